@@ -20,6 +20,7 @@ ST_BAD_PRIORITY = 0x4
 ST_BAD_REQUEST = 0x8
 ST_LEN_CLAMPED = 0x10
 ST_SCAN_ABORTED = 0x20
+ST_NO_PAGE = 0x40
 STATUS_WORDS = 4
 
 PART = 4096
@@ -31,7 +32,7 @@ IPC_HANDLE_BYTES = 64
 MAILBOX_BYTES = 2 * MAX_SHARDS * 16
 SEARCH_SCALE = 1
 
-DT_F32, DT_F64, DT_I64, DT_F16 = range(4)
+DT_F32, DT_F64, DT_I64, DT_F16, DT_BF16 = range(5)
 FILL_U32, FILL_F32_NORMAL, FILL_F32_UNIFORM, FILL_F32_LOGNORMAL, FILL_I32_RANGE, FILL_U8, FILL_U01_F64 = range(7)
 
 
@@ -162,6 +163,14 @@ _SIGS = {
     "gearb_ingest_client_step": (i64, [vp]),
     "gearb_ingest_client_writeback": (i64, [vp, C.c_int, C.c_int, f64]),
     "gearb_ingest_client_status": (C.c_int, [vp, pi64, C.POINTER(f64)]),
+    "gearb_handler_segment_lengths": (C.c_int, [vp, C.c_int, vp, vp, vp, i64, vp, vp]),
+    "gearb_handler_gather_packed": (C.c_int, [vp, pi32, C.c_int, vp, vp, vp, i64, vp, vp, i64, i64, vp, C.POINTER(vp),
+                                              pi64, vp, vp]),
+    "gearb_layout_scratch_bytes": (i64, [i64]),
+    "gearb_layout_paged": (C.c_int, [vp, vp]),
+    "gearb_recurrence_bytes": (C.c_int, [vp, C.c_int, pi64, pi64]),
+    "gearb_recurrence_forward": (C.c_int, [vp, vp]),
+    "gearb_recurrence_backward": (C.c_int, [vp, vp]),
     "gearb_fill": (C.c_int, [vp, i64, C.c_int, u64, u64, f64, f64, vp]),
 }
 
@@ -193,6 +202,25 @@ class PullArgs(C.Structure):
                 ("table", C.POINTER(vp)), ("variates", vp), ("b", i64), ("variate_stride", i64),
                 ("columns", pi32), ("ncols", C.c_int), ("dst", C.POINTER(vp)), ("zero_fill", C.c_int),
                 ("ring", C.c_int), ("out_flat", vp), ("out_idx", vp), ("out_ts", vp)]
+
+
+class LayoutArgs(C.Structure):
+    """gearb_layout_args of include/gear_b200.h."""
+    _fields_ = [("lengths", vp), ("past", vp), ("requests", i64), ("page", i64), ("max_blocks", i64),
+                ("block_table", vp), ("free_pages", vp), ("num_pages", i64), ("used_in", vp), ("used_out", vp),
+                ("offsets", vp), ("slot_map", vp), ("max_tokens", i64), ("scratch", vp), ("scratch_bytes", i64),
+                ("status", vp)]
+
+
+class RecurrenceArgs(C.Structure):
+    """gearb_recurrence_args of include/gear_b200.h."""
+    _fields_ = [("x", vp), ("gate", vp), ("x_dtype", i32), ("gate_dtype", i32), ("batch", i64), ("time", i64),
+                ("width", i64), ("gates", i64), ("x_batch_stride", i64), ("x_row_stride", i64),
+                ("gate_batch_stride", i64), ("gate_row_stride", i64), ("offsets", vp), ("lengths", vp),
+                ("sequences", i64), ("h0", vp), ("reverse", i32), ("gate_log", i32), ("zero_rest", i32), ("out", vp),
+                ("state_out", vp), ("carry", vp), ("dout", vp), ("dout_batch_stride", i64), ("dout_row_stride", i64),
+                ("dstate", vp), ("dx", vp), ("dgate", vp), ("dh0", vp), ("scratch", vp), ("scratch_bytes", i64),
+                ("status", vp)]
 
 
 def declared_symbols() -> list[str]:

@@ -8,6 +8,7 @@ CpuTrajectoryStorageHandler, Indexset; src/storage, include/index/set.h).
 from __future__ import annotations
 
 import ctypes as C
+from contextlib import nullcontext
 from dataclasses import dataclass
 from typing import Optional, Sequence
 
@@ -42,6 +43,15 @@ def _stream(stream=None) -> C.c_void_p:
             return C.c_void_p(_RAW_STREAM(_RAW_DEVICE()))
         stream = torch.cuda.current_stream()
     return C.c_void_p(stream.cuda_stream if hasattr(stream, "cuda_stream") else int(stream))
+
+
+def _stream_scope(stream):
+    """Context in which torch allocates for, and _stream() returns, the given stream (None: the current one)."""
+    if stream is None:
+        return nullcontext()
+    if not hasattr(stream, "cuda_stream"):
+        stream = torch.cuda.ExternalStream(int(stream))
+    return torch.cuda.stream(stream)
 
 
 def _dev_i64(t: torch.Tensor, what: str) -> C.c_void_p:
@@ -243,6 +253,74 @@ class StorageHandler:
              _dev_i64(idx, "idx"), _dev_i64(ts, "ts"), _dev_i64(ln, "len"), n,
              (C.c_void_p * nc)(*[d.data_ptr() for d in dsts]), int(bool(zero_fill)), _ptr(st),
              _stream(stream))
+
+    def segment_lengths(self, idx: torch.Tensor, ts: torch.Tensor, ln: torch.Tensor, column: int,
+                        out: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
+        """Rows that each request's clipped segment of `column` has: what gather() copies of it, int64."""
+        n = idx.numel()
+        if not (ts.numel() == n and ln.numel() == n):
+            raise GearError(N.ERR_INVALID, "idx, ts and len must have the same number of entries")
+        if out is not None and out.numel() != n:
+            raise GearError(N.ERR_INVALID, "out must have one entry per request")
+        ptrs = [_dev_i64(t, w) for t, w in ((idx, "idx"), (ts, "ts"), (ln, "len"))]
+        with torch.cuda.device(idx.device), _stream_scope(stream):
+            if out is None:
+                out = torch.empty(n, dtype=torch.int64, device=idx.device)
+            call("gearb_handler_segment_lengths", self._h, int(column), *ptrs, n, _dev_i64(out, "out"), _stream())
+        return out
+
+    def gather_packed(self, columns: Sequence[int], idx: torch.Tensor, ts: torch.Tensor, ln: torch.Tensor,
+                      offsets: torch.Tensor, dsts: Sequence[torch.Tensor],
+                      block_table: Optional[torch.Tensor] = None, page: int = 0,
+                      past: Optional[torch.Tensor] = None, stream=None) -> None:
+        """gather() without padding: row t of request r goes to row offsets[r] + t of each destination, or,
+        with a block table (int32 [requests, max_blocks]) and past lengths (int64, default 0), to row
+        block_table[r][(past[r] + t) // page] * page + (past[r] + t) % page.
+
+        The destinations are [rows, ...] with the column's bytes per row; rows no request owns are left as
+        they are.  At most offsets[r + 1] - offsets[r] rows of a request are copied.  Rows that would land
+        outside a destination, and pages below 0, are skipped and flagged (ST_BAD_REQUEST in status()).  The
+        columns must share one pattern offset and length; their pad option plays no role."""
+        n = idx.numel()
+        if not (ts.numel() == n and ln.numel() == n):
+            raise GearError(N.ERR_INVALID, "idx, ts and len must have the same number of entries")
+        if offsets.numel() != n + 1:
+            raise GearError(N.ERR_INVALID, "offsets must have one entry more than there are requests")
+        if len(dsts) != len(columns):
+            raise GearError(N.ERR_INVALID, "one destination per column is required")
+        for c in columns:
+            if not 0 <= int(c) < self.table.ncolumns:
+                raise GearError(N.ERR_INVALID, f"column id {int(c)} out of range")
+        rows = []
+        for c, d in zip(columns, dsts):
+            rb = self.table.row_bytes[int(c)]
+            if not d.is_cuda or d.device != idx.device or not d.is_contiguous() or d.dim() < 1 \
+                    or (d.shape[0] and d.numel() * d.element_size() != d.shape[0] * rb):
+                raise GearError(N.ERR_INVALID, f"destination of column {c} must be a contiguous CUDA tensor "
+                                               f"[rows, ...] of {rb} bytes per row, on the requests' device")
+            rows.append(d.shape[0])
+        bt, max_blocks = None, 0
+        if block_table is not None:
+            if block_table.dtype != torch.int32 or not block_table.is_cuda or not block_table.is_contiguous() \
+                    or block_table.dim() != 2 or block_table.shape[0] != n:
+                raise GearError(N.ERR_INVALID, "block_table must be a contiguous int32 CUDA tensor [requests, max_blocks]")
+            bt, max_blocks = block_table, block_table.shape[1]
+        if past is not None and past.numel() != n:
+            raise GearError(N.ERR_INVALID, "past must have one entry per request")
+        for t, what in ((ts, "ts"), (ln, "len"), (offsets, "offsets"), (bt, "block_table"), (past, "past")):
+            if t is not None and t.device != idx.device:
+                raise GearError(N.ERR_INVALID, f"{what} is on {t.device}, idx on {idx.device}")
+        nc = len(columns)
+        if n == 0 or nc == 0:
+            return
+        st = self.status_tensor(idx.device)
+        with torch.cuda.device(idx.device):
+            call("gearb_handler_gather_packed", self._h, (C.c_int32 * nc)(*[int(c) for c in columns]), nc,
+                 _dev_i64(idx, "idx"), _dev_i64(ts, "ts"), _dev_i64(ln, "len"), n, _dev_i64(offsets, "offsets"),
+                 _ptr(bt), max_blocks, int(page), None if past is None else _dev_i64(past, "past"),
+                 (C.c_void_p * nc)(*[d.data_ptr() or idx.data_ptr() for d in dsts]),   # 0 rows: never written
+                 (C.c_int64 * nc)(*rows), _ptr(st),
+                 _stream(stream))
 
     def view(self, index: int, column: int) -> np.ndarray:
         """Host bytes of one column of one trajectory (handler.cc:223-233)."""

@@ -565,6 +565,60 @@ int gearb_handler_gather(gearb_handler *h, const int32_t *columns, int ncols, co
   return launch_gather(p, as_stream(stream));
 }
 
+int gearb_handler_segment_lengths(const gearb_handler *h, int column, const int64_t *idx, const int64_t *ts,
+                                  const int64_t *len, int64_t n, int64_t *out, void *stream) {
+  TraceRange trace("gearb:segment_lengths");
+  const Pattern *pat = nullptr;
+  int rc = pattern_of(h, column, &pat);
+  if (rc != GEARB_OK) return rc;
+  GEARB_REQUIRE(n >= 0, "segment_lengths: negative request count");
+  if (n == 0) return GEARB_OK;
+  GEARB_REQUIRE(idx && ts && len && out, "segment_lengths: null argument");
+  GatherParams p = {};
+  p.idx = idx; p.ts = ts; p.len = len;
+  p.n = n;
+  p.capacity = h->table->capacity;
+  p.T = h->table->T;
+  p.cols[0].row = 1;
+  p.cols[0].pat_offset = pat->offset;
+  p.cols[0].pat_length = static_cast<int32_t>(pat->length);
+  return launch_segment_lengths(p, out, as_stream(stream));
+}
+
+int gearb_handler_gather_packed(gearb_handler *h, const int32_t *columns, int ncols, const int64_t *idx,
+                                const int64_t *ts, const int64_t *len, int64_t n, const int64_t *offsets,
+                                const int32_t *block_table, int64_t max_blocks, int64_t page, const int64_t *past,
+                                void *const *dst, const int64_t *dst_rows, int32_t *status, void *stream) {
+  TraceRange trace("gearb:gather_packed");
+  GatherParams p;
+  int rc = build_gather_params(h, columns, ncols, n, dst, 0, status, p);
+  if (rc != GEARB_OK) return rc;
+  for (int i = 1; i < ncols; ++i) {
+    const Pattern &a = *h->patterns[columns[0]], &b = *h->patterns[columns[i]];
+    GEARB_REQUIRE(a.offset == b.offset && a.length == b.length,
+                  "gather_packed: columns %d and %d have different patterns, gather them in calls of their own",
+                  columns[0], columns[i]);
+  }
+  GEARB_REQUIRE(!block_table || (page > 0 && max_blocks > 0 && page <= (int64_t(1) << 31) / max_blocks),
+                "gather_packed: a block table needs page and max_blocks, with page * max_blocks at most 2^31");
+  GEARB_REQUIRE(block_table || !past, "gather_packed: past lengths belong to a block table");
+  if (n == 0 || p.ncols == 0) return GEARB_OK;
+  GEARB_REQUIRE(idx && ts && len && offsets && dst_rows, "gather_packed: null argument");
+  p.idx = idx; p.ts = ts; p.len = len;
+  PackedDst d = {};
+  d.offsets = offsets;
+  d.block_table = block_table;
+  d.max_blocks = max_blocks;
+  d.page = page;
+  d.past = past;
+  // The listed columns share one pattern, so none was dropped from p.cols unless all were.
+  for (int i = 0; i < ncols; ++i) {
+    GEARB_REQUIRE(dst_rows[i] >= 0, "gather_packed: negative destination size");
+    d.dst_rows[i] = dst_rows[i];
+  }
+  return launch_gather_packed(p, d, as_stream(stream));
+}
+
 int gearb_handler_subcopy(gearb_handler *h, const int64_t *idx, const int64_t *ts,
                           const int64_t *len, int64_t n, int column, void *dst, int32_t *status,
                           void *stream) {

@@ -201,6 +201,16 @@ int64_t mailbox_blk_base(int64_t n);
 int launch_publish(const double *l1, int64_t nparts, int world, int rank, void *const *mailboxes,
                    unsigned long long epoch, int copy_l1, unsigned *counter, cudaStream_t stream,
                    const float *blk = nullptr);
+// Where the rows of a packed or paged gather go.
+struct PackedDst {
+  const int64_t *offsets;       // [n + 1]
+  const int32_t *block_table;   // null: packed
+  int64_t max_blocks, page;
+  const int64_t *past;          // may be null
+  int64_t dst_rows[GEARB_MAX_COLUMNS];  // by position in GatherParams::cols
+};
+int launch_gather_packed(const GatherParams &p, const PackedDst &d, cudaStream_t stream);
+int launch_segment_lengths(const GatherParams &p, int64_t *out, cudaStream_t stream);
 int launch_vcopy(const uint8_t *src, uint8_t *dst, const int64_t *src_off,
                  const int64_t *dst_off, const int64_t *lengths, int64_t fixed_length,
                  int64_t n, int64_t max_length, cudaStream_t stream);

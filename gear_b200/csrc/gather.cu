@@ -75,6 +75,71 @@ __global__ void __launch_bounds__(kThreads) vcopy_kernel(const VcopyArgs a) {
   }
 }
 
+__global__ void segment_lengths_kernel(const __grid_constant__ GatherParams P, int64_t *out) {
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
+  if (i >= P.n) return;
+  int64_t start, rows;
+  unsigned flags = 0;
+  dev::clip_segment(P, P.cols[0], P.idx[i], P.ts[i], P.len[i], start, rows, flags);
+  out[i] = rows;
+}
+
+// Packed / paged gather: one warp moves one 2 KiB piece of a request's column, cut at the page
+// boundaries that fall into it.
+__global__ void __launch_bounds__(kThreads) gather_packed_kernel(const __grid_constant__ GatherParams P,
+                                                                 const __grid_constant__ PackedDst D) {
+  const int lane = threadIdx.x & 31;
+  const int64_t warps_total = static_cast<int64_t>(gridDim.x) * kWarpsPerBlock;
+  const int64_t items = P.n * P.chunks_per_request;
+  unsigned flags = 0;
+  for (int64_t item = static_cast<int64_t>(blockIdx.x) * kWarpsPerBlock + (threadIdx.x >> 5); item < items;
+       item += warps_total) {
+    const int64_t g = item / P.chunks_per_request;
+    const int q = static_cast<int>(item - g * P.chunks_per_request);
+    const int ci = dev::column_of_piece(P, q);
+    const GatherColumn &col = P.cols[ci];
+    const int64_t idx = __ldg(P.idx + g), o0 = __ldg(D.offsets + g), o1 = __ldg(D.offsets + g + 1);
+    int64_t start, bytes;
+    dev::clip_segment(P, col, idx, __ldg(P.ts + g), __ldg(P.len + g), start, bytes, flags);
+    const int64_t row = col.row;
+    if (o0 < 0 || o1 <= o0) {
+      if (o0 < 0) flags |= GEARB_ST_BAD_REQUEST;
+      continue;
+    }
+    if (bytes / row > o1 - o0) bytes = (o1 - o0) * row;
+    const int64_t c0 = static_cast<int64_t>(q - col.chunk_first) * P.chunk_bytes;
+    const int64_t c1 = c0 + P.chunk_bytes < bytes ? c0 + P.chunk_bytes : bytes;
+    if (c1 <= c0) continue;
+    const uint8_t *src = dev::segment_src(P, col, idx, start, P.table);
+    if (!D.block_table) {
+      // bytes of the piece that lie inside the destination
+      const int64_t left = o0 < D.dst_rows[ci] ? (D.dst_rows[ci] - o0) * row : 0;
+      if (c1 > left) flags |= GEARB_ST_BAD_REQUEST;
+      const int64_t b = c1 < left ? c1 : left;
+      if (b > c0) dev::warp_copy(col.dst + o0 * row + c0, src + c0, static_cast<int>(b - c0), lane);
+      continue;
+    }
+    const int64_t past = D.past ? __ldg(D.past + g) : 0;
+    if (past < 0 || past > D.max_blocks * D.page) {
+      flags |= GEARB_ST_BAD_REQUEST;
+      continue;
+    }
+    for (int64_t c = c0; c < c1;) {
+      const int64_t t = c / row, pos = past + t, blk = pos / D.page;
+      const int64_t in_page = pos - blk * D.page;
+      int64_t e = (t + D.page - in_page) * row;  // first byte of the next page
+      if (e > c1) e = c1;
+      const int64_t page = blk < D.max_blocks ? __ldg(D.block_table + g * D.max_blocks + blk) : -1;
+      const int64_t slot = page * D.page + in_page;  // row of t; (c - t * row) bytes of it went before
+      const int64_t rows = (e - 1) / row - t + 1;
+      if (page < 0 || slot + rows > D.dst_rows[ci]) flags |= GEARB_ST_BAD_REQUEST;
+      else dev::warp_copy(col.dst + slot * row + (c - t * row), src + c, static_cast<int>(e - c), lane);
+      c = e;
+    }
+  }
+  if (flags && P.status && lane == 0) atomicOr(reinterpret_cast<unsigned *>(P.status), flags);
+}
+
 int grid_for(int64_t items) {
   int64_t blocks = (items + kWarpsPerBlock - 1) / kWarpsPerBlock;
   const int64_t cap = static_cast<int64_t>(sm_count()) * 64;
@@ -89,6 +154,20 @@ int launch_gather(const GatherParams &p, cudaStream_t stream) {
   if (p.n == 0 || p.ncols == 0) return GEARB_OK;
   const int64_t items = p.n * p.chunks_per_request;
   gather_kernel<<<grid_for(items), kThreads, 0, stream>>>(p);
+  GEARB_CUDA(cudaGetLastError());
+  return GEARB_OK;
+}
+
+int launch_segment_lengths(const GatherParams &p, int64_t *out, cudaStream_t stream) {
+  const int64_t blocks = (p.n + kThreads - 1) / kThreads;
+  GEARB_REQUIRE(blocks < (int64_t(1) << 31), "segment_lengths: too many requests");
+  segment_lengths_kernel<<<static_cast<unsigned>(blocks), kThreads, 0, stream>>>(p, out);
+  GEARB_CUDA(cudaGetLastError());
+  return GEARB_OK;
+}
+
+int launch_gather_packed(const GatherParams &p, const PackedDst &d, cudaStream_t stream) {
+  gather_packed_kernel<<<grid_for(p.n * p.chunks_per_request), kThreads, 0, stream>>>(p, d);
   GEARB_CUDA(cudaGetLastError());
   return GEARB_OK;
 }

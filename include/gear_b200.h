@@ -40,6 +40,7 @@ extern "C" {
 #define GEARB_ST_LEN_CLAMPED 0x10     /* gather: a length beyond trajectory_length was clamped */
 #define GEARB_ST_SCAN_ABORTED 0x20    /* a bounded wait inside a kernel ran out (a lost copy, a peer that never
                                          published): the tables or the batch of that launch are NOT valid */
+#define GEARB_ST_NO_PAGE 0x40         /* layout: the pool ran out of pages, the entries and slots concerned are -1 */
 /* status[1] = number of variates that landed within one float32 ulp of a
  * cumulative-priority boundary (search), accumulated until cleared.
  * status[2] = low 32 bits of the epoch at which a pull launch last gave up waiting for its peers.
@@ -332,6 +333,7 @@ int gearb_comm_recv(gearb_comm *c, void *buf, int64_t bytes, int peer, void *str
 #define GEARB_DT_F64 1
 #define GEARB_DT_I64 2
 #define GEARB_DT_F16 3
+#define GEARB_DT_BF16 4 /* recurrences only */
 int gearb_comm_allreduce_sum(gearb_comm *c, void *buf, int64_t count, int dtype, void *stream);
 int gearb_comm_allgather(gearb_comm *c, const void *send, void *recv, int64_t bytes_per_rank,
                          void *stream);
@@ -482,6 +484,106 @@ int gearb_ingest_client_release(gearb_ingest_client *c);
 int64_t gearb_ingest_client_step(gearb_ingest_client *c);
 int64_t gearb_ingest_client_writeback(gearb_ingest_client *c, int terminated, int alloc_new, double weight);
 int gearb_ingest_client_status(const gearb_ingest_client *c, int64_t *out7, double *weight);
+
+/* ======================= sequence batches ================================ */
+/* What a sequence model needs next to sampled segments: how a batch of unequal
+ * lengths is laid out (packed rows, or pages of a pool), the gather into that
+ * layout, and the linear recurrences over it (discounted returns, advantages,
+ * recurrent layers).  The reference has no counterpart: it pads every segment
+ * to its pattern's length (gear/loader/offline_loader.py:178-203).            */
+
+/* Rows each request's clipped segment has (the copy length of handler.sub, src/storage/handler.cc:104-115,
+ * in rows of `column`'s pattern): out[i] = max(0, min(len, trajectory_length, start + pattern length) - start),
+ * 0 for a trajectory index outside the table.                                                      */
+int gearb_handler_segment_lengths(const gearb_handler *h, int column, const int64_t *idx, const int64_t *ts,
+                                  const int64_t *len, int64_t n, int64_t *out, void *stream);
+
+/* Packed (block_table == NULL) or paged form of gearb_handler_gather: row t of request r goes to row
+ * offsets[r] + t of dst[c], or to row block_table[r][(past[r]+t) / page] * page + (past[r]+t) % page.
+ * At most offsets[r+1] - offsets[r] rows of a request are copied; rows that would land outside
+ * [0, dst_rows[c]) and pages below 0 are skipped (GEARB_ST_BAD_REQUEST).  All listed columns must have the
+ * same pattern offset and length.  Rows of dst that no request owns are left as they are.           */
+int gearb_handler_gather_packed(gearb_handler *h, const int32_t *columns, int ncols, const int64_t *idx,
+                                const int64_t *ts, const int64_t *len, int64_t n, const int64_t *offsets,
+                                const int32_t *block_table, int64_t max_blocks, int64_t page, const int64_t *past,
+                                void *const *dst, const int64_t *dst_rows, int32_t *status, void *stream);
+
+/* Offsets, block table and slot map of a batch from its request lengths.
+ *   n_r        = lengths[r] clamped to [0, max_blocks * page - past[r]]  (GEARB_ST_LEN_CLAMPED when it was)
+ *   offsets[r] = n_0 + ... + n_(r-1);  requests + 1 entries
+ *   need_r     = ceil((past[r] + n_r) / page) - ceil(past[r] / page) new pages, taken in request order
+ *                from free_pages[used_in ...] (NULL: page k of the pool itself), at most up to num_pages
+ *   block_table[r][ceil(past[r] / page) ...] = those pages; its other entries are left as they are
+ *   slot_map[offsets[r] + t] = block_table[r][(past[r]+t) / page] * page + (past[r]+t) % page;
+ *                entries from offsets[requests] to max_tokens are -1
+ *   used_out   = min(used_in + sum of need_r, num_pages); may be the same address as used_in
+ * Where the pool runs out the entries and slots are -1 (GEARB_ST_NO_PAGE).  Tokens beyond max_tokens have
+ * their pages but no entry in slot_map.  past may be NULL (all 0); slot_map may be NULL (max_tokens 0).
+ * scratch: gearb_layout_scratch_bytes(requests) bytes, contents irrelevant, one per call in flight.   */
+typedef struct gearb_layout_args {
+  const int64_t *lengths;
+  const int64_t *past;
+  int64_t requests;
+  int64_t page;
+  int64_t max_blocks;
+  int32_t *block_table;
+  const int32_t *free_pages;
+  int64_t num_pages;
+  const int64_t *used_in;
+  int64_t *used_out;
+  int64_t *offsets;
+  int64_t *slot_map;
+  int64_t max_tokens;
+  void *scratch;
+  int64_t scratch_bytes;
+  int32_t *status;
+} gearb_layout_args;
+int64_t gearb_layout_scratch_bytes(int64_t requests);
+int gearb_layout_paged(const gearb_layout_args *args, void *stream);
+
+/* Linear recurrence  h_t = a_t * h_(t-1) + x_t  for every sequence and channel; a_t = gate, or exp(gate)
+ * with gate_log.  Rows are batch * time; row (b, t) of x starts at x + b * x_batch_stride + t * x_row_stride
+ * elements, its channels are consecutive; likewise gate (gates channels, each shared by width / gates
+ * consecutive channels of x) and dout.  out, dx ([rows][width]) and dgate ([rows][gates]) are contiguous.
+ * Sequences:  offsets != NULL  packed: batch is 1, sequence s is rows [offsets[s], offsets[s+1])
+ *             lengths != NULL  padded: sequence b is the first lengths[b] rows of batch entry b
+ *             neither          dense:  sequence b is all rows of batch entry b
+ * Rows of no sequence are not used; out, dx and dgate get zeros there with zero_rest, else are left as
+ * they are.  reverse: from the last row of a sequence to its first.  h0, state_out, dstate, dh0:
+ * float32 [sequences][width], each may be NULL (h0: zeros); state_out of an empty sequence is its h0.
+ * Types: x, out, dout, dx of x_dtype; gate, dgate of gate_dtype, either x_dtype or GEARB_DT_F32.
+ * All arithmetic is float32; the result does not depend on timing.
+ * carry: what the backward pass needs besides x and gate, written by the forward pass when not NULL.
+ * gearb_recurrence_bytes gives the sizes of scratch (contents irrelevant, one per call in flight) and
+ * carry.  The backward pass reads x, gate, h0, dout, dstate and carry, writes dx, dgate and dh0.     */
+typedef struct gearb_recurrence_args {
+  const void *x;
+  const void *gate;
+  int32_t x_dtype, gate_dtype;
+  int64_t batch, time, width, gates;
+  int64_t x_batch_stride, x_row_stride, gate_batch_stride, gate_row_stride;
+  const int64_t *offsets;
+  const int64_t *lengths;
+  int64_t sequences;
+  const float *h0;
+  int32_t reverse, gate_log, zero_rest;
+  void *out;
+  float *state_out;
+  float *carry;
+  const void *dout;
+  int64_t dout_batch_stride, dout_row_stride;
+  const float *dstate;
+  void *dx;
+  void *dgate;
+  float *dh0;
+  void *scratch;
+  int64_t scratch_bytes;
+  int32_t *status;
+} gearb_recurrence_args;
+int gearb_recurrence_bytes(const gearb_recurrence_args *args, int backward, int64_t *scratch_bytes,
+                           int64_t *carry_bytes);
+int gearb_recurrence_forward(const gearb_recurrence_args *args, void *stream);
+int gearb_recurrence_backward(const gearb_recurrence_args *args, void *stream);
 
 /* ======================= synthetic data ================================= */
 /* Device-side Philox4x32-10 fills for benchmark tables that are too large to

@@ -1,0 +1,421 @@
+"""Linear recurrences on the GPU against a row-by-row float64 reference (recurrence_ref.py derives the tolerances)."""
+import numpy as np
+import pytest
+import torch
+
+import recurrence_ref as R
+from gear_b200 import _native as N
+from gear_b200 import core, recurrence
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+
+
+def make(seed, lead, width, gates, dtype, gate_dtype, log, one_step=False):
+    rng = np.random.default_rng(seed)
+    x = torch.from_numpy(rng.standard_normal(lead + (width,)).astype(np.float32)).to(dtype).to(DEV)
+    a = np.exp(-np.exp(rng.uniform(-7, 1, lead + (gates,))))
+    if not log:
+        a = a * np.where(rng.random(a.shape) < 0.02, 0.0, np.sign(rng.uniform(-0.2, 1, a.shape)))
+    gate = torch.from_numpy((np.log(a) if log else a).astype(np.float32)).to(gate_dtype).to(DEV)
+    return x, gate
+
+
+def dbl(t):
+    return None if t is None else t.detach().double().cpu().numpy()
+
+
+def run_and_check(x, gate, h0=None, offsets=None, lengths=None, reverse=False, log=False, train=True, seed=0,
+                  with_dstate=True):
+    """Forward without and with gradients, backward; everything against the reference."""
+    width, gates = x.shape[-1], gate.shape[-1]
+    time = x.shape[0] if offsets is not None else x.shape[1]
+    rows = x.shape[0] if offsets is not None else x.shape[0] * x.shape[1]
+    ns = offsets.numel() - 1 if offsets is not None else x.shape[0]
+    seqs = R.spans(rows, time, dbl(offsets), dbl(lengths))
+    kind = "log" if log else "decay"
+    rng = np.random.default_rng(seed + 99)
+    dh = torch.from_numpy(rng.standard_normal(tuple(x.shape)).astype(np.float32)).to(x.dtype).to(DEV)
+    dstate = torch.from_numpy(rng.standard_normal((ns, width)).astype(np.float32)).to(DEV) if with_dstate else None
+    owned = np.zeros(rows, bool)
+    for lo, hi in seqs:
+        owned[lo:hi] = True
+    # what no sequence owns must not matter: NaN there for the kernel, zeros for the reference
+    hole = torch.from_numpy(~owned).to(DEV).reshape(x.shape[:-1] + (1,))
+    xk, gk, dk = (torch.where(hole, float("nan"), t.float()).to(t.dtype) for t in (x, gate, dh))
+    flat = lambda t, c: dbl(t).reshape(rows, c)
+    want = R.reference(flat(x, width), flat(gate, gates), seqs, dbl(h0), reverse, log, flat(dh, width), dbl(dstate))
+    kw = dict(offsets=offsets, lengths=lengths, reverse=reverse, gate_kind=kind)
+
+    h, state = recurrence.linear_recurrence(xk, gk, h0=h0, **kw)
+    R.check(h, want["h"], x.dtype, "h")
+    R.check(state, want["state"], F32, "state")
+    assert h.dtype == x.dtype and state.dtype == F32 and h.shape == x.shape
+    if not owned.all():
+        assert (h.reshape(rows, width)[torch.from_numpy(~owned).to(DEV)] == 0).all()
+    if not train:
+        return h, state
+    leaves = [t.clone().requires_grad_(True) for t in (xk, gk)] + ([h0.clone().requires_grad_(True)] if h0 is not None else [])
+    h2, state2 = recurrence.linear_recurrence(leaves[0], leaves[1], h0=leaves[2] if h0 is not None else None, **kw)
+    assert torch.equal(h2, h) and torch.equal(state2, state)
+    outs, gouts = ([h2, state2], [dk, dstate]) if with_dstate else ([h2], [dk])
+    grads = torch.autograd.grad(outs, leaves, gouts)
+    R.check(grads[0], want["dx"], x.dtype, "dx")
+    R.check(grads[1], want["dgate"], gate.dtype, "dgate")
+    if h0 is not None:
+        R.check(grads[2], want["dh0"], F32, "dh0")
+    if not owned.all():
+        sel = torch.from_numpy(~owned).to(DEV)
+        assert (grads[0].reshape(rows, width)[sel] == 0).all() and (grads[1].reshape(rows, gates)[sel] == 0).all()
+    return h, state
+
+
+def state_of(seed, n, width):
+    return torch.from_numpy(np.random.default_rng(seed).standard_normal((n, width)).astype(np.float32)).to(DEV)
+
+
+DENSE = [
+    # batch, time, width, gates
+    (1, 1, 1, 1), (1, 1, 5, 5), (3, 1, 64, 64), (7, 1, 130, 2), (1, 2, 33, 33), (2, 63, 32, 32), (2, 64, 32, 1),
+    (2, 65, 31, 31), (1, 127, 64, 64), (1, 128, 128, 4), (3, 129, 129, 1), (1, 1000, 1, 1), (5, 333, 1, 1),
+    (2, 517, 2, 2), (1, 700, 3, 1), (2, 300, 7, 7), (1, 900, 16, 4), (2, 257, 100, 5), (1, 2500, 40, 8),
+    (1, 1537, 256, 256), (2, 640, 300, 3), (9, 40, 257, 257), (1, 5000, 8, 8), (1, 20000, 1, 1), (300, 3, 4, 2),
+]
+
+
+@pytest.mark.parametrize("batch,time,width,gates", DENSE)
+@pytest.mark.parametrize("dtype,gate_dtype", [(F32, F32), (BF16, F32)])
+def test_dense(batch, time, width, gates, dtype, gate_dtype):
+    seed = batch * 1000003 + time * 101 + width
+    log, reverse = bool((time + width) & 1), bool((batch + gates) & 1)
+    x, gate = make(seed, (batch, time), width, gates, dtype, gate_dtype, log)
+    h0 = state_of(seed, batch, width) if (time + gates) % 3 else None
+    run_and_check(x, gate, h0, reverse=reverse, log=log, seed=seed, with_dstate=bool(time % 2))
+
+
+@pytest.mark.parametrize("dtype,gate_dtype", [(F32, F32), (F16, F32), (F16, F16), (BF16, F32), (BF16, BF16)])
+@pytest.mark.parametrize("log", [False, True])
+@pytest.mark.parametrize("reverse", [False, True])
+@pytest.mark.parametrize("width,gates", [(96, 96), (96, 3), (6, 6), (6, 2)])
+def test_types_and_directions(dtype, gate_dtype, log, reverse, width, gates):
+    x, gate = make(7, (3, 210), width, gates, dtype, gate_dtype, log)
+    run_and_check(x, gate, state_of(8, 3, width), reverse=reverse, log=log)
+
+
+LENGTHS = [
+    [0], [0, 0, 0], [5], [1, 1, 1, 1], [64, 64, 64], [63, 1, 64, 0, 65, 0], [0, 300, 0, 0, 7, 129, 0],
+    [1] * 200, [0, 1] * 100, [1000, 3, 0, 500, 31, 32, 33], [2000],
+]
+
+
+@pytest.mark.parametrize("lens", LENGTHS)
+@pytest.mark.parametrize("width,gates", [(1, 1), (3, 3), (40, 8), (64, 1), (200, 200)])
+@pytest.mark.parametrize("reverse", [False, True])
+def test_packed(lens, width, gates, reverse):
+    off = torch.from_numpy(np.concatenate([[0], np.cumsum(lens)])).to(DEV)
+    rows = sum(lens) + (len(lens) % 3) * 50        # rows behind the last sequence
+    seed = rows + width
+    log = bool(len(lens) & 1)
+    x, gate = make(seed, (rows,), width, gates, BF16 if gates == 8 else F32, F32, log)
+    h0 = state_of(seed, len(lens), width) if len(lens) % 2 or reverse else None
+    run_and_check(x, gate, h0, offsets=off, reverse=reverse, log=log)
+
+
+@pytest.mark.parametrize("width,gates", [(1, 1), (5, 1), (48, 48), (136, 2)])
+@pytest.mark.parametrize("reverse", [False, True])
+@pytest.mark.parametrize("time", [1, 31, 64, 200, 777])
+def test_padded(width, gates, reverse, time):
+    rng = np.random.default_rng(time)
+    lens = rng.integers(0, time + 1, 9)
+    lens[0], lens[1] = 0, time
+    x, gate = make(time, (9, time), width, gates, F32, F32, True)
+    run_and_check(x, gate, state_of(time, 9, width), lengths=torch.from_numpy(lens).to(DEV), reverse=reverse, log=True)
+
+
+def test_offsets_need_not_start_at_row_zero():
+    off = torch.tensor([10, 10, 75, 200], device=DEV)
+    for width, reverse in ((1, True), (70, False), (70, True), (4, False)):
+        x, gate = make(3, (260,), width, width, F32, F32, False)
+        run_and_check(x, gate, state_of(1, 3, width), offsets=off, reverse=reverse)
+
+
+@pytest.mark.parametrize("width,gates", [(64, 64), (2, 1), (72, 8)])
+def test_strides(width, gates):
+    """Slices of wider rows, time-major storage, a gate expanded over time or over the batch, odd base addresses."""
+    rng = np.random.default_rng(0)
+    wide = torch.from_numpy(rng.standard_normal((3, 150, 2 * width + 3)).astype(np.float32)).to(DEV)
+    x, g = wide[..., 3:3 + width], torch.sigmoid(wide[..., 1:1 + gates])
+    run_and_check(x, g, state_of(0, 3, width))
+    tm = torch.from_numpy(rng.standard_normal((150, 3, width)).astype(np.float32)).to(BF16).to(DEV).transpose(0, 1)
+    run_and_check(tm, g, state_of(0, 3, width))
+    per_channel = torch.sigmoid(wide[0, 0, :gates]).expand(3, 150, gates)
+    per_step = torch.sigmoid(wide[0, :, :gates]).unsqueeze(0).expand(3, 150, gates)
+    for e in (per_channel, per_step):
+        h, _ = recurrence.linear_recurrence(x, e)
+        assert torch.equal(h, recurrence.linear_recurrence(x.contiguous(), e.contiguous())[0])
+    p = wide.reshape(-1, 2 * width + 3)[:, 2:2 + width]
+    off = torch.tensor([0, 100, 450], device=DEV)
+    run_and_check(p, torch.sigmoid(wide.reshape(-1, 2 * width + 3)[:, :gates]), None, offsets=off, reverse=True)
+    # last dimension not consecutive: copied
+    t = torch.from_numpy(rng.standard_normal((2, width, 50)).astype(np.float32)).to(DEV).transpose(1, 2)
+    run_and_check(t, torch.sigmoid(t[..., :gates]), None)
+
+
+def test_gradient_of_a_broadcast_gate_and_of_a_summed_loss():
+    x, gate = make(5, (2, 130), 32, 32, F32, F32, False)
+    decay = gate[0, 0].clone().requires_grad_(True)
+    h, _ = recurrence.linear_recurrence(x, decay.expand(2, 130, 32), return_state=False)
+    h.sum().backward()                     # an expanded gradient of ones: strides 0
+    d2 = gate[0, 0].clone().double().cpu().requires_grad_(True)
+    cur, tot = torch.zeros(2, 32, dtype=torch.float64), 0.0
+    for t in range(130):
+        cur = d2 * cur + x[:, t].double().cpu()
+        tot = tot + cur.sum()
+    tot.backward()
+    scale = d2.grad.abs().max()
+    # 260 rows are summed, each a few dozen roundings of values that may be hundreds of times the result
+    assert (decay.grad.double().cpu() - d2.grad).abs().max() <= 1e-4 * scale
+
+
+@pytest.mark.parametrize("width,gates,reverse,log", [(3, 3, False, True), (64, 4, True, False), (1, 1, True, False)])
+def test_gradients_against_differences(width, gates, reverse, log):
+    """<gradient, v> against central differences of the float64 reference's loss along v."""
+    x, gate = make(11, (2, 90), width, gates, F32, F32, log)
+    h0 = state_of(12, 2, width)
+    rng = np.random.default_rng(1)
+    dh, dst = rng.standard_normal((180, width)), rng.standard_normal((2, width))
+    dh, dst = dh.astype(np.float32).astype(np.float64), dst.astype(np.float32).astype(np.float64)
+    seqs = R.spans(180, 90, None, None)
+
+    def loss(xx, gg, hh):
+        r = R.reference(xx, gg, seqs, hh, reverse, log)
+        return (r["h"][0] * dh).sum() + (r["state"][0] * dst).sum()
+
+    base = [dbl(x).reshape(180, width), dbl(gate).reshape(180, gates), dbl(h0)]
+    full = R.reference(*base[:2], seqs, base[2], reverse, log, dh, dst)
+    leaves = [t.clone().requires_grad_(True) for t in (x, gate, h0)]
+    h, s = recurrence.linear_recurrence(*leaves[:2], h0=leaves[2], reverse=reverse, gate_kind="log" if log else "decay")
+    grads = torch.autograd.grad([h, s], leaves, [torch.from_numpy(dh).float().reshape(h.shape).to(DEV),
+                                                 torch.from_numpy(dst).float().to(DEV)])
+    for i, key in enumerate(("dx", "dgate", "dh0")):
+        v = rng.standard_normal(base[i].shape)
+        eps = 1e-5
+        up, dn = list(base), list(base)
+        up[i], dn[i] = base[i] + eps * v, base[i] - eps * v
+        diff = (loss(*up) - loss(*dn)) / (2 * eps)
+        got = (dbl(grads[i]).reshape(v.shape) * v).sum()
+        # the kernel's own bound, and what the difference loses: 1e-11 of the loss's size over eps, eps^2 relative
+        size = np.abs(full[key][0] * v).sum()
+        tol = ((full[key][1] + U32 * np.abs(full[key][0])) * np.abs(v)).sum() + 1e-6 * size + 1e-6
+        assert abs(got - diff) <= tol, (key, got, diff, tol)
+
+
+U32 = 2.0 ** -24
+
+
+def test_a_poisoned_sequence_stays_alone():
+    """NaN and infinities inside one sequence do not reach its neighbours, in either direction or pass."""
+    lens = [70, 64, 1, 200, 90]
+    off = torch.from_numpy(np.concatenate([[0], np.cumsum(lens)])).to(DEV)
+    for width in (1, 4, 64):
+        for reverse in (False, True):
+            x, gate = make(2, (sum(lens),), width, width, F32, F32, False)
+            clean = run_and_check(x, gate, None, offsets=off, reverse=reverse)[0]
+            bx, bg = x.clone(), gate.clone()
+            bx[140:150], bg[150:160] = float("nan"), float("inf")     # in sequence 3 (rows 135..334)
+            leaves = [bx.requires_grad_(True), bg.requires_grad_(True)]
+            h, _ = recurrence.linear_recurrence(*leaves, offsets=off, reverse=reverse)
+            assert torch.equal(h[:135], clean[:135]) and torch.equal(h[335:], clean[335:])
+            dx, dg = torch.autograd.grad(h, leaves, torch.ones_like(h))
+            for t in (dx, dg):
+                assert torch.isfinite(t[:135]).all() and torch.isfinite(t[335:]).all()
+
+
+def test_log_gate_of_minus_infinity_forgets():
+    x, gate = make(4, (1, 200), 64, 64, F32, F32, True)
+    gate[:, 77] = -float("inf")
+    h, _ = recurrence.linear_recurrence(x, gate, gate_kind="log")
+    assert torch.equal(h[:, 77], x[:, 77])
+    rest, _ = recurrence.linear_recurrence(x[:, 77:], gate[:, 77:], gate_kind="log")
+    want = R.reference(dbl(x[0, 77:]), dbl(gate[0, 77:]), [(0, 123)], log=True)["h"]
+    R.check(h[0, 77:], want, F32, "h behind the reset")
+    R.check(rest[0], want, F32, "h from the reset")
+
+
+@pytest.mark.parametrize("width,gates,lead", [(1, 1, (4, 3000)), (64, 64, (1, 4000)), (96, 3, (2, 2000))])
+def test_same_bits_every_time(width, gates, lead):
+    x, gate = make(6, lead, width, gates, BF16, F32, True)
+    dh = torch.randn(lead + (width,), device=DEV).to(BF16)
+
+    def once():
+        leaves = [x.clone().requires_grad_(True), gate.clone().requires_grad_(True)]
+        h, s = recurrence.linear_recurrence(*leaves, gate_kind="log")
+        return [h, s, *torch.autograd.grad(h, leaves, dh)]
+
+    first = once()
+    for _ in range(5):
+        assert all(torch.equal(a, b) for a, b in zip(first, once()))
+
+
+def test_out_state_out_and_rows_left_alone():
+    lens = [30, 0, 101]
+    off = torch.tensor([0, 30, 30, 131], device=DEV)
+    for width in (1, 64):
+        x, gate = make(9, (150,), width, width, F32, F32, False)
+        h0 = state_of(1, 3, width)
+        want, ws = recurrence.linear_recurrence(x, gate, h0=h0, offsets=off)
+        out = torch.full_like(x, 7.0)
+        state = h0.clone()
+        h, s = recurrence.linear_recurrence(x, gate, h0=state, offsets=off, out=out, state_out=state)
+        assert h is out and s is state
+        assert torch.equal(out[:131], want[:131]) and (out[131:] == 7.0).all() and torch.equal(state, ws)
+        assert torch.equal(ws[1], h0[1])
+
+
+def test_step_by_step_equals_the_whole():
+    """One token at a time with the carried state gives the whole sequence's values (within float32 rounding)."""
+    x, gate = make(10, (3, 25), 130, 130, F32, F32, True)
+    want = R.reference(dbl(x).reshape(75, 130), dbl(gate).reshape(75, 130), R.spans(75, 25, None, None), log=True)
+    state = torch.zeros(3, 130, device=DEV)
+    got = []
+    for t in range(25):
+        h, _ = recurrence.linear_recurrence(x[:, t:t + 1], gate[:, t:t + 1], h0=state, state_out=state, gate_kind="log")
+        got.append(h)
+    R.check(torch.cat(got, 1), want["h"], F32, "h")
+    R.check(state, want["state"], F32, "state")
+
+
+def test_graph_replay_and_other_streams():
+    x, gate = make(13, (2, 900), 72, 72, BF16, F32, True)
+    want, ws = recurrence.linear_recurrence(x, gate, gate_kind="log")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    h, s = recurrence.linear_recurrence(x, gate, gate_kind="log", stream=side)
+    side.synchronize()
+    assert torch.equal(h, want) and torch.equal(s, ws)
+    # two captured graphs of the forward and one of a training step, replayed together on two streams
+    xs = [x.clone(), x.clone()]
+    graphs, outs = [], []
+    for i in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(recurrence.linear_recurrence(xs[i], gate, gate_kind="log"))
+        graphs.append(g)
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    for k in range(3):
+        xs[0].copy_(x * (k + 1)), xs[1].copy_(x * -(k + 1))
+        torch.cuda.synchronize()
+        for g, s in zip(graphs, (s1, s2)):
+            with torch.cuda.stream(s):
+                for _ in range(4):
+                    g.replay()
+        torch.cuda.synchronize()
+        for i in range(2):
+            e, _ = recurrence.linear_recurrence(xs[i], gate, gate_kind="log")
+            assert torch.equal(outs[i][0], e)
+
+
+def test_training_step_in_a_graph():
+    x, gate = make(14, (2, 300), 64, 64, F32, F32, False)
+    dh = torch.randn_like(x)
+    eager = [t.clone().requires_grad_(True) for t in (x, gate)]
+    h, _ = recurrence.linear_recurrence(*eager)
+    want = torch.autograd.grad(h, eager, dh)
+    leaves = [t.clone().requires_grad_(True) for t in (x, gate)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):                  # warm up as torch asks
+        hh, _ = recurrence.linear_recurrence(*leaves)
+        torch.autograd.grad(hh, leaves, dh)
+        del hh
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        hh, _ = recurrence.linear_recurrence(*leaves)
+        got = torch.autograd.grad(hh, leaves, dh)
+    g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_concurrent_calls_on_two_streams():
+    x, gate = make(15, (1, 6000), 64, 64, F32, F32, True)
+    want, _ = recurrence.linear_recurrence(x, gate, gate_kind="log")
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    outs = []
+    for _ in range(10):
+        for s in streams:
+            outs.append(recurrence.linear_recurrence(x, gate, gate_kind="log", stream=s)[0])
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for o in outs)
+
+
+def test_empty_batches():
+    for width in (1, 64):
+        e = torch.zeros(0, width, device=DEV)
+        h0 = state_of(0, 2, width)
+        h, s = recurrence.linear_recurrence(e, e, h0=h0, offsets=torch.zeros(3, dtype=torch.int64, device=DEV))
+        assert h.shape == (0, width) and torch.equal(s, h0)
+        h, s = recurrence.linear_recurrence(e, e, offsets=torch.zeros(1, dtype=torch.int64, device=DEV))
+        assert s.shape == (0, width)
+        z = torch.zeros(3, 0, width, device=DEV, requires_grad=True)
+        h0 = state_of(0, 3, width).requires_grad_(True)
+        h, s = recurrence.linear_recurrence(z, torch.zeros(3, 0, width, device=DEV), h0=h0)
+        assert torch.equal(s, h0)
+        d, = torch.autograd.grad(s, [h0], torch.ones_like(s))
+        assert (d == 1).all()
+        n = torch.zeros(0, 4, width, device=DEV)
+        h, s = recurrence.linear_recurrence(n, n)
+        assert h.shape == (0, 4, width) and s.shape == (0, width)
+        # rows, but no sequence
+        h, s = recurrence.linear_recurrence(torch.ones(5, width, device=DEV), torch.ones(5, width, device=DEV),
+                                            offsets=torch.zeros(1, dtype=torch.int64, device=DEV))
+        assert (h == 0).all()
+
+
+def test_offsets_and_lengths_outside_the_rows_are_cut():
+    x, gate = make(1, (100,), 64, 64, F32, F32, False)
+    off = torch.tensor([0, 40, 1 << 40], device=DEV)
+    h, s = recurrence.linear_recurrence(x, gate, offsets=off)
+    want, ws = recurrence.linear_recurrence(x, gate, offsets=torch.tensor([0, 40, 100], device=DEV))
+    assert torch.equal(h, want) and torch.equal(s, ws)
+    h, s = recurrence.linear_recurrence(x[None], gate[None], lengths=torch.tensor([1 << 50], device=DEV))
+    assert torch.equal(h, recurrence.linear_recurrence(x[None], gate[None])[0])
+    h, s = recurrence.linear_recurrence(x[None], gate[None], lengths=torch.tensor([-3], device=DEV))
+    assert (h == 0).all() and (s == 0).all()
+
+
+def test_refusals():
+    x = torch.zeros(2, 5, 6, device=DEV)
+    g = torch.zeros(2, 5, 6, device=DEV)
+    bad = [
+        lambda: recurrence.linear_recurrence(x.double(), g.double()),
+        lambda: recurrence.linear_recurrence(x, g.half()),
+        lambda: recurrence.linear_recurrence(x, g[..., :4]),
+        lambda: recurrence.linear_recurrence(x, g[:, :4]),
+        lambda: recurrence.linear_recurrence(x, g, gate_kind="tanh"),
+        lambda: recurrence.linear_recurrence(x, g, h0=torch.zeros(2, 5, device=DEV)),
+        lambda: recurrence.linear_recurrence(x, g, h0=torch.zeros(2, 6, device=DEV).half()),
+        lambda: recurrence.linear_recurrence(x, g, h0=torch.zeros(2, 6)),
+        lambda: recurrence.linear_recurrence(x, g, lengths=torch.zeros(3, dtype=torch.int64, device=DEV)),
+        lambda: recurrence.linear_recurrence(x, g, lengths=torch.zeros(2, dtype=torch.int32, device=DEV)),
+        lambda: recurrence.linear_recurrence(x, g, offsets=torch.zeros(2, dtype=torch.int64, device=DEV)),
+        lambda: recurrence.linear_recurrence(x, g, out=torch.zeros(2, 5, 5, device=DEV)),
+        lambda: recurrence.linear_recurrence(x, g, out=torch.zeros(2, 6, 5, device=DEV).transpose(1, 2)),
+        lambda: recurrence.linear_recurrence(x.clone().requires_grad_(True), g, out=torch.zeros_like(x)),
+        lambda: recurrence.linear_recurrence(x, g, status=torch.zeros(2, dtype=torch.int32, device=DEV)),
+        lambda: recurrence.linear_recurrence(x.cpu(), g.cpu()),
+        lambda: recurrence.linear_recurrence(x, g.cpu()),
+    ]
+    for f in bad:
+        with pytest.raises(core.GearError) as e:
+            f()
+        assert e.value.code == N.ERR_INVALID
+    # only once differentiable
+    xg = x.clone().requires_grad_(True)
+    h, _ = recurrence.linear_recurrence(xg, g)
+    d, = torch.autograd.grad(h.sum(), xg, create_graph=True)
+    with pytest.raises(RuntimeError):
+        d.sum().backward()
