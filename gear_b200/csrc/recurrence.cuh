@@ -1,0 +1,393 @@
+// Linear recurrences over sequences, forward and backward.
+//
+//   h_t = a_t * h_(t-1) + x_t                      h_(-1) = h0
+//   g_t = dh_t + a_(t+1) * g_(t+1)                 g_last = dh_last + dstate
+//   dx_t = g_t,  da_t = sum over the gate's channels of g_t * h_(t-1),  dh0 = a_0 * g_0
+//
+// with a_t = gate, or exp(gate) (then dgate = da * a).  This file has what the kernels share.
+//
+// Any run of rows maps the state before it to the state behind it as S -> A*S + H (A the product of its a_t,
+// H its own result from zero), and such maps compose, so rows can be worked on in parallel: all rows of a call,
+// sequence after sequence, are cut into tiles of 64; a CTA takes one tile and one block of channels, keeps
+// gate and x in registers (8 rows a warp, one channel or a few a lane), forms (A, H), learns the state before
+// its tile, and runs its rows again from there.  Every input is read once and every output written once.
+//
+// The state before a tile.  Tiles publish their (A, H); 16 consecutive tiles form a superblock, and the last
+// tile of one publishes the state behind it.  A tile composes the tiles before it in its superblock, in
+// order, onto the state in front of the superblock: the same operations whatever the timing, so results are the
+// same bits every time, and the chain of waiting CTAs has one link per 1024 rows.  A tile needs nothing from
+// before the start of the sequence its first row belongs to.  Tiles are handed out by a counter in scan order,
+// so a CTA only ever waits for CTAs that are already running; every wait has a limit, after which the
+// launch goes on with NaN and says so in the status word.  Published words are 32 bits that read
+// 0xffffffff until they are written (a value of those bits is published as another NaN), so no flags and
+// fences are needed beside them.
+//
+// Backward.  In terms of c_t = a_t * g_t the gradients obey c_t = a_t * c_(t+1) + a_t * dh_t, the same
+// recurrence from the last row to the first, over the same tiles.  h_(t-1) is not read back (it was rounded to
+// x's type) but formed again in float32 from x, gate and the state before the tile, which the forward
+// pass leaves in `carry`.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "common.h"
+#include "warp_search.cuh"
+
+namespace gearb {
+namespace rec {
+
+constexpr int kWarps = 8;
+constexpr int kThreads = kWarps * 32;
+constexpr int kRows = 8;                     // rows a warp keeps in registers
+constexpr int kTile = kWarps * kRows;        // rows per tile
+constexpr int kSuper = 16;                   // tiles per superblock
+constexpr unsigned kAll = 0xffffffffu;
+constexpr unsigned kUnset = 0xffffffffu;     // a published word that has not been written
+constexpr int kPollLimit = 1 << 20;          // polls of one word, the better part of a second
+
+template <typename T> __device__ __forceinline__ float to_f(T v);
+template <> __device__ __forceinline__ float to_f(float v) { return v; }
+template <> __device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
+template <> __device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T> __device__ __forceinline__ T from_f(float v);
+template <> __device__ __forceinline__ float from_f(float v) { return v; }
+template <> __device__ __forceinline__ __half from_f(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f(float v) { return __float2bfloat16_rn(v); }
+
+// V consecutive values of T, loaded and stored as one access.
+template <typename T, int V>
+struct alignas(sizeof(T) * V) Pack {
+  T v[V];
+};
+template <typename T, int V>
+__device__ __forceinline__ Pack<T, V> load_pack(const T *p) {
+  constexpr int kBytes = sizeof(T) * V;
+  Pack<T, V> r;
+  if constexpr (kBytes == 16) {
+    *reinterpret_cast<uint4 *>(&r) = __ldcs(reinterpret_cast<const uint4 *>(p));
+  } else if constexpr (kBytes == 8) {
+    *reinterpret_cast<uint2 *>(&r) = __ldcs(reinterpret_cast<const uint2 *>(p));
+  } else if constexpr (kBytes == 4) {
+    *reinterpret_cast<unsigned *>(&r) = __ldcs(reinterpret_cast<const unsigned *>(p));
+  } else {
+    *reinterpret_cast<unsigned short *>(&r) = __ldcs(reinterpret_cast<const unsigned short *>(p));
+  }
+  return r;
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_pack(T *p, const float (&f)[V]) {
+  Pack<T, V> r;
+#pragma unroll
+  for (int v = 0; v < V; ++v) r.v[v] = from_f<T>(f[v]);
+  *reinterpret_cast<Pack<T, V> *>(p) = r;
+}
+
+// What the kernels need beyond the caller's arguments.
+struct Params {
+  gearb_recurrence_args A;
+  int64_t rows;
+  int64_t tiles;
+  int tile_rows;         // kTile, or the largest multiple of `time` below it when tiles then need nothing from each other
+  int chain;             // tiles publish to each other
+  int per;               // channels per gate
+  int blocks_per_gate;   // column blocks of a gate's channels (shared gates)
+  int ncol;              // column blocks
+  // Address periods: rows per batch entry, or all rows where one row stride covers the whole batch.
+  int64_t x_period, gate_period, dout_period;
+  unsigned *ticket;
+  float2 *agg;           // [tiles][width]: (A, H) of every tile
+  float *super;          // [superblocks][width]: state in front of every superblock
+  int V;                 // channels a lane, by alignment and width
+  float *gate_part;      // [blocks_per_gate][rows][gates], when a gate's channels span several column blocks
+};
+
+__device__ __forceinline__ unsigned poll_word(const unsigned *p, bool &lost) {
+  unsigned v;
+  for (int n = 0;; ++n) {
+    asm volatile("ld.relaxed.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+    if (v != kUnset) return v;
+    if (lost || n == kPollLimit) break;
+    __nanosleep(20);
+  }
+  lost = true;
+  return 0x7fffffffu;  // NaN
+}
+__device__ __forceinline__ float2 peek_pair(const float2 *p) {
+  unsigned a, h;
+  asm volatile("ld.relaxed.gpu.global.v2.u32 {%0,%1}, [%2];" : "=r"(a), "=r"(h) : "l"(p) : "memory");
+  return make_float2(__uint_as_float(a), __uint_as_float(h));
+}
+__device__ __forceinline__ float2 poll_pair(const float2 *p, bool &lost) {
+  unsigned a, h;
+  for (int n = 0;; ++n) {
+    asm volatile("ld.relaxed.gpu.global.v2.u32 {%0,%1}, [%2];" : "=r"(a), "=r"(h) : "l"(p) : "memory");
+    if (a != kUnset && h != kUnset) return make_float2(__uint_as_float(a), __uint_as_float(h));
+    if (lost || n == kPollLimit) break;
+    __nanosleep(20);
+  }
+  lost = true;
+  return make_float2(__uint_as_float(0x7fffffffu), __uint_as_float(0x7fffffffu));
+}
+__device__ __forceinline__ unsigned word_of(float v) {
+  const unsigned u = __float_as_uint(v);
+  return u == kUnset ? 0x7fffffffu : u;
+}
+__device__ __forceinline__ void publish_pair(float2 *p, float a, float h) {
+  asm volatile("st.relaxed.gpu.global.v2.u32 [%0], {%1,%2};" ::"l"(p), "r"(word_of(a)), "r"(word_of(h)) : "memory");
+}
+__device__ __forceinline__ void publish_word(float *p, float v) {
+  asm volatile("st.relaxed.gpu.global.u32 [%0], %1;" ::"l"(p), "r"(word_of(v)) : "memory");
+}
+
+// Offset s of the packed sequences in scan order: as given, or mirrored for a reverse call.  Kept inside the rows.
+struct ScanOffsets {
+  const int64_t *off;
+  int64_t rows, n;
+  int reverse;
+  __device__ __forceinline__ int64_t at(int64_t s) const {
+    int64_t v = __ldg(off + (reverse ? n - s : s));
+    v = v < 0 ? 0 : (v > rows ? rows : v);
+    return reverse ? rows - v : v;
+  }
+  // For warp_upper_bound, which walks a pointer.
+  __device__ __forceinline__ int64_t operator()(const int64_t *p) const { return at(p - off); }
+};
+
+// a / b of non-negative numbers, in 32 bits where both have no more (the usual case by far).
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+  if (((a | b) >> 32) == 0) return static_cast<unsigned>(a) / static_cast<unsigned>(b);
+  return a / b;
+}
+
+// Rows [i0, i0 + n) of the scan as one warp sees them; row k is bit k.  Lane k holds the sequence of row k.
+struct RowMap {
+  unsigned live, start, end;
+  int seq;
+  int64_t first_start;  // scan index at which the sequence of row i0 starts
+  int64_t last_end;     // scan index at which the sequence of row i0 + n - 1 ends
+};
+
+__device__ __forceinline__ RowMap map_rows(const gearb_recurrence_args &A, int64_t rows, int64_t i0, int n, int lane) {
+  RowMap m;
+  m.seq = 0;
+  m.first_start = m.last_end = 0;
+  const int64_t i = i0 + lane;
+  bool live = lane < n, start = false, end = false;
+  if (!A.offsets) {
+    int64_t s0 = 0, s1 = 0;
+    if (live) {
+      const int64_t b = quotient(i, A.time), u = i - b * A.time;
+      const int64_t seq = A.reverse ? A.batch - 1 - b : b;
+      int64_t len = A.time;
+      if (A.lengths) {
+        len = __ldg(A.lengths + seq);
+        len = len < 0 ? 0 : (len > A.time ? A.time : len);
+      }
+      const int64_t lo = A.reverse ? A.time - len : 0;  // first live row of this batch entry, in scan order
+      live = u >= lo && u < lo + len;
+      start = live && u == lo;
+      end = live && u == lo + len - 1;
+      m.seq = static_cast<int>(seq);
+      s0 = i - u + lo;
+      s1 = s0 + len - 1;
+    }
+    m.first_start = __shfl_sync(kAll, s0, 0);
+    m.last_end = __shfl_sync(kAll, s1, n > 0 ? n - 1 : 0);
+  } else {
+    const ScanOffsets so{A.offsets, rows, A.sequences, A.reverse};
+    const int64_t total = so.at(A.sequences);
+    live = live && i < total;
+    int64_t my_seq = -1, my_start = 0, my_end = 0;
+    if (n > 0 && i0 < total) {
+      int64_t s = warp_upper_bound<int64_t>(A.offsets, 0, A.sequences, i0, lane, so);  // first offset behind row i0
+      int64_t before = s > 0 ? so.at(s - 1) : -1;  // the offset in front of the window; -1: rows of no sequence
+      bool settled = lane >= n;
+      const int64_t behind = so.at(s);
+      if (behind > i0 + n) {  // no sequence starts or ends behind the first row: nearly always
+        settled = true;
+        my_seq = s - 1;
+        my_start = before;
+        my_end = behind;
+      }
+      while (!__all_sync(kAll, settled)) {  // 32 offsets at a time: one round unless many sequences end within these rows
+        const int64_t b = s + lane <= A.sequences ? so.at(s + lane) : rows + 1;
+        int count = 0;  // offsets of the window at or before this lane's row
+        for (int k = 0; k < n; ++k) {
+          const unsigned c = __ballot_sync(kAll, b <= i0 + k);
+          if (lane == k) count = __popc(c);
+        }
+        const int64_t st = __shfl_sync(kAll, b, count > 0 ? count - 1 : 0);
+        const int64_t nx = __shfl_sync(kAll, b, count < 32 ? count : 31);
+        if (!settled && count < 32) {
+          settled = true;
+          my_seq = s + count - 1;
+          my_start = count > 0 ? st : before;
+          my_end = nx;
+        }
+        before = __shfl_sync(kAll, b, 31);
+        s += 32;
+      }
+    }
+    live = live && my_seq >= 0;
+    start = live && my_start == i;
+    end = live && my_end == i + 1;
+    // offsets that do not ascend give nonsense, but nothing outside the rows
+    if (my_start > i || my_start < 0) my_start = i;
+    if (my_end <= i || my_end > rows) my_end = i + 1;
+    m.seq = live ? static_cast<int>(A.reverse ? A.sequences - 1 - my_seq : my_seq) : 0;
+    m.first_start = __shfl_sync(kAll, my_start, 0);
+    m.last_end = __shfl_sync(kAll, my_end - 1, n > 0 ? n - 1 : 0);
+  }
+  m.live = __ballot_sync(kAll, live);
+  m.start = __ballot_sync(kAll, start && live);
+  m.end = __ballot_sync(kAll, end && live);
+  return m;
+}
+
+// Element offset of consecutive rows of the scan in one tensor.
+struct RowWalk {
+  int64_t off, t, period, step, wrap;
+  int reverse;
+  __device__ __forceinline__ RowWalk(int64_t row, int64_t period_, int64_t sb, int64_t sr, int reverse_)
+      : period(period_), reverse(reverse_) {
+    const int64_t b = quotient(row, period);
+    t = row - b * period;
+    off = b * sb + t * sr;
+    step = reverse ? -sr : sr;
+    wrap = reverse ? period * sr - sb : sb - period * sr;
+  }
+  __device__ __forceinline__ void next() {
+    off += step;
+    if (reverse) {
+      if (t-- == 0) {
+        t = period - 1;
+        off += wrap;
+      }
+    } else if (++t == period) {
+      t = 0;
+      off += wrap;
+    }
+  }
+};
+
+__device__ __forceinline__ int64_t row_of(const Params &P, int64_t i) { return P.A.reverse ? P.rows - 1 - i : i; }
+
+// The CTA's tile and column block.
+struct Place {
+  int64_t tile;
+  int64_t i0, i1;  // rows of the scan
+  int64_t gate;    // shared gates: the gate of this column block
+  int64_t d0, d1;  // channels
+  int part;        // which column block of the gate
+};
+
+template <int V, bool kShared>
+__device__ __forceinline__ Place take_place(const Params &P, unsigned *smem_ticket, bool backward) {
+  unsigned item;
+  if (P.chain) {
+    if (threadIdx.x == 0) *smem_ticket = atomicAdd(P.ticket, 1u) + 1u;  // the counter starts at 0xffffffff
+    __syncthreads();
+    item = *smem_ticket;
+  } else {
+    item = blockIdx.x;
+  }
+  Place p;
+  const unsigned t = item / static_cast<unsigned>(P.ncol);
+  const int c = static_cast<int>(item - t * static_cast<unsigned>(P.ncol));
+  p.tile = backward ? P.tiles - 1 - t : t;
+  p.i0 = p.tile * P.tile_rows;
+  p.i1 = p.i0 + P.tile_rows < P.rows ? p.i0 + P.tile_rows : P.rows;
+  if (kShared) {
+    p.gate = c / P.blocks_per_gate;
+    p.part = c - static_cast<int>(p.gate) * P.blocks_per_gate;
+    p.d0 = p.gate * P.per + static_cast<int64_t>(p.part) * 32 * V;
+    p.d1 = (p.gate + 1) * P.per;
+  } else {
+    p.gate = 0;
+    p.part = 0;
+    p.d0 = static_cast<int64_t>(c) * 32 * V;
+    p.d1 = P.A.width;
+  }
+  return p;
+}
+
+// V consecutive channels of n rows of the scan (zeros where there is no row or channel).
+template <typename T, int V>
+__device__ __forceinline__ void load_rows(const T *base, const Params &P, int64_t i0, int64_t period, int64_t sb, int64_t sr,
+                                          int n, int64_t d, bool on, Pack<T, V> (&r)[kRows]) {
+#pragma unroll
+  for (int k = 0; k < kRows; ++k)
+#pragma unroll
+    for (int v = 0; v < V; ++v) r[k].v[v] = from_f<T>(0.0f);
+  if (n == 0 || !on) return;
+  RowWalk w(row_of(P, i0), period, sb, sr, P.A.reverse);
+  if (n == kRows && (P.A.reverse ? w.t >= kRows - 1 : w.t + kRows <= period)) {
+    const T *p = base + w.off + d;  // eight rows of one batch entry: one stride
+#pragma unroll
+    for (int k = 0; k < kRows; ++k) r[k] = load_pack<T, V>(p + k * w.step);
+  } else {
+#pragma unroll
+    for (int k = 0; k < kRows; ++k) {
+      if (k < n) r[k] = load_pack<T, V>(base + w.off + d);
+      w.next();
+    }
+  }
+}
+
+// What the tiles before this one (in the order of the tickets, `at` of them) hand on: the state of channel d in front of
+// the tile.  lo: the first tile that matters.
+__device__ __forceinline__ float look_back(const Params &P, int64_t at, int64_t lo, int64_t d, bool &lost) {
+  const int64_t sb = at / kSuper, sb0 = sb * kSuper;
+  const bool need_super = lo < sb0;
+  const int64_t j0 = need_super ? sb0 : lo;
+  float pa = 1.0f, ph = 0.0f;
+  for (int64_t j = j0; j < at; j += 5) {
+    float2 q[5];
+#pragma unroll
+    for (int u = 0; u < 5; ++u)
+      if (j + u < at) q[u] = peek_pair(P.agg + (j + u) * P.A.width + d);
+#pragma unroll
+    for (int u = 0; u < 5; ++u)
+      if (j + u < at) {
+        if (__float_as_uint(q[u].x) == kUnset || __float_as_uint(q[u].y) == kUnset)
+          q[u] = poll_pair(P.agg + (j + u) * P.A.width + d, lost);
+        // nothing in front of the sequence's start counts
+        ph = (j + u == j0 && !need_super) ? q[u].y : fmaf(q[u].x, ph, q[u].y);
+        pa *= q[u].x;
+      }
+  }
+  if (!need_super) return ph;
+  const float s = __uint_as_float(poll_word(reinterpret_cast<const unsigned *>(P.super + sb * P.A.width + d), lost));
+  return fmaf(pa, s, ph);
+}
+
+// Hands a sequence without rows its state (forward) or its gradient (backward): the CTAs of a launch share the
+// sequences among them.
+__device__ __forceinline__ void empty_sequences(const Params &P, const Place &pl, int64_t block, const float *from,
+                                                float *to) {
+  const gearb_recurrence_args &A = P.A;
+  if (!to) return;
+  const int64_t step = P.tiles * kThreads;
+  for (int64_t s = pl.tile * kThreads + threadIdx.x; s < A.sequences; s += step) {
+    int64_t n;
+    if (A.offsets) {
+      const ScanOffsets so{A.offsets, P.rows, A.sequences, 0};
+      n = so.at(s + 1) - so.at(s);
+    } else if (!A.lengths) {
+      return;
+    } else {
+      n = __ldg(A.lengths + s);
+    }
+    if (n > 0) continue;
+    const int64_t d1 = pl.d0 + block < pl.d1 ? pl.d0 + block : pl.d1;
+    for (int64_t d = pl.d0; d < d1; ++d) to[s * A.width + d] = from ? from[s * A.width + d] : 0.0f;
+  }
+}
+
+int launch_f32(Params &p, bool backward, cudaStream_t stream);
+int launch_f16(Params &p, bool backward, cudaStream_t stream);
+int launch_bf16(Params &p, bool backward, cudaStream_t stream);
+
+}  // namespace rec
+}  // namespace gearb

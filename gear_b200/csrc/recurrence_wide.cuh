@@ -1,0 +1,445 @@
+// Kernels of the recurrences for rows of many channels: one warp a row, V channels a lane.
+//
+// Three phases with a barrier between them.  Every warp forms (A, H) of its eight rows; then one thread per channel goes
+// through the eight warps' pairs, publishes the tile's, learns the state before the tile and leaves the state before
+// each warp; then every warp runs its rows from there.
+#pragma once
+
+#include "recurrence.cuh"
+
+namespace gearb {
+namespace rec {
+
+template <typename TA, int V, bool kShared>
+__device__ __forceinline__ void load_gate(const Params &P, const Place &pl, int64_t i0, int n, int64_t d, bool on,
+                                          float (&a)[kRows][kShared ? 1 : V]) {
+  constexpr int kG = kShared ? 1 : V;
+  Pack<TA, kG> raw[kRows];
+  load_rows<TA, kG>(static_cast<const TA *>(P.A.gate), P, i0, P.gate_period, P.A.gate_batch_stride, P.A.gate_row_stride, n,
+                    kShared ? pl.gate : d, on, raw);
+#pragma unroll
+  for (int k = 0; k < kRows; ++k)
+#pragma unroll
+    for (int v = 0; v < kG; ++v) a[k][v] = to_f(raw[k].v[v]);
+}
+
+template <int kG>
+__device__ __forceinline__ void exp_gate(float (&a)[kRows][kG]) {
+#pragma unroll
+  for (int k = 0; k < kRows; ++k)
+#pragma unroll
+    for (int v = 0; v < kG; ++v) a[k][v] = expf(a[k][v]);
+}
+
+// A float of every channel of [sequences][width], of V channels of one sequence.
+template <int V>
+__device__ __forceinline__ void state_load(const float *p, int seq, int64_t width, int64_t d, bool on, float (&r)[V]) {
+#pragma unroll
+  for (int v = 0; v < V; ++v) r[v] = (p && on) ? p[static_cast<int64_t>(seq) * width + d + v] : 0.0f;
+}
+template <int V>
+__device__ __forceinline__ void state_store(float *p, int seq, int64_t width, int64_t d, bool on, const float (&r)[V]) {
+  if (p && on)
+#pragma unroll
+    for (int v = 0; v < V; ++v) p[static_cast<int64_t>(seq) * width + d + v] = r[v];
+}
+
+template <typename TX, typename TA, int V, bool kShared>
+__global__ void __launch_bounds__(kThreads, V == 4 ? 2 : 3) forward_kernel(const __grid_constant__ Params P) {
+  constexpr int kG = kShared ? 1 : V;
+  constexpr int kW = 32 * V;  // channels of a block
+  __shared__ float sa[kWarps][kW], sh[kWarps][kW];
+  __shared__ int scut[kWarps];
+  __shared__ unsigned sticket;
+  __shared__ int64_t sfirst;  // scan index at which the first row's sequence starts, or -1: nothing is needed from before
+  const gearb_recurrence_args &A = P.A;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const Place pl = take_place<V, kShared>(P, &sticket, false);
+  const int64_t d = pl.d0 + lane * V;
+  const bool on = d < pl.d1;
+  const int64_t i0 = pl.i0 + warp * kRows;
+  const int n = static_cast<int>(i0 >= pl.i1 ? 0 : (pl.i1 - i0 < kRows ? pl.i1 - i0 : kRows));
+
+  Pack<TX, V> x[kRows];
+  float a[kRows][kG];
+  load_rows<TX, V>(static_cast<const TX *>(A.x), P, i0, P.x_period, A.x_batch_stride, A.x_row_stride, n, d, on, x);
+  load_gate<TA, V, kShared>(P, pl, i0, n, d, on, a);
+  const RowMap m = map_rows(A, P.rows, i0, n, lane);
+  if (A.gate_log) exp_gate(a);
+  const bool plain = m.live == (1u << kRows) - 1u && (m.start | m.end) == 0;
+
+  // (A, H) of this warp's rows; behind a start only H counts
+  float ca[V], ch[V], first[V];  // first: h of the last start row, see below
+#pragma unroll
+  for (int v = 0; v < V; ++v) { ca[v] = 1.0f; ch[v] = first[v] = 0.0f; }
+  if (plain) {
+#pragma unroll
+    for (int k = 0; k < kRows; ++k)
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const float av = a[k][kShared ? 0 : v];
+        ch[v] = fmaf(av, ch[v], to_f(x[k].v[v]));
+        ca[v] *= av;
+      }
+  } else {
+#pragma unroll
+    for (int k = 0; k < kRows; ++k) {
+      if (!(m.live >> k & 1u)) continue;
+      const bool st = m.start >> k & 1u;
+      float s[V];
+      if (st) state_load<V>(A.h0, __shfl_sync(kAll, m.seq, k), A.width, d, on, s);
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const float av = a[k][kShared ? 0 : v], xv = to_f(x[k].v[v]);
+        if (st) ch[v] = first[v] = A.h0 ? fmaf(av, s[v], xv) : xv;
+        else ch[v] = fmaf(av, ch[v], xv);
+        ca[v] *= av;
+      }
+    }
+  }
+#pragma unroll
+  for (int v = 0; v < V; ++v) { sa[warp][lane * V + v] = ca[v]; sh[warp][lane * V + v] = ch[v]; }
+  if (lane == 0) {
+    scut[warp] = m.start != 0;
+    if (warp == 0) sfirst = ((m.live & ~m.start) & 1u) ? m.first_start : -1;
+  }
+  __syncthreads();
+
+  const int64_t ch2 = pl.d0 + threadIdx.x;
+  if (threadIdx.x < kW && ch2 < pl.d1) {
+    float cin = 0.0f;
+    if (P.chain) {
+      float ta = 1.0f, th = 0.0f;
+#pragma unroll
+      for (int q = 0; q < kWarps; ++q) {
+        const float b = sa[q][threadIdx.x], h = sh[q][threadIdx.x];
+        th = scut[q] ? h : fmaf(b, th, h);
+        ta *= b;
+      }
+      publish_pair(P.agg + pl.tile * A.width + ch2, ta, th);
+      const int64_t lo = sfirst >= 0 ? quotient(sfirst, P.tile_rows) : pl.tile;
+      if (lo < pl.tile) {
+        bool lost = false;
+        cin = look_back(P, pl.tile, lo, ch2, lost);
+        if (lost && A.status) atomicOr(reinterpret_cast<unsigned *>(A.status), GEARB_ST_SCAN_ABORTED);
+        if (A.carry) A.carry[pl.tile * A.width + ch2] = cin;
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < kWarps; ++q) {
+      const float b = sa[q][threadIdx.x], h = sh[q][threadIdx.x];
+      sh[q][threadIdx.x] = cin;  // the state before warp q
+      cin = scut[q] ? h : fmaf(b, cin, h);
+    }
+    if (P.chain && pl.tile % kSuper == kSuper - 1 && pl.tile + 1 < P.tiles)
+      publish_word(P.super + (pl.tile / kSuper + 1) * A.width + ch2, cin);
+  }
+  __syncthreads();
+
+  if (n > 0) {
+    float h[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) h[v] = sh[warp][lane * V + v];
+    TX *out = static_cast<TX *>(A.out) + row_of(P, i0) * A.width + d;
+    const int64_t step = A.reverse ? -A.width : A.width;
+    if (plain) {
+#pragma unroll
+      for (int k = 0; k < kRows; ++k) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) h[v] = fmaf(a[k][kShared ? 0 : v], h[v], to_f(x[k].v[v]));
+        if (on) store_pack<TX, V>(out + k * step, h);
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < kRows; ++k) {
+        if (k >= n) break;
+        if (!(m.live >> k & 1u)) {
+          if (A.zero_rest && on) {
+            const float z[V] = {};
+            store_pack<TX, V>(out + k * step, z);
+          }
+          continue;
+        }
+        const int seq = __shfl_sync(kAll, m.seq, k);
+        if (m.start >> k == 1u) {
+          // The sequence may end in another warp or tile, which may by now have put its state where h0 was
+          // (state_out may be h0): h of this row is kept from the first look at it.
+#pragma unroll
+          for (int v = 0; v < V; ++v) h[v] = first[v];
+        } else if (m.start >> k & 1u) {
+          float s[V];
+          state_load<V>(A.h0, seq, A.width, d, on, s);
+#pragma unroll
+          for (int v = 0; v < V; ++v) {
+            const float xv = to_f(x[k].v[v]);
+            h[v] = A.h0 ? fmaf(a[k][kShared ? 0 : v], s[v], xv) : xv;
+          }
+        } else {
+#pragma unroll
+          for (int v = 0; v < V; ++v) h[v] = fmaf(a[k][kShared ? 0 : v], h[v], to_f(x[k].v[v]));
+        }
+        if (on) store_pack<TX, V>(out + k * step, h);
+        if (m.end >> k & 1u) state_store<V>(A.state_out, seq, A.width, d, on, h);
+      }
+    }
+  }
+  empty_sequences(P, pl, kW, A.h0, A.state_out);
+}
+
+// Sums of eight values over the 32 lanes: lane l with l % 4 == 0 ends up with the sum of value
+// (l >> 4 & 1) * 4 + (l >> 3 & 1) * 2 + (l >> 2 & 1).  Nine shuffles instead of forty.
+__device__ __forceinline__ float sum_rows(float (&v)[kRows], int lane) {
+  static_assert(kRows == 8, "three halvings");
+#pragma unroll
+  for (int half = 4, m = 16; half > 0; half >>= 1, m >>= 1) {
+    const bool up = lane & m;
+#pragma unroll
+    for (int j = 0; j < half; ++j) {
+      const float give = up ? v[j] : v[j + half], keep = up ? v[j + half] : v[j];
+      v[j] = keep + __shfl_xor_sync(kAll, give, m);
+    }
+  }
+  v[0] += __shfl_xor_sync(kAll, v[0], 2);
+  v[0] += __shfl_xor_sync(kAll, v[0], 1);
+  return v[0];
+}
+
+template <typename TX, typename TA, int V, bool kShared>
+__global__ void __launch_bounds__(kThreads, V == 4 ? 2 : 3) backward_kernel(const __grid_constant__ Params P) {
+  constexpr int kG = kShared ? 1 : V;
+  constexpr int kW = 32 * V;
+  __shared__ float sa[kWarps][kW], sh[kWarps][kW], sc[kWarps][kW];
+  __shared__ int scut[kWarps], send[kWarps];
+  __shared__ unsigned sticket;
+  __shared__ int64_t slast;   // scan index at which the last row's sequence ends, or -1: nothing is needed from behind
+  __shared__ int sopen;       // the first row continues a sequence of an earlier tile
+  const gearb_recurrence_args &A = P.A;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const Place pl = take_place<V, kShared>(P, &sticket, true);
+  const int64_t d = pl.d0 + lane * V;
+  const bool on = d < pl.d1;
+  const int64_t i0 = pl.i0 + warp * kRows;
+  const int n = static_cast<int>(i0 >= pl.i1 ? 0 : (pl.i1 - i0 < kRows ? pl.i1 - i0 : kRows));
+
+  Pack<TX, V> x[kRows], dh[kRows];
+  float a[kRows][kG];
+  load_rows<TX, V>(static_cast<const TX *>(A.x), P, i0, P.x_period, A.x_batch_stride, A.x_row_stride, n, d, on, x);
+  load_gate<TA, V, kShared>(P, pl, i0, n, d, on, a);
+  load_rows<TX, V>(static_cast<const TX *>(A.dout), P, i0, P.dout_period, A.dout_batch_stride, A.dout_row_stride, n, d, on,
+                   dh);
+  const RowMap m = map_rows(A, P.rows, i0, n, lane);
+  if (A.gate_log) exp_gate(a);
+  const bool plain = m.live == (1u << kRows) - 1u && (m.start | m.end) == 0;
+
+  // (A, H) of this warp's rows forward, (A, C) backward
+  float ca[V], ch[V], cc[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) { ca[v] = 1.0f; ch[v] = 0.0f; cc[v] = 0.0f; }
+  if (plain) {
+#pragma unroll
+    for (int k = 0; k < kRows; ++k)
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const float av = a[k][kShared ? 0 : v];
+        ch[v] = fmaf(av, ch[v], to_f(x[k].v[v]));
+        ca[v] *= av;
+      }
+#pragma unroll
+    for (int k = kRows - 1; k >= 0; --k)
+#pragma unroll
+      for (int v = 0; v < V; ++v) cc[v] = a[k][kShared ? 0 : v] * (to_f(dh[k].v[v]) + cc[v]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < kRows; ++k) {
+      if (!(m.live >> k & 1u)) continue;
+      const bool st = m.start >> k & 1u;
+      float s[V];
+      if (st) state_load<V>(A.h0, __shfl_sync(kAll, m.seq, k), A.width, d, on, s);
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const float av = a[k][kShared ? 0 : v], xv = to_f(x[k].v[v]);
+        if (st) ch[v] = A.h0 ? fmaf(av, s[v], xv) : xv;
+        else ch[v] = fmaf(av, ch[v], xv);
+        ca[v] *= av;
+      }
+    }
+#pragma unroll
+    for (int k = kRows - 1; k >= 0; --k) {
+      if (!(m.live >> k & 1u)) continue;
+      if (m.end >> k & 1u) state_load<V>(A.dstate, __shfl_sync(kAll, m.seq, k), A.width, d, on, cc);
+#pragma unroll
+      for (int v = 0; v < V; ++v) cc[v] = a[k][kShared ? 0 : v] * (to_f(dh[k].v[v]) + cc[v]);
+    }
+  }
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    sa[warp][lane * V + v] = ca[v];
+    sh[warp][lane * V + v] = ch[v];
+    sc[warp][lane * V + v] = cc[v];
+  }
+  if (lane == 0) {
+    scut[warp] = m.start != 0;
+    send[warp] = m.end != 0;
+    if (warp == 0) sopen = ((m.live & ~m.start) & 1u) && quotient(m.first_start, P.tile_rows) < pl.tile;
+    if (n > 0 && i0 + n == pl.i1) slast = ((m.live & ~m.end) >> (n - 1) & 1u) ? m.last_end : -1;
+  }
+  __syncthreads();
+
+  // one thread per channel backward, another forward
+  if (threadIdx.x < kW) {
+    const int64_t ch2 = pl.d0 + threadIdx.x;
+    if (ch2 < pl.d1) {
+      const int64_t at = P.tiles - 1 - pl.tile;  // place of the tile in the order of the tickets
+      float cin = 0.0f;
+      if (P.chain) {
+        float ta = 1.0f, tc = 0.0f;
+#pragma unroll
+        for (int q = kWarps - 1; q >= 0; --q) {
+          const float b = sa[q][threadIdx.x], c = sc[q][threadIdx.x];
+          tc = send[q] ? c : fmaf(b, tc, c);
+          ta *= b;
+        }
+        publish_pair(P.agg + at * A.width + ch2, ta, tc);
+        const int64_t lo = slast >= 0 ? P.tiles - 1 - quotient(slast, P.tile_rows) : at;
+        if (lo < at) {
+          bool lost = false;
+          cin = look_back(P, at, lo, ch2, lost);
+          if (lost && A.status) atomicOr(reinterpret_cast<unsigned *>(A.status), GEARB_ST_SCAN_ABORTED);
+        }
+      }
+#pragma unroll
+      for (int q = kWarps - 1; q >= 0; --q) {
+        const float b = sa[q][threadIdx.x], c = sc[q][threadIdx.x];
+        sc[q][threadIdx.x] = cin;
+        cin = send[q] ? c : fmaf(b, cin, c);
+      }
+      if (P.chain && at % kSuper == kSuper - 1 && at + 1 < P.tiles)
+        publish_word(P.super + (at / kSuper + 1) * A.width + ch2, cin);
+    }
+  } else if (threadIdx.x < 2 * kW) {
+    const int c0 = threadIdx.x - kW;
+    const int64_t ch2 = pl.d0 + c0;
+    if (ch2 < pl.d1) {
+      float hin = (P.chain && sopen) ? __ldg(A.carry + pl.tile * A.width + ch2) : 0.0f;
+#pragma unroll
+      for (int q = 0; q < kWarps; ++q) {
+        const float b = sa[q][c0], h = sh[q][c0];
+        sh[q][c0] = hin;
+        hin = scut[q] ? h : fmaf(b, hin, h);
+      }
+    }
+  }
+  __syncthreads();
+
+  if (n > 0) {
+    float hp[kRows][V], h[V], c[V], part[kRows];  // hp: h_(t-1) of every row
+#pragma unroll
+    for (int v = 0; v < V; ++v) { h[v] = sh[warp][lane * V + v]; c[v] = sc[warp][lane * V + v]; }
+    const int64_t row0 = row_of(P, i0), sign = A.reverse ? -1 : 1;
+    TX *dx = static_cast<TX *>(A.dx) + row0 * A.width + d;
+    TA *dgate = static_cast<TA *>(A.dgate) + row0 * A.gates + (kShared ? pl.gate : d);
+    const int64_t xs = sign * A.width, gs = sign * A.gates;
+    if (plain) {
+#pragma unroll
+      for (int k = 0; k < kRows; ++k)
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          hp[k][v] = h[v];
+          h[v] = fmaf(a[k][kShared ? 0 : v], h[v], to_f(x[k].v[v]));
+        }
+#pragma unroll
+      for (int k = kRows - 1; k >= 0; --k) {
+        float g[V], da[V];
+        part[k] = 0.0f;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          const float av = a[k][kShared ? 0 : v];
+          g[v] = to_f(dh[k].v[v]) + c[v];
+          c[v] = av * g[v];
+          da[v] = (A.gate_log ? c[v] : g[v]) * hp[k][v];
+          part[k] += on ? da[v] : 0.0f;
+        }
+        if (on) {
+          store_pack<TX, V>(dx + k * xs, g);
+          if constexpr (!kShared) store_pack<TA, V>(dgate + k * gs, da);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < kRows; ++k) {
+        const bool st = m.start >> k & 1u, lv = m.live >> k & 1u;
+        if (st) state_load<V>(A.h0, __shfl_sync(kAll, m.seq, k), A.width, d, on, h);
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          const float xv = to_f(x[k].v[v]);
+          hp[k][v] = h[v];
+          if (lv) h[v] = (st && !A.h0) ? xv : fmaf(a[k][kShared ? 0 : v], h[v], xv);
+        }
+      }
+#pragma unroll
+      for (int k = kRows - 1; k >= 0; --k) {
+        part[k] = 0.0f;
+        if (k >= n) continue;
+        const bool lv = m.live >> k & 1u, st = m.start >> k & 1u;
+        const int seq = __shfl_sync(kAll, m.seq, k);
+        if (m.end >> k & 1u) state_load<V>(A.dstate, seq, A.width, d, on, c);
+        float g[V], da[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          const float av = a[k][kShared ? 0 : v];
+          g[v] = lv ? to_f(dh[k].v[v]) + c[v] : 0.0f;
+          if (lv) c[v] = av * g[v];
+          // the first row of a sequence without h0 is h = x: its gate plays no part
+          da[v] = (lv && !(st && !A.h0)) ? (A.gate_log ? c[v] : g[v]) * hp[k][v] : 0.0f;
+          part[k] += on ? da[v] : 0.0f;
+        }
+        if (on && (lv || A.zero_rest)) {
+          store_pack<TX, V>(dx + k * xs, g);
+          if constexpr (!kShared) store_pack<TA, V>(dgate + k * gs, da);
+        }
+        if (st) state_store<V>(A.dh0, seq, A.width, d, on, c);
+      }
+    }
+    if constexpr (kShared) {
+      const float sum = sum_rows(part, lane);
+      const int k = (lane >> 4 & 1) * 4 + (lane >> 3 & 1) * 2 + (lane >> 2 & 1);
+      if ((lane & 3) == 0 && k < n && ((m.live >> k & 1u) || A.zero_rest)) {
+        if (P.blocks_per_gate == 1) dgate[k * gs] = from_f<TA>(sum);
+        else P.gate_part[(pl.part * P.rows + row0 + k * sign) * A.gates + pl.gate] = sum;
+      }
+    }
+  }
+  empty_sequences(P, pl, kW, A.dstate, A.dh0);
+}
+
+template <typename TX, typename TA, int V>
+int launch_wide(Params &p, bool backward, cudaStream_t stream) {
+  const gearb_recurrence_args &a = p.A;
+  const bool shared = a.gates < a.width;
+  p.blocks_per_gate = shared ? (p.per + 32 * V - 1) / (32 * V) : 1;
+  const int64_t ncol = shared ? a.gates * p.blocks_per_gate : (a.width + 32 * V - 1) / (32 * V);
+  GEARB_REQUIRE(p.tiles <= (int64_t(1) << 31) / ncol - 1, "recurrence: too many tiles for one launch");
+  p.ncol = static_cast<int>(ncol);
+  const unsigned grid = static_cast<unsigned>(p.tiles * ncol);
+  if (backward) {
+    if (shared) backward_kernel<TX, TA, V, true><<<grid, kThreads, 0, stream>>>(p);
+    else backward_kernel<TX, TA, V, false><<<grid, kThreads, 0, stream>>>(p);
+  } else {
+    if (shared) forward_kernel<TX, TA, V, true><<<grid, kThreads, 0, stream>>>(p);
+    else forward_kernel<TX, TA, V, false><<<grid, kThreads, 0, stream>>>(p);
+  }
+  GEARB_CUDA(cudaGetLastError());
+  return GEARB_OK;
+}
+
+template <typename TX, typename TA>
+int launch_wide_any(Params &p, bool backward, cudaStream_t stream) {
+  switch (p.V) {
+    case 4: return launch_wide<TX, TA, 4>(p, backward, stream);
+    case 2: return launch_wide<TX, TA, 2>(p, backward, stream);
+    default: return launch_wide<TX, TA, 1>(p, backward, stream);
+  }
+}
+
+}  // namespace rec
+}  // namespace gearb
