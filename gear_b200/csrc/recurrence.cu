@@ -1,13 +1,44 @@
 // Host side of the recurrences: checks, sizes, choice of the kernel, and the entry points.
-#include "recurrence.cuh"
+#include <cuda.h>
 
-#ifndef GEARB_REC_MAXV
-#define GEARB_REC_MAXV 4
-#endif
+#include <atomic>
+
+#include "recurrence.cuh"
 
 namespace gearb {
 
 using namespace rec;
+
+namespace rec {
+
+// cuTensorMapEncodeTiled, looked up in the driver once (the library links the runtime only).
+int encode_map(CUtensorMap *map, CUtensorMapDataType type, void *base, int64_t width, int64_t rows, int64_t row_bytes, int box_w,
+               int box_h) {
+  using Encode = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
+                              const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  static std::atomic<Encode> known{nullptr};
+  Encode encode = known.load(std::memory_order_acquire);
+  if (!encode) {
+    void *fn = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    GEARB_CUDA(cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &found));
+    if (found != cudaDriverEntryPointSuccess || !fn)
+      return fail(GEARB_ERR_UNSUPPORTED, "the driver has no cuTensorMapEncodeTiled");
+    encode = reinterpret_cast<Encode>(fn);
+    known.store(encode, std::memory_order_release);
+  }
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(width), static_cast<cuuint64_t>(rows)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(row_bytes)};
+  const cuuint32_t box[2] = {static_cast<cuuint32_t>(box_w), static_cast<cuuint32_t>(box_h)}, step[2] = {1, 1};
+  const CUresult r = encode(map, type, 2, base, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                            CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(GEARB_ERR_CUDA, "cuTensorMapEncodeTiled failed with %d", static_cast<int>(r));
+  return GEARB_OK;
+}
+
+}  // namespace rec
 
 namespace {
 
@@ -135,11 +166,12 @@ int launch(const gearb_recurrence_args &a, bool backward, cudaStream_t stream) {
   p.x_period = period(a.x_batch_stride, a.x_row_stride);
   p.gate_period = period(a.gate_batch_stride, a.gate_row_stride);
   p.dout_period = period(a.dout_batch_stride, a.dout_row_stride);
+  p.flat = p.x_period == p.rows && p.gate_period == p.rows && (!backward || p.dout_period == p.rows);
   // Channels a lane: as many as alignment allows and the width (of a gate's channels) fills.
   const bool shared = a.gates < a.width;
   const int64_t unit = shared ? p.per : a.width;
   const int xs = a.x_dtype == GEARB_DT_F32 ? 4 : 2, gs = a.gate_dtype == GEARB_DT_F32 ? 4 : 2;
-  for (p.V = GEARB_REC_MAXV; p.V > 1; p.V /= 2) {
+  for (p.V = 4; p.V > 1; p.V /= 2) {
     const int v = p.V;
     if (unit % v != 0 || unit <= 32 * (v / 2)) continue;
     if (!vector_ok(a.x, a.x_batch_stride, a.x_row_stride, xs, v)) continue;

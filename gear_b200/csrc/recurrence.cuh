@@ -9,13 +9,13 @@
 // Any run of rows maps the state before it to the state behind it as S -> A*S + H (A the product of its a_t,
 // H its own result from zero), and such maps compose, so rows can be worked on in parallel: all rows of a call,
 // sequence after sequence, are cut into tiles of 64; a CTA takes one tile and one block of channels, keeps
-// gate and x in registers (8 rows a warp, one channel or a few a lane), forms (A, H), learns the state before
+// gate and x in registers (eight rows a warp, up to four channels a lane), forms (A, H), learns the state before
 // its tile, and runs its rows again from there.  Every input is read once and every output written once.
 //
-// The state before a tile.  Tiles publish their (A, H); 16 consecutive tiles form a superblock, and the last
+// The state before a tile.  Tiles publish their (A, H); 8 consecutive tiles form a superblock, and the last
 // tile of one publishes the state behind it.  A tile composes the tiles before it in its superblock, in
 // order, onto the state in front of the superblock: the same operations whatever the timing, so results are the
-// same bits every time, and the chain of waiting CTAs has one link per 1024 rows.  A tile needs nothing from
+// same bits every time, and the chain of waiting CTAs has one link per 512 rows.  A tile needs nothing from
 // before the start of the sequence its first row belongs to.  Tiles are handed out by a counter in scan order,
 // so a CTA only ever waits for CTAs that are already running; every wait has a limit, after which the
 // launch goes on with NaN and says so in the status word.  Published words are 32 bits that read
@@ -41,7 +41,7 @@ constexpr int kWarps = 8;
 constexpr int kThreads = kWarps * 32;
 constexpr int kRows = 8;                     // rows a warp keeps in registers
 constexpr int kTile = kWarps * kRows;        // rows per tile
-constexpr int kSuper = 16;                   // tiles per superblock
+constexpr int kSuper = 8;                    // tiles per superblock
 constexpr unsigned kAll = 0xffffffffu;
 constexpr unsigned kUnset = 0xffffffffu;     // a published word that has not been written
 constexpr int kPollLimit = 1 << 20;          // polls of one word, the better part of a second
@@ -64,7 +64,10 @@ template <typename T, int V>
 __device__ __forceinline__ Pack<T, V> load_pack(const T *p) {
   constexpr int kBytes = sizeof(T) * V;
   Pack<T, V> r;
-  if constexpr (kBytes == 16) {
+  if constexpr (kBytes == 32) {
+    reinterpret_cast<uint4 *>(&r)[0] = __ldcs(reinterpret_cast<const uint4 *>(p));
+    reinterpret_cast<uint4 *>(&r)[1] = __ldcs(reinterpret_cast<const uint4 *>(p) + 1);
+  } else if constexpr (kBytes == 16) {
     *reinterpret_cast<uint4 *>(&r) = __ldcs(reinterpret_cast<const uint4 *>(p));
   } else if constexpr (kBytes == 8) {
     *reinterpret_cast<uint2 *>(&r) = __ldcs(reinterpret_cast<const uint2 *>(p));
@@ -93,6 +96,7 @@ struct Params {
   int per;               // channels per gate
   int blocks_per_gate;   // column blocks of a gate's channels (shared gates)
   int ncol;              // column blocks
+  int flat;              // every tensor's rows lie one stride apart over the whole batch
   // Address periods: rows per batch entry, or all rows where one row stride covers the whole batch.
   int64_t x_period, gate_period, dout_period;
   unsigned *ticket;
@@ -312,26 +316,83 @@ __device__ __forceinline__ Place take_place(const Params &P, unsigned *smem_tick
   return p;
 }
 
-// V consecutive channels of n rows of the scan (zeros where there is no row or channel).
+// How the rows of a tile lie: what is the same for all of its warps.
+struct TileRows {
+  int64_t bb, tt;  // batch entry and row in it of the tile's first row
+  bool linear;     // the tile's rows lie one row stride apart in every tensor
+  bool interior;   // one sequence goes through the whole tile: no row of it is its first or last
+  int64_t first_start, last_end;  // with interior: scan indexes of that sequence's first and last row
+};
+
+// Dense and padded rows, from the tile's place alone.
+__device__ __forceinline__ TileRows tile_rows_dense(const Params &P, const Place &pl) {
+  const gearb_recurrence_args &A = P.A;
+  const int64_t b = quotient(pl.i0, A.time), u = pl.i0 - b * A.time, n = pl.i1 - pl.i0;
+  TileRows t;
+  t.bb = A.reverse ? A.batch - 1 - b : b;
+  t.tt = A.reverse ? A.time - 1 - u : u;
+  t.linear = P.flat || u + n <= A.time;
+  int64_t lo = 0, hi = A.time;  // rows of the sequence, in scan order within the batch entry
+  if (A.lengths) {
+    int64_t len = __ldg(A.lengths + t.bb);
+    len = len < 0 ? 0 : (len > A.time ? A.time : len);
+    if (A.reverse) lo = A.time - len;
+    else hi = len;
+  }
+  t.interior = u > lo && u + n < hi;
+  t.first_start = pl.i0 - u + lo;
+  t.last_end = pl.i0 - u + hi - 1;
+  return t;
+}
+
+// Packed rows: one warp looks the tile's place up in the offsets.
+__device__ __forceinline__ TileRows tile_rows_packed(const Params &P, const Place &pl, int lane) {
+  const gearb_recurrence_args &A = P.A;
+  TileRows t;
+  t.bb = 0;
+  t.tt = row_of(P, pl.i0);
+  t.linear = true;
+  t.interior = false;
+  t.first_start = t.last_end = 0;
+  const ScanOffsets so{A.offsets, P.rows, A.sequences, A.reverse};
+  if (pl.i0 < so.at(A.sequences)) {
+    const int64_t s = warp_upper_bound<int64_t>(A.offsets, 0, A.sequences, pl.i0, lane, so);
+    if (s > 0) {
+      t.first_start = so.at(s - 1);
+      const int64_t behind = so.at(s);
+      t.last_end = behind - 1;
+      t.interior = t.first_start < pl.i0 && behind > pl.i1 && behind <= P.rows;
+    }
+  }
+  return t;
+}
+
+// V consecutive channels of a warp's n rows of the scan (zeros where there is no row or channel).  
 template <typename T, int V>
-__device__ __forceinline__ void load_rows(const T *base, const Params &P, int64_t i0, int64_t period, int64_t sb, int64_t sr,
-                                          int n, int64_t d, bool on, Pack<T, V> (&r)[kRows]) {
+__device__ __forceinline__ void load_rows(const T *base, const Params &P, const Place &pl, const TileRows &tr, int64_t period,
+                                          int64_t sb, int64_t sr, int warp, int n, int64_t d, bool on, Pack<T, V> (&r)[kRows]) {
+  if (n == kRows && tr.linear) {
+    const int64_t step = P.A.reverse ? -sr : sr;
+    const T *p = base + (tr.bb * sb + tr.tt * sr + warp * kRows * step + d);
+#pragma unroll
+    for (int k = 0; k < kRows; ++k) {
+      if (on) r[k] = load_pack<T, V>(p + k * step);
+      else
+#pragma unroll
+        for (int v = 0; v < V; ++v) r[k].v[v] = from_f<T>(0.0f);
+    }
+    return;
+  }
 #pragma unroll
   for (int k = 0; k < kRows; ++k)
 #pragma unroll
     for (int v = 0; v < V; ++v) r[k].v[v] = from_f<T>(0.0f);
   if (n == 0 || !on) return;
-  RowWalk w(row_of(P, i0), period, sb, sr, P.A.reverse);
-  if (n == kRows && (P.A.reverse ? w.t >= kRows - 1 : w.t + kRows <= period)) {
-    const T *p = base + w.off + d;  // eight rows of one batch entry: one stride
+  RowWalk w(row_of(P, pl.i0 + warp * kRows), period, sb, sr, P.A.reverse);
 #pragma unroll
-    for (int k = 0; k < kRows; ++k) r[k] = load_pack<T, V>(p + k * w.step);
-  } else {
-#pragma unroll
-    for (int k = 0; k < kRows; ++k) {
-      if (k < n) r[k] = load_pack<T, V>(base + w.off + d);
-      w.next();
-    }
+  for (int k = 0; k < kRows; ++k) {
+    if (k < n) r[k] = load_pack<T, V>(base + w.off + d);
+    w.next();
   }
 }
 
@@ -341,19 +402,21 @@ __device__ __forceinline__ float look_back(const Params &P, int64_t at, int64_t 
   const int64_t sb = at / kSuper, sb0 = sb * kSuper;
   const bool need_super = lo < sb0;
   const int64_t j0 = need_super ? sb0 : lo;
+  const int count = static_cast<int>(at - j0);
+  const float2 *p = P.agg + j0 * P.A.width + d;
   float pa = 1.0f, ph = 0.0f;
-  for (int64_t j = j0; j < at; j += 5) {
+  for (int j = 0; j < count; j += 5) {
     float2 q[5];
 #pragma unroll
     for (int u = 0; u < 5; ++u)
-      if (j + u < at) q[u] = peek_pair(P.agg + (j + u) * P.A.width + d);
+      if (j + u < count) q[u] = peek_pair(p + (j + u) * P.A.width);
 #pragma unroll
     for (int u = 0; u < 5; ++u)
-      if (j + u < at) {
+      if (j + u < count) {
         if (__float_as_uint(q[u].x) == kUnset || __float_as_uint(q[u].y) == kUnset)
-          q[u] = poll_pair(P.agg + (j + u) * P.A.width + d, lost);
+          q[u] = poll_pair(p + (j + u) * P.A.width, lost);
         // nothing in front of the sequence's start counts
-        ph = (j + u == j0 && !need_super) ? q[u].y : fmaf(q[u].x, ph, q[u].y);
+        ph = (j + u == 0 && !need_super) ? q[u].y : fmaf(q[u].x, ph, q[u].y);
         pa *= q[u].x;
       }
   }
@@ -362,14 +425,29 @@ __device__ __forceinline__ float look_back(const Params &P, int64_t at, int64_t 
   return fmaf(pa, s, ph);
 }
 
+// e^x in float32 from 2^t (one instruction, 2 units in the last place): with t = x / ln 2 rounded, e^x = 2^t * e^r for
+// the r = x - t ln 2 that the rounding left, and e^r = 1 + r to 2^-30 for x above -150, below which e^x is 0.
+constexpr float kLog2E = 1.4426950408889634f;
+constexpr float kLn2Hi = 0.693147180559945309f;                       // rounded to float32
+constexpr float kLn2Lo = static_cast<float>(0.693147180559945309 - static_cast<double>(kLn2Hi));
+__device__ __forceinline__ float exp_of(float x) {
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(x) : "f"(x), "f"(-150.0f));
+  const float t = x * kLog2E;
+  const float r = fmaf(-t, kLn2Lo, fmaf(-t, kLn2Hi, x));
+  float e;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
+  return fmaf(e, r, e);
+}
+
 // Hands a sequence without rows its state (forward) or its gradient (backward): the CTAs of a launch share the
 // sequences among them.
 __device__ __forceinline__ void empty_sequences(const Params &P, const Place &pl, int64_t block, const float *from,
-                                                float *to) {
+                                                float *to, int lane = -1) {
   const gearb_recurrence_args &A = P.A;
   if (!to) return;
-  const int64_t step = P.tiles * kThreads;
-  for (int64_t s = pl.tile * kThreads + threadIdx.x; s < A.sequences; s += step) {
+  // by all threads of the CTA, or by one warp's lanes
+  const int64_t each = lane < 0 ? kThreads : 32, step = P.tiles * each;
+  for (int64_t s = pl.tile * each + (lane < 0 ? threadIdx.x : lane); s < A.sequences; s += step) {
     int64_t n;
     if (A.offsets) {
       const ScanOffsets so{A.offsets, P.rows, A.sequences, 0};

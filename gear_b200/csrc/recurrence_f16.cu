@@ -1,12 +1,12 @@
 // Recurrences over x of type __half.
-#include "recurrence_wide.cuh"
+#include "recurrence_stream.cuh"
 
 namespace gearb {
 namespace rec {
 
 int launch_f16(Params &p, bool backward, cudaStream_t stream) {
-  return p.A.gate_dtype == GEARB_DT_F32 ? launch_wide_any<__half, float>(p, backward, stream)
-                                        : launch_wide_any<__half, __half>(p, backward, stream);
+  return p.A.gate_dtype == GEARB_DT_F32 ? launch_any<__half, float>(p, backward, stream)
+                                        : launch_any<__half, __half>(p, backward, stream);
 }
 
 }  // namespace rec

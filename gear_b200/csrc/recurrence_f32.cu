@@ -1,11 +1,11 @@
 // Recurrences over x of type float.
-#include "recurrence_wide.cuh"
+#include "recurrence_stream.cuh"
 
 namespace gearb {
 namespace rec {
 
 int launch_f32(Params &p, bool backward, cudaStream_t stream) {
-  return launch_wide_any<float, float>(p, backward, stream);
+  return launch_any<float, float>(p, backward, stream);
 }
 
 }  // namespace rec

@@ -1,7 +1,7 @@
 // Kernels of the recurrences for rows of many channels: one warp a row, V channels a lane.
 //
 // Three phases with a barrier between them.  Every warp forms (A, H) of its eight rows; then one thread per channel goes
-// through the eight warps' pairs, publishes the tile's, learns the state before the tile and leaves the state before
+// through the warps' pairs, publishes the tile's, learns the state before the tile and leaves the state before
 // each warp; then every warp runs its rows from there.
 #pragma once
 
@@ -11,12 +11,12 @@ namespace gearb {
 namespace rec {
 
 template <typename TA, int V, bool kShared>
-__device__ __forceinline__ void load_gate(const Params &P, const Place &pl, int64_t i0, int n, int64_t d, bool on,
-                                          float (&a)[kRows][kShared ? 1 : V]) {
+__device__ __forceinline__ void load_gate(const Params &P, const Place &pl, const TileRows &tr, int warp, int n, int64_t d,
+                                          bool on, float (&a)[kRows][kShared ? 1 : V]) {
   constexpr int kG = kShared ? 1 : V;
   Pack<TA, kG> raw[kRows];
-  load_rows<TA, kG>(static_cast<const TA *>(P.A.gate), P, i0, P.gate_period, P.A.gate_batch_stride, P.A.gate_row_stride, n,
-                    kShared ? pl.gate : d, on, raw);
+  load_rows<TA, kG>(static_cast<const TA *>(P.A.gate), P, pl, tr, P.gate_period, P.A.gate_batch_stride, P.A.gate_row_stride,
+                    warp, n, kShared ? pl.gate : d, on, raw);
 #pragma unroll
   for (int k = 0; k < kRows; ++k)
 #pragma unroll
@@ -28,7 +28,44 @@ __device__ __forceinline__ void exp_gate(float (&a)[kRows][kG]) {
 #pragma unroll
   for (int k = 0; k < kRows; ++k)
 #pragma unroll
-    for (int v = 0; v < kG; ++v) a[k][v] = expf(a[k][v]);
+    for (int v = 0; v < kG; ++v) a[k][v] = exp_of(a[k][v]);
+}
+
+constexpr unsigned kAllRows = (1u << kRows) - 1u;
+
+// The tile's rows, and this warp's: looked up for the whole tile first, by each warp only where a sequence starts or
+// ends in it.
+struct SharedRows {
+  TileRows t;
+};
+__device__ __forceinline__ TileRows rows_of_tile(const Params &P, const Place &pl) {
+  if (!P.A.offsets) return tile_rows_dense(P, pl);
+  TileRows t;
+  t.bb = 0;
+  t.tt = row_of(P, pl.i0);
+  t.linear = true;
+  t.interior = false;
+  t.first_start = t.last_end = 0;
+  return t;
+}
+__device__ __forceinline__ RowMap rows_of_warp(const Params &P, const Place &pl, TileRows &t, SharedRows &sm, int64_t i0, int n,
+                                               int warp, int lane) {
+  if (P.A.offsets) {
+    if (warp == 0) {
+      const TileRows found = tile_rows_packed(P, pl, lane);
+      if (lane == 0) sm.t = found;
+    }
+    __syncthreads();
+    t = sm.t;
+  }
+  if (!t.interior) return map_rows(P.A, P.rows, i0, n, lane);
+  RowMap m;
+  m.live = kAllRows;
+  m.start = m.end = 0;
+  m.seq = 0;
+  m.first_start = t.first_start;
+  m.last_end = t.last_end;
+  return m;
 }
 
 // A float of every channel of [sequences][width], of V channels of one sequence.
@@ -51,6 +88,7 @@ __global__ void __launch_bounds__(kThreads, V == 4 ? 2 : 3) forward_kernel(const
   __shared__ float sa[kWarps][kW], sh[kWarps][kW];
   __shared__ int scut[kWarps];
   __shared__ unsigned sticket;
+  __shared__ SharedRows srows;
   __shared__ int64_t sfirst;  // scan index at which the first row's sequence starts, or -1: nothing is needed from before
   const gearb_recurrence_args &A = P.A;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -62,16 +100,17 @@ __global__ void __launch_bounds__(kThreads, V == 4 ? 2 : 3) forward_kernel(const
 
   Pack<TX, V> x[kRows];
   float a[kRows][kG];
-  load_rows<TX, V>(static_cast<const TX *>(A.x), P, i0, P.x_period, A.x_batch_stride, A.x_row_stride, n, d, on, x);
-  load_gate<TA, V, kShared>(P, pl, i0, n, d, on, a);
-  const RowMap m = map_rows(A, P.rows, i0, n, lane);
+  TileRows tr = rows_of_tile(P, pl);
+  load_rows<TX, V>(static_cast<const TX *>(A.x), P, pl, tr, P.x_period, A.x_batch_stride, A.x_row_stride, warp, n, d, on, x);
+  load_gate<TA, V, kShared>(P, pl, tr, warp, n, d, on, a);
+  const RowMap m = rows_of_warp(P, pl, tr, srows, i0, n, warp, lane);
   if (A.gate_log) exp_gate(a);
-  const bool plain = m.live == (1u << kRows) - 1u && (m.start | m.end) == 0;
+  const bool plain = m.live == kAllRows && (m.start | m.end) == 0;
 
   // (A, H) of this warp's rows; behind a start only H counts
-  float ca[V], ch[V], first[V];  // first: h of the last start row, see below
+  float ca[V], ch[V];
 #pragma unroll
-  for (int v = 0; v < V; ++v) { ca[v] = 1.0f; ch[v] = first[v] = 0.0f; }
+  for (int v = 0; v < V; ++v) { ca[v] = 1.0f; ch[v] = 0.0f; }
   if (plain) {
 #pragma unroll
     for (int k = 0; k < kRows; ++k)
@@ -91,7 +130,7 @@ __global__ void __launch_bounds__(kThreads, V == 4 ? 2 : 3) forward_kernel(const
 #pragma unroll
       for (int v = 0; v < V; ++v) {
         const float av = a[k][kShared ? 0 : v], xv = to_f(x[k].v[v]);
-        if (st) ch[v] = first[v] = A.h0 ? fmaf(av, s[v], xv) : xv;
+        if (st) ch[v] = A.h0 ? fmaf(av, s[v], xv) : xv;
         else ch[v] = fmaf(av, ch[v], xv);
         ca[v] *= av;
       }
@@ -161,12 +200,7 @@ __global__ void __launch_bounds__(kThreads, V == 4 ? 2 : 3) forward_kernel(const
           continue;
         }
         const int seq = __shfl_sync(kAll, m.seq, k);
-        if (m.start >> k == 1u) {
-          // The sequence may end in another warp or tile, which may by now have put its state where h0 was
-          // (state_out may be h0): h of this row is kept from the first look at it.
-#pragma unroll
-          for (int v = 0; v < V; ++v) h[v] = first[v];
-        } else if (m.start >> k & 1u) {
+        if (m.start >> k & 1u) {
           float s[V];
           state_load<V>(A.h0, seq, A.width, d, on, s);
 #pragma unroll
@@ -186,12 +220,13 @@ __global__ void __launch_bounds__(kThreads, V == 4 ? 2 : 3) forward_kernel(const
   empty_sequences(P, pl, kW, A.h0, A.state_out);
 }
 
-// Sums of eight values over the 32 lanes: lane l with l % 4 == 0 ends up with the sum of value
-// (l >> 4 & 1) * 4 + (l >> 3 & 1) * 2 + (l >> 2 & 1).  Nine shuffles instead of forty.
+// Sums of kRows values over the 32 lanes, by halving: with every shuffle a lane gives away half of the values it still
+// holds.  Lane l ends up with the sum of value row_of_lane(l); 7 + 2 shuffles for eight values instead of forty.
+constexpr int kSpare = 32 / kRows;  // lanes that hold the same value in the end
+__device__ __forceinline__ int row_of_lane(int lane) { return lane / kSpare; }
 __device__ __forceinline__ float sum_rows(float (&v)[kRows], int lane) {
-  static_assert(kRows == 8, "three halvings");
 #pragma unroll
-  for (int half = 4, m = 16; half > 0; half >>= 1, m >>= 1) {
+  for (int half = kRows / 2, m = 16; half > 0; half >>= 1, m >>= 1) {
     const bool up = lane & m;
 #pragma unroll
     for (int j = 0; j < half; ++j) {
@@ -199,8 +234,8 @@ __device__ __forceinline__ float sum_rows(float (&v)[kRows], int lane) {
       v[j] = keep + __shfl_xor_sync(kAll, give, m);
     }
   }
-  v[0] += __shfl_xor_sync(kAll, v[0], 2);
-  v[0] += __shfl_xor_sync(kAll, v[0], 1);
+#pragma unroll
+  for (int m = kSpare / 2; m > 0; m >>= 1) v[0] += __shfl_xor_sync(kAll, v[0], m);
   return v[0];
 }
 
@@ -211,6 +246,7 @@ __global__ void __launch_bounds__(kThreads, V == 4 ? 2 : 3) backward_kernel(cons
   __shared__ float sa[kWarps][kW], sh[kWarps][kW], sc[kWarps][kW];
   __shared__ int scut[kWarps], send[kWarps];
   __shared__ unsigned sticket;
+  __shared__ SharedRows srows;
   __shared__ int64_t slast;   // scan index at which the last row's sequence ends, or -1: nothing is needed from behind
   __shared__ int sopen;       // the first row continues a sequence of an earlier tile
   const gearb_recurrence_args &A = P.A;
@@ -223,13 +259,14 @@ __global__ void __launch_bounds__(kThreads, V == 4 ? 2 : 3) backward_kernel(cons
 
   Pack<TX, V> x[kRows], dh[kRows];
   float a[kRows][kG];
-  load_rows<TX, V>(static_cast<const TX *>(A.x), P, i0, P.x_period, A.x_batch_stride, A.x_row_stride, n, d, on, x);
-  load_gate<TA, V, kShared>(P, pl, i0, n, d, on, a);
-  load_rows<TX, V>(static_cast<const TX *>(A.dout), P, i0, P.dout_period, A.dout_batch_stride, A.dout_row_stride, n, d, on,
-                   dh);
-  const RowMap m = map_rows(A, P.rows, i0, n, lane);
+  TileRows tr = rows_of_tile(P, pl);
+  load_rows<TX, V>(static_cast<const TX *>(A.x), P, pl, tr, P.x_period, A.x_batch_stride, A.x_row_stride, warp, n, d, on, x);
+  load_gate<TA, V, kShared>(P, pl, tr, warp, n, d, on, a);
+  load_rows<TX, V>(static_cast<const TX *>(A.dout), P, pl, tr, P.dout_period, A.dout_batch_stride, A.dout_row_stride, warp, n,
+                   d, on, dh);
+  const RowMap m = rows_of_warp(P, pl, tr, srows, i0, n, warp, lane);
   if (A.gate_log) exp_gate(a);
-  const bool plain = m.live == (1u << kRows) - 1u && (m.start | m.end) == 0;
+  const bool plain = m.live == kAllRows && (m.start | m.end) == 0;
 
   // (A, H) of this warp's rows forward, (A, C) backward
   float ca[V], ch[V], cc[V];
@@ -402,8 +439,8 @@ __global__ void __launch_bounds__(kThreads, V == 4 ? 2 : 3) backward_kernel(cons
     }
     if constexpr (kShared) {
       const float sum = sum_rows(part, lane);
-      const int k = (lane >> 4 & 1) * 4 + (lane >> 3 & 1) * 2 + (lane >> 2 & 1);
-      if ((lane & 3) == 0 && k < n && ((m.live >> k & 1u) || A.zero_rest)) {
+      const int k = row_of_lane(lane);
+      if (lane % kSpare == 0 && k < n && ((m.live >> k & 1u) || A.zero_rest)) {
         if (P.blocks_per_gate == 1) dgate[k * gs] = from_f<TA>(sum);
         else P.gate_part[(pl.part * P.rows + row0 + k * sign) * A.gates + pl.gate] = sum;
       }

@@ -109,6 +109,8 @@ class _Problem:
 
 
 def _forward(p, x, gate, h0, offsets, lengths, need_carry, return_state, out, state_out, status):
+    if state_out is not None and h0 is not None and p.time != 1 and state_out.data_ptr() == h0.data_ptr():
+        h0 = h0.clone()    # rows of one sequence are worked on in several places: one may be done before another reads h0
     a = p.args(x, gate, h0, offsets, lengths)
     a.zero_rest = int(out is None)
     h = torch.empty(x.shape, dtype=x.dtype, device=x.device) if out is None else out
@@ -174,7 +176,7 @@ def linear_recurrence(x: torch.Tensor, gate: torch.Tensor, *, h0: Optional[torch
     reverse     from each sequence's last row to its first
     state       float32 [sequences, width] (None with return_state=False); an empty sequence keeps its h0
     out, state_out   write there instead of allocating (no gradients then); with `out` the rows of no
-                sequence are left as they were.  state_out may be h0 itself
+                sequence are left as they were.  state_out may be h0 itself; apart from that nothing may overlap
     status      int32[4] as of the other launches: ST_SCAN_ABORTED if a wait inside the launch ran out (h is
                 NaN from there on)
 

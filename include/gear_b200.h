@@ -551,6 +551,7 @@ int gearb_layout_paged(const gearb_layout_args *args, void *stream);
  * Rows of no sequence are not used; out, dx and dgate get zeros there with zero_rest, else are left as
  * they are.  reverse: from the last row of a sequence to its first.  h0, state_out, dstate, dh0:
  * float32 [sequences][width], each may be NULL (h0: zeros); state_out of an empty sequence is its h0.
+ * Nothing that is written may overlap what is read, except that with time 1 state_out may be h0.
  * Types: x, out, dout, dx of x_dtype; gate, dgate of gate_dtype, either x_dtype or GEARB_DT_F32.
  * All arithmetic is float32; the result does not depend on timing.
  * carry: what the backward pass needs besides x and gate, written by the forward pass when not NULL.
