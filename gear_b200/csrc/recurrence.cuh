@@ -37,9 +37,12 @@
 namespace gearb {
 namespace rec {
 
-constexpr int kWarps = 8;
+#ifndef GEARB_REC_WARPS
+#define GEARB_REC_WARPS 8
+#endif
+constexpr int kWarps = GEARB_REC_WARPS;
 constexpr int kThreads = kWarps * 32;
-constexpr int kRows = 8;                     // rows a warp keeps in registers
+constexpr int kRows = 64 / kWarps;           // rows a warp keeps in registers
 constexpr int kTile = kWarps * kRows;        // rows per tile
 constexpr int kSuper = 8;                    // tiles per superblock
 constexpr unsigned kAll = 0xffffffffu;

@@ -1,22 +1,20 @@
 // Kernels of the recurrences for long calls whose rows lie in one TMA-addressable matrix.
 //
-// The tiles are those of recurrence_wide.cuh (64 rows, eight warps of eight rows), but the CTAs stay, one per SM, and
-// work on two tiles at a time: the rows of tile m come out of shared memory into registers, its (A, H) is formed and
-// published, and only then tile m - 1 is finished, whose neighbours have by then published theirs.  So no CTA holds up
-// those behind it while it waits.  (Finishing each tile before the next is begun: every tile spent 6700 of its 11000
-// cycles looking back, and 2 x 16384 x 2048 bf16 took 170 us whatever the types.)
-//
-// A ninth warp plans: it takes the next tile's number from the counter, works out once for everybody where the tile
-// lies and which rows start or end a sequence, and starts its copies, one tensor copy per input (64 rows of 32 * V
-// channels).  (One bulk copy per row instead: an SM starts one about every 35 cycles, which is too few.  Every warp
-// working out its own rows' place: 600 of 1000 instructions per warp and tile.)
-//
-//   per tile:   wait for its copies; registers <- shared memory; (A, H) of each warp's rows
-//               barrier
-//               lower threads: one per channel joins the warps' pairs and publishes the tile's     } of tile m
-//               upper threads: one per channel takes what the tiles before have published          } of tile m - 1
-//               barrier
-//               each warp runs its rows of tile m - 1 from the state before them and stores them
+// The tiles are those of recurrence_wide.cuh, but the CTAs stay, one per SM, and their warps have roles, so that
+// nothing waits in line:
+//   planner     takes the next tile's number from the counter, works out once for everybody where the tile lies and
+//               which rows start or end a sequence, and starts its copies (one tensor copy per input)
+//   compute     first look at tile m: (A, H) of each warp's rows; then, tile m - 1 again: its rows from the state
+//               before them, and out
+//   publishers  one thread per channel: turn the warps' pairs into those of all rows before each warp, publish the
+//               tile's
+//   finishers   one thread per channel: the state in front of the tile from what the tiles before published
+// They meet at mbarriers only.  Measured on the way, 2 x 16384 x 2048 bf16 with float32 gates (82 us at the copy rate):
+// a CTA per tile 170 us whatever the types; CTAs that stay but finish a tile before they begin the next: every tile
+// spent 6700 of 11000 cycles looking back; one bulk copy per row: an SM starts one about every 35 cycles, 180 us;
+// every warp finding its rows' place itself: 600 of 1000 instructions; both phases' rows in registers: spills, 234 us;
+// several tiles' numbers taken at once: tiles wait for others far back in another CTA's queue, 250 to 600 us; two CTA
+// barriers a tile in place of the roles: 136 us.
 #pragma once
 
 #include <cuda.h>
@@ -26,9 +24,11 @@
 namespace gearb {
 namespace rec {
 
-constexpr int kStreamThreads = kThreads + 32;
+constexpr int kStreamThreads = kThreads + 9 * 32;  // compute, 4 publishers, 4 finishers, planner
 constexpr int kSmemMost = 227 * 1024;
-constexpr unsigned kPlans = 8;  // plans outlive the stages of their tiles by one tile
+#ifndef GEARB_REC_STAGES
+#define GEARB_REC_STAGES 6
+#endif
 
 constexpr unsigned kWaitLimit = 1u << 20;  // mbarrier polls before a copy is declared lost
 
@@ -110,13 +110,15 @@ __device__ __forceinline__ void unpack(const Pack<T, V> &p, float (&f)[V]) {
   for (int v = 0; v < V; ++v) f[v] = to_f(p.v[v]);
 }
 
+__device__ __forceinline__ bool warp_wait(uint64_t *bar, unsigned parity) {
+  return __all_sync(kAll, mbar_wait(bar, parity));
+}
 __device__ __forceinline__ void mbar_init_count(uint64_t *bar, unsigned n) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_addr(bar)), "r"(n));
 }
 __device__ __forceinline__ void mbar_arrive(uint64_t *bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
 }
-__device__ __forceinline__ void compute_barrier() { asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory"); }
 
 // Shared memory of one stage.  A tensor copy writes to 128-byte boundaries.
 template <typename TX, typename TA, int V, bool kShared, bool kBackward>
@@ -139,30 +141,40 @@ struct Plan {
   int plain;       // one sequence goes through the whole tile: no row of it is its first or last
   int lo;          // look back as far as this tile, counted in the order of the tickets; -1: nothing is needed from before
   int open;        // backward: the first row continues a sequence of an earlier tile
-  alignas(8) unsigned char live[kWarps], start[kWarps], end[kWarps];  // bits: rows of each warp
+  unsigned starts, ends;  // bit w: a sequence starts (ends) in warp w's rows
+  unsigned cut;    // bit w: a sequence starts in rows of the tile before warp w's (bit kWarps: anywhere in it)
+  unsigned bcut;   // bit w: a sequence ends in rows of the tile behind warp w's (bit kWarps: anywhere in it)
+  alignas(16) unsigned char live[kWarps], start[kWarps], end[kWarps];  // bits: rows of each warp
   int seq[kTile];                                                     // sequence of each row (unless plain)
   float a[kTile];                                                     // shared gates: a of each row
 };
 
 template <int V, bool kBackward>
-struct Pairs {  // of the warps of one tile
+struct Pairs {  // of the warps of one tile; then of all rows before (backward: behind) each warp's
   alignas(16) float a[kWarps][32 * V];
   alignas(16) float h[kWarps][32 * V];
+  alignas(16) float b[kBackward ? kWarps : 1][kBackward ? 32 * V : 4];
   alignas(16) float c[kBackward ? kWarps : 1][kBackward ? 32 * V : 4];
 };
-static_assert(sizeof(Pairs<4, false>) % 16 == 0 && sizeof(Pairs<2, true>) % 16 == 0, "vector accesses");
+template <int V>
+struct Edge {  // of one tile: its own pair, and the state in front of it
+  float a[32 * V], h[32 * V], in[32 * V];
+};
 
 template <typename TX, typename TA, int V, bool kShared, bool kBackward>
 struct StreamShared {
   using StageT = Stage<TX, TA, V, kShared, kBackward>;
-  static constexpr int kFixed = 2 * sizeof(Pairs<V, kBackward>) + kPlans * sizeof(Plan) + 512;
-  static constexpr int kFit = (kSmemMost - kFixed) / static_cast<int>(sizeof(StageT));
-  static constexpr int kStages = kFit > 4 ? 4 : kFit;
-  static_assert(kStages >= 2 && kStages + 2 <= static_cast<int>(kPlans), "");
+  static constexpr int kEach = static_cast<int>(sizeof(StageT) + sizeof(Edge<V>) + sizeof(Plan)) + 64;
+  static constexpr int kFit = (kSmemMost - 2 * static_cast<int>(sizeof(Pairs<V, kBackward>)) - 256) / kEach;
+  static constexpr unsigned kStages = kFit > GEARB_REC_STAGES ? GEARB_REC_STAGES : kFit;
+  static_assert(kStages >= 3, "two tiles in work and one on its way");
   StageT stage[kStages];
   Pairs<V, kBackward> pairs[2];
-  Plan plan[kPlans];
-  uint64_t full[kStages], empty[kStages];
+  Edge<V> edge[kStages];
+  Plan plan[kStages];
+  uint64_t full[kStages], empty[kStages];  // the tile's rows and plan are there; the tile is done with
+  uint64_t entered[kStages];               // edge.in is there
+  uint64_t paired[2], ready[2], read[2];   // the warps' pairs; turned and edge.a, edge.h there; read again
 };
 
 // The tile before (in the order of the tickets): what its predecessors published, asked for early.
@@ -213,8 +225,10 @@ __device__ __forceinline__ void plan_tiles(const Params &P, const Maps &maps, St
   constexpr unsigned kStages = Shared::kStages;
   const gearb_recurrence_args &A = P.A;
   const unsigned items = static_cast<unsigned>(P.tiles * P.ncol);
-  unsigned next = 0;  // lane 0: the next number
-  if (lane == 0) next = P.chain ? atomicAdd(P.ticket, kStages) + 1u : blockIdx.x;  // the counter starts at 0xffffffff
+  // lane 0: the next number.  One at a time from the start: CTAs that took several at once would come to tiles much
+  // later than others come to the tiles behind them, and those would wait.
+  unsigned next = 0;
+  if (lane == 0) next = P.chain ? atomicAdd(P.ticket, 1u) + 1u : blockIdx.x;  // the counter starts at 0xffffffff
   unsigned stage = 0, parity = 0;
   for (unsigned m = 0;; ++m) {
     if (m >= kStages) {
@@ -225,7 +239,7 @@ __device__ __forceinline__ void plan_tiles(const Params &P, const Maps &maps, St
       }
     }
     const unsigned item = __shfl_sync(kAll, next, 0);
-    Plan &pl = sm.plan[m % kPlans];
+    Plan &pl = sm.plan[stage];
     if (item >= items) {
       if (lane == 0) {
         pl.valid = 0;
@@ -235,9 +249,7 @@ __device__ __forceinline__ void plan_tiles(const Params &P, const Maps &maps, St
       return;
     }
     if (lane == 0) {  // asked for now, needed a tile later
-      if (!P.chain) next = item + gridDim.x;
-      else if (m + 1 < kStages) next = item + 1;
-      else next = atomicAdd(P.ticket, 1u) + 1u;
+      next = P.chain ? atomicAdd(P.ticket, 1u) + 1u : item + gridDim.x;
     }
     Place at;
     const unsigned t = item / static_cast<unsigned>(P.ncol);
@@ -277,10 +289,11 @@ __device__ __forceinline__ void plan_tiles(const Params &P, const Maps &maps, St
         const int n0 = n - half * 32, nn = n0 < 0 ? 0 : (n0 > 32 ? 32 : n0);
         const RowMap rm = map_rows(A, P.rows, at.i0 + half * 32, nn, lane);
         pl.seq[half * 32 + lane] = rm.seq;
-        if (lane < 4) {
-          pl.live[half * 4 + lane] = static_cast<unsigned char>(rm.live >> (8 * lane));
-          pl.start[half * 4 + lane] = static_cast<unsigned char>(rm.start >> (8 * lane));
-          pl.end[half * 4 + lane] = static_cast<unsigned char>(rm.end >> (8 * lane));
+        if (lane < 32 / kRows) {
+          const int w = half * (32 / kRows) + lane;
+          pl.live[w] = static_cast<unsigned char>(rm.live >> (kRows * lane) & kAllRows);
+          pl.start[w] = static_cast<unsigned char>(rm.start >> (kRows * lane) & kAllRows);
+          pl.end[w] = static_cast<unsigned char>(rm.end >> (kRows * lane) & kAllRows);
         }
         if (half == 0) {
           first_start = rm.first_start;
@@ -291,11 +304,11 @@ __device__ __forceinline__ void plan_tiles(const Params &P, const Maps &maps, St
           last_open = (rm.live & ~rm.end) >> (nn - 1) & 1u;
         }
       }
-    } else if (lane < 2) {
-      reinterpret_cast<unsigned *>(pl.live)[lane] = 0xffffffffu;
-      reinterpret_cast<unsigned *>(pl.start)[lane] = 0u;
-      reinterpret_cast<unsigned *>(pl.end)[lane] = 0u;
+    } else if (lane < kWarps) {
+      pl.live[lane] = static_cast<unsigned char>(kAllRows);
+      pl.start[lane] = pl.end[lane] = 0;
     }
+    __syncwarp();
     if (lane == 0) {
       pl.valid = 1;
       pl.tile = static_cast<int>(at.tile);
@@ -306,6 +319,24 @@ __device__ __forceinline__ void plan_tiles(const Params &P, const Maps &maps, St
       pl.gate = static_cast<int>(at.gate);
       pl.part = at.part;
       pl.plain = tr.interior;
+      unsigned cut = 0, bcut = 0, starts = 0, ends = 0;
+      if (!tr.interior) {
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          if (pl.start[w]) {
+            starts |= 1u << w;
+            cut |= ~0u << (w + 1);
+          }
+          if (pl.end[w]) {
+            ends |= 1u << w;
+            bcut |= ((1u << w) - 1u) | 1u << kWarps;
+          }
+        }
+      }
+      pl.starts = starts;
+      pl.ends = ends;
+      pl.cut = cut;
+      pl.bcut = bcut;
       const int64_t from = quotient(first_start, P.tile_rows);
       pl.open = P.chain && first_open && from < at.tile;
       pl.lo = -1;
@@ -365,49 +396,90 @@ struct WarpRows {
   }
 };
 
-__device__ __forceinline__ unsigned long long flags_of(const unsigned char (&f)[kWarps]) {
-  return *reinterpret_cast<const unsigned long long *>(f);
+// Finishers: the state in front of every tile (backward: behind it), and that in front of the next superblock.
+template <typename TX, typename TA, int V, bool kShared, bool kBackward>
+__device__ __forceinline__ bool finish_tiles(const Params &P, StreamShared<TX, TA, V, kShared, kBackward> &sm, int c, int lane) {
+  using Shared = StreamShared<TX, TA, V, kShared, kBackward>;
+  const gearb_recurrence_args &A = P.A;
+  bool lost = false;
+  unsigned stage = 0, parity = 0;
+  for (unsigned m = 0;; ++m) {
+    if (!warp_wait(&sm.full[stage], parity)) return true;
+    const Plan &pl = sm.plan[stage];
+    if (!pl.valid) return lost;
+    const int tile = kBackward ? static_cast<int>(P.tiles) - 1 - pl.tile : pl.tile, lo = pl.lo, d = pl.d0 + c;
+    const bool on = c < pl.cols;
+    float in = 0.0f;
+    if (on && lo >= 0) {
+      Peek peek;
+      peek_back(P, tile, lo, d, peek);
+      in = settle_back(P, tile, lo, d, peek, lost);
+      if (!kBackward && A.carry) A.carry[pl.tile * A.width + d] = in;
+    }
+    if (P.chain && tile % kSuper == kSuper - 1 && tile + 1 < P.tiles) {
+      const bool cut = (kBackward ? pl.bcut : pl.cut) >> kWarps & 1u;
+      if (!warp_wait(&sm.ready[m & 1], m >> 1 & 1u)) return true;
+      if (on) {
+        const float h = sm.edge[stage].h[c];
+        publish_word(P.super + ((tile / kSuper + 1) * A.width + d), cut ? h : fmaf(sm.edge[stage].a[c], in, h));
+      }
+    }
+    if (c < 32 * V) sm.edge[stage].in[c] = in;
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&sm.entered[stage]);
+    if (++stage == Shared::kStages) {
+      stage = 0;
+      parity ^= 1u;
+    }
+  }
 }
-__device__ __forceinline__ bool any_in(unsigned long long flags, int warp) { return flags >> (8 * warp) & 0xffu; }
 
 template <typename TX, typename TA, int V, bool kShared>
-__global__ void __launch_bounds__(kStreamThreads, 1) forward_stream_kernel(const __grid_constant__ Params P,
-                                                                           const __grid_constant__ Maps maps) {
-  constexpr int kG = kShared ? 1 : V, kW = 32 * V, R = kRows;
+__device__ __forceinline__ bool publish_tiles(const Params &P, StreamShared<TX, TA, V, kShared, false> &sm, int c, int lane) {
   using Shared = StreamShared<TX, TA, V, kShared, false>;
-  constexpr unsigned kStages = Shared::kStages;
-  static_assert(2 * kW <= kThreads, "publishing and finishing threads");
-  extern __shared__ __align__(1024) unsigned char raw_smem[];
-  auto &sm = *reinterpret_cast<Shared *>(raw_smem);
-  const gearb_recurrence_args &A = P.A;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  if (threadIdx.x == 0) {
-    for (unsigned s = 0; s < kStages; ++s) {
-      mbar_init_count(&sm.full[s], 2);  // the expected bytes, and the plan
-      mbar_init_count(&sm.empty[s], kWarps);
-    }
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-  }
-  __syncthreads();
-  if (warp == kWarps) {
-    plan_tiles<TX, TA, V, kShared, false>(P, maps, sm, lane);
-    return;
-  }
-
-  bool lost = false, have_old = false;
   unsigned stage = 0, parity = 0;
-  const int oc = static_cast<int>(threadIdx.x) - kThreads / 2;  // finishing threads: their channel
-  // One round: tile m's first phase, tile m - 1's last.
   for (unsigned m = 0;; ++m) {
-    const Plan &opl = sm.plan[(m + kPlans - 1) % kPlans];
-    const Plan &pl = sm.plan[m % kPlans];
-    auto &np = sm.pairs[m & 1], &op = sm.pairs[m & 1 ^ 1];
-    Peek peek;
-    const bool finishes = have_old && oc >= 0 && oc < opl.cols;
-    const int olo = have_old ? opl.lo : -1;
-    if (finishes && olo >= 0) peek_back(P, opl.tile, olo, opl.d0 + oc, peek);
-    if (!__all_sync(kAll, mbar_wait(&sm.full[stage], parity))) lost = true;
-    const bool valid = !lost && pl.valid;
+    if (!warp_wait(&sm.full[stage], parity)) return true;
+    const Plan &pl = sm.plan[stage];
+    if (!pl.valid) return false;
+    if (!warp_wait(&sm.paired[m & 1], m >> 1 & 1u)) return true;
+    if (c < pl.cols) {
+      auto &pr = sm.pairs[m & 1];
+      const unsigned starts = pl.starts;
+      float b[kWarps], h[kWarps], ta = 1.0f, th = 0.0f;
+#pragma unroll
+      for (int q = 0; q < kWarps; ++q) { b[q] = pr.a[q][c]; h[q] = pr.h[q][c]; }
+#pragma unroll
+      for (int q = 0; q < kWarps; ++q) {
+        pr.a[q][c] = ta;
+        pr.h[q][c] = th;
+        th = (starts >> q & 1u) ? h[q] : fmaf(b[q], th, h[q]);
+        ta *= b[q];
+      }
+      if (P.chain) publish_pair(P.agg + (pl.tile * P.A.width + pl.d0 + c), ta, th);
+      sm.edge[stage].a[c] = ta;
+      sm.edge[stage].h[c] = th;
+    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&sm.ready[m & 1]);
+    if (++stage == Shared::kStages) {
+      stage = 0;
+      parity ^= 1u;
+    }
+  }
+}
+
+template <typename TX, typename TA, int V, bool kShared>
+__device__ __forceinline__ bool compute_forward(const Params &P, StreamShared<TX, TA, V, kShared, false> &sm, int warp,
+                                                int lane) {
+  using Shared = StreamShared<TX, TA, V, kShared, false>;
+  constexpr int kG = kShared ? 1 : V, R = kRows;
+  const gearb_recurrence_args &A = P.A;
+  unsigned stage = 0, parity = 0, ostage = 0, oparity = 0;
+  for (unsigned m = 0;; ++m) {
+    if (!warp_wait(&sm.full[stage], parity)) return true;
+    const Plan &pl = sm.plan[stage];
+    const bool valid = pl.valid;
     if (valid) {
       const WarpRows<TX, TA, V, kShared, false> rows(P, pl, sm.stage[stage], warp, lane);
       float a[kG], ca[V], ch[V], x[V];
@@ -444,58 +516,30 @@ __global__ void __launch_bounds__(kStreamThreads, 1) forward_stream_kernel(const
           mul_v(ca, a, ca);
         }
       }
-      store_pack<float, V>(&np.a[warp][lane * V], ca);
-      store_pack<float, V>(&np.h[warp][lane * V], ch);
+      if (m >= 2 && !warp_wait(&sm.read[m & 1], (m >> 1) - 1u & 1u)) return true;
+      store_pack<float, V>(&sm.pairs[m & 1].a[warp][lane * V], ca);
+      store_pack<float, V>(&sm.pairs[m & 1].h[warp][lane * V], ch);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.paired[m & 1]);
     }
-    if (!valid && !have_old) break;
-    compute_barrier();
-
-    const int c = threadIdx.x;
-    if (valid && P.chain && c < pl.cols) {  // the new tile's pair
-      const unsigned long long cut = flags_of(pl.start);
-      float ta = 1.0f, th = 0.0f;
-#pragma unroll
-      for (int q = 0; q < kWarps; ++q) {
-        const float b = np.a[q][c], h = np.h[q][c];
-        th = any_in(cut, q) ? h : fmaf(b, th, h);
-        ta *= b;
-      }
-      publish_pair(P.agg + (pl.tile * A.width + pl.d0 + c), ta, th);
-    }
-    if (finishes) {  // the old tile's states
-      const int d = opl.d0 + oc, tile = opl.tile;
-      float cin = 0.0f;
-      if (olo >= 0) {
-        bool gone = false;
-        cin = settle_back(P, tile, olo, d, peek, gone);
-        if (gone && A.status) atomicOr(reinterpret_cast<unsigned *>(A.status), GEARB_ST_SCAN_ABORTED);
-        if (A.carry) A.carry[tile * A.width + d] = cin;
-      }
-      const unsigned long long cut = flags_of(opl.start);
-      float b[kWarps], h[kWarps];
-#pragma unroll
-      for (int q = 0; q < kWarps; ++q) { b[q] = op.a[q][oc]; h[q] = op.h[q][oc]; }
-#pragma unroll
-      for (int q = 0; q < kWarps; ++q) {
-        op.h[q][oc] = cin;  // the state before warp q
-        cin = any_in(cut, q) ? h[q] : fmaf(b[q], cin, h[q]);
-      }
-      if (P.chain && tile % kSuper == kSuper - 1 && tile + 1 < P.tiles)
-        publish_word(P.super + ((tile / kSuper + 1) * A.width + d), cin);
-    }
-    compute_barrier();
-
-    if (have_old) {
-      const unsigned ostage = stage == 0 ? kStages - 1 : stage - 1;
+    if (m > 0) {
+      const unsigned o = m - 1;
+      const Plan &opl = sm.plan[ostage];
       const int n = opl.rows - warp * R, d = opl.d0 + lane * V;
       const bool on = lane * V < opl.cols;
+      if (!warp_wait(&sm.ready[o & 1], o >> 1 & 1u) || !warp_wait(&sm.entered[ostage], oparity)) return true;
+      float a[kG], h[V], x[V], in[V];
+      unpack(*reinterpret_cast<const Pack<float, V> *>(&sm.pairs[o & 1].h[warp][lane * V]), h);
+      if (!(opl.cut >> warp & 1u)) {
+        float pa[V];
+        unpack(*reinterpret_cast<const Pack<float, V> *>(&sm.pairs[o & 1].a[warp][lane * V]), pa);
+        unpack(*reinterpret_cast<const Pack<float, V> *>(&sm.edge[ostage].in[lane * V]), in);
+        fma_v(h, pa, in, h);
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.read[o & 1]);
       if (n > 0) {
         const WarpRows<TX, TA, V, kShared, false> rows(P, opl, sm.stage[ostage], warp, lane);
-        float a[kG], h[V], x[V];
-        unpack(*reinterpret_cast<const Pack<float, V> *>(&op.h[warp][lane * V]), h);
-        if (lost)
-#pragma unroll
-          for (int v = 0; v < V; ++v) h[v] = __int_as_float(0x7fffffff);
         const int64_t step = A.reverse ? -A.width : A.width;
         TX *out = static_cast<TX *>(A.out) + ((A.reverse ? opl.row0 - warp * R : opl.row0 + warp * R) * A.width + d);
         if (opl.plain) {
@@ -539,15 +583,51 @@ __global__ void __launch_bounds__(kStreamThreads, 1) forward_stream_kernel(const
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // a was written where the next copy will write
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm.empty[ostage]);
+      if (++ostage == Shared::kStages) {
+        ostage = 0;
+        oparity ^= 1u;
+      }
     }
-    if (!valid) break;
-    have_old = true;
-    if (++stage == kStages) {
+    if (!valid) return false;
+    if (++stage == Shared::kStages) {
       stage = 0;
       parity ^= 1u;
     }
   }
-  if (lost && lane == 0 && A.status) atomicOr(reinterpret_cast<unsigned *>(A.status), GEARB_ST_SCAN_ABORTED);
+}
+
+template <typename TX, typename TA, int V, bool kShared, bool kBackward>
+__device__ __forceinline__ void init_barriers(StreamShared<TX, TA, V, kShared, kBackward> &sm) {
+  if (threadIdx.x == 0) {
+    for (unsigned s = 0; s < StreamShared<TX, TA, V, kShared, kBackward>::kStages; ++s) {
+      mbar_init_count(&sm.full[s], 2);  // the expected bytes, and the plan
+      mbar_init_count(&sm.empty[s], kWarps);
+      mbar_init_count(&sm.entered[s], 4);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init_count(&sm.paired[s], kWarps);
+      mbar_init_count(&sm.ready[s], 4);
+      mbar_init_count(&sm.read[s], kWarps);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  __syncthreads();
+}
+
+template <typename TX, typename TA, int V, bool kShared>
+__global__ void __launch_bounds__(kStreamThreads, 1) forward_stream_kernel(const __grid_constant__ Params P,
+                                                                           const __grid_constant__ Maps maps) {
+  using Shared = StreamShared<TX, TA, V, kShared, false>;
+  extern __shared__ __align__(1024) unsigned char raw_smem[];
+  auto &sm = *reinterpret_cast<Shared *>(raw_smem);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  init_barriers(sm);
+  bool lost = false;
+  if (warp < kWarps) lost = compute_forward<TX, TA, V, kShared>(P, sm, warp, lane);
+  else if (warp < kWarps + 4) lost = publish_tiles<TX, TA, V, kShared>(P, sm, threadIdx.x - kThreads, lane);
+  else if (warp < kWarps + 8) lost = finish_tiles<TX, TA, V, kShared, false>(P, sm, threadIdx.x - kThreads - 128, lane);
+  else plan_tiles<TX, TA, V, kShared, false>(P, maps, sm, lane);
+  if (lost && lane == 0 && P.A.status) atomicOr(reinterpret_cast<unsigned *>(P.A.status), GEARB_ST_SCAN_ABORTED);
 }
 
 // A matrix of [rows][width] for boxes of kTile rows and 32 * V channels.
@@ -598,7 +678,9 @@ int launch_any(Params &p, bool backward, cudaStream_t stream) {
   if (!stream_fits<TX, TA>(p, backward)) return launch_wide_any<TX, TA>(p, backward, stream);
   const bool shared = p.A.gates < p.A.width;
   if (shared) return p.V == 4 ? launch_stream<TX, TA, 4, true>(p, stream) : launch_stream<TX, TA, 2, true>(p, stream);
-  return p.V == 4 ? launch_stream<TX, TA, 4, false>(p, stream) : launch_stream<TX, TA, 2, false>(p, stream);
+  if constexpr (sizeof(TX) + sizeof(TA) <= 6)
+    if (p.V == 4) return launch_stream<TX, TA, 4, false>(p, stream);
+  return launch_stream<TX, TA, 2, false>(p, stream);
 }
 
 }  // namespace rec

@@ -82,7 +82,7 @@ __device__ __forceinline__ void state_store(float *p, int seq, int64_t width, in
 }
 
 template <typename TX, typename TA, int V, bool kShared>
-__global__ void __launch_bounds__(kThreads, V == 4 ? 2 : 3) forward_kernel(const __grid_constant__ Params P) {
+__global__ void __launch_bounds__(kThreads, V == 4 ? 2 : 2) forward_kernel(const __grid_constant__ Params P) {
   constexpr int kG = kShared ? 1 : V;
   constexpr int kW = 32 * V;  // channels of a block
   __shared__ float sa[kWarps][kW], sh[kWarps][kW];
@@ -146,15 +146,20 @@ __global__ void __launch_bounds__(kThreads, V == 4 ? 2 : 3) forward_kernel(const
 
   const int64_t ch2 = pl.d0 + threadIdx.x;
   if (threadIdx.x < kW && ch2 < pl.d1) {
+    float ta = 1.0f, th = 0.0f;  // of the rows before warp q
+    bool cut = false;
+    float pa[kWarps], ph[kWarps];
+#pragma unroll
+    for (int q = 0; q < kWarps; ++q) {
+      const float b = sa[q][threadIdx.x], h = sh[q][threadIdx.x];
+      pa[q] = ta;
+      ph[q] = th;
+      th = scut[q] ? h : fmaf(b, th, h);
+      ta *= b;
+      cut |= scut[q] != 0;
+    }
     float cin = 0.0f;
     if (P.chain) {
-      float ta = 1.0f, th = 0.0f;
-#pragma unroll
-      for (int q = 0; q < kWarps; ++q) {
-        const float b = sa[q][threadIdx.x], h = sh[q][threadIdx.x];
-        th = scut[q] ? h : fmaf(b, th, h);
-        ta *= b;
-      }
       publish_pair(P.agg + pl.tile * A.width + ch2, ta, th);
       const int64_t lo = sfirst >= 0 ? quotient(sfirst, P.tile_rows) : pl.tile;
       if (lo < pl.tile) {
@@ -163,15 +168,15 @@ __global__ void __launch_bounds__(kThreads, V == 4 ? 2 : 3) forward_kernel(const
         if (lost && A.status) atomicOr(reinterpret_cast<unsigned *>(A.status), GEARB_ST_SCAN_ABORTED);
         if (A.carry) A.carry[pl.tile * A.width + ch2] = cin;
       }
+      if (pl.tile % kSuper == kSuper - 1 && pl.tile + 1 < P.tiles)
+        publish_word(P.super + (pl.tile / kSuper + 1) * A.width + ch2, cut ? th : fmaf(ta, cin, th));
     }
+    cut = false;
 #pragma unroll
-    for (int q = 0; q < kWarps; ++q) {
-      const float b = sa[q][threadIdx.x], h = sh[q][threadIdx.x];
-      sh[q][threadIdx.x] = cin;  // the state before warp q
-      cin = scut[q] ? h : fmaf(b, cin, h);
+    for (int q = 0; q < kWarps; ++q) {  // the state before warp q
+      sh[q][threadIdx.x] = cut ? ph[q] : fmaf(pa[q], cin, ph[q]);
+      cut |= scut[q] != 0;
     }
-    if (P.chain && pl.tile % kSuper == kSuper - 1 && pl.tile + 1 < P.tiles)
-      publish_word(P.super + (pl.tile / kSuper + 1) * A.width + ch2, cin);
   }
   __syncthreads();
 
@@ -240,7 +245,7 @@ __device__ __forceinline__ float sum_rows(float (&v)[kRows], int lane) {
 }
 
 template <typename TX, typename TA, int V, bool kShared>
-__global__ void __launch_bounds__(kThreads, V == 4 ? 2 : 3) backward_kernel(const __grid_constant__ Params P) {
+__global__ void __launch_bounds__(kThreads, V == 4 ? 1 : 2) backward_kernel(const __grid_constant__ Params P) {
   constexpr int kG = kShared ? 1 : V;
   constexpr int kW = 32 * V;
   __shared__ float sa[kWarps][kW], sh[kWarps][kW], sc[kWarps][kW];
@@ -327,15 +332,20 @@ __global__ void __launch_bounds__(kThreads, V == 4 ? 2 : 3) backward_kernel(cons
     const int64_t ch2 = pl.d0 + threadIdx.x;
     if (ch2 < pl.d1) {
       const int64_t at = P.tiles - 1 - pl.tile;  // place of the tile in the order of the tickets
+      float ta = 1.0f, tc = 0.0f;  // of the rows behind warp q
+      bool cut = false;
+      float pa[kWarps], pc[kWarps];
+#pragma unroll
+      for (int q = kWarps - 1; q >= 0; --q) {
+        const float b = sa[q][threadIdx.x], c = sc[q][threadIdx.x];
+        pa[q] = ta;
+        pc[q] = tc;
+        tc = send[q] ? c : fmaf(b, tc, c);
+        ta *= b;
+        cut |= send[q] != 0;
+      }
       float cin = 0.0f;
       if (P.chain) {
-        float ta = 1.0f, tc = 0.0f;
-#pragma unroll
-        for (int q = kWarps - 1; q >= 0; --q) {
-          const float b = sa[q][threadIdx.x], c = sc[q][threadIdx.x];
-          tc = send[q] ? c : fmaf(b, tc, c);
-          ta *= b;
-        }
         publish_pair(P.agg + at * A.width + ch2, ta, tc);
         const int64_t lo = slast >= 0 ? P.tiles - 1 - quotient(slast, P.tile_rows) : at;
         if (lo < at) {
@@ -343,26 +353,30 @@ __global__ void __launch_bounds__(kThreads, V == 4 ? 2 : 3) backward_kernel(cons
           cin = look_back(P, at, lo, ch2, lost);
           if (lost && A.status) atomicOr(reinterpret_cast<unsigned *>(A.status), GEARB_ST_SCAN_ABORTED);
         }
+        if (at % kSuper == kSuper - 1 && at + 1 < P.tiles)
+          publish_word(P.super + (at / kSuper + 1) * A.width + ch2, cut ? tc : fmaf(ta, cin, tc));
       }
+      cut = false;
 #pragma unroll
       for (int q = kWarps - 1; q >= 0; --q) {
-        const float b = sa[q][threadIdx.x], c = sc[q][threadIdx.x];
-        sc[q][threadIdx.x] = cin;
-        cin = send[q] ? c : fmaf(b, cin, c);
+        sc[q][threadIdx.x] = cut ? pc[q] : fmaf(pa[q], cin, pc[q]);
+        cut |= send[q] != 0;
       }
-      if (P.chain && at % kSuper == kSuper - 1 && at + 1 < P.tiles)
-        publish_word(P.super + (at / kSuper + 1) * A.width + ch2, cin);
     }
   } else if (threadIdx.x < 2 * kW) {
     const int c0 = threadIdx.x - kW;
     const int64_t ch2 = pl.d0 + c0;
     if (ch2 < pl.d1) {
-      float hin = (P.chain && sopen) ? __ldg(A.carry + pl.tile * A.width + ch2) : 0.0f;
+      const float hin = (P.chain && sopen) ? __ldg(A.carry + pl.tile * A.width + ch2) : 0.0f;
+      float ta = 1.0f, th = 0.0f;
+      bool cut = false;
 #pragma unroll
       for (int q = 0; q < kWarps; ++q) {
         const float b = sa[q][c0], h = sh[q][c0];
-        sh[q][c0] = hin;
-        hin = scut[q] ? h : fmaf(b, hin, h);
+        sh[q][c0] = cut ? th : fmaf(ta, hin, th);
+        th = scut[q] ? h : fmaf(b, th, h);
+        ta *= b;
+        cut |= scut[q] != 0;
       }
     }
   }
