@@ -105,10 +105,6 @@ Scratch scratch_of(const gearb_recurrence_args &a, bool backward) {
   return s;
 }
 
-bool vector_ok(const void *p, int64_t sb, int64_t sr, int size, int v) {
-  return reinterpret_cast<uintptr_t>(p) % (size * v) == 0 && sb % v == 0 && sr % v == 0;
-}
-
 int check_sizes(const gearb_recurrence_args *a) {
   GEARB_REQUIRE(a, "recurrence: null argument");
   GEARB_REQUIRE(a->batch >= 0 && a->time >= 0 && a->width > 0 && a->gates > 0 && a->sequences >= 0,

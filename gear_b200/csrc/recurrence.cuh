@@ -37,12 +37,9 @@
 namespace gearb {
 namespace rec {
 
-#ifndef GEARB_REC_WARPS
-#define GEARB_REC_WARPS 8
-#endif
-constexpr int kWarps = GEARB_REC_WARPS;
+constexpr int kWarps = 8;
 constexpr int kThreads = kWarps * 32;
-constexpr int kRows = 64 / kWarps;           // rows a warp keeps in registers
+constexpr int kRows = 8;                     // rows a warp keeps in registers
 constexpr int kTile = kWarps * kRows;        // rows per tile
 constexpr int kSuper = 8;                    // tiles per superblock
 constexpr unsigned kAll = 0xffffffffu;
@@ -464,6 +461,11 @@ __device__ __forceinline__ void empty_sequences(const Params &P, const Place &pl
     const int64_t d1 = pl.d0 + block < pl.d1 ? pl.d0 + block : pl.d1;
     for (int64_t d = pl.d0; d < d1; ++d) to[s * A.width + d] = from ? from[s * A.width + d] : 0.0f;
   }
+}
+
+// Whether rows can be read or written v values at a time.
+inline bool vector_ok(const void *p, int64_t sb, int64_t sr, int size, int v) {
+  return reinterpret_cast<uintptr_t>(p) % (size * v) == 0 && sb % v == 0 && sr % v == 0;
 }
 
 int launch_f32(Params &p, bool backward, cudaStream_t stream);

@@ -26,9 +26,12 @@ namespace rec {
 
 constexpr int kStreamThreads = kThreads + 9 * 32;  // compute, 4 publishers, 4 finishers, planner
 constexpr int kSmemMost = 227 * 1024;
-#ifndef GEARB_REC_STAGES
-#define GEARB_REC_STAGES 6
-#endif
+constexpr unsigned kLag = 2;  // tiles that compute warps begin before they come back to one (1: 124 us in place of 110)
+constexpr unsigned kRing = kLag + 1;
+constexpr int kMostStages = 6;
+// How a block of channels gets its gates: a gate each; one for the whole block; by a table of the few that it spans.
+enum { kOwn = 0, kOne = 1, kTable = 2 };
+constexpr int kTableGates = 8;
 
 constexpr unsigned kWaitLimit = 1u << 20;  // mbarrier polls before a copy is declared lost
 
@@ -121,13 +124,13 @@ __device__ __forceinline__ void mbar_arrive(uint64_t *bar) {
 }
 
 // Shared memory of one stage.  A tensor copy writes to 128-byte boundaries.
-template <typename TX, typename TA, int V, bool kShared, bool kBackward>
+template <typename TX, typename TA, int V, int kGate, bool kBackward>
 struct Stage {
   alignas(128) TX x[kTile][32 * V];
   alignas(128) TX dout[kBackward ? kTile : 1][kBackward ? 32 * V : 8];
-  alignas(128) TA gate[kShared ? 1 : kTile][kShared ? 8 : 32 * V];
+  alignas(128) TA gate[kGate != kOwn ? 1 : kTile][kGate != kOwn ? 8 : 32 * V];
   static constexpr unsigned kBytes = sizeof(TX) * 32 * V * kTile * (kBackward ? 2 : 1) +
-                                     (kShared ? 0 : sizeof(TA) * 32 * V * kTile);
+                                     (kGate != kOwn ? 0 : sizeof(TA) * 32 * V * kTile);
 };
 
 // What the planning warp works out about a tile.  Rows are counted in 32 bits here (the entry point sends longer calls
@@ -146,7 +149,10 @@ struct Plan {
   unsigned bcut;   // bit w: a sequence ends in rows of the tile behind warp w's (bit kWarps: anywhere in it)
   alignas(16) unsigned char live[kWarps], start[kWarps], end[kWarps];  // bits: rows of each warp
   int seq[kTile];                                                     // sequence of each row (unless plain)
-  float a[kTile];                                                     // shared gates: a of each row
+};
+template <int kGate>
+struct GateRows {  // a of each row, for gates that are not copied with the rows
+  float a[kGate == kOwn ? 1 : kTile][kGate == kTable ? kTableGates : 1];
 };
 
 template <int V, bool kBackward>
@@ -156,25 +162,40 @@ struct Pairs {  // of the warps of one tile; then of all rows before (backward: 
   alignas(16) float b[kBackward ? kWarps : 1][kBackward ? 32 * V : 4];
   alignas(16) float c[kBackward ? kWarps : 1][kBackward ? 32 * V : 4];
 };
-template <int V>
-struct Edge {  // of one tile: its own pair, and the state in front of it
-  float a[32 * V], h[32 * V], in[32 * V];
+// A place in a ring of barriers, and the parity of its use.
+template <unsigned kSize>
+struct Turn {
+  unsigned i = 0, parity = 0;
+  __device__ __forceinline__ void next() {
+    if (++i == kSize) {
+      i = 0;
+      parity ^= 1u;
+    }
+  }
+};
+template <int V, bool kBackward>
+struct Edge {  // of one tile: its own pair, and the state that enters it (backward: from behind, and from in front)
+  alignas(16) float a[32 * V];
+  alignas(16) float h[32 * V];
+  alignas(16) float in[32 * V];
+  alignas(16) float front[kBackward ? 32 * V : 4];
 };
 
-template <typename TX, typename TA, int V, bool kShared, bool kBackward>
+template <typename TX, typename TA, int V, int kGate, bool kBackward>
 struct StreamShared {
-  using StageT = Stage<TX, TA, V, kShared, kBackward>;
-  static constexpr int kEach = static_cast<int>(sizeof(StageT) + sizeof(Edge<V>) + sizeof(Plan)) + 64;
-  static constexpr int kFit = (kSmemMost - 2 * static_cast<int>(sizeof(Pairs<V, kBackward>)) - 256) / kEach;
-  static constexpr unsigned kStages = kFit > GEARB_REC_STAGES ? GEARB_REC_STAGES : kFit;
-  static_assert(kStages >= 3, "two tiles in work and one on its way");
+  using StageT = Stage<TX, TA, V, kGate, kBackward>;
+  static constexpr int kEach = static_cast<int>(sizeof(StageT) + sizeof(Edge<V, kBackward>) + sizeof(Plan) + sizeof(GateRows<kGate>)) + 64;
+  static constexpr int kFit = (kSmemMost - static_cast<int>(kRing * sizeof(Pairs<V, kBackward>)) - 256) / kEach;
+  static constexpr unsigned kStages = kFit > kMostStages ? kMostStages : kFit;
+  static_assert(kStages >= kLag + 2, "the tiles in work and one on its way");
   StageT stage[kStages];
-  Pairs<V, kBackward> pairs[2];
-  Edge<V> edge[kStages];
+  Pairs<V, kBackward> pairs[kRing];
+  Edge<V, kBackward> edge[kStages];
   Plan plan[kStages];
+  GateRows<kGate> gates[kStages];
   uint64_t full[kStages], empty[kStages];  // the tile's rows and plan are there; the tile is done with
   uint64_t entered[kStages];               // edge.in is there
-  uint64_t paired[2], ready[2], read[2];   // the warps' pairs; turned and edge.a, edge.h there; read again
+  uint64_t paired[kRing], ready[kRing], read[kRing];   // the warps' pairs; turned and edge.a, edge.h there; read again
 };
 
 // The tile before (in the order of the tickets): what its predecessors published, asked for early.
@@ -218,10 +239,10 @@ __device__ __forceinline__ float settle_back(const Params &P, int at, int lo, in
 }
 
 // The planning warp.
-template <typename TX, typename TA, int V, bool kShared, bool kBackward>
-__device__ __forceinline__ void plan_tiles(const Params &P, const Maps &maps, StreamShared<TX, TA, V, kShared, kBackward> &sm,
+template <typename TX, typename TA, int V, int kGate, bool kBackward>
+__device__ __forceinline__ void plan_tiles(const Params &P, const Maps &maps, StreamShared<TX, TA, V, kGate, kBackward> &sm,
                                            int lane) {
-  using Shared = StreamShared<TX, TA, V, kShared, kBackward>;
+  using Shared = StreamShared<TX, TA, V, kGate, kBackward>;
   constexpr unsigned kStages = Shared::kStages;
   const gearb_recurrence_args &A = P.A;
   const unsigned items = static_cast<unsigned>(P.tiles * P.ncol);
@@ -257,10 +278,10 @@ __device__ __forceinline__ void plan_tiles(const Params &P, const Maps &maps, St
     at.tile = kBackward ? P.tiles - 1 - t : t;
     at.i0 = at.tile * P.tile_rows;
     at.i1 = at.i0 + P.tile_rows < P.rows ? at.i0 + P.tile_rows : P.rows;
-    at.gate = kShared ? c / P.blocks_per_gate : 0;
-    at.part = kShared ? c - static_cast<int>(at.gate) * P.blocks_per_gate : 0;
-    at.d0 = kShared ? at.gate * P.per + at.part * 32 * V : c * 32 * V;
-    at.d1 = kShared ? (at.gate + 1) * P.per : A.width;
+    at.gate = kGate == kOne ? c / P.blocks_per_gate : 0;
+    at.part = kGate == kOne ? c - static_cast<int>(at.gate) * P.blocks_per_gate : 0;
+    at.d0 = kGate == kOne ? at.gate * P.per + at.part * 32 * V : c * 32 * V;
+    at.d1 = kGate == kOne ? (at.gate + 1) * P.per : A.width;
     const int n = static_cast<int>(at.i1 - at.i0);
     const int row0 = static_cast<int>(row_of(P, at.i0));
     if (lane == 0) {
@@ -268,17 +289,31 @@ __device__ __forceinline__ void plan_tiles(const Params &P, const Maps &maps, St
       const int bc = static_cast<int>(at.d0), br = A.reverse ? row0 - (kTile - 1) : row0;
       mbar_expect(&sm.full[stage], Shared::StageT::kBytes);  // arrives below
       tensor_load(sm.stage[stage].x, &maps.x, bc, br, &sm.full[stage]);
-      if constexpr (!kShared) tensor_load(sm.stage[stage].gate, &maps.gate, bc, br, &sm.full[stage]);
+      if constexpr (kGate == kOwn) tensor_load(sm.stage[stage].gate, &maps.gate, bc, br, &sm.full[stage]);
       if constexpr (kBackward) tensor_load(sm.stage[stage].dout, &maps.dout, bc, br, &sm.full[stage]);
     }
-    if constexpr (kShared) {
+    if constexpr (kGate == kOne) {
 #pragma unroll
       for (int k = lane; k < kTile; k += 32) {
         float own = 0.0f;
         if (k < n)
           own = to_f(static_cast<const TA *>(A.gate)[(A.reverse ? row0 - k : row0 + k) * A.gate_row_stride + at.gate]);
-        pl.a[k] = A.gate_log ? exp_of(own) : own;
+        sm.gates[stage].a[k][0] = A.gate_log ? exp_of(own) : own;
       }
+    } else if constexpr (kGate == kTable) {
+      // eight gates a row: lane l looks at rows l / 8, l / 8 + 4, ...
+      const int g0 = static_cast<int>(at.d0) / P.per, g = g0 + (lane & 7);
+      float own[kTile / 4];
+#pragma unroll
+      for (int u = 0; u < kTile / 4; ++u) {
+        const int k = (lane >> 3) + 4 * u;
+        own[u] = 0.0f;
+        if (k < n && g < A.gates && static_cast<int64_t>(g) * P.per < at.d0 + 32 * V)
+          own[u] = to_f(static_cast<const TA *>(A.gate)[(A.reverse ? row0 - k : row0 + k) * A.gate_row_stride + g]);
+      }
+#pragma unroll
+      for (int u = 0; u < kTile / 4; ++u)
+        sm.gates[stage].a[(lane >> 3) + 4 * u][lane & 7] = A.gate_log ? exp_of(own[u]) : own[u];
     }
     const TileRows tr = A.offsets ? tile_rows_packed(P, at, lane) : tile_rows_dense(P, at);
     int64_t first_start = tr.first_start, last_end = tr.last_end;
@@ -358,21 +393,27 @@ __device__ __forceinline__ void plan_tiles(const Params &P, const Maps &maps, St
 }
 
 // A warp's rows of a tile in its stage: row k of the warp (in scan order) at k * step.
-template <typename TX, typename TA, int V, bool kShared, bool kBackward>
+template <typename TX, typename TA, int V, int kGate, bool kBackward>
 struct WarpRows {
-  static constexpr int kW = 32 * V, kG = kShared ? 1 : V;
+  static constexpr int kW = 32 * V, kG = kGate == kOne ? 1 : V;
   TX *x, *dout;
   TA *gate;
-  const float *shared_a;
-  int step;
-  __device__ __forceinline__ WarpRows(const Params &P, const Plan &pl, Stage<TX, TA, V, kShared, kBackward> &st, int warp,
-                                      int lane) {
+  const float *table;
+  int step, column[kGate == kTable ? V : 1];
+  __device__ __forceinline__ WarpRows(const Params &P, const Plan &pl, StreamShared<TX, TA, V, kGate, kBackward> &sm,
+                                      unsigned stage, int warp, int lane) {
+    auto &st = sm.stage[stage];
     const int k0 = P.A.reverse ? kTile - 1 - warp * kRows : warp * kRows, at = k0 * kW + lane * V;
     step = P.A.reverse ? -kW : kW;
     x = st.x[0] + at;
     dout = st.dout[0] + (kBackward ? at : 0);
-    gate = st.gate[0] + (kShared ? 0 : at);
-    shared_a = pl.a + warp * kRows;
+    gate = st.gate[0] + (kGate != kOwn ? 0 : at);
+    table = sm.gates[stage].a[kGate == kOwn ? 0 : warp * kRows];
+    if constexpr (kGate == kTable) {
+      const int d = pl.d0 + lane * V, g0 = pl.d0 / P.per;
+#pragma unroll
+      for (int v = 0; v < V; ++v) column[v] = min((d + v) / P.per - g0, kTableGates - 1);  // channels beyond the width too
+    }
   }
   __device__ __forceinline__ void get_x(int k, float (&f)[V]) const {
     unpack(*reinterpret_cast<const Pack<TX, V> *>(x + k * step), f);
@@ -382,8 +423,11 @@ struct WarpRows {
   }
   // a of row k.  The first look turns a float32 log gate into a where it lies; a 16-bit one is turned at every look.
   __device__ __forceinline__ void get_a(int k, int log, bool first, float (&a)[kG]) const {
-    if constexpr (kShared) {
-      a[0] = shared_a[k];
+    if constexpr (kGate == kOne) {
+      a[0] = table[k];
+    } else if constexpr (kGate == kTable) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) a[v] = table[k * kTableGates + column[v]];
     } else {
       unpack(*reinterpret_cast<const Pack<TA, V> *>(gate + k * step), a);
       if (log && (first || sizeof(TA) == 2)) {
@@ -396,14 +440,33 @@ struct WarpRows {
   }
 };
 
+// h = a * h + x for one row.  At a sequence's first row h comes from h0, or the row is h = x.  What a row of no
+// sequence leaves is never used: the next row of one is its first.
+template <int V, int kG>
+__device__ __forceinline__ void step_row(const gearb_recurrence_args &A, const Plan &pl, unsigned start, int k, int row, int d,
+                                         bool on, float (&a)[kG], const float (&x)[V], float (&h)[V]) {
+  if (start >> k & 1u) {
+    if (A.h0) {
+      state_load<V>(A.h0, pl.seq[row], A.width, d, on, h);
+    } else {
+#pragma unroll
+      for (int v = 0; v < V; ++v) h[v] = 0.0f;
+#pragma unroll
+      for (int v = 0; v < kG; ++v) a[v] = 0.0f;
+    }
+  }
+  fma_v(h, a, h, x);
+}
+
 // Finishers: the state in front of every tile (backward: behind it), and that in front of the next superblock.
-template <typename TX, typename TA, int V, bool kShared, bool kBackward>
-__device__ __forceinline__ bool finish_tiles(const Params &P, StreamShared<TX, TA, V, kShared, kBackward> &sm, int c, int lane) {
-  using Shared = StreamShared<TX, TA, V, kShared, kBackward>;
+template <typename TX, typename TA, int V, int kGate, bool kBackward>
+__device__ __forceinline__ bool finish_tiles(const Params &P, StreamShared<TX, TA, V, kGate, kBackward> &sm, int c, int lane) {
+  using Shared = StreamShared<TX, TA, V, kGate, kBackward>;
   const gearb_recurrence_args &A = P.A;
   bool lost = false;
   unsigned stage = 0, parity = 0;
-  for (unsigned m = 0;; ++m) {
+  Turn<kRing> pair;
+  for (;; pair.next()) {
     if (!warp_wait(&sm.full[stage], parity)) return true;
     const Plan &pl = sm.plan[stage];
     if (!pl.valid) return lost;
@@ -418,13 +481,16 @@ __device__ __forceinline__ bool finish_tiles(const Params &P, StreamShared<TX, T
     }
     if (P.chain && tile % kSuper == kSuper - 1 && tile + 1 < P.tiles) {
       const bool cut = (kBackward ? pl.bcut : pl.cut) >> kWarps & 1u;
-      if (!warp_wait(&sm.ready[m & 1], m >> 1 & 1u)) return true;
+      if (!warp_wait(&sm.ready[pair.i], pair.parity)) return true;
       if (on) {
         const float h = sm.edge[stage].h[c];
         publish_word(P.super + ((tile / kSuper + 1) * A.width + d), cut ? h : fmaf(sm.edge[stage].a[c], in, h));
       }
     }
-    if (c < 32 * V) sm.edge[stage].in[c] = in;
+    if (c < 32 * V) {
+      sm.edge[stage].in[c] = in;
+      if constexpr (kBackward) sm.edge[stage].front[c] = (on && pl.open) ? __ldg(A.carry + (pl.tile * A.width + d)) : 0.0f;
+    }
     __syncwarp();
     if (lane == 0) mbar_arrive(&sm.entered[stage]);
     if (++stage == Shared::kStages) {
@@ -434,54 +500,74 @@ __device__ __forceinline__ bool finish_tiles(const Params &P, StreamShared<TX, T
   }
 }
 
-template <typename TX, typename TA, int V, bool kShared>
-__device__ __forceinline__ bool publish_tiles(const Params &P, StreamShared<TX, TA, V, kShared, false> &sm, int c, int lane) {
-  using Shared = StreamShared<TX, TA, V, kShared, false>;
-  unsigned stage = 0, parity = 0;
-  for (unsigned m = 0;; ++m) {
-    if (!warp_wait(&sm.full[stage], parity)) return true;
-    const Plan &pl = sm.plan[stage];
+// Publishers.  In place of its own pair every warp finds that of all rows before it in the tile (h: forward) and, going
+// backward, that of all rows behind it (c).
+template <typename TX, typename TA, int V, int kGate, bool kBackward>
+__device__ __forceinline__ bool publish_tiles(const Params &P, StreamShared<TX, TA, V, kGate, kBackward> &sm, int c, int lane) {
+  using Shared = StreamShared<TX, TA, V, kGate, kBackward>;
+  Turn<Shared::kStages> now;
+  Turn<kRing> pair;
+  for (;; pair.next(), now.next()) {
+    if (!warp_wait(&sm.full[now.i], now.parity)) return true;
+    const Plan &pl = sm.plan[now.i];
     if (!pl.valid) return false;
-    if (!warp_wait(&sm.paired[m & 1], m >> 1 & 1u)) return true;
+    if (!warp_wait(&sm.paired[pair.i], pair.parity)) return true;
     if (c < pl.cols) {
-      auto &pr = sm.pairs[m & 1];
+      auto &pr = sm.pairs[pair.i];
       const unsigned starts = pl.starts;
-      float b[kWarps], h[kWarps], ta = 1.0f, th = 0.0f;
+      float a[kWarps], h[kWarps], ta = 1.0f, th = 0.0f;
 #pragma unroll
-      for (int q = 0; q < kWarps; ++q) { b[q] = pr.a[q][c]; h[q] = pr.h[q][c]; }
+      for (int q = 0; q < kWarps; ++q) { a[q] = pr.a[q][c]; h[q] = pr.h[q][c]; }
 #pragma unroll
       for (int q = 0; q < kWarps; ++q) {
         pr.a[q][c] = ta;
         pr.h[q][c] = th;
-        th = (starts >> q & 1u) ? h[q] : fmaf(b[q], th, h[q]);
-        ta *= b[q];
+        th = (starts >> q & 1u) ? h[q] : fmaf(a[q], th, h[q]);
+        ta *= a[q];
       }
-      if (P.chain) publish_pair(P.agg + (pl.tile * P.A.width + pl.d0 + c), ta, th);
-      sm.edge[stage].a[c] = ta;
-      sm.edge[stage].h[c] = th;
+      int at = pl.tile;
+      if constexpr (kBackward) {
+        const unsigned ends = pl.ends;
+        at = static_cast<int>(P.tiles) - 1 - at;
+#pragma unroll
+        for (int q = 0; q < kWarps; ++q) h[q] = pr.c[q][c];
+        ta = 1.0f;
+        th = 0.0f;
+#pragma unroll
+        for (int q = kWarps - 1; q >= 0; --q) {
+          pr.b[q][c] = ta;
+          pr.c[q][c] = th;
+          th = (ends >> q & 1u) ? h[q] : fmaf(a[q], th, h[q]);
+          ta *= a[q];
+        }
+      }
+      if (P.chain) publish_pair(P.agg + (at * P.A.width + pl.d0 + c), ta, th);
+      sm.edge[now.i].a[c] = ta;
+      sm.edge[now.i].h[c] = th;
     }
     __syncwarp();
-    if (lane == 0) mbar_arrive(&sm.ready[m & 1]);
-    if (++stage == Shared::kStages) {
-      stage = 0;
-      parity ^= 1u;
-    }
+    if (lane == 0) mbar_arrive(&sm.ready[pair.i]);
   }
 }
 
-template <typename TX, typename TA, int V, bool kShared>
-__device__ __forceinline__ bool compute_forward(const Params &P, StreamShared<TX, TA, V, kShared, false> &sm, int warp,
+template <typename TX, typename TA, int V, int kGate>
+__device__ __forceinline__ bool compute_forward(const Params &P, StreamShared<TX, TA, V, kGate, false> &sm, int warp,
                                                 int lane) {
-  using Shared = StreamShared<TX, TA, V, kShared, false>;
-  constexpr int kG = kShared ? 1 : V, R = kRows;
+  using Shared = StreamShared<TX, TA, V, kGate, false>;
+  constexpr int kG = kGate == kOne ? 1 : V, R = kRows;
   const gearb_recurrence_args &A = P.A;
-  unsigned stage = 0, parity = 0, ostage = 0, oparity = 0;
-  for (unsigned m = 0;; ++m) {
-    if (!warp_wait(&sm.full[stage], parity)) return true;
-    const Plan &pl = sm.plan[stage];
-    const bool valid = pl.valid;
-    if (valid) {
-      const WarpRows<TX, TA, V, kShared, false> rows(P, pl, sm.stage[stage], warp, lane);
+  Turn<Shared::kStages> now, old;
+  Turn<kRing> pair, opair;
+  unsigned m = 0, tiles = 0xffffffffu;  // tiles of this CTA, known when the planner has said that there are no more
+  for (; m < kLag || m - kLag < tiles; ++m) {
+    if (tiles == 0xffffffffu) {
+      if (!warp_wait(&sm.full[now.i], now.parity)) return true;
+      if (!sm.plan[now.i].valid) tiles = m;
+    }
+    if (m < tiles) {
+      const unsigned stage = now.i;
+      const Plan &pl = sm.plan[stage];
+      const WarpRows<TX, TA, V, kGate, false> rows(P, pl, sm, stage, warp, lane);
       float a[kG], ca[V], ch[V], x[V];
 #pragma unroll
       for (int v = 0; v < V; ++v) { ca[v] = 1.0f; ch[v] = 0.0f; }
@@ -494,52 +580,47 @@ __device__ __forceinline__ bool compute_forward(const Params &P, StreamShared<TX
           mul_v(ca, a, ca);
         }
       } else {
-        const unsigned live = pl.live[warp], start = pl.start[warp];
+        const unsigned start = pl.start[warp];
         const int d = pl.d0 + lane * V;
+        const bool on = lane * V < pl.cols;
+        float as[R][kG], xs[R][V];
 #pragma unroll
         for (int k = 0; k < R; ++k) {
-          rows.get_a(k, A.gate_log, true, a);
-          if (!(live >> k & 1u)) continue;
-          rows.get_x(k, x);
-          if (start >> k & 1u) {
-            if (A.h0) {
-              float h0[V];
-              state_load<V>(A.h0, pl.seq[warp * R + k], A.width, d, lane * V < pl.cols, h0);
-              fma_v(ch, a, h0, x);
-            } else {
+          rows.get_a(k, A.gate_log, true, as[k]);
+          rows.get_x(k, xs[k]);
+        }
 #pragma unroll
-              for (int v = 0; v < V; ++v) ch[v] = x[v];
-            }
-          } else {
-            fma_v(ch, a, ch, x);
-          }
-          mul_v(ca, a, ca);
+        for (int k = 0; k < R; ++k) {
+          mul_v(ca, as[k], ca);
+          step_row(A, pl, start, k, warp * R + k, d, on, as[k], xs[k], ch);
         }
       }
-      if (m >= 2 && !warp_wait(&sm.read[m & 1], (m >> 1) - 1u & 1u)) return true;
-      store_pack<float, V>(&sm.pairs[m & 1].a[warp][lane * V], ca);
-      store_pack<float, V>(&sm.pairs[m & 1].h[warp][lane * V], ch);
+      if (m >= kRing && !warp_wait(&sm.read[pair.i], pair.parity ^ 1u)) return true;
+      store_pack<float, V>(&sm.pairs[pair.i].a[warp][lane * V], ca);
+      store_pack<float, V>(&sm.pairs[pair.i].h[warp][lane * V], ch);
       __syncwarp();
-      if (lane == 0) mbar_arrive(&sm.paired[m & 1]);
+      if (lane == 0) mbar_arrive(&sm.paired[pair.i]);
+      now.next();
+      pair.next();
     }
-    if (m > 0) {
-      const unsigned o = m - 1;
+    if (m >= kLag && m - kLag < tiles) {
+      const unsigned ostage = old.i;
       const Plan &opl = sm.plan[ostage];
       const int n = opl.rows - warp * R, d = opl.d0 + lane * V;
       const bool on = lane * V < opl.cols;
-      if (!warp_wait(&sm.ready[o & 1], o >> 1 & 1u) || !warp_wait(&sm.entered[ostage], oparity)) return true;
+      if (!warp_wait(&sm.ready[opair.i], opair.parity) || !warp_wait(&sm.entered[ostage], old.parity)) return true;
       float a[kG], h[V], x[V], in[V];
-      unpack(*reinterpret_cast<const Pack<float, V> *>(&sm.pairs[o & 1].h[warp][lane * V]), h);
+      unpack(*reinterpret_cast<const Pack<float, V> *>(&sm.pairs[opair.i].h[warp][lane * V]), h);
       if (!(opl.cut >> warp & 1u)) {
         float pa[V];
-        unpack(*reinterpret_cast<const Pack<float, V> *>(&sm.pairs[o & 1].a[warp][lane * V]), pa);
+        unpack(*reinterpret_cast<const Pack<float, V> *>(&sm.pairs[opair.i].a[warp][lane * V]), pa);
         unpack(*reinterpret_cast<const Pack<float, V> *>(&sm.edge[ostage].in[lane * V]), in);
         fma_v(h, pa, in, h);
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive(&sm.read[o & 1]);
+      if (lane == 0) mbar_arrive(&sm.read[opair.i]);
       if (n > 0) {
-        const WarpRows<TX, TA, V, kShared, false> rows(P, opl, sm.stage[ostage], warp, lane);
+        const WarpRows<TX, TA, V, kGate, false> rows(P, opl, sm, ostage, warp, lane);
         const int64_t step = A.reverse ? -A.width : A.width;
         TX *out = static_cast<TX *>(A.out) + ((A.reverse ? opl.row0 - warp * R : opl.row0 + warp * R) * A.width + d);
         if (opl.plain) {
@@ -553,29 +634,21 @@ __device__ __forceinline__ bool compute_forward(const Params &P, StreamShared<TX
           }
         } else {
           const unsigned live = opl.live[warp], start = opl.start[warp], end = opl.end[warp];
+          float as[R][kG], xs[R][V];
 #pragma unroll
           for (int k = 0; k < R; ++k) {
-            if (live >> k & 1u) {
-              rows.get_a(k, A.gate_log, false, a);
-              rows.get_x(k, x);
-              if (start >> k & 1u) {
-                if (A.h0) {
-                  float h0[V];
-                  state_load<V>(A.h0, opl.seq[warp * R + k], A.width, d, on, h0);
-                  fma_v(h, a, h0, x);
-                } else {
+            rows.get_a(k, A.gate_log, false, as[k]);
+            rows.get_x(k, xs[k]);
+          }
 #pragma unroll
-                  for (int v = 0; v < V; ++v) h[v] = x[v];
-                }
-              } else {
-                fma_v(h, a, h, x);
-              }
-              if (on) store_pack<TX, V>(out, h);
-              if (end >> k & 1u) state_store<V>(A.state_out, opl.seq[warp * R + k], A.width, d, on, h);
-            } else if (k < n && A.zero_rest && on) {
-              const float z[V] = {};
-              store_pack<TX, V>(out, z);
-            }
+          for (int k = 0; k < R; ++k) {
+            step_row(A, opl, start, k, warp * R + k, d, on, as[k], xs[k], h);
+            const bool lv = live >> k & 1u;
+            float o[V];
+#pragma unroll
+            for (int v = 0; v < V; ++v) o[v] = lv ? h[v] : 0.0f;
+            if (on && (lv || (A.zero_rest && k < n))) store_pack<TX, V>(out, o);
+            if (end >> k & 1u) state_store<V>(A.state_out, opl.seq[warp * R + k], A.width, d, on, h);
             out += step;
           }
         }
@@ -583,28 +656,207 @@ __device__ __forceinline__ bool compute_forward(const Params &P, StreamShared<TX
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // a was written where the next copy will write
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm.empty[ostage]);
-      if (++ostage == Shared::kStages) {
-        ostage = 0;
-        oparity ^= 1u;
-      }
-    }
-    if (!valid) return false;
-    if (++stage == Shared::kStages) {
-      stage = 0;
-      parity ^= 1u;
+      old.next();
+      opair.next();
     }
   }
+  return false;
 }
 
-template <typename TX, typename TA, int V, bool kShared, bool kBackward>
-__device__ __forceinline__ void init_barriers(StreamShared<TX, TA, V, kShared, kBackward> &sm) {
+template <typename TX, typename TA, int V, int kGate>
+__device__ __forceinline__ bool compute_backward(const Params &P, StreamShared<TX, TA, V, kGate, true> &sm, int warp, int lane) {
+  using Shared = StreamShared<TX, TA, V, kGate, true>;
+  constexpr int kG = kGate == kOne ? 1 : V, R = kRows;
+  const gearb_recurrence_args &A = P.A;
+  Turn<Shared::kStages> now, old;
+  Turn<kRing> pair, opair;
+  unsigned m = 0, tiles = 0xffffffffu;
+  for (; m < kLag || m - kLag < tiles; ++m) {
+    if (tiles == 0xffffffffu) {
+      if (!warp_wait(&sm.full[now.i], now.parity)) return true;
+      if (!sm.plan[now.i].valid) tiles = m;
+    }
+    if (m < tiles) {
+      const Plan &pl = sm.plan[now.i];
+      const WarpRows<TX, TA, V, kGate, true> rows(P, pl, sm, now.i, warp, lane);
+      float as[R][kG], x[V], ca[V], ch[V], cc[V];
+#pragma unroll
+      for (int v = 0; v < V; ++v) { ca[v] = 1.0f; ch[v] = cc[v] = 0.0f; }
+#pragma unroll
+      for (int k = 0; k < R; ++k) rows.get_a(k, A.gate_log, true, as[k]);
+      if (pl.plain) {
+#pragma unroll
+        for (int k = 0; k < R; ++k) {
+          rows.get_x(k, x);
+          fma_v(ch, as[k], ch, x);
+          mul_v(ca, as[k], ca);
+        }
+#pragma unroll
+        for (int k = R - 1; k >= 0; --k) {
+          rows.get_dout(k, x);
+#pragma unroll
+          for (int v = 0; v < V; ++v) x[v] += cc[v];
+          mul_v(cc, as[k], x);
+        }
+      } else {
+        const unsigned live = pl.live[warp], start = pl.start[warp], end = pl.end[warp];
+        const int d = pl.d0 + lane * V;
+        const bool on = lane * V < pl.cols;
+#pragma unroll
+        for (int k = R - 1; k >= 0; --k) {
+          if (end >> k & 1u) state_load<V>(A.dstate, pl.seq[warp * R + k], A.width, d, on, cc);
+          rows.get_dout(k, x);
+          if (live >> k & 1u) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) x[v] += cc[v];
+            mul_v(cc, as[k], x);
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < R; ++k) {
+          rows.get_x(k, x);
+          if (live >> k & 1u) {
+            mul_v(ca, as[k], ca);
+            step_row(A, pl, start, k, warp * R + k, d, on, as[k], x, ch);
+          }
+        }
+      }
+      if (m >= kRing && !warp_wait(&sm.read[pair.i], pair.parity ^ 1u)) return true;
+      auto &pr = sm.pairs[pair.i];
+      store_pack<float, V>(&pr.a[warp][lane * V], ca);
+      store_pack<float, V>(&pr.h[warp][lane * V], ch);
+      store_pack<float, V>(&pr.c[warp][lane * V], cc);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.paired[pair.i]);
+      now.next();
+      pair.next();
+    }
+    if (m >= kLag && m - kLag < tiles) {
+      const Plan &pl = sm.plan[old.i];
+      const int n = pl.rows - warp * R, d = pl.d0 + lane * V;
+      const bool on = lane * V < pl.cols;
+      if (!warp_wait(&sm.ready[opair.i], opair.parity) || !warp_wait(&sm.entered[old.i], old.parity)) return true;
+      float h[V], c[V], f[V], e[V];
+      auto &pr = sm.pairs[opair.i];
+      auto &ed = sm.edge[old.i];
+      unpack(*reinterpret_cast<const Pack<float, V> *>(&pr.h[warp][lane * V]), h);
+      unpack(*reinterpret_cast<const Pack<float, V> *>(&pr.c[warp][lane * V]), c);
+      if (!(pl.cut >> warp & 1u)) {
+        unpack(*reinterpret_cast<const Pack<float, V> *>(&pr.a[warp][lane * V]), f);
+        unpack(*reinterpret_cast<const Pack<float, V> *>(&ed.front[lane * V]), e);
+        fma_v(h, f, e, h);
+      }
+      if (!(pl.bcut >> warp & 1u)) {
+        unpack(*reinterpret_cast<const Pack<float, V> *>(&pr.b[warp][lane * V]), f);
+        unpack(*reinterpret_cast<const Pack<float, V> *>(&ed.in[lane * V]), e);
+        fma_v(c, f, e, c);
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.read[opair.i]);
+      if (n > 0) {
+        const WarpRows<TX, TA, V, kGate, true> rows(P, pl, sm, old.i, warp, lane);
+        const int sign = A.reverse ? -1 : 1, row0 = pl.row0 + sign * warp * R;
+        const int64_t xs = sign * A.width, gs = sign * A.gates;
+        TX *dx = static_cast<TX *>(A.dx) + (row0 * A.width + d);
+        TA *dgate = static_cast<TA *>(A.dgate) + (row0 * A.gates + (kGate == kOne ? pl.gate : d));
+        float as[R][kG], hp[R][V], part[R], x[V];
+#pragma unroll
+        for (int k = 0; k < R; ++k) rows.get_a(k, A.gate_log, false, as[k]);
+        if (pl.plain) {
+#pragma unroll
+          for (int k = 0; k < R; ++k) {
+            rows.get_x(k, x);
+#pragma unroll
+            for (int v = 0; v < V; ++v) hp[k][v] = h[v];
+            fma_v(h, as[k], h, x);
+          }
+#pragma unroll
+          for (int k = R - 1; k >= 0; --k) {
+            float g[V], da[V];
+            rows.get_dout(k, g);
+            part[k] = 0.0f;
+#pragma unroll
+            for (int v = 0; v < V; ++v) g[v] += c[v];
+            mul_v(c, as[k], g);
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+              da[v] = (A.gate_log ? c[v] : g[v]) * hp[k][v];
+              part[k] += on ? da[v] : 0.0f;
+            }
+            if (on) {
+              store_pack<TX, V>(dx + k * xs, g);
+              if constexpr (kGate == kOwn) store_pack<TA, V>(dgate + k * gs, da);
+            }
+          }
+        } else {
+          const unsigned live = pl.live[warp], start = pl.start[warp], end = pl.end[warp];
+#pragma unroll
+          for (int k = 0; k < R; ++k) {
+            const bool st = start >> k & 1u;
+            if (st) state_load<V>(A.h0, pl.seq[warp * R + k], A.width, d, on, h);  // zeros without h0
+            rows.get_x(k, x);
+#pragma unroll
+            for (int v = 0; v < V; ++v) hp[k][v] = h[v];
+            if (live >> k & 1u) {
+              if (st && !A.h0) {
+#pragma unroll
+                for (int v = 0; v < V; ++v) h[v] = x[v];
+              } else {
+                fma_v(h, as[k], h, x);
+              }
+            }
+          }
+#pragma unroll
+          for (int k = R - 1; k >= 0; --k) {
+            const bool lv = live >> k & 1u, st = start >> k & 1u;
+            if (end >> k & 1u) state_load<V>(A.dstate, pl.seq[warp * R + k], A.width, d, on, c);
+            float g[V], da[V];
+            rows.get_dout(k, g);
+            part[k] = 0.0f;
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+              const float av = as[k][kGate == kOne ? 0 : v];
+              g[v] = lv ? g[v] + c[v] : 0.0f;
+              if (lv) c[v] = av * g[v];
+              // the first row of a sequence without h0 is h = x: its gate plays no part
+              da[v] = (lv && !(st && !A.h0)) ? (A.gate_log ? c[v] : g[v]) * hp[k][v] : 0.0f;
+              part[k] += on ? da[v] : 0.0f;
+            }
+            if (on && (lv || (A.zero_rest && k < n))) {
+              store_pack<TX, V>(dx + k * xs, g);
+              if constexpr (kGate == kOwn) store_pack<TA, V>(dgate + k * gs, da);
+            }
+            if (st) state_store<V>(A.dh0, pl.seq[warp * R + k], A.width, d, on, c);
+          }
+        }
+        if constexpr (kGate == kOne) {
+          const float sum = sum_rows(part, lane);
+          const int k = row_of_lane(lane);
+          if (lane % kSpare == 0 && k < n && ((pl.live[warp] >> k & 1u) || A.zero_rest)) {
+            if (P.blocks_per_gate == 1) dgate[k * gs] = from_f<TA>(sum);
+            else P.gate_part[(pl.part * P.rows + row0 + k * sign) * A.gates + pl.gate] = sum;
+          }
+        }
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // a was written where the next copy will write
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.empty[old.i]);
+      old.next();
+      opair.next();
+    }
+  }
+  return false;
+}
+
+template <typename TX, typename TA, int V, int kGate, bool kBackward>
+__device__ __forceinline__ void init_barriers(StreamShared<TX, TA, V, kGate, kBackward> &sm) {
   if (threadIdx.x == 0) {
-    for (unsigned s = 0; s < StreamShared<TX, TA, V, kShared, kBackward>::kStages; ++s) {
+    for (unsigned s = 0; s < StreamShared<TX, TA, V, kGate, kBackward>::kStages; ++s) {
       mbar_init_count(&sm.full[s], 2);  // the expected bytes, and the plan
       mbar_init_count(&sm.empty[s], kWarps);
       mbar_init_count(&sm.entered[s], 4);
     }
-    for (int s = 0; s < 2; ++s) {
+    for (unsigned s = 0; s < kRing; ++s) {
       mbar_init_count(&sm.paired[s], kWarps);
       mbar_init_count(&sm.ready[s], 4);
       mbar_init_count(&sm.read[s], kWarps);
@@ -614,19 +866,35 @@ __device__ __forceinline__ void init_barriers(StreamShared<TX, TA, V, kShared, k
   __syncthreads();
 }
 
-template <typename TX, typename TA, int V, bool kShared>
+template <typename TX, typename TA, int V, int kGate>
 __global__ void __launch_bounds__(kStreamThreads, 1) forward_stream_kernel(const __grid_constant__ Params P,
                                                                            const __grid_constant__ Maps maps) {
-  using Shared = StreamShared<TX, TA, V, kShared, false>;
+  using Shared = StreamShared<TX, TA, V, kGate, false>;
   extern __shared__ __align__(1024) unsigned char raw_smem[];
   auto &sm = *reinterpret_cast<Shared *>(raw_smem);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   init_barriers(sm);
   bool lost = false;
-  if (warp < kWarps) lost = compute_forward<TX, TA, V, kShared>(P, sm, warp, lane);
-  else if (warp < kWarps + 4) lost = publish_tiles<TX, TA, V, kShared>(P, sm, threadIdx.x - kThreads, lane);
-  else if (warp < kWarps + 8) lost = finish_tiles<TX, TA, V, kShared, false>(P, sm, threadIdx.x - kThreads - 128, lane);
-  else plan_tiles<TX, TA, V, kShared, false>(P, maps, sm, lane);
+  if (warp < kWarps) lost = compute_forward<TX, TA, V, kGate>(P, sm, warp, lane);
+  else if (warp < kWarps + 4) lost = publish_tiles<TX, TA, V, kGate, false>(P, sm, threadIdx.x - kThreads, lane);
+  else if (warp < kWarps + 8) lost = finish_tiles<TX, TA, V, kGate, false>(P, sm, threadIdx.x - kThreads - 128, lane);
+  else plan_tiles<TX, TA, V, kGate, false>(P, maps, sm, lane);
+  if (lost && lane == 0 && P.A.status) atomicOr(reinterpret_cast<unsigned *>(P.A.status), GEARB_ST_SCAN_ABORTED);
+}
+
+template <typename TX, typename TA, int V, int kGate>
+__global__ void __launch_bounds__(kStreamThreads, 1) backward_stream_kernel(const __grid_constant__ Params P,
+                                                                            const __grid_constant__ Maps maps) {
+  using Shared = StreamShared<TX, TA, V, kGate, true>;
+  extern __shared__ __align__(1024) unsigned char raw_smem[];
+  auto &sm = *reinterpret_cast<Shared *>(raw_smem);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  init_barriers(sm);
+  bool lost = false;
+  if (warp < kWarps) lost = compute_backward<TX, TA, V, kGate>(P, sm, warp, lane);
+  else if (warp < kWarps + 4) lost = publish_tiles<TX, TA, V, kGate, true>(P, sm, threadIdx.x - kThreads, lane);
+  else if (warp < kWarps + 8) lost = finish_tiles<TX, TA, V, kGate, true>(P, sm, threadIdx.x - kThreads - 128, lane);
+  else plan_tiles<TX, TA, V, kGate, true>(P, maps, sm, lane);
   if (lost && lane == 0 && P.A.status) atomicOr(reinterpret_cast<unsigned *>(P.A.status), GEARB_ST_SCAN_ABORTED);
 }
 
@@ -637,21 +905,24 @@ int make_map(CUtensorMap *map, const void *base, int64_t width, int64_t rows, in
   return encode_map(map, type, const_cast<void *>(base), width, rows, row_stride * static_cast<int64_t>(sizeof(T)), box, kTile);
 }
 
-template <typename TX, typename TA, int V, bool kShared>
+template <typename TX, typename TA, int V, int kGate, bool kBackward>
 int launch_stream(Params &p, cudaStream_t stream) {
   const gearb_recurrence_args &a = p.A;
-  p.blocks_per_gate = kShared ? (p.per + 32 * V - 1) / (32 * V) : 1;
-  const int64_t ncol = kShared ? a.gates * p.blocks_per_gate : (a.width + 32 * V - 1) / (32 * V);
-  // Items are counted in 32 bits, and every CTA takes two numbers beyond the last.
+  p.blocks_per_gate = kGate == kOne ? (p.per + 32 * V - 1) / (32 * V) : 1;
+  const int64_t ncol = kGate == kOne ? a.gates * p.blocks_per_gate : (a.width + 32 * V - 1) / (32 * V);
+  // Items are counted in 32 bits, and every CTA takes numbers beyond the last.
   GEARB_REQUIRE(p.tiles <= (int64_t(1) << 31) / ncol - 1, "recurrence: too many tiles for one launch");
   p.ncol = static_cast<int>(ncol);
   Maps maps;
   int rc = make_map<TX>(&maps.x, a.x, a.width, p.rows, a.x_row_stride, 32 * V);
-  if (rc == GEARB_OK && !kShared) rc = make_map<TA>(&maps.gate, a.gate, a.width, p.rows, a.gate_row_stride, 32 * V);
+  if (rc == GEARB_OK && kGate == kOwn) rc = make_map<TA>(&maps.gate, a.gate, a.width, p.rows, a.gate_row_stride, 32 * V);
+  if (rc == GEARB_OK && kBackward) rc = make_map<TX>(&maps.dout, a.dout, a.width, p.rows, a.dout_row_stride, 32 * V);
   if (rc != GEARB_OK) return rc;
-  constexpr int kSmem = sizeof(StreamShared<TX, TA, V, kShared, false>);
+  constexpr int kSmem = sizeof(StreamShared<TX, TA, V, kGate, kBackward>);
   static_assert(kSmem <= kSmemMost, "fits one SM");
-  auto kernel = forward_stream_kernel<TX, TA, V, kShared>;
+  void (*kernel)(Params, Maps);
+  if constexpr (kBackward) kernel = backward_stream_kernel<TX, TA, V, kGate>;
+  else kernel = forward_stream_kernel<TX, TA, V, kGate>;
   GEARB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
   const int64_t most = sm_count(), items = p.tiles * ncol;
   kernel<<<static_cast<unsigned>(items < most ? items : most), kStreamThreads, kSmem, stream>>>(p, maps);
@@ -663,24 +934,41 @@ int launch_stream(Params &p, cudaStream_t stream) {
 inline bool matrix_ok(const void *p, int64_t sr, int size) {
   return reinterpret_cast<uintptr_t>(p) % 16 == 0 && sr > 0 && sr * size % 16 == 0 && sr * size < (int64_t(1) << 40);
 }
+
+// Channels a lane in the streaming kernel, 0: not for it.
 template <typename TX, typename TA>
-bool stream_fits(const Params &p, bool backward) {
+int stream_width(const Params &p, bool backward) {
   const gearb_recurrence_args &a = p.A;
-  if (backward) return false;
   const bool shared = a.gates < a.width;
-  if (!p.flat || p.V < 2 || p.rows >= (int64_t(1) << 31) || !matrix_ok(a.x, a.x_row_stride, sizeof(TX))) return false;
-  if (shared) return p.per * sizeof(TX) % 16 == 0;
-  return matrix_ok(a.gate, a.gate_row_stride, sizeof(TA));
+  if (!p.flat || p.rows >= (int64_t(1) << 31) || !matrix_ok(a.x, a.x_row_stride, sizeof(TX))) return 0;
+  if (!shared && !matrix_ok(a.gate, a.gate_row_stride, sizeof(TA))) return 0;
+  if (backward) {
+    if (!matrix_ok(a.dout, a.dout_row_stride, sizeof(TX)) || a.width % 2 != 0) return 0;
+    if (!vector_ok(a.dx, 0, 0, sizeof(TX), 2) || (!shared && !vector_ok(a.dgate, 0, 0, sizeof(TA), 2))) return 0;
+    if (shared ? (p.per <= 32 || p.per * sizeof(TX) % 16 != 0) : a.width <= 32) return 0;
+    return 2;
+  }
+  if (a.width <= 32 || a.width % 2 != 0) return 0;
+  // a block's channels may span as many gates as the table holds
+  auto spans = [&](int v) { return !shared || (32 * v - 2) / p.per + 2 <= kTableGates; };
+  const bool four = a.width > 64 && a.width % 4 == 0 && vector_ok(a.out, 0, 0, sizeof(TX), 4) && spans(4);
+  if (four && (shared || sizeof(TX) + sizeof(TA) <= 6)) return 4;
+  return vector_ok(a.out, 0, 0, sizeof(TX), 2) && spans(2) ? 2 : 0;
 }
 
 template <typename TX, typename TA>
 int launch_any(Params &p, bool backward, cudaStream_t stream) {
-  if (!stream_fits<TX, TA>(p, backward)) return launch_wide_any<TX, TA>(p, backward, stream);
+  const int v = stream_width<TX, TA>(p, backward);
   const bool shared = p.A.gates < p.A.width;
-  if (shared) return p.V == 4 ? launch_stream<TX, TA, 4, true>(p, stream) : launch_stream<TX, TA, 2, true>(p, stream);
+  if (v == 0) return launch_wide_any<TX, TA>(p, backward, stream);
+  if (backward)
+    return shared ? launch_stream<TX, TA, 2, kOne, true>(p, stream) : launch_stream<TX, TA, 2, kOwn, true>(p, stream);
+  if (shared)
+    return v == 4 ? launch_stream<TX, TA, 4, kTable, false>(p, stream) : launch_stream<TX, TA, 2, kTable, false>(p, stream);
+  // four channels of eight bytes would leave room for two tiles
   if constexpr (sizeof(TX) + sizeof(TA) <= 6)
-    if (p.V == 4) return launch_stream<TX, TA, 4, false>(p, stream);
-  return launch_stream<TX, TA, 2, false>(p, stream);
+    if (v == 4) return launch_stream<TX, TA, 4, kOwn, false>(p, stream);
+  return launch_stream<TX, TA, 2, kOwn, false>(p, stream);
 }
 
 }  // namespace rec
