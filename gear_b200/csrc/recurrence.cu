@@ -70,6 +70,68 @@ __global__ void states_kernel(const float *from, float *to, int64_t n) {
     to[i] = from ? from[i] : 0.0f;
 }
 
+// One warp per tile: its rows among the sequences.  All warps: 0xff where tiles will publish.
+__global__ void __launch_bounds__(kThreads) prepare_kernel(const __grid_constant__ Params P) {
+  const gearb_recurrence_args &A = P.A;
+  const int lane = threadIdx.x & 31;
+  const int64_t threads = static_cast<int64_t>(gridDim.x) * kThreads, me = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
+  uint4 *fill = reinterpret_cast<uint4 *>(P.ticket);  // whole multiples of 256 bytes
+  for (int64_t i = me; i < P.chain_bytes / 16; i += threads) fill[i] = make_uint4(kUnset, kUnset, kUnset, kUnset);
+  for (int64_t tile = me >> 5; tile < P.tiles; tile += threads >> 5) {
+    Place at = {};
+    at.tile = tile;
+    at.i0 = tile * P.tile_rows;
+    at.i1 = at.i0 + P.tile_rows < P.rows ? at.i0 + P.tile_rows : P.rows;
+    const int n = static_cast<int>(at.i1 - at.i0);
+    const TileRows tr = A.offsets ? tile_rows_packed(P, at, lane) : tile_rows_dense(P, at);
+    TileRec &rec = P.recs[tile];
+    int64_t first_start = tr.first_start, last_end = tr.last_end;
+    bool first_open = true, last_open = true;  // the first (last) row's sequence began (goes on) elsewhere
+    uint64_t live = ~uint64_t(0), start = 0, end = 0;
+    if (!tr.interior) {
+      live = 0;
+#pragma unroll
+      for (int half = 0; half < kTile / 32; ++half) {
+        const int n0 = n - half * 32, nn = n0 < 0 ? 0 : (n0 > 32 ? 32 : n0);
+        const RowMap rm = map_rows(A, P.rows, at.i0 + half * 32, nn, lane);
+        rec.seq[half * 32 + lane] = rm.seq;
+        live |= static_cast<uint64_t>(rm.live) << (half * 32);
+        start |= static_cast<uint64_t>(rm.start) << (half * 32);
+        end |= static_cast<uint64_t>(rm.end) << (half * 32);
+        if (half == 0) {
+          first_start = rm.first_start;
+          first_open = rm.live & ~rm.start & 1u;
+        }
+        if (nn > 0) {
+          last_end = rm.last_end;
+          last_open = (rm.live & ~rm.end) >> (nn - 1) & 1u;
+        }
+      }
+    }
+    const bool s = lane < kWarps && (start >> (kRows * (lane & (kWarps - 1))) & kAllRows) != 0;
+    const bool e = lane < kWarps && (end >> (kRows * (lane & (kWarps - 1))) & kAllRows) != 0;
+    const unsigned starts = __ballot_sync(kAll, s), ends = __ballot_sync(kAll, e);
+    if (lane < kWarps) {
+      rec.live[lane] = static_cast<unsigned char>(live >> (kRows * lane) & kAllRows);
+      rec.start[lane] = static_cast<unsigned char>(start >> (kRows * lane) & kAllRows);
+      rec.end[lane] = static_cast<unsigned char>(end >> (kRows * lane) & kAllRows);
+    }
+    if (lane == 0) {
+      rec.starts = starts;
+      rec.ends = ends;
+      // all bits above the lowest start; all below the highest end, and bit kWarps
+      rec.cut = starts ? ~0u << __ffs(starts) : 0u;
+      rec.bcut = ends ? ((1u << (31 - __clz(ends))) - 1u) | 1u << kWarps : 0u;
+      rec.plain = tr.interior;
+      const int64_t from = quotient(first_start, P.tile_rows), back = P.tiles - 1 - tile;
+      rec.open = P.chain && first_open && from < tile;
+      rec.lo = rec.open ? static_cast<int>(from) : -1;
+      const int64_t lo = P.tiles - 1 - quotient(last_end, P.tile_rows);
+      rec.lo_back = P.chain && last_open && lo < back ? static_cast<int>(lo) : -1;
+    }
+  }
+}
+
 // ---- host -------------------------------------------------------------------
 int64_t up256(int64_t v) { return (v + 255) / 256 * 256; }
 
@@ -86,7 +148,7 @@ void tiling(const gearb_recurrence_args &a, int64_t *rows, int *tile_rows, int64
 }
 
 struct Scratch {
-  int64_t agg, super, part, chain_bytes, total;
+  int64_t agg, super, recs, part, chain_bytes, total;
 };
 Scratch scratch_of(const gearb_recurrence_args &a, bool backward) {
   int64_t rows, tiles;
@@ -98,7 +160,8 @@ Scratch scratch_of(const gearb_recurrence_args &a, bool backward) {
     s.super = s.agg + up256(tiles * a.width * 8);
     s.chain_bytes = s.super + up256((tiles / kSuper + 1) * a.width * 4);
   }
-  s.part = s.chain_bytes;
+  s.recs = s.chain_bytes;
+  s.part = s.recs + up256(tiles * static_cast<int64_t>(sizeof(TileRec)));
   s.total = s.part;
   const int64_t per = a.width / a.gates;
   if (backward && a.gates < a.width && per > 32) s.total += up256((per + 31) / 32 * rows * a.gates * 4);
@@ -155,8 +218,9 @@ int launch(const gearb_recurrence_args &a, bool backward, cudaStream_t stream) {
     p.ticket = reinterpret_cast<unsigned *>(base);
     p.agg = reinterpret_cast<float2 *>(base + s.agg);
     p.super = reinterpret_cast<float *>(base + s.super);
-    GEARB_CUDA(cudaMemsetAsync(base, 0xff, static_cast<size_t>(s.chain_bytes), stream));
+    p.chain_bytes = s.chain_bytes;
   }
+  p.recs = reinterpret_cast<TileRec *>(static_cast<char *>(a.scratch) + s.recs);
   p.gate_part = reinterpret_cast<float *>(static_cast<char *>(a.scratch) + s.part);
   auto period = [&](int64_t sb, int64_t sr) { return sb == a.time * sr || a.batch == 1 ? p.rows : a.time; };
   p.x_period = period(a.x_batch_stride, a.x_row_stride);
@@ -201,6 +265,14 @@ int run(const gearb_recurrence_args *args, bool backward, void *stream) {
 }
 
 }  // namespace
+
+int rec::launch_prepare(const Params &p, cudaStream_t stream) {
+  const int64_t warps = p.tiles > p.chain_bytes / 2048 ? p.tiles : p.chain_bytes / 2048;  // up to 64 bytes a thread
+  const int64_t blocks = (warps + kWarps - 1) / kWarps, most = static_cast<int64_t>(sm_count()) * 8;
+  prepare_kernel<<<static_cast<unsigned>(blocks < most ? (blocks > 0 ? blocks : 1) : most), kThreads, 0, stream>>>(p);
+  GEARB_CUDA(cudaGetLastError());
+  return GEARB_OK;
+}
 }  // namespace gearb
 
 using namespace gearb;

@@ -43,6 +43,7 @@ constexpr int kRows = 8;                     // rows a warp keeps in registers
 constexpr int kTile = kWarps * kRows;        // rows per tile
 constexpr int kSuper = 8;                    // tiles per superblock
 constexpr unsigned kAll = 0xffffffffu;
+constexpr unsigned kAllRows = (1u << kRows) - 1u;
 constexpr unsigned kUnset = 0xffffffffu;     // a published word that has not been written
 constexpr int kPollLimit = 1 << 20;          // polls of one word, the better part of a second
 
@@ -86,6 +87,18 @@ __device__ __forceinline__ void store_pack(T *p, const float (&f)[V]) {
   *reinterpret_cast<Pack<T, V> *>(p) = r;
 }
 
+// The rows of a tile among the sequences, for the streaming kernels.
+struct alignas(16) TileRec {
+  unsigned char live[kWarps], start[kWarps], end[kWarps];  // bits: rows of each warp
+  unsigned starts, ends;  // bit w: a sequence starts (ends) in warp w's rows
+  unsigned cut;           // bit w: a sequence starts in rows of the tile before warp w's (bit kWarps: anywhere in it)
+  unsigned bcut;          // bit w: a sequence ends in rows of the tile behind warp w's (bit kWarps: anywhere in it)
+  int plain;              // one sequence goes through the whole tile: no row of it is its first or last
+  int open;               // the first row continues a sequence of an earlier tile
+  int lo, lo_back;        // look back as far as this tile, counted in the order of the tickets; -1: nothing is needed
+  int seq[kTile];         // sequence of each row (unless plain)
+};
+
 // What the kernels need beyond the caller's arguments.
 struct Params {
   gearb_recurrence_args A;
@@ -103,6 +116,8 @@ struct Params {
   float2 *agg;           // [tiles][width]: (A, H) of every tile
   float *super;          // [superblocks][width]: state in front of every superblock
   int V;                 // channels a lane, by alignment and width
+  TileRec *recs;         // [tiles]
+  int64_t chain_bytes;   // at `ticket`: to be set to 0xff before tiles publish
   float *gate_part;      // [blocks_per_gate][rows][gates], when a gate's channels span several column blocks
 };
 
@@ -468,6 +483,8 @@ inline bool vector_ok(const void *p, int64_t sb, int64_t sr, int size, int v) {
   return reinterpret_cast<uintptr_t>(p) % (size * v) == 0 && sb % v == 0 && sr % v == 0;
 }
 
+// In front of a streaming kernel: finds out about the tiles' rows, and clears what they publish in.
+int launch_prepare(const Params &p, cudaStream_t stream);
 int launch_f32(Params &p, bool backward, cudaStream_t stream);
 int launch_f16(Params &p, bool backward, cudaStream_t stream);
 int launch_bf16(Params &p, bool backward, cudaStream_t stream);

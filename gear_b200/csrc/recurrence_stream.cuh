@@ -2,8 +2,8 @@
 //
 // The tiles are those of recurrence_wide.cuh, but the CTAs stay, one per SM, and their warps have roles, so that
 // nothing waits in line:
-//   planner     takes the next tile's number from the counter, works out once for everybody where the tile lies and
-//               which rows start or end a sequence, and starts its copies (one tensor copy per input)
+//   planner     takes the next tile's number from the counter and starts its copies (one tensor copy per input);
+//               which of its rows start or end a sequence was found out by the launch before, once for all columns
 //   compute     first look at tile m: (A, H) of each warp's rows; then, tile m - 1 again: its rows from the state
 //               before them, and out
 //   publishers  one thread per channel: turn the warps' pairs into those of all rows before each warp, publish the
@@ -13,7 +13,7 @@
 // a CTA per tile 170 us whatever the types; CTAs that stay but finish a tile before they begin the next: every tile
 // spent 6700 of 11000 cycles looking back; one bulk copy per row: an SM starts one about every 35 cycles, 180 us;
 // every warp finding its rows' place itself: 600 of 1000 instructions; both phases' rows in registers: spills, 234 us;
-// several tiles' numbers taken at once: tiles wait for others far back in another CTA's queue, 250 to 600 us; two CTA
+// the planner looking the rows up in the offsets: 4 us a tile; several tiles' numbers taken at once: tiles wait for others far back in another CTA's queue, 250 to 600 us; two CTA
 // barriers a tile in place of the roles: 136 us.
 #pragma once
 
@@ -133,22 +133,15 @@ struct Stage {
                                      (kGate != kOwn ? 0 : sizeof(TA) * 32 * V * kTile);
 };
 
-// What the planning warp works out about a tile.  Rows are counted in 32 bits here (the entry point sends longer calls
-// elsewhere).
+// What the warps need to know about a tile: what prepare_kernel found out about its rows, and its place.  Rows are
+// counted in 32 bits here (the entry point sends longer calls elsewhere).
 struct Plan {
+  TileRec rec;
   int valid;
   int tile, rows;  // rows of the scan in it
   int row0;        // matrix row of the first of them; the others follow it, or precede it in a reverse call
   int d0, cols;    // first channel, channels
   int gate, part;  // shared gates: the gate, and which block of its channels
-  int plain;       // one sequence goes through the whole tile: no row of it is its first or last
-  int lo;          // look back as far as this tile, counted in the order of the tickets; -1: nothing is needed from before
-  int open;        // backward: the first row continues a sequence of an earlier tile
-  unsigned starts, ends;  // bit w: a sequence starts (ends) in warp w's rows
-  unsigned cut;    // bit w: a sequence starts in rows of the tile before warp w's (bit kWarps: anywhere in it)
-  unsigned bcut;   // bit w: a sequence ends in rows of the tile behind warp w's (bit kWarps: anywhere in it)
-  alignas(16) unsigned char live[kWarps], start[kWarps], end[kWarps];  // bits: rows of each warp
-  int seq[kTile];                                                     // sequence of each row (unless plain)
 };
 template <int kGate>
 struct GateRows {  // a of each row, for gates that are not copied with the rows
@@ -315,35 +308,13 @@ __device__ __forceinline__ void plan_tiles(const Params &P, const Maps &maps, St
       for (int u = 0; u < kTile / 4; ++u)
         sm.gates[stage].a[(lane >> 3) + 4 * u][lane & 7] = A.gate_log ? exp_of(own[u]) : own[u];
     }
-    const TileRows tr = A.offsets ? tile_rows_packed(P, at, lane) : tile_rows_dense(P, at);
-    int64_t first_start = tr.first_start, last_end = tr.last_end;
-    bool first_open = true, last_open = true;  // the first (last) row's sequence began (goes on) elsewhere
-    if (!tr.interior) {
+    {
+      const int *from = reinterpret_cast<const int *>(P.recs + at.tile);
+      int *to = reinterpret_cast<int *>(&pl.rec);
 #pragma unroll
-      for (int half = 0; half < kTile / 32; ++half) {
-        const int n0 = n - half * 32, nn = n0 < 0 ? 0 : (n0 > 32 ? 32 : n0);
-        const RowMap rm = map_rows(A, P.rows, at.i0 + half * 32, nn, lane);
-        pl.seq[half * 32 + lane] = rm.seq;
-        if (lane < 32 / kRows) {
-          const int w = half * (32 / kRows) + lane;
-          pl.live[w] = static_cast<unsigned char>(rm.live >> (kRows * lane) & kAllRows);
-          pl.start[w] = static_cast<unsigned char>(rm.start >> (kRows * lane) & kAllRows);
-          pl.end[w] = static_cast<unsigned char>(rm.end >> (kRows * lane) & kAllRows);
-        }
-        if (half == 0) {
-          first_start = rm.first_start;
-          first_open = rm.live & ~rm.start & 1u;
-        }
-        if (nn > 0) {
-          last_end = rm.last_end;
-          last_open = (rm.live & ~rm.end) >> (nn - 1) & 1u;
-        }
-      }
-    } else if (lane < kWarps) {
-      pl.live[lane] = static_cast<unsigned char>(kAllRows);
-      pl.start[lane] = pl.end[lane] = 0;
+      for (int w = 0; w < static_cast<int>(sizeof(TileRec) / 4 + 31) / 32; ++w)
+        if (w * 32 + lane < static_cast<int>(sizeof(TileRec) / 4)) to[w * 32 + lane] = __ldg(from + w * 32 + lane);
     }
-    __syncwarp();
     if (lane == 0) {
       pl.valid = 1;
       pl.tile = static_cast<int>(at.tile);
@@ -353,34 +324,6 @@ __device__ __forceinline__ void plan_tiles(const Params &P, const Maps &maps, St
       pl.cols = static_cast<int>(at.d1 - at.d0 < 32 * V ? at.d1 - at.d0 : 32 * V);
       pl.gate = static_cast<int>(at.gate);
       pl.part = at.part;
-      pl.plain = tr.interior;
-      unsigned cut = 0, bcut = 0, starts = 0, ends = 0;
-      if (!tr.interior) {
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-          if (pl.start[w]) {
-            starts |= 1u << w;
-            cut |= ~0u << (w + 1);
-          }
-          if (pl.end[w]) {
-            ends |= 1u << w;
-            bcut |= ((1u << w) - 1u) | 1u << kWarps;
-          }
-        }
-      }
-      pl.starts = starts;
-      pl.ends = ends;
-      pl.cut = cut;
-      pl.bcut = bcut;
-      const int64_t from = quotient(first_start, P.tile_rows);
-      pl.open = P.chain && first_open && from < at.tile;
-      pl.lo = -1;
-      if (!kBackward) {
-        if (pl.open) pl.lo = static_cast<int>(from);
-      } else if (P.chain && last_open) {
-        const int64_t lo = P.tiles - 1 - quotient(last_end, P.tile_rows);
-        if (lo < static_cast<int64_t>(t)) pl.lo = static_cast<int>(lo);
-      }
     }
     __syncwarp();
     if (lane == 0) mbar_arrive(&sm.full[stage]);  // the plan is there; the copies count themselves
@@ -447,7 +390,7 @@ __device__ __forceinline__ void step_row(const gearb_recurrence_args &A, const P
                                          bool on, float (&a)[kG], const float (&x)[V], float (&h)[V]) {
   if (start >> k & 1u) {
     if (A.h0) {
-      state_load<V>(A.h0, pl.seq[row], A.width, d, on, h);
+      state_load<V>(A.h0, pl.rec.seq[row], A.width, d, on, h);
     } else {
 #pragma unroll
       for (int v = 0; v < V; ++v) h[v] = 0.0f;
@@ -470,7 +413,7 @@ __device__ __forceinline__ bool finish_tiles(const Params &P, StreamShared<TX, T
     if (!warp_wait(&sm.full[stage], parity)) return true;
     const Plan &pl = sm.plan[stage];
     if (!pl.valid) return lost;
-    const int tile = kBackward ? static_cast<int>(P.tiles) - 1 - pl.tile : pl.tile, lo = pl.lo, d = pl.d0 + c;
+    const int tile = kBackward ? static_cast<int>(P.tiles) - 1 - pl.tile : pl.tile, lo = kBackward ? pl.rec.lo_back : pl.rec.lo, d = pl.d0 + c;
     const bool on = c < pl.cols;
     float in = 0.0f;
     if (on && lo >= 0) {
@@ -480,7 +423,7 @@ __device__ __forceinline__ bool finish_tiles(const Params &P, StreamShared<TX, T
       if (!kBackward && A.carry) A.carry[pl.tile * A.width + d] = in;
     }
     if (P.chain && tile % kSuper == kSuper - 1 && tile + 1 < P.tiles) {
-      const bool cut = (kBackward ? pl.bcut : pl.cut) >> kWarps & 1u;
+      const bool cut = (kBackward ? pl.rec.bcut : pl.rec.cut) >> kWarps & 1u;
       if (!warp_wait(&sm.ready[pair.i], pair.parity)) return true;
       if (on) {
         const float h = sm.edge[stage].h[c];
@@ -489,7 +432,7 @@ __device__ __forceinline__ bool finish_tiles(const Params &P, StreamShared<TX, T
     }
     if (c < 32 * V) {
       sm.edge[stage].in[c] = in;
-      if constexpr (kBackward) sm.edge[stage].front[c] = (on && pl.open) ? __ldg(A.carry + (pl.tile * A.width + d)) : 0.0f;
+      if constexpr (kBackward) sm.edge[stage].front[c] = (on && pl.rec.open) ? __ldg(A.carry + (pl.tile * A.width + d)) : 0.0f;
     }
     __syncwarp();
     if (lane == 0) mbar_arrive(&sm.entered[stage]);
@@ -514,7 +457,7 @@ __device__ __forceinline__ bool publish_tiles(const Params &P, StreamShared<TX, 
     if (!warp_wait(&sm.paired[pair.i], pair.parity)) return true;
     if (c < pl.cols) {
       auto &pr = sm.pairs[pair.i];
-      const unsigned starts = pl.starts;
+      const unsigned starts = pl.rec.starts;
       float a[kWarps], h[kWarps], ta = 1.0f, th = 0.0f;
 #pragma unroll
       for (int q = 0; q < kWarps; ++q) { a[q] = pr.a[q][c]; h[q] = pr.h[q][c]; }
@@ -527,7 +470,7 @@ __device__ __forceinline__ bool publish_tiles(const Params &P, StreamShared<TX, 
       }
       int at = pl.tile;
       if constexpr (kBackward) {
-        const unsigned ends = pl.ends;
+        const unsigned ends = pl.rec.ends;
         at = static_cast<int>(P.tiles) - 1 - at;
 #pragma unroll
         for (int q = 0; q < kWarps; ++q) h[q] = pr.c[q][c];
@@ -571,7 +514,7 @@ __device__ __forceinline__ bool compute_forward(const Params &P, StreamShared<TX
       float a[kG], ca[V], ch[V], x[V];
 #pragma unroll
       for (int v = 0; v < V; ++v) { ca[v] = 1.0f; ch[v] = 0.0f; }
-      if (pl.plain) {
+      if (pl.rec.plain) {
 #pragma unroll
         for (int k = 0; k < R; ++k) {
           rows.get_a(k, A.gate_log, true, a);
@@ -580,7 +523,7 @@ __device__ __forceinline__ bool compute_forward(const Params &P, StreamShared<TX
           mul_v(ca, a, ca);
         }
       } else {
-        const unsigned start = pl.start[warp];
+        const unsigned start = pl.rec.start[warp];
         const int d = pl.d0 + lane * V;
         const bool on = lane * V < pl.cols;
         float as[R][kG], xs[R][V];
@@ -611,7 +554,7 @@ __device__ __forceinline__ bool compute_forward(const Params &P, StreamShared<TX
       if (!warp_wait(&sm.ready[opair.i], opair.parity) || !warp_wait(&sm.entered[ostage], old.parity)) return true;
       float a[kG], h[V], x[V], in[V];
       unpack(*reinterpret_cast<const Pack<float, V> *>(&sm.pairs[opair.i].h[warp][lane * V]), h);
-      if (!(opl.cut >> warp & 1u)) {
+      if (!(opl.rec.cut >> warp & 1u)) {
         float pa[V];
         unpack(*reinterpret_cast<const Pack<float, V> *>(&sm.pairs[opair.i].a[warp][lane * V]), pa);
         unpack(*reinterpret_cast<const Pack<float, V> *>(&sm.edge[ostage].in[lane * V]), in);
@@ -623,7 +566,7 @@ __device__ __forceinline__ bool compute_forward(const Params &P, StreamShared<TX
         const WarpRows<TX, TA, V, kGate, false> rows(P, opl, sm, ostage, warp, lane);
         const int64_t step = A.reverse ? -A.width : A.width;
         TX *out = static_cast<TX *>(A.out) + ((A.reverse ? opl.row0 - warp * R : opl.row0 + warp * R) * A.width + d);
-        if (opl.plain) {
+        if (opl.rec.plain) {
 #pragma unroll
           for (int k = 0; k < R; ++k) {
             rows.get_a(k, A.gate_log, false, a);
@@ -633,7 +576,7 @@ __device__ __forceinline__ bool compute_forward(const Params &P, StreamShared<TX
             out += step;
           }
         } else {
-          const unsigned live = opl.live[warp], start = opl.start[warp], end = opl.end[warp];
+          const unsigned live = opl.rec.live[warp], start = opl.rec.start[warp], end = opl.rec.end[warp];
           float as[R][kG], xs[R][V];
 #pragma unroll
           for (int k = 0; k < R; ++k) {
@@ -648,7 +591,7 @@ __device__ __forceinline__ bool compute_forward(const Params &P, StreamShared<TX
 #pragma unroll
             for (int v = 0; v < V; ++v) o[v] = lv ? h[v] : 0.0f;
             if (on && (lv || (A.zero_rest && k < n))) store_pack<TX, V>(out, o);
-            if (end >> k & 1u) state_store<V>(A.state_out, opl.seq[warp * R + k], A.width, d, on, h);
+            if (end >> k & 1u) state_store<V>(A.state_out, opl.rec.seq[warp * R + k], A.width, d, on, h);
             out += step;
           }
         }
@@ -684,7 +627,7 @@ __device__ __forceinline__ bool compute_backward(const Params &P, StreamShared<T
       for (int v = 0; v < V; ++v) { ca[v] = 1.0f; ch[v] = cc[v] = 0.0f; }
 #pragma unroll
       for (int k = 0; k < R; ++k) rows.get_a(k, A.gate_log, true, as[k]);
-      if (pl.plain) {
+      if (pl.rec.plain) {
 #pragma unroll
         for (int k = 0; k < R; ++k) {
           rows.get_x(k, x);
@@ -699,12 +642,12 @@ __device__ __forceinline__ bool compute_backward(const Params &P, StreamShared<T
           mul_v(cc, as[k], x);
         }
       } else {
-        const unsigned live = pl.live[warp], start = pl.start[warp], end = pl.end[warp];
+        const unsigned live = pl.rec.live[warp], start = pl.rec.start[warp], end = pl.rec.end[warp];
         const int d = pl.d0 + lane * V;
         const bool on = lane * V < pl.cols;
 #pragma unroll
         for (int k = R - 1; k >= 0; --k) {
-          if (end >> k & 1u) state_load<V>(A.dstate, pl.seq[warp * R + k], A.width, d, on, cc);
+          if (end >> k & 1u) state_load<V>(A.dstate, pl.rec.seq[warp * R + k], A.width, d, on, cc);
           rows.get_dout(k, x);
           if (live >> k & 1u) {
 #pragma unroll
@@ -741,12 +684,12 @@ __device__ __forceinline__ bool compute_backward(const Params &P, StreamShared<T
       auto &ed = sm.edge[old.i];
       unpack(*reinterpret_cast<const Pack<float, V> *>(&pr.h[warp][lane * V]), h);
       unpack(*reinterpret_cast<const Pack<float, V> *>(&pr.c[warp][lane * V]), c);
-      if (!(pl.cut >> warp & 1u)) {
+      if (!(pl.rec.cut >> warp & 1u)) {
         unpack(*reinterpret_cast<const Pack<float, V> *>(&pr.a[warp][lane * V]), f);
         unpack(*reinterpret_cast<const Pack<float, V> *>(&ed.front[lane * V]), e);
         fma_v(h, f, e, h);
       }
-      if (!(pl.bcut >> warp & 1u)) {
+      if (!(pl.rec.bcut >> warp & 1u)) {
         unpack(*reinterpret_cast<const Pack<float, V> *>(&pr.b[warp][lane * V]), f);
         unpack(*reinterpret_cast<const Pack<float, V> *>(&ed.in[lane * V]), e);
         fma_v(c, f, e, c);
@@ -762,7 +705,7 @@ __device__ __forceinline__ bool compute_backward(const Params &P, StreamShared<T
         float as[R][kG], hp[R][V], part[R], x[V];
 #pragma unroll
         for (int k = 0; k < R; ++k) rows.get_a(k, A.gate_log, false, as[k]);
-        if (pl.plain) {
+        if (pl.rec.plain) {
 #pragma unroll
           for (int k = 0; k < R; ++k) {
             rows.get_x(k, x);
@@ -789,11 +732,11 @@ __device__ __forceinline__ bool compute_backward(const Params &P, StreamShared<T
             }
           }
         } else {
-          const unsigned live = pl.live[warp], start = pl.start[warp], end = pl.end[warp];
+          const unsigned live = pl.rec.live[warp], start = pl.rec.start[warp], end = pl.rec.end[warp];
 #pragma unroll
           for (int k = 0; k < R; ++k) {
             const bool st = start >> k & 1u;
-            if (st) state_load<V>(A.h0, pl.seq[warp * R + k], A.width, d, on, h);  // zeros without h0
+            if (st) state_load<V>(A.h0, pl.rec.seq[warp * R + k], A.width, d, on, h);  // zeros without h0
             rows.get_x(k, x);
 #pragma unroll
             for (int v = 0; v < V; ++v) hp[k][v] = h[v];
@@ -809,7 +752,7 @@ __device__ __forceinline__ bool compute_backward(const Params &P, StreamShared<T
 #pragma unroll
           for (int k = R - 1; k >= 0; --k) {
             const bool lv = live >> k & 1u, st = start >> k & 1u;
-            if (end >> k & 1u) state_load<V>(A.dstate, pl.seq[warp * R + k], A.width, d, on, c);
+            if (end >> k & 1u) state_load<V>(A.dstate, pl.rec.seq[warp * R + k], A.width, d, on, c);
             float g[V], da[V];
             rows.get_dout(k, g);
             part[k] = 0.0f;
@@ -826,13 +769,13 @@ __device__ __forceinline__ bool compute_backward(const Params &P, StreamShared<T
               store_pack<TX, V>(dx + k * xs, g);
               if constexpr (kGate == kOwn) store_pack<TA, V>(dgate + k * gs, da);
             }
-            if (st) state_store<V>(A.dh0, pl.seq[warp * R + k], A.width, d, on, c);
+            if (st) state_store<V>(A.dh0, pl.rec.seq[warp * R + k], A.width, d, on, c);
           }
         }
         if constexpr (kGate == kOne) {
           const float sum = sum_rows(part, lane);
           const int k = row_of_lane(lane);
-          if (lane % kSpare == 0 && k < n && ((pl.live[warp] >> k & 1u) || A.zero_rest)) {
+          if (lane % kSpare == 0 && k < n && ((pl.rec.live[warp] >> k & 1u) || A.zero_rest)) {
             if (P.blocks_per_gate == 1) dgate[k * gs] = from_f<TA>(sum);
             else P.gate_part[(pl.part * P.rows + row0 + k * sign) * A.gates + pl.gate] = sum;
           }
@@ -913,8 +856,10 @@ int launch_stream(Params &p, cudaStream_t stream) {
   // Items are counted in 32 bits, and every CTA takes numbers beyond the last.
   GEARB_REQUIRE(p.tiles <= (int64_t(1) << 31) / ncol - 1, "recurrence: too many tiles for one launch");
   p.ncol = static_cast<int>(ncol);
+  int rc = launch_prepare(p, stream);
+  if (rc != GEARB_OK) return rc;
   Maps maps;
-  int rc = make_map<TX>(&maps.x, a.x, a.width, p.rows, a.x_row_stride, 32 * V);
+  rc = make_map<TX>(&maps.x, a.x, a.width, p.rows, a.x_row_stride, 32 * V);
   if (rc == GEARB_OK && kGate == kOwn) rc = make_map<TA>(&maps.gate, a.gate, a.width, p.rows, a.gate_row_stride, 32 * V);
   if (rc == GEARB_OK && kBackward) rc = make_map<TX>(&maps.dout, a.dout, a.width, p.rows, a.dout_row_stride, 32 * V);
   if (rc != GEARB_OK) return rc;

@@ -31,7 +31,6 @@ __device__ __forceinline__ void exp_gate(float (&a)[kRows][kG]) {
     for (int v = 0; v < kG; ++v) a[k][v] = exp_of(a[k][v]);
 }
 
-constexpr unsigned kAllRows = (1u << kRows) - 1u;
 
 // The tile's rows, and this warp's: looked up for the whole tile first, by each warp only where a sequence starts or
 // ends in it.
@@ -472,6 +471,7 @@ int launch_wide(Params &p, bool backward, cudaStream_t stream) {
   GEARB_REQUIRE(p.tiles <= (int64_t(1) << 31) / ncol - 1, "recurrence: too many tiles for one launch");
   p.ncol = static_cast<int>(ncol);
   const unsigned grid = static_cast<unsigned>(p.tiles * ncol);
+  if (p.chain) GEARB_CUDA(cudaMemsetAsync(p.ticket, 0xff, static_cast<size_t>(p.chain_bytes), stream));
   if (backward) {
     if (shared) backward_kernel<TX, TA, V, true><<<grid, kThreads, 0, stream>>>(p);
     else backward_kernel<TX, TA, V, false><<<grid, kThreads, 0, stream>>>(p);
