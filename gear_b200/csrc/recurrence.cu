@@ -77,6 +77,15 @@ __global__ void __launch_bounds__(kThreads) prepare_kernel(const __grid_constant
   const int64_t threads = static_cast<int64_t>(gridDim.x) * kThreads, me = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
   uint4 *fill = reinterpret_cast<uint4 *>(P.ticket);  // whole multiples of 256 bytes
   for (int64_t i = me; i < P.chain_bytes / 16; i += threads) fill[i] = make_uint4(kUnset, kUnset, kUnset, kUnset);
+  // sequences without rows keep their state (backward: their gradient)
+  float *to = P.backward ? A.dh0 : A.state_out;
+  const float *old = P.backward ? A.dstate : A.h0;
+  if (to && to != old && (A.offsets || A.lengths))
+    for (int64_t s = me >> 5; s < A.sequences; s += threads >> 5) {
+      const ScanOffsets so{A.offsets, P.rows, A.sequences, 0};
+      if ((A.offsets ? so.at(s + 1) - so.at(s) : __ldg(A.lengths + s)) > 0) continue;
+      for (int64_t d = lane; d < A.width; d += 32) to[s * A.width + d] = old ? old[s * A.width + d] : 0.0f;
+    }
   for (int64_t tile = me >> 5; tile < P.tiles; tile += threads >> 5) {
     Place at = {};
     at.tile = tile;
@@ -123,6 +132,7 @@ __global__ void __launch_bounds__(kThreads) prepare_kernel(const __grid_constant
       rec.cut = starts ? ~0u << __ffs(starts) : 0u;
       rec.bcut = ends ? ((1u << (31 - __clz(ends))) - 1u) | 1u << kWarps : 0u;
       rec.plain = tr.interior;
+      rec.dead = live == 0;
       const int64_t from = quotient(first_start, P.tile_rows), back = P.tiles - 1 - tile;
       rec.open = P.chain && first_open && from < tile;
       rec.lo = rec.open ? static_cast<int>(from) : -1;
@@ -200,6 +210,7 @@ int check_pointers(const gearb_recurrence_args *a, bool backward) {
 int launch(const gearb_recurrence_args &a, bool backward, cudaStream_t stream) {
   Params p = {};
   p.A = a;
+  p.backward = backward;
   tiling(a, &p.rows, &p.tile_rows, &p.tiles, &p.chain);
   if (p.rows == 0) {
     const float *from = backward ? a.dstate : a.h0;
@@ -267,7 +278,8 @@ int run(const gearb_recurrence_args *args, bool backward, void *stream) {
 }  // namespace
 
 int rec::launch_prepare(const Params &p, cudaStream_t stream) {
-  const int64_t warps = p.tiles > p.chain_bytes / 2048 ? p.tiles : p.chain_bytes / 2048;  // up to 64 bytes a thread
+  int64_t warps = p.tiles > p.chain_bytes / 2048 ? p.tiles : p.chain_bytes / 2048;  // up to 64 bytes a thread
+  if ((p.A.offsets || p.A.lengths) && warps < p.A.sequences) warps = p.A.sequences;
   const int64_t blocks = (warps + kWarps - 1) / kWarps, most = static_cast<int64_t>(sm_count()) * 8;
   prepare_kernel<<<static_cast<unsigned>(blocks < most ? (blocks > 0 ? blocks : 1) : most), kThreads, 0, stream>>>(p);
   GEARB_CUDA(cudaGetLastError());

@@ -93,6 +93,7 @@ struct alignas(16) TileRec {
   unsigned starts, ends;  // bit w: a sequence starts (ends) in warp w's rows
   unsigned cut;           // bit w: a sequence starts in rows of the tile before warp w's (bit kWarps: anywhere in it)
   unsigned bcut;          // bit w: a sequence ends in rows of the tile behind warp w's (bit kWarps: anywhere in it)
+  int dead;               // no row of the tile belongs to a sequence
   int plain;              // one sequence goes through the whole tile: no row of it is its first or last
   int open;               // the first row continues a sequence of an earlier tile
   int lo, lo_back;        // look back as far as this tile, counted in the order of the tickets; -1: nothing is needed
@@ -105,6 +106,7 @@ struct Params {
   int64_t rows;
   int64_t tiles;
   int tile_rows;         // kTile, or the largest multiple of `time` below it when tiles then need nothing from each other
+  int backward;
   int chain;             // tiles publish to each other
   int per;               // channels per gate
   int blocks_per_gate;   // column blocks of a gate's channels (shared gates)

@@ -24,11 +24,12 @@
 namespace gearb {
 namespace rec {
 
-constexpr int kStreamThreads = kThreads + 9 * 32;  // compute, 4 publishers, 4 finishers, planner
+constexpr int kStreamThreads = kThreads + 11 * 32;  // compute, 4 publishers, 4 finishers, issuer, 2 recorders
 constexpr int kSmemMost = 227 * 1024;
 constexpr unsigned kLag = 2;  // tiles that compute warps begin before they come back to one (1: 124 us in place of 110)
 constexpr unsigned kRing = kLag + 1;
 constexpr int kMostStages = 6;
+constexpr int kRecorders = 2;  // one takes 3 us a tile: two dependent trips to L2
 // How a block of channels gets its gates: a gate each; one for the whole block; by a table of the few that it spans.
 enum { kOwn = 0, kOne = 1, kTable = 2 };
 constexpr int kTableGates = 8;
@@ -123,6 +124,17 @@ __device__ __forceinline__ void mbar_arrive(uint64_t *bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
 }
 
+// A place in a ring of barriers, and the parity of its use.
+template <unsigned kSize>
+struct Turn {
+  unsigned i = 0, parity = 0;
+  __device__ __forceinline__ void next() {
+    if (++i == kSize) {
+      i = 0;
+      parity ^= 1u;
+    }
+  }
+};
 // Shared memory of one stage.  A tensor copy writes to 128-byte boundaries.
 template <typename TX, typename TA, int V, int kGate, bool kBackward>
 struct Stage {
@@ -155,17 +167,6 @@ struct Pairs {  // of the warps of one tile; then of all rows before (backward: 
   alignas(16) float b[kBackward ? kWarps : 1][kBackward ? 32 * V : 4];
   alignas(16) float c[kBackward ? kWarps : 1][kBackward ? 32 * V : 4];
 };
-// A place in a ring of barriers, and the parity of its use.
-template <unsigned kSize>
-struct Turn {
-  unsigned i = 0, parity = 0;
-  __device__ __forceinline__ void next() {
-    if (++i == kSize) {
-      i = 0;
-      parity ^= 1u;
-    }
-  }
-};
 template <int V, bool kBackward>
 struct Edge {  // of one tile: its own pair, and the state that enters it (backward: from behind, and from in front)
   alignas(16) float a[32 * V];
@@ -187,6 +188,8 @@ struct StreamShared {
   Plan plan[kStages];
   GateRows<kGate> gates[kStages];
   uint64_t full[kStages], empty[kStages];  // the tile's rows and plan are there; the tile is done with
+  uint64_t issued[kStages];                // item is there
+  unsigned item[kStages];
   uint64_t entered[kStages];               // edge.in is there
   uint64_t paired[kRing], ready[kRing], read[kRing];   // the warps' pairs; turned and edge.a, edge.h there; read again
 };
@@ -231,89 +234,123 @@ __device__ __forceinline__ float settle_back(const Params &P, int at, int lo, in
   return fmaf(pa, k.s, ph);
 }
 
-// The planning warp.
+// Where an item lies.
+template <int V, int kGate, bool kBackward>
+__device__ __forceinline__ Place place_of_item(const Params &P, unsigned item) {
+  Place at;
+  const unsigned t = item / static_cast<unsigned>(P.ncol);
+  const int c = static_cast<int>(item - t * static_cast<unsigned>(P.ncol));
+  at.tile = kBackward ? P.tiles - 1 - t : t;
+  at.i0 = at.tile * P.tile_rows;
+  at.i1 = at.i0 + P.tile_rows < P.rows ? at.i0 + P.tile_rows : P.rows;
+  at.gate = kGate == kOne ? c / P.blocks_per_gate : 0;
+  at.part = kGate == kOne ? c - static_cast<int>(at.gate) * P.blocks_per_gate : 0;
+  at.d0 = kGate == kOne ? at.gate * P.per + at.part * 32 * V : c * 32 * V;
+  at.d1 = kGate == kOne ? (at.gate + 1) * P.per : P.A.width;
+  return at;
+}
+
+// The issuing warp (one lane of it): numbers and copies.
 template <typename TX, typename TA, int V, int kGate, bool kBackward>
-__device__ __forceinline__ void plan_tiles(const Params &P, const Maps &maps, StreamShared<TX, TA, V, kGate, kBackward> &sm,
-                                           int lane) {
+__device__ __forceinline__ bool issue_tiles(const Params &P, const Maps &maps, StreamShared<TX, TA, V, kGate, kBackward> &sm) {
   using Shared = StreamShared<TX, TA, V, kGate, kBackward>;
-  constexpr unsigned kStages = Shared::kStages;
   const gearb_recurrence_args &A = P.A;
   const unsigned items = static_cast<unsigned>(P.tiles * P.ncol);
-  // lane 0: the next number.  One at a time from the start: CTAs that took several at once would come to tiles much
-  // later than others come to the tiles behind them, and those would wait.
-  unsigned next = 0;
-  if (lane == 0) next = P.chain ? atomicAdd(P.ticket, 1u) + 1u : blockIdx.x;  // the counter starts at 0xffffffff
-  unsigned stage = 0, parity = 0;
-  for (unsigned m = 0;; ++m) {
-    if (m >= kStages) {
-      const bool free = mbar_wait(&sm.empty[stage], parity ^ 1u);
-      if (!__all_sync(kAll, free)) {  // a warp of this CTA is stuck: nothing more is started
-        if (lane == 0 && A.status) atomicOr(reinterpret_cast<unsigned *>(A.status), GEARB_ST_SCAN_ABORTED);
-        return;
+  // Packed rows of no sequence need no copies.
+  int64_t lo = 0, hi = P.rows;
+  if (A.offsets) {
+    const ScanOffsets so{A.offsets, P.rows, A.sequences, A.reverse};
+    lo = so.at(0);
+    hi = so.at(A.sequences);
+  }
+  // One number at a time from the start: CTAs that took several at once would come to tiles much later than others come to
+  // the tiles behind them, and those would wait.
+  unsigned next = P.chain ? atomicAdd(P.ticket, 1u) + 1u : blockIdx.x;  // the counter starts at 0xffffffff
+  Turn<Shared::kStages> now;
+  for (unsigned m = 0;; ++m, now.next()) {
+    if (m >= Shared::kStages && !mbar_wait(&sm.empty[now.i], now.parity ^ 1u)) return true;
+    const unsigned item = next;
+    sm.item[now.i] = item;
+    if (item >= items) {
+      mbar_arrive(&sm.full[now.i]);
+      for (int r = 0; r < kRecorders; ++r) {  // every recorder has to learn that there are no more
+        mbar_arrive(&sm.issued[now.i]);
+        now.next();
+        if (r + 1 < kRecorders) {
+          ++m;
+          if (m >= Shared::kStages && !mbar_wait(&sm.empty[now.i], now.parity ^ 1u)) return true;
+          sm.item[now.i] = item;
+        }
       }
+      return false;
     }
-    const unsigned item = __shfl_sync(kAll, next, 0);
-    Plan &pl = sm.plan[stage];
+    const Place at = place_of_item<V, kGate, kBackward>(P, item);
+    uint64_t *full = &sm.full[now.i];
+    if (at.i0 < hi && at.i1 > lo) {
+      // a reverse call's tile ends at row_of(i0): its box begins kTile - 1 rows before, if need be in front of the matrix
+      const int row0 = static_cast<int>(row_of(P, at.i0)), c = static_cast<int>(at.d0), r = A.reverse ? row0 - (kTile - 1) : row0;
+      mbar_expect(full, Shared::StageT::kBytes);
+      tensor_load(sm.stage[now.i].x, &maps.x, c, r, full);
+      if constexpr (kGate == kOwn) tensor_load(sm.stage[now.i].gate, &maps.gate, c, r, full);
+      if constexpr (kBackward) tensor_load(sm.stage[now.i].dout, &maps.dout, c, r, full);
+    } else {
+      mbar_arrive(full);
+    }
+    mbar_arrive(&sm.issued[now.i]);
+    next = P.chain ? atomicAdd(P.ticket, 1u) + 1u : item + gridDim.x;  // needed a tile later
+  }
+}
+
+// The recording warps, every kRecorders-th tile each: what is known about a tile's rows, and gates that are not copied.
+template <typename TX, typename TA, int V, int kGate, bool kBackward>
+__device__ __forceinline__ bool record_tiles(const Params &P, StreamShared<TX, TA, V, kGate, kBackward> &sm, int which, int lane) {
+  using Shared = StreamShared<TX, TA, V, kGate, kBackward>;
+  const gearb_recurrence_args &A = P.A;
+  const unsigned items = static_cast<unsigned>(P.tiles * P.ncol);
+  Turn<Shared::kStages> now;
+  for (int k = 0; k < which; ++k) now.next();
+  for (;;) {
+    if (!warp_wait(&sm.issued[now.i], now.parity)) return true;
+    const unsigned item = sm.item[now.i];
+    Plan &pl = sm.plan[now.i];
     if (item >= items) {
       if (lane == 0) {
         pl.valid = 0;
-        mbar_arrive(&sm.full[stage]);
-        mbar_arrive(&sm.full[stage]);
+        mbar_arrive(&sm.full[now.i]);
       }
-      return;
+      return false;
     }
-    if (lane == 0) {  // asked for now, needed a tile later
-      next = P.chain ? atomicAdd(P.ticket, 1u) + 1u : item + gridDim.x;
-    }
-    Place at;
-    const unsigned t = item / static_cast<unsigned>(P.ncol);
-    const int c = static_cast<int>(item - t * static_cast<unsigned>(P.ncol));
-    at.tile = kBackward ? P.tiles - 1 - t : t;
-    at.i0 = at.tile * P.tile_rows;
-    at.i1 = at.i0 + P.tile_rows < P.rows ? at.i0 + P.tile_rows : P.rows;
-    at.gate = kGate == kOne ? c / P.blocks_per_gate : 0;
-    at.part = kGate == kOne ? c - static_cast<int>(at.gate) * P.blocks_per_gate : 0;
-    at.d0 = kGate == kOne ? at.gate * P.per + at.part * 32 * V : c * 32 * V;
-    at.d1 = kGate == kOne ? (at.gate + 1) * P.per : A.width;
-    const int n = static_cast<int>(at.i1 - at.i0);
-    const int row0 = static_cast<int>(row_of(P, at.i0));
-    if (lane == 0) {
-      // a reverse call's tile ends at row0: its box begins kTile - 1 rows before, if need be in front of the matrix
-      const int bc = static_cast<int>(at.d0), br = A.reverse ? row0 - (kTile - 1) : row0;
-      mbar_expect(&sm.full[stage], Shared::StageT::kBytes);  // arrives below
-      tensor_load(sm.stage[stage].x, &maps.x, bc, br, &sm.full[stage]);
-      if constexpr (kGate == kOwn) tensor_load(sm.stage[stage].gate, &maps.gate, bc, br, &sm.full[stage]);
-      if constexpr (kBackward) tensor_load(sm.stage[stage].dout, &maps.dout, bc, br, &sm.full[stage]);
-    }
-    if constexpr (kGate == kOne) {
+    const Place at = place_of_item<V, kGate, kBackward>(P, item);
+    const int n = static_cast<int>(at.i1 - at.i0), row0 = static_cast<int>(row_of(P, at.i0));
+    constexpr int kWords = static_cast<int>(sizeof(TileRec) / 4), kEach = (kWords + 31) / 32;
+    const int *from = reinterpret_cast<const int *>(P.recs + at.tile);
+    int word[kEach];
 #pragma unroll
-      for (int k = lane; k < kTile; k += 32) {
-        float own = 0.0f;
-        if (k < n)
-          own = to_f(static_cast<const TA *>(A.gate)[(A.reverse ? row0 - k : row0 + k) * A.gate_row_stride + at.gate]);
-        sm.gates[stage].a[k][0] = A.gate_log ? exp_of(own) : own;
-      }
-    } else if constexpr (kGate == kTable) {
-      // eight gates a row: lane l looks at rows l / 8, l / 8 + 4, ...
-      const int g0 = static_cast<int>(at.d0) / P.per, g = g0 + (lane & 7);
-      float own[kTile / 4];
+    for (int w = 0; w < kEach; ++w) word[w] = w * 32 + lane < kWords ? __ldg(from + w * 32 + lane) : 0;
+    // gates: all 64 rows of one, or of eight (lane l: gate l % 8 of rows l / 8, l / 8 + 4, ...)
+    constexpr int kLooks = kGate == kOwn ? 1 : (kGate == kOne ? kTile / 32 : kTile / 4);
+    float own[kLooks];
+    if constexpr (kGate != kOwn) {
+      const int g = kGate == kOne ? static_cast<int>(at.gate) : static_cast<int>(at.d0) / P.per + (lane & 7);
+      const bool wanted = g < A.gates && (kGate == kOne || static_cast<int64_t>(g) * P.per < at.d0 + 32 * V);
 #pragma unroll
-      for (int u = 0; u < kTile / 4; ++u) {
-        const int k = (lane >> 3) + 4 * u;
+      for (int u = 0; u < kLooks; ++u) {
+        const int k = kGate == kOne ? lane + 32 * u : (lane >> 3) + 4 * u;
         own[u] = 0.0f;
-        if (k < n && g < A.gates && static_cast<int64_t>(g) * P.per < at.d0 + 32 * V)
+        if (k < n && wanted)
           own[u] = to_f(static_cast<const TA *>(A.gate)[(A.reverse ? row0 - k : row0 + k) * A.gate_row_stride + g]);
       }
-#pragma unroll
-      for (int u = 0; u < kTile / 4; ++u)
-        sm.gates[stage].a[(lane >> 3) + 4 * u][lane & 7] = A.gate_log ? exp_of(own[u]) : own[u];
     }
-    {
-      const int *from = reinterpret_cast<const int *>(P.recs + at.tile);
-      int *to = reinterpret_cast<int *>(&pl.rec);
 #pragma unroll
-      for (int w = 0; w < static_cast<int>(sizeof(TileRec) / 4 + 31) / 32; ++w)
-        if (w * 32 + lane < static_cast<int>(sizeof(TileRec) / 4)) to[w * 32 + lane] = __ldg(from + w * 32 + lane);
+    for (int w = 0; w < kEach; ++w)
+      if (w * 32 + lane < kWords) reinterpret_cast<int *>(&pl.rec)[w * 32 + lane] = word[w];
+    if constexpr (kGate != kOwn) {
+#pragma unroll
+      for (int u = 0; u < kLooks; ++u) {
+        const float a = A.gate_log ? exp_of(own[u]) : own[u];
+        if constexpr (kGate == kOne) sm.gates[now.i].a[lane + 32 * u][0] = a;
+        else sm.gates[now.i].a[(lane >> 3) + 4 * u][lane & 7] = a;
+      }
     }
     if (lane == 0) {
       pl.valid = 1;
@@ -326,12 +363,8 @@ __device__ __forceinline__ void plan_tiles(const Params &P, const Maps &maps, St
       pl.part = at.part;
     }
     __syncwarp();
-    if (lane == 0) mbar_arrive(&sm.full[stage]);  // the plan is there; the copies count themselves
-    empty_sequences(P, at, 32 * V, kBackward ? A.dstate : A.h0, kBackward ? A.dh0 : A.state_out, lane);
-    if (++stage == kStages) {
-      stage = 0;
-      parity ^= 1u;
-    }
+    if (lane == 0) mbar_arrive(&sm.full[now.i]);
+    for (int k = 0; k < kRecorders; ++k) now.next();
   }
 }
 
@@ -514,7 +547,8 @@ __device__ __forceinline__ bool compute_forward(const Params &P, StreamShared<TX
       float a[kG], ca[V], ch[V], x[V];
 #pragma unroll
       for (int v = 0; v < V; ++v) { ca[v] = 1.0f; ch[v] = 0.0f; }
-      if (pl.rec.plain) {
+      if (pl.rec.dead) {
+      } else if (pl.rec.plain) {
 #pragma unroll
         for (int k = 0; k < R; ++k) {
           rows.get_a(k, A.gate_log, true, a);
@@ -795,9 +829,10 @@ template <typename TX, typename TA, int V, int kGate, bool kBackward>
 __device__ __forceinline__ void init_barriers(StreamShared<TX, TA, V, kGate, kBackward> &sm) {
   if (threadIdx.x == 0) {
     for (unsigned s = 0; s < StreamShared<TX, TA, V, kGate, kBackward>::kStages; ++s) {
-      mbar_init_count(&sm.full[s], 2);  // the expected bytes, and the plan
+      mbar_init_count(&sm.full[s], 2);  // the issuer (and its copies' bytes), the recorder
       mbar_init_count(&sm.empty[s], kWarps);
       mbar_init_count(&sm.entered[s], 4);
+      mbar_init_count(&sm.issued[s], 1);
     }
     for (unsigned s = 0; s < kRing; ++s) {
       mbar_init_count(&sm.paired[s], kWarps);
@@ -821,7 +856,8 @@ __global__ void __launch_bounds__(kStreamThreads, 1) forward_stream_kernel(const
   if (warp < kWarps) lost = compute_forward<TX, TA, V, kGate>(P, sm, warp, lane);
   else if (warp < kWarps + 4) lost = publish_tiles<TX, TA, V, kGate, false>(P, sm, threadIdx.x - kThreads, lane);
   else if (warp < kWarps + 8) lost = finish_tiles<TX, TA, V, kGate, false>(P, sm, threadIdx.x - kThreads - 128, lane);
-  else plan_tiles<TX, TA, V, kGate, false>(P, maps, sm, lane);
+  else if (warp < kWarps + 8 + kRecorders) lost = record_tiles<TX, TA, V, kGate, false>(P, sm, warp - kWarps - 8, lane);
+  else if (lane == 0) lost = issue_tiles<TX, TA, V, kGate, false>(P, maps, sm);
   if (lost && lane == 0 && P.A.status) atomicOr(reinterpret_cast<unsigned *>(P.A.status), GEARB_ST_SCAN_ABORTED);
 }
 
@@ -837,7 +873,8 @@ __global__ void __launch_bounds__(kStreamThreads, 1) backward_stream_kernel(cons
   if (warp < kWarps) lost = compute_backward<TX, TA, V, kGate>(P, sm, warp, lane);
   else if (warp < kWarps + 4) lost = publish_tiles<TX, TA, V, kGate, true>(P, sm, threadIdx.x - kThreads, lane);
   else if (warp < kWarps + 8) lost = finish_tiles<TX, TA, V, kGate, true>(P, sm, threadIdx.x - kThreads - 128, lane);
-  else plan_tiles<TX, TA, V, kGate, true>(P, maps, sm, lane);
+  else if (warp < kWarps + 8 + kRecorders) lost = record_tiles<TX, TA, V, kGate, true>(P, sm, warp - kWarps - 8, lane);
+  else if (lane == 0) lost = issue_tiles<TX, TA, V, kGate, true>(P, maps, sm);
   if (lost && lane == 0 && P.A.status) atomicOr(reinterpret_cast<unsigned *>(P.A.status), GEARB_ST_SCAN_ABORTED);
 }
 
