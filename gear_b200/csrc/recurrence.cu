@@ -3,7 +3,7 @@
 
 #include <atomic>
 
-#include "recurrence.cuh"
+#include "recurrence_narrow.cuh"
 
 namespace gearb {
 
@@ -145,27 +145,40 @@ __global__ void __launch_bounds__(kThreads) prepare_kernel(const __grid_constant
 // ---- host -------------------------------------------------------------------
 int64_t up256(int64_t v) { return (v + 255) / 256 * 256; }
 
-// Tiling of a call: rows per tile, and whether tiles need anything from each other.
-void tiling(const gearb_recurrence_args &a, int64_t *rows, int *tile_rows, int64_t *tiles, int *chain) {
-  *rows = a.batch * a.time;
-  *tile_rows = kTile;
-  *chain = *rows > kTile;
-  if (!a.offsets && a.time > 0 && a.time <= kTile) {  // whole sequences per tile
-    *tile_rows = static_cast<int>(kTile / a.time * a.time);
-    *chain = 0;
+// Tiling of a call, the same for its forward and backward pass: which kind of kernel, rows per tile, and whether tiles
+// need anything from each other.
+struct Tiling {
+  int64_t rows, tiles;
+  int tile_rows, chain, narrow_rows;
+};
+Tiling tiling_of(const gearb_recurrence_args &a) {
+  Tiling t = {};
+  t.rows = a.batch * a.time;
+  int most = kTile;
+  if (a.width <= kNarrowWidth) {
+    // 16 rows a thread keep the memory busy; with 4 a small call is spread over four times as many SMs
+    const int groups = kWarps * narrow_groups(static_cast<int>(a.width));
+    t.narrow_rows = t.rows > int64_t(16) * groups * 148 ? 16 : 4;
+    most = t.narrow_rows * groups;
   }
-  *tiles = (*rows + *tile_rows - 1) / *tile_rows;
+  t.tile_rows = most;
+  t.chain = t.rows > most;
+  if (!a.offsets && a.time > 0 && a.time <= most) {  // whole sequences per tile
+    t.tile_rows = static_cast<int>(most / a.time * a.time);
+    t.chain = 0;
+  }
+  t.tiles = (t.rows + t.tile_rows - 1) / t.tile_rows;
+  return t;
 }
 
 struct Scratch {
   int64_t agg, super, recs, part, chain_bytes, total;
 };
 Scratch scratch_of(const gearb_recurrence_args &a, bool backward) {
-  int64_t rows, tiles;
-  int tile_rows, chain;
-  tiling(a, &rows, &tile_rows, &tiles, &chain);
+  const Tiling t = tiling_of(a);
+  const int64_t rows = t.rows, tiles = t.tiles;
   Scratch s = {};
-  if (chain) {
+  if (t.chain) {
     s.agg = 256;
     s.super = s.agg + up256(tiles * a.width * 8);
     s.chain_bytes = s.super + up256((tiles / kSuper + 1) * a.width * 4);
@@ -211,7 +224,12 @@ int launch(const gearb_recurrence_args &a, bool backward, cudaStream_t stream) {
   Params p = {};
   p.A = a;
   p.backward = backward;
-  tiling(a, &p.rows, &p.tile_rows, &p.tiles, &p.chain);
+  const Tiling t = tiling_of(a);
+  p.rows = t.rows;
+  p.tiles = t.tiles;
+  p.tile_rows = t.tile_rows;
+  p.chain = t.chain;
+  p.narrow_rows = t.narrow_rows;
   if (p.rows == 0) {
     const float *from = backward ? a.dstate : a.h0;
     float *to = backward ? a.dh0 : a.state_out;
@@ -296,11 +314,9 @@ int gearb_recurrence_bytes(const gearb_recurrence_args *args, int backward, int6
   GEARB_REQUIRE(scratch_bytes && carry_bytes, "recurrence_bytes: null argument");
   const int rc = check_sizes(args);
   if (rc != GEARB_OK) return rc;
-  int64_t rows, tiles;
-  int tile_rows, chain;
-  tiling(*args, &rows, &tile_rows, &tiles, &chain);
+  const Tiling t = tiling_of(*args);
   *scratch_bytes = scratch_of(*args, backward != 0).total;
-  *carry_bytes = chain ? tiles * args->width * 4 : 0;
+  *carry_bytes = t.chain ? t.tiles * args->width * 4 : 0;
   return GEARB_OK;
 }
 

@@ -105,8 +105,10 @@ struct Params {
   gearb_recurrence_args A;
   int64_t rows;
   int64_t tiles;
-  int tile_rows;         // kTile, or the largest multiple of `time` below it when tiles then need nothing from each other
+  int tile_rows;         // kTile (narrow_kernel: more), or the largest multiple of `time` below it when tiles then need
+                         // nothing from each other
   int backward;
+  int narrow_rows;       // rows a thread takes in narrow_kernel; 0: another kernel
   int chain;             // tiles publish to each other
   int per;               // channels per gate
   int blocks_per_gate;   // column blocks of a gate's channels (shared gates)

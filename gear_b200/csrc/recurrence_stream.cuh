@@ -19,6 +19,7 @@
 
 #include <cuda.h>
 
+#include "recurrence_narrow.cuh"
 #include "recurrence_wide.cuh"
 
 namespace gearb {
@@ -940,6 +941,8 @@ int stream_width(const Params &p, bool backward) {
 
 template <typename TX, typename TA>
 int launch_any(Params &p, bool backward, cudaStream_t stream) {
+  if (p.narrow_rows == 16) return launch_narrow<TX, TA, 16>(p, backward, stream);
+  if (p.narrow_rows == 4) return launch_narrow<TX, TA, 4>(p, backward, stream);
   const int v = stream_width<TX, TA>(p, backward);
   const bool shared = p.A.gates < p.A.width;
   if (v == 0) return launch_wide_any<TX, TA>(p, backward, stream);
