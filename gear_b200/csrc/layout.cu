@@ -1,24 +1,50 @@
 // Offsets, block table and slot map of a batch of requests, from their lengths.
 //
-// n_r tokens are added to request r behind the past_r it has.  Two prefix sums over the requests
-// (tokens, new pages) place every request; then every token's slot and every new page's table
-// entry follow from its request alone.  All of it is integer arithmetic in 64 bits.
+// n_r tokens are added to request r behind the past_r it has.  Two prefix sums over the requests (tokens, new pages)
+// place every request; then every token's slot and every new page's table entry follow from its request alone.  All of it
+// is integer arithmetic, in 64 bits where a sum or a slot may need them.
+//
+// What bounds it: writing 8 bytes per token (the slot map); for a decoding step, the launches.
+//   layout_scan_kernel    one CTA, eight requests a thread: up to 8192 requests in one round.
+//   layout_sums_kernel, layout_offsets_kernel   more requests: 4096 a CTA; a CTA adds up the sums before its own.
+//   layout_fill_kernel    every warp takes one stretch of the tokens, looks its first request up once and walks on from
+//                         there: 128 tokens a step, four a lane, while they belong to one request; otherwise 32 a step,
+//                         each lane finding its request among the next 32 offsets, which the warp holds.
+// Up to 8192 requests and 16384 slots the scan and the fill are one launch of one CTA.  Measured: 131072 requests,
+// 65 M tokens: 1950 us with a binary search per token and one CTA's prefix sums.
 #include "common.h"
+#include "warp_search.cuh"
 
 namespace gearb {
 namespace {
 
-constexpr int kThreads = 1024;
+constexpr int kScanThreads = 1024;
+constexpr int kPer = 8;                                // requests a thread
+constexpr int64_t kScanMost = kScanThreads * kPer;
+constexpr int64_t kFusedSlots = 16384;                 // beyond them the fill gets the whole GPU
+constexpr int kBlock = 4096;                           // requests a CTA of the longer way
+constexpr int kFillThreads = 256;
+constexpr int kStep = 128;                             // tokens a warp step
+constexpr unsigned kAll = 0xffffffffu;
 
 struct LayoutParams {
   gearb_layout_args a;
-  int64_t *first_page;  // [requests]: place of the request's first new page in the free list
+  int64_t *first_page;   // [requests]: place of the request's first new page in the free list
+  int64_t *sums;         // [2][blocks]: tokens, then pages; then the pages of all
+  int64_t blocks;
+  int page_shift;        // log2 of the page size, -1: not a power of two
+  int vector;            // the slot map can be written 16 bytes at a time
 };
 
+__device__ __forceinline__ unsigned page_of(const LayoutParams &P, unsigned pos) {
+  return P.page_shift >= 0 ? pos >> P.page_shift : pos / static_cast<unsigned>(P.a.page);
+}
+
 // Tokens the request adds and pages it needs for them.
-__device__ __forceinline__ void request_need(const gearb_layout_args &a, int64_t r, int64_t &past, int64_t &n,
-                                             int64_t &have, int64_t &need, unsigned &flags) {
-  const int64_t room = a.max_blocks * a.page;
+__device__ __forceinline__ void request_need(const LayoutParams &P, int64_t r, int64_t &past, int64_t &n, int64_t &have,
+                                             int64_t &need, unsigned &flags) {
+  const gearb_layout_args &a = P.a;
+  const int64_t room = a.max_blocks * a.page;  // at most 2^31
   past = a.past ? __ldg(a.past + r) : 0;
   if (past < 0 || past > room) {
     past = past < 0 ? 0 : room;
@@ -29,54 +55,76 @@ __device__ __forceinline__ void request_need(const gearb_layout_args &a, int64_t
     n = n < 0 ? 0 : room - past;
     flags |= GEARB_ST_LEN_CLAMPED;
   }
-  have = (past + a.page - 1) / a.page;
-  need = (past + n + a.page - 1) / a.page - have;
+  // ceil(x / page) for x <= 2^31: (x - 1) / page + 1 stays inside 32 bits
+  have = past > 0 ? static_cast<int64_t>(page_of(P, static_cast<unsigned>(past - 1))) + 1 : 0;
+  const int64_t end = past + n;
+  need = (end > 0 ? static_cast<int64_t>(page_of(P, static_cast<unsigned>(end - 1))) + 1 : 0) - have;
 }
 
-__device__ __forceinline__ int64_t warp_inclusive(int64_t v, int lane) {
+// Inclusive sums over the CTA's threads of two values; totals to all.  `sm`: 2 x 32 words.
+__device__ __forceinline__ void block_sums(int64_t &x, int64_t &y, int64_t &tx, int64_t &ty, int64_t (*sm)[32]) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
-    const int64_t u = __shfl_up_sync(0xffffffffu, v, d);
-    if (lane >= d) v += u;
+    const int64_t u = __shfl_up_sync(kAll, x, d), v = __shfl_up_sync(kAll, y, d);
+    if (lane >= d) { x += u; y += v; }
   }
-  return v;
+  if (lane == 31) { sm[0][warp] = x; sm[1][warp] = y; }
+  __syncthreads();
+  int64_t u = lane < warps ? sm[0][lane] : 0, v = lane < warps ? sm[1][lane] : 0;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int64_t s = __shfl_up_sync(kAll, u, d), t = __shfl_up_sync(kAll, v, d);
+    if (lane >= d) { u += s; v += t; }
+  }
+  const int64_t bx = __shfl_sync(kAll, u, warp > 0 ? warp - 1 : 0), by = __shfl_sync(kAll, v, warp > 0 ? warp - 1 : 0);
+  if (warp > 0) { x += bx; y += by; }
+  tx = __shfl_sync(kAll, u, 31);
+  ty = __shfl_sync(kAll, v, 31);
+  __syncthreads();
 }
 
-__global__ void __launch_bounds__(kThreads) layout_scan_kernel(const __grid_constant__ LayoutParams P) {
-  __shared__ int64_t wt[kThreads / 32], wp[kThreads / 32];
+// `per` requests a thread from r0 on, in front of them `tokens` tokens and `pages` pages; what follows is added to both.
+template <int kRequests>
+__device__ __forceinline__ void place_requests(const LayoutParams &P, int64_t r0, int64_t end, int64_t &tokens, int64_t &pages,
+                                               unsigned &flags, int64_t (*sm)[32]) {
   const gearb_layout_args &a = P.a;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int64_t tokens = 0, used = *a.used_in;
-  if (used < 0) used = 0;
-  unsigned flags = 0;
-  for (int64_t r0 = 0; r0 < a.requests; r0 += kThreads) {
-    const int64_t r = r0 + threadIdx.x;
-    int64_t past, n = 0, have, need = 0;
-    if (r < a.requests) request_need(a, r, past, n, have, need, flags);
-    const int64_t it = warp_inclusive(n, lane), ip = warp_inclusive(need, lane);
-    if (lane == 31) { wt[warp] = it; wp[warp] = ip; }
-    __syncthreads();
-    int64_t bt = tokens, bp = used;
-    for (int w = 0; w < kThreads / 32; ++w) {
-      if (w < warp) { bt += wt[w]; bp += wp[w]; }
-      tokens += wt[w];
-      used += wp[w];
-    }
-    if (r < a.requests) {
-      a.offsets[r] = bt + it - n;
-      P.first_page[r] = bp + ip - need;
-    }
-    __syncthreads();
+  int64_t n[kRequests], need[kRequests], x = 0, y = 0, tx, ty;
+  const int64_t r = r0 + static_cast<int64_t>(threadIdx.x) * kRequests;
+#pragma unroll
+  for (int k = 0; k < kRequests; ++k) {
+    n[k] = need[k] = 0;
+    int64_t past, have;
+    if (r + k < end) request_need(P, r + k, past, n[k], have, need[k], flags);
+    x += n[k];
+    y += need[k];
   }
-  if (threadIdx.x == 0) {
-    a.offsets[a.requests] = tokens;
-    if (used > a.num_pages) {
-      used = a.num_pages;
-      flags |= GEARB_ST_NO_PAGE;
+  const int64_t ox = x, oy = y;
+  block_sums(x, y, tx, ty, sm);
+  int64_t t = tokens + x - ox, p = pages + y - oy;
+#pragma unroll
+  for (int k = 0; k < kRequests; ++k)
+    if (r + k < end) {
+      a.offsets[r + k] = t;
+      P.first_page[r + k] = p;
+      t += n[k];
+      p += need[k];
     }
-    *a.used_out = used;
+  tokens += tx;
+  pages += ty;
+}
+
+__device__ __forceinline__ int64_t used_before(const gearb_layout_args &a) {
+  const int64_t u = *a.used_in;
+  return u < 0 ? 0 : u;
+}
+__device__ __forceinline__ void finish_sums(const gearb_layout_args &a, int64_t tokens, int64_t pages, unsigned &flags) {
+  a.offsets[a.requests] = tokens;
+  if (pages > a.num_pages) {
+    pages = a.num_pages;
+    flags |= GEARB_ST_NO_PAGE;
   }
-  if (flags && a.status) atomicOr(reinterpret_cast<unsigned *>(a.status), flags);
+  *a.used_out = pages;
 }
 
 __device__ __forceinline__ int32_t page_at(const gearb_layout_args &a, int64_t k) {
@@ -84,33 +132,205 @@ __device__ __forceinline__ int32_t page_at(const gearb_layout_args &a, int64_t k
   return a.free_pages ? __ldg(a.free_pages + k) : static_cast<int32_t>(k);
 }
 
-// One thread per token: its slot, and the table entry of the page it is the first new token of.
-__global__ void layout_fill_kernel(const __grid_constant__ LayoutParams P) {
+// What placing one request's tokens takes.
+struct Request {
+  int64_t r, first, end;   // its tokens are [first, end) of the batch
+  int64_t past, have, page0;
+};
+__device__ __forceinline__ Request load_request(const LayoutParams &P, int64_t r) {
+  Request q;
+  int64_t n, need;
+  unsigned flags = 0;
+  request_need(P, r, q.past, n, q.have, need, flags);
+  q.r = r;
+  q.first = P.a.offsets[r];
+  q.end = q.first + n;
+  q.page0 = P.first_page[r];
+  return q;
+}
+// Slot of token i; writes the table entry of a page whose first new token it is.
+__device__ __forceinline__ int64_t place_token(const LayoutParams &P, const Request &q, int64_t i) {
+  const gearb_layout_args &a = P.a;
+  const unsigned pos = static_cast<unsigned>(q.past + (i - q.first)), blk = page_of(P, pos);
+  const unsigned in_page = pos - blk * static_cast<unsigned>(a.page);
+  int32_t *entry = a.block_table + q.r * a.max_blocks + blk;
+  const bool fresh = blk >= q.have;
+  const int32_t page = fresh ? page_at(a, q.page0 + (blk - q.have)) : *entry;
+  if (fresh && in_page == 0) *entry = page;
+  return page < 0 ? -1 : static_cast<int64_t>(page) * a.page + in_page;
+}
+
+// Tokens [lo, hi) by one warp.
+__device__ __forceinline__ void fill_stretch(const LayoutParams &P, int64_t total, int64_t lo, int64_t hi, int lane) {
+  const gearb_layout_args &a = P.a;
+  int64_t i = lo;
+  if (i < total && i < hi) {
+    // last request whose offset is <= i: it has this token
+    Request q = load_request(P, warp_upper_bound<int64_t>(a.offsets, 0, a.requests, i, lane, LoadPlain()) - 1);
+    while (i < hi && i < total) {
+      if (i >= q.end) {  // usually among the next 32 requests
+        const int64_t near = q.r + 31 < a.requests ? q.r + 31 : a.requests;
+        q = load_request(P, warp_upper_bound<int64_t>(a.offsets, q.r, a.offsets[near] > i ? near : a.requests, i, lane,
+                                                      LoadPlain()) - 1);
+      }
+      const int64_t stop = i + kStep < hi ? i + kStep : hi;
+      if (stop == i + kStep && stop <= q.end && (stop <= a.max_tokens || i >= a.max_tokens)) {
+        // 128 tokens of one request, four a lane
+        const int64_t t = i + 4 * lane;
+        const unsigned pos = static_cast<unsigned>(q.past + (t - q.first)), blk = page_of(P, pos);
+        const unsigned in_page = pos - blk * static_cast<unsigned>(a.page);
+        int64_t s[4];
+        if (static_cast<int64_t>(in_page) + 3 < a.page) {
+          int32_t *entry = a.block_table + q.r * a.max_blocks + blk;
+          const bool fresh = blk >= q.have;
+          const int32_t page = fresh ? page_at(a, q.page0 + (blk - q.have)) : *entry;
+          if (fresh && in_page == 0) *entry = page;
+          const int64_t base = static_cast<int64_t>(page) * a.page + in_page;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) s[k] = page < 0 ? -1 : base + k;
+        } else {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) s[k] = place_token(P, q, t + k);
+        }
+        if (i >= a.max_tokens) {
+          // rows without an entry: their pages only
+        } else if (P.vector) {
+          longlong2 *to = reinterpret_cast<longlong2 *>(a.slot_map + t);
+          __stcs(to, make_longlong2(s[0], s[1]));
+          __stcs(to + 1, make_longlong2(s[2], s[3]));
+        } else {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) a.slot_map[t + k] = s[k];
+        }
+        i = stop;
+        continue;
+      }
+      // up to 32 tokens of any requests: each lane finds its own among 32 offsets at a time
+      const int64_t t = i + lane;
+      const bool mine = t < hi && t < total;
+      bool settled = !mine;
+      int64_t r = q.r;
+      for (int64_t s = q.r + 1; !__all_sync(kAll, settled); s += 32) {
+        const int64_t b = s + lane <= a.requests ? a.offsets[s + lane] : total + 1;
+        int count = 0;  // offsets of the window at or before this lane's token
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) {
+          const int64_t probe = __shfl_sync(kAll, b, count + d - 1);
+          if (probe <= t) count += d;
+        }
+        const int64_t top = __shfl_sync(kAll, b, 31);
+        if (count == 31 && top <= t) count = 32;
+        if (!settled && count < 32) {
+          settled = true;
+          r = s + count - 1;
+        }
+      }
+      if (mine) {
+        const Request own = r == q.r ? q : load_request(P, r);
+        const int64_t slot = place_token(P, own, t);
+        if (t < a.max_tokens) a.slot_map[t] = slot;
+      }
+      i += 32;
+    }
+  }
+  for (int64_t t = (total > lo ? total : lo) + lane; t < hi; t += 32)  // behind the last token
+    if (t < a.max_tokens) a.slot_map[t] = -1;
+}
+
+// One CTA: the prefix sums, and with kFill everything.
+template <bool kFill>
+__global__ void __launch_bounds__(kScanThreads) layout_scan_kernel(const __grid_constant__ LayoutParams P) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  __shared__ int64_t sm[2][32];
+  const gearb_layout_args &a = P.a;
+  int64_t tokens = 0, pages = used_before(a);
+  unsigned flags = 0;
+  __syncthreads();  // everybody has read used_in: used_out may be the same word
+  if (a.requests <= kScanThreads) place_requests<1>(P, 0, a.requests, tokens, pages, flags, sm);
+  else place_requests<kPer>(P, 0, a.requests, tokens, pages, flags, sm);
+  if (threadIdx.x == 0) finish_sums(a, tokens, pages, flags);
+  if (flags && a.status) atomicOr(reinterpret_cast<unsigned *>(a.status), flags);
+  if constexpr (kFill) {
+    __syncthreads();
+    const int64_t end = tokens > a.max_tokens ? tokens : a.max_tokens;
+    const int64_t each = ((end + 31) / 32 + kStep - 1) / kStep * kStep, lo = (threadIdx.x >> 5) * each;
+    if (lo < end) fill_stretch(P, tokens, lo, lo + each < end ? lo + each : end, threadIdx.x & 31);
+  }
+}
+
+__global__ void __launch_bounds__(kScanThreads) layout_sums_kernel(const __grid_constant__ LayoutParams P) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  __shared__ int64_t sm[2][32];
+  int64_t x = 0, y = 0, tx, ty;
+  unsigned flags = 0;
+  const int64_t r0 = static_cast<int64_t>(blockIdx.x) * kBlock;
+#pragma unroll
+  for (int k = 0; k < kBlock / kScanThreads; ++k) {
+    const int64_t r = r0 + threadIdx.x + k * kScanThreads;
+    int64_t past, n, have, need;
+    if (r < P.a.requests) {
+      request_need(P, r, past, n, have, need, flags);
+      x += n;
+      y += need;
+    }
+  }
+  block_sums(x, y, tx, ty, sm);
+  if (threadIdx.x == 0) {
+    P.sums[blockIdx.x] = tx;
+    P.sums[P.blocks + blockIdx.x] = ty;
+  }
+}
+
+__global__ void __launch_bounds__(kScanThreads) layout_offsets_kernel(const __grid_constant__ LayoutParams P) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  __shared__ int64_t sm[2][32];
+  int64_t x = 0, y = 0, tokens, pages;
+  for (int64_t b = threadIdx.x; b < blockIdx.x; b += kScanThreads) {
+    x += P.sums[b];
+    y += P.sums[P.blocks + b];
+  }
+  block_sums(x, y, tokens, pages, sm);
+  // used_out, which may be the same word, is written by the fill, when all CTAs of this launch have ended
+  pages += used_before(P.a);
+  unsigned flags = 0;
+  const int64_t r0 = static_cast<int64_t>(blockIdx.x) * kBlock, end = r0 + kBlock < P.a.requests ? r0 + kBlock : P.a.requests;
+  place_requests<kBlock / kScanThreads>(P, r0, end, tokens, pages, flags, sm);
+  if (threadIdx.x == 0 && blockIdx.x == gridDim.x - 1) {
+    P.a.offsets[P.a.requests] = tokens;
+    P.sums[2 * P.blocks] = pages;
+  }
+  if (flags && P.a.status) atomicOr(reinterpret_cast<unsigned *>(P.a.status), flags);
+}
+
+__global__ void __launch_bounds__(kFillThreads) layout_fill_kernel(const __grid_constant__ LayoutParams P) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const gearb_layout_args &a = P.a;
   const int64_t total = a.offsets[a.requests];
-  const int64_t end = total > a.max_tokens ? total : a.max_tokens;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < end;
-       i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
-    if (i >= total) {
-      a.slot_map[i] = -1;
-      continue;
-    }
-    int64_t lo = 0, hi = a.requests - 1;  // last request whose offset is <= i: it has this token
-    while (lo < hi) {
-      const int64_t mid = (lo + hi + 1) >> 1;
-      if (a.offsets[mid] <= i) lo = mid;
-      else hi = mid - 1;
-    }
-    const int64_t r = lo;
-    int64_t past, n, have, need;
+  if (P.blocks && blockIdx.x == 0 && threadIdx.x == 0) {
     unsigned flags = 0;
-    request_need(a, r, past, n, have, need, flags);
-    const int64_t pos = past + (i - a.offsets[r]), blk = pos / a.page, in_page = pos - blk * a.page;
-    int32_t *entry = a.block_table + r * a.max_blocks + blk;
-    const int32_t page = blk < have ? *entry : page_at(a, P.first_page[r] + (blk - have));
-    if (blk >= have && in_page == 0) *entry = page;
-    if (i < a.max_tokens) a.slot_map[i] = page < 0 ? -1 : page * a.page + in_page;
+    finish_sums(a, total, P.sums[2 * P.blocks], flags);
+    if (flags && a.status) atomicOr(reinterpret_cast<unsigned *>(a.status), flags);
   }
+  const int64_t end = total > a.max_tokens ? total : a.max_tokens;
+  const int64_t warps = static_cast<int64_t>(gridDim.x) * (kFillThreads / 32);
+  const int64_t each = ((end + warps - 1) / warps + kStep - 1) / kStep * kStep;
+  const int64_t lo = (static_cast<int64_t>(blockIdx.x) * (kFillThreads / 32) + (threadIdx.x >> 5)) * each;
+  if (lo < end) fill_stretch(P, total, lo, lo + each < end ? lo + each : end, threadIdx.x & 31);
+}
+
+int launch_after(void (*kernel)(LayoutParams), unsigned grid, unsigned threads, const LayoutParams &p, cudaStream_t stream) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  GEARB_CUDA(cudaLaunchKernelEx(&cfg, kernel, p));
+  return GEARB_OK;
 }
 
 }  // namespace
@@ -120,7 +340,9 @@ using namespace gearb;
 
 extern "C" {
 
-int64_t gearb_layout_scratch_bytes(int64_t requests) { return requests > 0 ? requests * 8 : 0; }
+int64_t gearb_layout_scratch_bytes(int64_t requests) {
+  return requests > 0 ? requests * 8 + 16 * ((requests + kBlock - 1) / kBlock) + 8 : 0;
+}
 
 int gearb_layout_paged(const gearb_layout_args *args, void *stream) {
   TraceRange trace("gearb:layout");
@@ -130,7 +352,7 @@ int gearb_layout_paged(const gearb_layout_args *args, void *stream) {
   const gearb_layout_args &a = p.a;
   GEARB_REQUIRE(a.requests >= 0 && a.max_tokens >= 0 && a.num_pages >= 0, "layout: negative size");
   GEARB_REQUIRE(a.page > 0 && a.max_blocks > 0, "layout: page and max_blocks must be positive");
-  // keeps every sum of lengths inside 64 bits
+  // keeps positions in 32 bits and every sum of lengths inside 64
   GEARB_REQUIRE(a.page <= (int64_t(1) << 31) / a.max_blocks && a.requests < (int64_t(1) << 31) &&
                     a.num_pages <= (int64_t(1) << 31),
                 "layout: page * max_blocks, requests and num_pages are limited to 2^31");
@@ -140,11 +362,28 @@ int gearb_layout_paged(const gearb_layout_args *args, void *stream) {
   GEARB_REQUIRE(a.scratch_bytes >= gearb_layout_scratch_bytes(a.requests) && (a.requests == 0 || a.scratch),
                 "layout: scratch of %lld bytes needed", (long long)gearb_layout_scratch_bytes(a.requests));
   p.first_page = static_cast<int64_t *>(a.scratch);
-  layout_scan_kernel<<<1, kThreads, 0, as_stream(stream)>>>(p);
-  GEARB_CUDA(cudaGetLastError());
-  layout_fill_kernel<<<sm_count() * 8, 256, 0, as_stream(stream)>>>(p);
-  GEARB_CUDA(cudaGetLastError());
-  return GEARB_OK;
+  p.blocks = a.requests > kScanMost ? (a.requests + kBlock - 1) / kBlock : 0;
+  p.sums = p.first_page + a.requests;
+  p.page_shift = -1;
+  for (int s = 0; s <= 31; ++s)
+    if (a.page == int64_t(1) << s) p.page_shift = s;
+  p.vector = reinterpret_cast<uintptr_t>(a.slot_map) % 16 == 0;
+  cudaStream_t st = as_stream(stream);
+  if (p.blocks == 0) {
+    if (a.max_tokens > 0 && a.max_tokens <= kFusedSlots) {
+      layout_scan_kernel<true><<<1, kScanThreads, 0, st>>>(p);
+      GEARB_CUDA(cudaGetLastError());
+      return GEARB_OK;
+    }
+    layout_scan_kernel<false><<<1, kScanThreads, 0, st>>>(p);
+    GEARB_CUDA(cudaGetLastError());
+  } else {
+    layout_sums_kernel<<<static_cast<unsigned>(p.blocks), kScanThreads, 0, st>>>(p);
+    GEARB_CUDA(cudaGetLastError());
+    const int rc = launch_after(layout_offsets_kernel, static_cast<unsigned>(p.blocks), kScanThreads, p, st);
+    if (rc != GEARB_OK) return rc;
+  }
+  return launch_after(layout_fill_kernel, static_cast<unsigned>(sm_count() * 8), kFillThreads, p, st);
 }
 
 }  // extern "C"
