@@ -129,7 +129,7 @@ struct GatherColumn {
   int32_t chunk_first; // first chunk id of this column inside a request
   int32_t chunk_count; // chunks this column's slot is cut into
   int32_t stage_off;   // byte offset of this column's staging area in shared memory
-  int32_t reserved;
+  int32_t reserved;    // gather_packed: pieces of a page's run
 };
 
 struct GatherParams {
@@ -208,6 +208,10 @@ struct PackedDst {
   int64_t max_blocks, page;
   const int64_t *past;          // may be null
   int64_t dst_rows[GEARB_MAX_COLUMNS];  // by position in GatherParams::cols
+  // set by launch_gather_packed
+  int64_t room;         // rows a request's pages hold
+  int32_t page_shift;   // log2 of page, -1 if it is no power of two
+  int32_t big;          // columns copied in runs, in front of the others
 };
 int launch_gather_packed(const GatherParams &p, const PackedDst &d, cudaStream_t stream);
 int launch_segment_lengths(const GatherParams &p, int64_t *out, cudaStream_t stream);

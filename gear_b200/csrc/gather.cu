@@ -84,60 +84,154 @@ __global__ void segment_lengths_kernel(const __grid_constant__ GatherParams P, i
   out[i] = rows;
 }
 
-// Packed / paged gather: one warp moves one 2 KiB piece of a request's column, cut at the page
-// boundaries that fall into it.
-__global__ void __launch_bounds__(kThreads) gather_packed_kernel(const __grid_constant__ GatherParams P,
-                                                                 const __grid_constant__ PackedDst D) {
-  const int lane = threadIdx.x & 31;
-  const int64_t warps_total = static_cast<int64_t>(gridDim.x) * kWarpsPerBlock;
-  const int64_t items = P.n * P.chunks_per_request;
-  unsigned flags = 0;
-  for (int64_t item = static_cast<int64_t>(blockIdx.x) * kWarpsPerBlock + (threadIdx.x >> 5); item < items;
-       item += warps_total) {
-    const int64_t g = item / P.chunks_per_request;
-    const int q = static_cast<int>(item - g * P.chunks_per_request);
-    const int ci = dev::column_of_piece(P, q);
-    const GatherColumn &col = P.cols[ci];
-    const int64_t idx = __ldg(P.idx + g), o0 = __ldg(D.offsets + g), o1 = __ldg(D.offsets + g + 1);
-    int64_t start, bytes;
-    dev::clip_segment(P, col, idx, __ldg(P.ts + g), __ldg(P.len + g), start, bytes, flags);
-    const int64_t row = col.row;
-    if (o0 < 0 || o1 <= o0) {
-      if (o0 < 0) flags |= GEARB_ST_BAD_REQUEST;
-      continue;
-    }
-    if (bytes / row > o1 - o0) bytes = (o1 - o0) * row;
-    const int64_t c0 = static_cast<int64_t>(q - col.chunk_first) * P.chunk_bytes;
-    const int64_t c1 = c0 + P.chunk_bytes < bytes ? c0 + P.chunk_bytes : bytes;
-    if (c1 <= c0) continue;
-    const uint8_t *src = dev::segment_src(P, col, idx, start, P.table);
-    if (!D.block_table) {
-      // bytes of the piece that lie inside the destination
-      const int64_t left = o0 < D.dst_rows[ci] ? (D.dst_rows[ci] - o0) * row : 0;
-      if (c1 > left) flags |= GEARB_ST_BAD_REQUEST;
-      const int64_t b = c1 < left ? c1 : left;
-      if (b > c0) dev::warp_copy(col.dst + o0 * row + c0, src + c0, static_cast<int>(b - c0), lane);
-      continue;
-    }
-    const int64_t past = D.past ? __ldg(D.past + g) : 0;
-    if (past < 0 || past > D.max_blocks * D.page) {
-      flags |= GEARB_ST_BAD_REQUEST;
-      continue;
-    }
-    for (int64_t c = c0; c < c1;) {
-      const int64_t t = c / row, pos = past + t, blk = pos / D.page;
-      const int64_t in_page = pos - blk * D.page;
-      int64_t e = (t + D.page - in_page) * row;  // first byte of the next page
-      if (e > c1) e = c1;
-      const int64_t page = blk < D.max_blocks ? __ldg(D.block_table + g * D.max_blocks + blk) : -1;
-      const int64_t slot = page * D.page + in_page;  // row of t; (c - t * row) bytes of it went before
-      const int64_t rows = (e - 1) / row - t + 1;
-      if (page < 0 || slot + rows > D.dst_rows[ci]) flags |= GEARB_ST_BAD_REQUEST;
-      else dev::warp_copy(col.dst + slot * row + (c - t * row), src + c, static_cast<int>(e - c), lane);
-      c = e;
+// Packed / paged gather.
+//
+// A CTA takes a request (or a slice of one, where the requests are few): its indexes are looked up once, and its warps
+// share its rows out.  Packed rows of a column are one run of bytes; so are the rows of a page.  Columns that are
+// packed, or have 64 bytes a row or 512 a page, go in pieces of at most 4 KiB of a run.  The smaller columns of a paged
+// request go together, 64 rows a warp, a row a lane, each row's slot looked up once for all of them: a page's run of
+// them would occupy a few lanes only.  Bound by memory: 2 x bytes; what it takes is many warps with few registers.
+// Measured on 8192 requests of config 3's rows in pages of 16 (118 us at the copy rate): a warp per 2 KiB of any
+// column, a page's run at a time, 2180 us; a warp per piece of some request, with four 16-byte blocks a lane in
+// flight, 340 to 750 us, faster with fewer registers than with fewer spills.
+constexpr int kPackedPiece = 4096;
+
+__device__ __forceinline__ void copy_run(uint8_t *d, const uint8_t *s, int nbytes, int lane) {
+  int head = static_cast<int>((16u - (reinterpret_cast<uintptr_t>(d) & 15u)) & 15u);
+  if (head > nbytes) head = nbytes;
+  if (lane < head) d[lane] = s[lane];
+  d += head;
+  s += head;
+  nbytes -= head;
+  const int nvec = nbytes >> 4;
+  const unsigned sh = static_cast<unsigned>(reinterpret_cast<uintptr_t>(s) & 15u);
+  uint4 *dv = reinterpret_cast<uint4 *>(d);
+  // two aligned blocks hold a block of the destination, where the source is not aligned like it
+  const uint4 *sv = reinterpret_cast<const uint4 *>(s - sh);
+  const unsigned ws = sh >> 2, bs = (sh & 3u) * 8u;
+#pragma unroll 2
+  for (int v = lane; v < nvec; v += 32) {
+    const uint4 a = __ldg(sv + v);
+    if (sh == 0) {
+      dv[v] = a;
+    } else {
+      const uint4 b = __ldg(sv + v + 1);
+      dv[v] = dev::shift_pair(a, b, ws, bs);
     }
   }
-  if (flags && P.status && lane == 0) atomicOr(reinterpret_cast<unsigned *>(P.status), flags);
+  const int done = nvec << 4;
+  if (lane < nbytes - done) d[done + lane] = s[done + lane];
+}
+
+template <typename U>
+__device__ __forceinline__ void copy_rows(uint8_t *dst, const uint8_t *src, int row, int64_t s0, int64_t s1, int lane) {
+  src += lane * row;
+  for (int c = 0; c < row; c += static_cast<int>(sizeof(U))) {
+    U a, b;
+    if (s0 >= 0) a = __ldg(reinterpret_cast<const U *>(src + c));
+    if (s1 >= 0) b = __ldg(reinterpret_cast<const U *>(src + 32 * row + c));
+    if (s0 >= 0) *reinterpret_cast<U *>(dst + s0 * row + c) = a;
+    if (s1 >= 0) *reinterpret_cast<U *>(dst + s1 * row + c) = b;
+  }
+}
+
+__global__ void __launch_bounds__(kThreads, 6) gather_packed_kernel(const __grid_constant__ GatherParams P,
+                                                                    const __grid_constant__ PackedDst D) {
+  const int lane = threadIdx.x & 31;
+  const int64_t g = blockIdx.x;
+  unsigned flags = 0;
+  const int64_t idx = __ldg(P.idx + g), o0 = __ldg(D.offsets + g), o1 = __ldg(D.offsets + g + 1);
+  const int64_t past = D.past ? __ldg(D.past + g) : 0;
+  int64_t start, count64;
+  {
+    GatherColumn rows_of = {};  // the columns share one pattern: the clipped segment in rows
+    rows_of.row = 1;
+    rows_of.pat_offset = P.cols[0].pat_offset;
+    rows_of.pat_length = P.cols[0].pat_length;
+    dev::clip_segment(P, rows_of, idx, __ldg(P.ts + g), __ldg(P.len + g), start, count64, flags);
+  }
+  if (o0 < 0 || past < 0 || past > D.room) {
+    flags |= GEARB_ST_BAD_REQUEST;
+    count64 = 0;
+  } else if (count64 > o1 - o0) {
+    count64 = o1 > o0 ? o1 - o0 : 0;
+  }
+  const int count = static_cast<int>(count64);  // at most the pattern's length
+  const uint8_t *base = P.table + idx * P.traj_stride;
+  // positions are at most 2^31 + the pattern's length
+  auto block_of = [&](uint64_t pos) -> uint64_t {
+    if (D.page_shift >= 0) return pos >> D.page_shift;
+    if ((pos >> 32) == 0) return static_cast<unsigned>(pos) / static_cast<unsigned>(D.page);
+    return pos / static_cast<uint64_t>(D.page);
+  };
+  auto page_at = [&](uint64_t blk) -> int64_t {
+    return blk < static_cast<uint64_t>(D.max_blocks) ? __ldg(D.block_table + g * D.max_blocks + static_cast<int64_t>(blk)) : -1;
+  };
+  const uint64_t blk0 = D.block_table ? block_of(static_cast<uint64_t>(past)) : 0;
+  const int in0 = D.block_table ? static_cast<int>(past - static_cast<int64_t>(blk0) * D.page) : 0;
+  // runs a column's rows make, and 64-row groups of the small columns
+  const int runs = count == 0 ? 0 : !D.block_table ? 1 : static_cast<int>(block_of(static_cast<uint64_t>(in0) + count - 1)) + 1;
+  const int first = static_cast<int>(blockIdx.y) * kWarpsPerBlock + (threadIdx.x >> 5);
+  const int step = static_cast<int>(gridDim.y) * kWarpsPerBlock;
+  int at = first;  // this warp's next piece, counted from the current column's first
+  for (int ci = 0; ci < D.big; ++ci) {
+    const GatherColumn &col = P.cols[ci];
+    const int row = col.row;
+    const int64_t limit = D.dst_rows[ci];
+    const uint8_t *src = base + col.col_offset + start * row;
+    const int pieces = col.reserved ? col.reserved : static_cast<int>((static_cast<int64_t>(count) * row + kPackedPiece - 1) / kPackedPiece);
+    const int64_t total = static_cast<int64_t>(runs) * pieces;
+    int64_t k = at;
+    for (; k < total; k += step) {
+      const int run = static_cast<int>(k / pieces), piece = static_cast<int>(k - static_cast<int64_t>(run) * pieces);
+      int64_t t = 0, rows = count, slot = o0;
+      if (D.block_table) {
+        const int64_t page = page_at(blk0 + run), in = run == 0 ? in0 : 0;
+        t = run == 0 ? 0 : static_cast<int64_t>(run) * D.page - in0;
+        rows = D.page - in < count - t ? D.page - in : count - t;
+        slot = page < 0 ? limit : page * D.page + in;
+      }
+      int64_t n = slot < limit ? limit - slot : 0;  // rows inside the destination
+      if (n < rows) flags |= GEARB_ST_BAD_REQUEST;
+      else n = rows;
+      const int64_t b0 = static_cast<int64_t>(piece) * kPackedPiece, b1 = n * row < b0 + kPackedPiece ? n * row : b0 + kPackedPiece;
+      if (b1 > b0) copy_run(col.dst + slot * row + b0, src + t * row + b0, static_cast<int>(b1 - b0), lane);
+    }
+    at = static_cast<int>(k - total);
+  }
+  if (D.big == P.ncols) {
+    if (flags && P.status) atomicOr(reinterpret_cast<unsigned *>(P.status), flags);
+    return;
+  }
+  for (int64_t t = static_cast<int64_t>(at) * 64; t < count; t += static_cast<int64_t>(step) * 64) {
+    int64_t slot[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int64_t r = t + 32 * k + lane;
+      slot[k] = -1;
+      if (r >= count) continue;
+      const uint64_t pos = static_cast<uint64_t>(past + r), blk = block_of(pos);
+      const int64_t page = page_at(blk);
+      if (page >= 0) slot[k] = page * D.page + static_cast<int64_t>(pos - blk * D.page);
+      else flags |= GEARB_ST_BAD_REQUEST;
+    }
+    for (int c = D.big; c < P.ncols; ++c) {
+      const GatherColumn &col = P.cols[c];
+      const int64_t limit = D.dst_rows[c];
+      int64_t s0 = slot[0], s1 = slot[1];
+      if (s0 >= limit || s1 >= limit) flags |= GEARB_ST_BAD_REQUEST;
+      if (s0 >= limit) s0 = -1;
+      if (s1 >= limit) s1 = -1;
+      const uint8_t *from = base + col.col_offset + (start + t) * col.row;
+      const uintptr_t bits = reinterpret_cast<uintptr_t>(from) | reinterpret_cast<uintptr_t>(col.dst) |
+                             static_cast<uintptr_t>(col.row);
+      if ((bits & 7) == 0) copy_rows<uint2>(col.dst, from, col.row, s0, s1, lane);
+      else if ((bits & 3) == 0) copy_rows<unsigned>(col.dst, from, col.row, s0, s1, lane);
+      else if ((bits & 1) == 0) copy_rows<unsigned short>(col.dst, from, col.row, s0, s1, lane);
+      else copy_rows<unsigned char>(col.dst, from, col.row, s0, s1, lane);
+    }
+  }
+  if (flags && P.status) atomicOr(reinterpret_cast<unsigned *>(P.status), flags);
 }
 
 int grid_for(int64_t items) {
@@ -166,8 +260,42 @@ int launch_segment_lengths(const GatherParams &p, int64_t *out, cudaStream_t str
   return GEARB_OK;
 }
 
-int launch_gather_packed(const GatherParams &p, const PackedDst &d, cudaStream_t stream) {
-  gather_packed_kernel<<<grid_for(p.n * p.chunks_per_request), kThreads, 0, stream>>>(p, d);
+int launch_gather_packed(const GatherParams &params, const PackedDst &dst, cudaStream_t stream) {
+  GatherParams p = params;
+  PackedDst d = dst;
+  d.page_shift = -1;
+  for (int s = 0; s < 32; ++s)
+    if (d.page == int64_t(1) << s) d.page_shift = s;
+  d.room = d.block_table ? d.max_blocks * d.page : 0;
+  auto small = [&](const GatherColumn &c) { return d.block_table && c.row < 64 && c.row * d.page < 512; };
+  // the columns that are copied in runs first
+  d.big = 0;
+  int at = 0;
+  for (int pass = 0; pass < 2; ++pass)
+    for (int c = 0; c < params.ncols; ++c)
+      if (small(params.cols[c]) == (pass == 1)) {
+        p.cols[at] = params.cols[c];
+        d.dst_rows[at++] = dst.dst_rows[c];
+        if (pass == 0) ++d.big;
+      }
+  int64_t pieces = 1;  // of a request of the pattern's length
+  for (int c = 0; c < p.ncols; ++c) {
+    GatherColumn &col = p.cols[c];
+    const int64_t of_run = (d.page * col.row + kPackedPiece - 1) / kPackedPiece;
+    GEARB_REQUIRE(static_cast<int64_t>(col.pat_length) * col.row < (int64_t(1) << 40) && of_run < (int64_t(1) << 31),
+                  "gather_packed: request too large");
+    col.reserved = d.block_table ? static_cast<int32_t>(of_run) : 0;  // pieces of a page's run; packed: by the request's rows
+    if (c >= d.big) pieces += (col.pat_length + 63) / 64 / (p.ncols - d.big);
+    else if (d.block_table) pieces += ((col.pat_length - 1) / d.page + 2) * of_run;
+    else pieces += (static_cast<int64_t>(col.pat_length) * col.row + kPackedPiece - 1) / kPackedPiece;
+  }
+  GEARB_REQUIRE(p.n < (int64_t(1) << 31) && pieces < (int64_t(1) << 31), "gather_packed: request too large");
+  // Slices: enough CTAs for the GPU where the requests alone are too few, but no CTA without a piece for its warps.
+  const int64_t want = (static_cast<int64_t>(sm_count()) * 12 + p.n - 1) / p.n;
+  int64_t slices = (pieces + kWarpsPerBlock - 1) / kWarpsPerBlock;
+  if (slices > want) slices = want;
+  if (slices > 65535) slices = 65535;
+  gather_packed_kernel<<<dim3(static_cast<unsigned>(p.n), static_cast<unsigned>(slices < 1 ? 1 : slices)), kThreads, 0, stream>>>(p, d);
   GEARB_CUDA(cudaGetLastError());
   return GEARB_OK;
 }
