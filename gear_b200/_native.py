@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -210,6 +211,11 @@ class LayoutArgs(C.Structure):
                 ("block_table", vp), ("free_pages", vp), ("num_pages", i64), ("used_in", vp), ("used_out", vp),
                 ("offsets", vp), ("slot_map", vp), ("max_tokens", i64), ("scratch", vp), ("scratch_bytes", i64),
                 ("status", vp)]
+
+
+# The same layouts for struct.pack: filling a ctypes structure field by field takes several times as long.
+LAYOUT_ARGS = struct.Struct("@PPqqqPPqPPPPqPqP")
+RECURRENCE_ARGS = struct.Struct("@PPii8qPPqPiiiPPPPqqPPPPPqP")
 
 
 class RecurrenceArgs(C.Structure):

@@ -8,7 +8,6 @@ CpuTrajectoryStorageHandler, Indexset; src/storage, include/index/set.h).
 from __future__ import annotations
 
 import ctypes as C
-from contextlib import nullcontext
 from dataclasses import dataclass
 from typing import Optional, Sequence
 
@@ -45,13 +44,29 @@ def _stream(stream=None) -> C.c_void_p:
     return C.c_void_p(stream.cuda_stream if hasattr(stream, "cuda_stream") else int(stream))
 
 
-def _stream_scope(stream):
-    """Context in which torch allocates for, and _stream() returns, the given stream (None: the current one)."""
-    if stream is None:
-        return nullcontext()
-    if not hasattr(stream, "cuda_stream"):
-        stream = torch.cuda.ExternalStream(int(stream))
-    return torch.cuda.stream(stream)
+class _Scope:
+    """Context in which torch allocates on, and _stream() returns a stream of, the given device: the given stream,
+    or (None) that device's current one.  Costs nothing where both are current already."""
+
+    def __init__(self, device: torch.device, stream=None):
+        self._inner = None
+        if stream is not None:
+            if not hasattr(stream, "cuda_stream"):
+                with torch.cuda.device(device):
+                    stream = torch.cuda.ExternalStream(int(stream))
+            elif stream.device != device:
+                raise GearError(N.ERR_INVALID, f"the stream is on {stream.device}, the tensors on {device}")
+            self._inner = torch.cuda.stream(stream)
+        elif _RAW_DEVICE is None or _RAW_DEVICE() != device.index:
+            self._inner = torch.cuda.device(device)
+
+    def __enter__(self):
+        if self._inner is not None:
+            self._inner.__enter__()
+
+    def __exit__(self, *exc):
+        if self._inner is not None:
+            self._inner.__exit__(*exc)
 
 
 def _dev_i64(t: torch.Tensor, what: str) -> C.c_void_p:
@@ -263,7 +278,7 @@ class StorageHandler:
         if out is not None and out.numel() != n:
             raise GearError(N.ERR_INVALID, "out must have one entry per request")
         ptrs = [_dev_i64(t, w) for t, w in ((idx, "idx"), (ts, "ts"), (ln, "len"))]
-        with torch.cuda.device(idx.device), _stream_scope(stream):
+        with _Scope(idx.device, stream):
             if out is None:
                 out = torch.empty(n, dtype=torch.int64, device=idx.device)
             call("gearb_handler_segment_lengths", self._h, int(column), *ptrs, n, _dev_i64(out, "out"), _stream())
@@ -314,13 +329,12 @@ class StorageHandler:
         if n == 0 or nc == 0:
             return
         st = self.status_tensor(idx.device)
-        with torch.cuda.device(idx.device):
+        with _Scope(idx.device, stream):
             call("gearb_handler_gather_packed", self._h, (C.c_int32 * nc)(*[int(c) for c in columns]), nc,
                  _dev_i64(idx, "idx"), _dev_i64(ts, "ts"), _dev_i64(ln, "len"), n, _dev_i64(offsets, "offsets"),
                  _ptr(bt), max_blocks, int(page), None if past is None else _dev_i64(past, "past"),
                  (C.c_void_p * nc)(*[d.data_ptr() or idx.data_ptr() for d in dsts]),   # 0 rows: never written
-                 (C.c_int64 * nc)(*rows), _ptr(st),
-                 _stream(stream))
+                 (C.c_int64 * nc)(*rows), _ptr(st), _stream())
 
     def view(self, index: int, column: int) -> np.ndarray:
         """Host bytes of one column of one trajectory (handler.cc:223-233)."""

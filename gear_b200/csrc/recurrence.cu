@@ -142,6 +142,55 @@ __global__ void __launch_bounds__(kThreads) prepare_kernel(const __grid_constant
   }
 }
 
+// One row a sequence, as in decoding: nothing to hand on, so every thread takes V channels of one row.  Bound by the
+// launch for the usual sizes, by memory for large ones.
+template <typename TX, typename TA, int V>
+__global__ void __launch_bounds__(kThreads) step_kernel(const __grid_constant__ Params P) {
+  const gearb_recurrence_args &A = P.A;
+  const int64_t per_row = (A.width + V - 1) / V, n = A.batch * per_row;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < n;
+       i += static_cast<int64_t>(gridDim.x) * kThreads) {
+    const int64_t b = quotient(i, per_row), d = (i - b * per_row) * V;
+    const TA *gate = static_cast<const TA *>(A.gate) + b * A.gate_batch_stride;
+    float x[V], a[V], h[V];
+    const Pack<TX, V> px = load_pack<TX, V>(static_cast<const TX *>(A.x) + b * A.x_batch_stride + d);
+#pragma unroll
+    for (int v = 0; v < V; ++v) x[v] = to_f(px.v[v]);
+    if (P.per == 1) {
+      const Pack<TA, V> pg = load_pack<TA, V>(gate + d);
+#pragma unroll
+      for (int v = 0; v < V; ++v) a[v] = to_f(pg.v[v]);
+    } else {
+#pragma unroll
+      for (int v = 0; v < V; ++v) a[v] = to_f(gate[(d + v) / P.per]);
+    }
+    if (A.h0) {
+      const Pack<float, V> p0 = load_pack<float, V>(A.h0 + b * A.width + d);
+#pragma unroll
+      for (int v = 0; v < V; ++v) h[v] = fmaf(A.gate_log ? exp_of(a[v]) : a[v], p0.v[v], x[v]);
+    } else {
+#pragma unroll
+      for (int v = 0; v < V; ++v) h[v] = x[v];
+    }
+    store_pack<TX, V>(static_cast<TX *>(A.out) + b * A.width + d, h);
+    if (A.state_out) store_pack<float, V>(A.state_out + b * A.width + d, h);
+  }
+}
+template <typename TX, typename TA>
+int launch_step(const Params &p, cudaStream_t stream) {
+  const gearb_recurrence_args &a = p.A;
+  const bool four = a.width % 4 == 0 && vector_ok(a.x, a.x_batch_stride, 0, sizeof(TX), 4) &&
+                    vector_ok(a.out, 0, 0, sizeof(TX), 4) && vector_ok(a.h0, 0, 0, 4, 4) && vector_ok(a.state_out, 0, 0, 4, 4) &&
+                    (p.per > 1 || vector_ok(a.gate, a.gate_batch_stride, 0, sizeof(TA), 4));
+  const int64_t n = a.batch * (four ? a.width / 4 : a.width), blocks = (n + kThreads - 1) / kThreads;
+  const int64_t most = static_cast<int64_t>(sm_count()) * 64;
+  const unsigned grid = static_cast<unsigned>(blocks < most ? blocks : most);
+  if (four) step_kernel<TX, TA, 4><<<grid, kThreads, 0, stream>>>(p);
+  else step_kernel<TX, TA, 1><<<grid, kThreads, 0, stream>>>(p);
+  GEARB_CUDA(cudaGetLastError());
+  return GEARB_OK;
+}
+
 // ---- host -------------------------------------------------------------------
 int64_t up256(int64_t v) { return (v + 255) / 256 * 256; }
 
@@ -241,6 +290,12 @@ int launch(const gearb_recurrence_args &a, bool backward, cudaStream_t stream) {
     return GEARB_OK;
   }
   p.per = static_cast<int>(a.width / a.gates);
+  if (!backward && a.time == 1 && !a.offsets && !a.lengths) {
+    const bool own = a.gate_dtype == a.x_dtype;
+    if (a.x_dtype == GEARB_DT_F32) return launch_step<float, float>(p, stream);
+    if (a.x_dtype == GEARB_DT_F16) return own ? launch_step<__half, __half>(p, stream) : launch_step<__half, float>(p, stream);
+    return own ? launch_step<__nv_bfloat16, __nv_bfloat16>(p, stream) : launch_step<__nv_bfloat16, float>(p, stream);
+  }
   const Scratch s = scratch_of(a, backward);
   if (p.chain) {
     char *base = static_cast<char *>(a.scratch);

@@ -57,8 +57,9 @@ __device__ __forceinline__ GroupRows group_rows_dense(const gearb_recurrence_arg
   return g;
 }
 
-// The sequence of a live row.
-__device__ __forceinline__ int64_t sequence_of(const gearb_recurrence_args &A, int64_t rows, int64_t i) {
+// The sequence of a live row.  Called where a sequence starts or ends and has a state; out of line, as it would stand in
+// the code for every row a thread has.
+static __device__ __noinline__ int64_t sequence_of(const gearb_recurrence_args &A, int64_t rows, int64_t i) {
   if (!A.offsets) {
     const int64_t b = quotient(i, A.time);
     return A.reverse ? A.batch - 1 - b : b;
@@ -125,25 +126,70 @@ __device__ __forceinline__ GroupRows group_rows_packed(const Params &P, const Na
   return g;
 }
 
-// Copies a tile's rows of one tensor into (or out of) shared memory, in memory order; f(word, element offset).
-template <typename F>
-__device__ __forceinline__ void each_value(const Params &P, int64_t i0, int n, const NarrowLayout &lay, int k, int64_t period,
-                                           int64_t sb, int64_t sr, F f) {
-  const int total = n * lay.w;
-  const int64_t row_low = P.A.reverse ? P.rows - i0 - n : i0;  // matrix row of the first value in memory order
-  const unsigned magic = (0x10000u + lay.w - 1) / lay.w;       // e / w for e < 4096, w <= 16
-  const int64_t first = quotient(row_low, period);
-  const bool flat = row_low - first * period + n <= period;
-  const int64_t base = first * sb + (row_low - first * period) * sr;
-  for (int e = threadIdx.x; e < total; e += kThreads) {
-    const int r = static_cast<int>((static_cast<unsigned>(e) * magic) >> 16), c = e - r * lay.w;
-    const int scan = P.A.reverse ? n - 1 - r : r, g = scan / k;
-    int64_t at = base + r * sr;
-    if (!flat) {
-      const int64_t b = quotient(row_low + r, period);
-      at = b * sb + (row_low + r - b * period) * sr;
+// Where the values of a tile's rows of one tensor lie, in memory order.
+struct NarrowWalk {
+  int n, w, k, stride, reverse;
+  unsigned magic;  // e / w for e < 4096, w <= 16
+  bool flat;       // one row stride
+  int64_t row_low, base, period, sb, sr;
+  __device__ __forceinline__ NarrowWalk(const Params &P, int64_t i0, int n_, const NarrowLayout &lay, int k_, int64_t period_,
+                                        int64_t sb_, int64_t sr_)
+      : n(n_), w(lay.w), k(k_), stride(lay.stride), reverse(P.A.reverse), period(period_), sb(sb_), sr(sr_) {
+    row_low = reverse ? P.rows - i0 - n : i0;  // matrix row of the first value
+    magic = (0x10000u + w - 1) / w;
+    const int64_t first = quotient(row_low, period);
+    flat = row_low - first * period + n <= period;
+    base = first * sb + (row_low - first * period) * sr;
+  }
+  // Value e: its word in shared memory, its row in scan order and its place in the row.
+  __device__ __forceinline__ int word(int e, int &scan, int &c) const {
+    const int r = static_cast<int>((static_cast<unsigned>(e) * magic) >> 16);
+    c = e - r * w;
+    scan = reverse ? n - 1 - r : r;
+    const int g = scan / k;
+    return g * stride + (scan - g * k) * w + c;
+  }
+  // Its element in memory.
+  __device__ __forceinline__ int64_t element(int e) const {
+    const int r = static_cast<int>((static_cast<unsigned>(e) * magic) >> 16), c = e - r * w;
+    if (flat) return base + r * sr + c;
+    const int64_t b = quotient(row_low + r, period);
+    return b * sb + (row_low + r - b * period) * sr + c;
+  }
+};
+
+// Rows into shared memory: 16-byte (or 8-byte) loads where the values follow one another, several loads in flight.
+template <typename T, typename F>
+__device__ __forceinline__ void load_values(const T *p, const NarrowWalk &m, float *to, F f) {
+  const int total = m.n * m.w;
+  int scan, c;
+  if (m.flat && m.sr == m.w && reinterpret_cast<uintptr_t>(p + m.base) % (4 * sizeof(T)) == 0) {
+    for (int e0 = 4 * threadIdx.x; e0 < total; e0 += 4 * 4 * kThreads) {
+      Pack<T, 4> v[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (e0 + 4 * u * kThreads + 3 < total) v[u] = load_pack<T, 4>(p + m.base + e0 + 4 * u * kThreads);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int e = e0 + 4 * u * kThreads;
+        if (e + 3 < total) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) to[m.word(e + q, scan, c)] = f(to_f(v[u].v[q]));
+        } else {
+          for (int q = e; q < total; ++q) to[m.word(q, scan, c)] = f(to_f(p[m.base + q]));
+        }
+      }
     }
-    f(g * lay.stride + (scan - g * k) * lay.w + c, at + c, scan, c);
+    return;
+  }
+  for (int e0 = threadIdx.x; e0 < total; e0 += 8 * kThreads) {
+    T v[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+      if (e0 + u * kThreads < total) v[u] = p[m.element(e0 + u * kThreads)];
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+      if (e0 + u * kThreads < total) to[m.word(e0 + u * kThreads, scan, c)] = f(to_f(v[u]));
   }
 }
 
@@ -157,7 +203,7 @@ __device__ __forceinline__ Group join(const Group &before, const Group &g) {
 }
 
 template <typename TX, typename TA, int K, bool kBackward>
-__global__ void __launch_bounds__(kThreads) narrow_kernel(const __grid_constant__ Params P) {
+__global__ void __launch_bounds__(kThreads, kBackward ? 3 : 4) narrow_kernel(const __grid_constant__ Params P) {
   extern __shared__ float values[];
   __shared__ NarrowShared sm;
   const gearb_recurrence_args &A = P.A;
@@ -177,17 +223,13 @@ __global__ void __launch_bounds__(kThreads) narrow_kernel(const __grid_constant_
   const int64_t i0 = tile * P.tile_rows, i1 = i0 + P.tile_rows < P.rows ? i0 + P.tile_rows : P.rows;
   const int n = static_cast<int>(i1 - i0);
 
-  each_value(P, i0, n, xl, K, P.x_period, A.x_batch_stride, A.x_row_stride, [&](int to, int64_t from, int, int) {
-    sx[to] = to_f(static_cast<const TX *>(A.x)[from]);
-  });
-  each_value(P, i0, n, gl, K, P.gate_period, A.gate_batch_stride, A.gate_row_stride, [&](int to, int64_t from, int, int) {
-    const float g = to_f(static_cast<const TA *>(A.gate)[from]);
-    sg[to] = A.gate_log ? exp_of(g) : g;
-  });
+  auto same = [](float v) { return v; };
+  load_values(static_cast<const TX *>(A.x), NarrowWalk(P, i0, n, xl, K, P.x_period, A.x_batch_stride, A.x_row_stride), sx, same);
+  load_values(static_cast<const TA *>(A.gate), NarrowWalk(P, i0, n, gl, K, P.gate_period, A.gate_batch_stride, A.gate_row_stride),
+              sg, [&](float v) { return A.gate_log ? exp_of(v) : v; });
   if (kBackward)
-    each_value(P, i0, n, xl, K, P.dout_period, A.dout_batch_stride, A.dout_row_stride, [&](int to, int64_t from, int, int) {
-      sd[to] = to_f(static_cast<const TX *>(A.dout)[from]);
-    });
+    load_values(static_cast<const TX *>(A.dout),
+                NarrowWalk(P, i0, n, xl, K, P.dout_period, A.dout_batch_stride, A.dout_row_stride), sd, same);
   if (A.offsets) mark_starts(P, sm, i0, i1);
 
   // this thread's rows
@@ -398,22 +440,26 @@ __global__ void __launch_bounds__(kThreads) narrow_kernel(const __grid_constant_
     const int64_t row = row_of(P, i), b0 = quotient(row, A.time);
     return row - b0 * A.time < __ldg(A.lengths + b0);
   };
-  if (!kBackward) {
-    each_value(P, i0, n, xl, K, P.rows, 0, w, [&](int from, int64_t to, int scan, int) {
-      if (A.zero_rest || owned(scan)) static_cast<TX *>(A.out)[to] = from_f<TX>(sx[from]);
-    });
-  } else {
-    each_value(P, i0, n, xl, K, P.rows, 0, w, [&](int from, int64_t to, int scan, int) {
-      if (A.zero_rest || owned(scan)) static_cast<TX *>(A.dx)[to] = from_f<TX>(sd[from]);
-    });
-    each_value(P, i0, n, gl, K, P.rows, 0, gates, [&](int, int64_t to, int scan, int gate) {
-      if (!A.zero_rest && !owned(scan)) return;
+  const NarrowWalk xw(P, i0, n, xl, K, P.rows, 0, w), gwalk(P, i0, n, gl, K, P.rows, 0, gates);
+  TX *to = static_cast<TX *>(kBackward ? A.dx : A.out) + xw.base;
+  const float *from = kBackward ? sd : sx;
+  int scan, ch;
+#pragma unroll 4
+  for (int e = threadIdx.x; e < n * w; e += kThreads) {
+    const float v = from[xw.word(e, scan, ch)];
+    if (A.zero_rest || owned(scan)) to[e] = from_f<TX>(v);
+  }
+  if (kBackward) {
+    TA *dg = static_cast<TA *>(A.dgate) + gwalk.base;
+    for (int e = threadIdx.x; e < n * gates; e += kThreads) {
+      gwalk.word(e, scan, ch);
+      if (!A.zero_rest && !owned(scan)) continue;
       const int gg = scan / K;
-      const float *p = sx + gg * xl.stride + (scan - gg * K) * w + gate * per;
+      const float *p = sx + gg * xl.stride + (scan - gg * K) * w + ch * per;
       float sum = 0.0f;
       for (int v = 0; v < per; ++v) sum += p[v];
-      static_cast<TA *>(A.dgate)[to] = from_f<TA>(sum);
-    });
+      dg[e] = from_f<TA>(sum);
+    }
   }
   empty_sequences(P, Place{tile, i0, i1, 0, 0, w, 0}, w, kBackward ? A.dstate : A.h0, kBackward ? A.dh0 : A.state_out);
 }

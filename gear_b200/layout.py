@@ -15,16 +15,17 @@ The reference has no counterpart: its batches are padded (gear/loader/offline_lo
 """
 from __future__ import annotations
 
-import ctypes as C
 from typing import NamedTuple, Optional
 
 import torch
 
 from . import _native as N
-from ._native import GearError, call, lib
-from .core import _ptr, _stream, _stream_scope
+from ._native import GearError, check, lib
+from .core import _Scope, _stream
 
 __all__ = ["PagedLayout", "paged_layout"]
+
+_LAYOUT = lib.gearb_layout_paged
 
 
 class PagedLayout(NamedTuple):
@@ -35,14 +36,13 @@ class PagedLayout(NamedTuple):
 
 
 def _need(t, what: str, dtype, device, numel=None):
-    if t is None:
-        return
-    if not isinstance(t, torch.Tensor) or t.dtype != dtype or not t.is_cuda or not t.is_contiguous():
+    if not isinstance(t, torch.Tensor) or t.dtype is not dtype or not t.is_cuda or not t.is_contiguous():
         raise GearError(N.ERR_INVALID, f"paged_layout: {what} must be a contiguous {dtype} CUDA tensor")
     if t.device != device:
         raise GearError(N.ERR_INVALID, f"paged_layout: {what} is on {t.device}, lengths on {device}")
     if numel is not None and t.numel() != numel:
         raise GearError(N.ERR_INVALID, f"paged_layout: {what} must have {numel} entries")
+    return t.data_ptr()
 
 
 def paged_layout(lengths: torch.Tensor, page: int, block_table: torch.Tensor, used: torch.Tensor, *,
@@ -67,45 +67,43 @@ def paged_layout(lengths: torch.Tensor, page: int, block_table: torch.Tensor, us
     if not isinstance(lengths, torch.Tensor) or lengths.dim() != 1:
         raise GearError(N.ERR_INVALID, "paged_layout: lengths must be a one-dimensional int64 CUDA tensor")
     dev, r = lengths.device, lengths.numel()
-    _need(lengths, "lengths", torch.int64, dev)
-    _need(past, "past", torch.int64, dev, r)
-    _need(block_table, "block_table", torch.int32, dev)
-    if block_table is None or block_table.dim() != 2 or block_table.shape[0] != r or block_table.shape[1] < 1:
+    at_lengths = _need(lengths, "lengths", torch.int64, dev)
+    at_past = 0 if past is None else _need(past, "past", torch.int64, dev, r)
+    at_table = _need(block_table, "block_table", torch.int32, dev)
+    shape = block_table.shape
+    if len(shape) != 2 or shape[0] != r or shape[1] < 1:
         raise GearError(N.ERR_INVALID, f"paged_layout: block_table must be [{r}, max_blocks]")
-    _need(free_pages, "free_pages", torch.int32, dev)
-    if used is None:
-        raise GearError(N.ERR_INVALID, "paged_layout: used must be one int64")
-    _need(used, "used", torch.int64, dev, 1)
-    _need(used_out, "used_out", torch.int64, dev, 1)
-    _need(offsets, "offsets", torch.int64, dev, r + 1)
-    _need(slot_map, "slot_map", torch.int64, dev)
-    _need(status, "status", torch.int32, dev, N.STATUS_WORDS)
+    at_free = 0 if free_pages is None else _need(free_pages, "free_pages", torch.int32, dev)
+    at_used = _need(used, "used", torch.int64, dev, 1)
     if free_pages is None and num_pages is None:
         raise GearError(N.ERR_INVALID, "paged_layout: num_pages is required without free_pages")
     pages = free_pages.numel() if num_pages is None else int(num_pages)
     if free_pages is not None and pages > free_pages.numel():
         raise GearError(N.ERR_INVALID, "paged_layout: num_pages is more than free_pages has")
+    max_tokens = int(max_tokens)
     if slot_map is not None:
+        _need(slot_map, "slot_map", torch.int64, dev)
         if max_tokens not in (0, slot_map.numel()):
             raise GearError(N.ERR_INVALID, "paged_layout: slot_map must have max_tokens entries")
         max_tokens = slot_map.numel()
-    if int(max_tokens) < 0:
+    if max_tokens < 0:
         raise GearError(N.ERR_INVALID, "paged_layout: max_tokens must not be negative")
-    with torch.cuda.device(dev), _stream_scope(stream):
+    if offsets is not None:
+        _need(offsets, "offsets", torch.int64, dev, r + 1)
+    if used_out is not None:
+        _need(used_out, "used_out", torch.int64, dev, 1)
+    at_status = 0 if status is None else _need(status, "status", torch.int32, dev, N.STATUS_WORDS)
+    with _Scope(dev, stream):
         if offsets is None:
             offsets = torch.empty(r + 1, dtype=torch.int64, device=dev)
         if slot_map is None and max_tokens:
-            slot_map = torch.empty(int(max_tokens), dtype=torch.int64, device=dev)
+            slot_map = torch.empty(max_tokens, dtype=torch.int64, device=dev)
         if used_out is None:
             used_out = torch.empty(1, dtype=torch.int64, device=dev)
-        nbytes = int(lib.gearb_layout_scratch_bytes(r))
+        nbytes = lib.gearb_layout_scratch_bytes(r)
         scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        a = N.LayoutArgs()
-        a.lengths, a.past, a.requests, a.page = lengths.data_ptr(), _ptr(past), r, int(page)
-        a.max_blocks, a.block_table = block_table.shape[1], block_table.data_ptr()
-        a.free_pages, a.num_pages = _ptr(free_pages), pages
-        a.used_in, a.used_out, a.offsets = used.data_ptr(), used_out.data_ptr(), offsets.data_ptr()
-        a.slot_map, a.max_tokens = _ptr(slot_map), int(max_tokens)
-        a.scratch, a.scratch_bytes, a.status = scratch.data_ptr(), nbytes, _ptr(status)
-        call("gearb_layout_paged", C.byref(a), _stream())
+        check(_LAYOUT(N.LAYOUT_ARGS.pack(at_lengths, at_past, r, int(page), shape[1], at_table, at_free, pages, at_used,
+                                         used_out.data_ptr(), offsets.data_ptr(),
+                                         0 if slot_map is None else slot_map.data_ptr(), max_tokens,
+                                         scratch.data_ptr(), nbytes, at_status), _stream()))
     return PagedLayout(offsets, slot_map, block_table, used_out)
