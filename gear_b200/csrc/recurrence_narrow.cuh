@@ -17,7 +17,8 @@ constexpr int kNarrowWidth = 16;
 // Where the words of a tile's tensor of `w` values a row lie in shared memory.
 struct NarrowLayout {
   int w, stride;  // values a row, floats from one group to the next
-  __host__ __device__ NarrowLayout(int w_, int k) : w(w_) { stride = k * w + ((w - k * w) % 32 + 32) % 32; }
+  __host__ __device__ constexpr NarrowLayout(int w_, int k)
+      : w(w_), stride(w_ == 1 ? k + 1 : k * w_ + ((w_ - k * w_) % 32 + 32) % 32) {}
 };
 __host__ __device__ inline int narrow_groups(int width) { return 32 / width; }  // of a warp
 
@@ -114,27 +115,28 @@ __device__ __forceinline__ GroupRows group_rows_packed(const Params &P, const Na
   if (n <= 0) return g;
   const ScanOffsets so{P.A.offsets, P.rows, P.A.sequences, P.A.reverse};
   const int64_t first = so.at(0), total = so.at(P.A.sequences);
-  const unsigned lo = sm.bits[at >> 5], hi = sm.bits[(at >> 5) + 1];
-  const unsigned here = __funnelshift_r(lo, hi, at & 31);          // bits of rows at ...
+  const unsigned here = __funnelshift_r(sm.bits[at >> 5], sm.bits[(at >> 5) + 1], at & 31);  // bits of rows at ...
   const int next = at + 1;
   const unsigned follow = __funnelshift_r(sm.bits[next >> 5], sm.bits[(next >> 5) + 1], next & 31);
-#pragma unroll
-  for (int k = 0; k < K; ++k)
-    if (k < n && i0 + at + k >= first && i0 + at + k < total) g.live |= 1u << k;
+  const int64_t before = first - (i0 + at), after = total - (i0 + at);  // rows in front of the first and up to the last sequence
+  const int lo = before < 0 ? 0 : (before < n ? static_cast<int>(before) : n);
+  const int hi = after < 0 ? 0 : (after < n ? static_cast<int>(after) : n);
+  if (hi > lo) g.live = ((1u << hi) - 1u) & ~((1u << lo) - 1u);
   g.start = here & g.live;
   g.end = follow & g.live;
   return g;
 }
 
 // Where the values of a tile's rows of one tensor lie, in memory order.
+template <int K, bool kOne>
 struct NarrowWalk {
-  int n, w, k, stride, reverse;
+  int n, w, stride, reverse;
   unsigned magic;  // e / w for e < 4096, w <= 16
   bool flat;       // one row stride
   int64_t row_low, base, period, sb, sr;
-  __device__ __forceinline__ NarrowWalk(const Params &P, int64_t i0, int n_, const NarrowLayout &lay, int k_, int64_t period_,
+  __device__ __forceinline__ NarrowWalk(const Params &P, int64_t i0, int n_, const NarrowLayout &lay, int64_t period_,
                                         int64_t sb_, int64_t sr_)
-      : n(n_), w(lay.w), k(k_), stride(lay.stride), reverse(P.A.reverse), period(period_), sb(sb_), sr(sr_) {
+      : n(n_), w(lay.w), stride(lay.stride), reverse(P.A.reverse), period(period_), sb(sb_), sr(sr_) {
     row_low = reverse ? P.rows - i0 - n : i0;  // matrix row of the first value
     magic = (0x10000u + w - 1) / w;
     const int64_t first = quotient(row_low, period);
@@ -143,15 +145,20 @@ struct NarrowWalk {
   }
   // Value e: its word in shared memory, its row in scan order and its place in the row.
   __device__ __forceinline__ int word(int e, int &scan, int &c) const {
+    if constexpr (kOne) {
+      c = 0;
+      scan = reverse ? n - 1 - e : e;
+      return scan + scan / K;
+    }
     const int r = static_cast<int>((static_cast<unsigned>(e) * magic) >> 16);
     c = e - r * w;
     scan = reverse ? n - 1 - r : r;
-    const int g = scan / k;
-    return g * stride + (scan - g * k) * w + c;
+    const int g = scan / K;
+    return g * stride + (scan - g * K) * w + c;
   }
   // Its element in memory.
   __device__ __forceinline__ int64_t element(int e) const {
-    const int r = static_cast<int>((static_cast<unsigned>(e) * magic) >> 16), c = e - r * w;
+    const int r = kOne ? e : static_cast<int>((static_cast<unsigned>(e) * magic) >> 16), c = e - r * w;
     if (flat) return base + r * sr + c;
     const int64_t b = quotient(row_low + r, period);
     return b * sb + (row_low + r - b * period) * sr + c;
@@ -159,8 +166,8 @@ struct NarrowWalk {
 };
 
 // Rows into shared memory: 16-byte (or 8-byte) loads where the values follow one another, several loads in flight.
-template <typename T, typename F>
-__device__ __forceinline__ void load_values(const T *p, const NarrowWalk &m, float *to, F f) {
+template <typename T, int K, bool kOne, typename F>
+__device__ __forceinline__ void load_values(const T *p, const NarrowWalk<K, kOne> &m, float *to, F f) {
   const int total = m.n * m.w;
   int scan, c;
   if (m.flat && m.sr == m.w && reinterpret_cast<uintptr_t>(p + m.base) % (4 * sizeof(T)) == 0) {
@@ -202,13 +209,15 @@ __device__ __forceinline__ Group join(const Group &before, const Group &g) {
   return Group{before.a * g.a, g.cut ? g.h : fmaf(g.a, before.h, g.h), g.cut | before.cut};
 }
 
-template <typename TX, typename TA, int K, bool kBackward>
+template <typename TX, typename TA, int K, bool kBackward, bool kOne>
 __global__ void __launch_bounds__(kThreads, kBackward ? 3 : 4) narrow_kernel(const __grid_constant__ Params P) {
   extern __shared__ float values[];
   __shared__ NarrowShared sm;
   const gearb_recurrence_args &A = P.A;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int w = static_cast<int>(A.width), gates = static_cast<int>(A.gates), per = P.per, gw = narrow_groups(w);
+  const int w = kOne ? 1 : static_cast<int>(A.width), gates = kOne ? 1 : static_cast<int>(A.gates), per = kOne ? 1 : P.per;
+  const int gw = narrow_groups(w);
+  using Walk = NarrowWalk<K, kOne>;
   const NarrowLayout xl(w, K), gl(gates, K);
   float *sx = values, *sg = sx + kWarps * gw * xl.stride, *sd = sg + kWarps * gw * gl.stride;
 
@@ -224,12 +233,12 @@ __global__ void __launch_bounds__(kThreads, kBackward ? 3 : 4) narrow_kernel(con
   const int n = static_cast<int>(i1 - i0);
 
   auto same = [](float v) { return v; };
-  load_values(static_cast<const TX *>(A.x), NarrowWalk(P, i0, n, xl, K, P.x_period, A.x_batch_stride, A.x_row_stride), sx, same);
-  load_values(static_cast<const TA *>(A.gate), NarrowWalk(P, i0, n, gl, K, P.gate_period, A.gate_batch_stride, A.gate_row_stride),
+  load_values(static_cast<const TX *>(A.x), Walk(P, i0, n, xl, P.x_period, A.x_batch_stride, A.x_row_stride), sx, same);
+  load_values(static_cast<const TA *>(A.gate), Walk(P, i0, n, gl, P.gate_period, A.gate_batch_stride, A.gate_row_stride),
               sg, [&](float v) { return A.gate_log ? exp_of(v) : v; });
   if (kBackward)
     load_values(static_cast<const TX *>(A.dout),
-                NarrowWalk(P, i0, n, xl, K, P.dout_period, A.dout_batch_stride, A.dout_row_stride), sd, same);
+                Walk(P, i0, n, xl, P.dout_period, A.dout_batch_stride, A.dout_row_stride), sd, same);
   if (A.offsets) mark_starts(P, sm, i0, i1);
 
   // this thread's rows
@@ -243,6 +252,18 @@ __global__ void __launch_bounds__(kThreads, kBackward ? 3 : 4) narrow_kernel(con
   float h0v = 0.0f;  // of the last start looked at
   auto first_state = [&](const float *p, int k) { return p ? p[sequence_of(A, P.rows, i0 + at + k) * w + c] : 0.0f; };
   Group f{1.0f, 0.0f, m.start != 0}, b{1.0f, 0.0f, m.end != 0};
+  // Without states of their own sequences start from nothing: no branches.  (What a row of no sequence leaves is not
+  // used: the next row of one is its first.)
+  const bool stateless = !A.h0 && !(kBackward ? A.dstate : nullptr);
+  if (stateless && mine > 0) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const bool st = m.start >> k & 1u;
+      const float a = pg[k * gates];
+      f.h = fmaf(st ? 0.0f : a, st ? 0.0f : f.h, px[k * w]);
+      f.a *= a;
+    }
+  } else {
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     if (!(m.live >> k & 1u)) continue;
@@ -254,6 +275,7 @@ __global__ void __launch_bounds__(kThreads, kBackward ? 3 : 4) narrow_kernel(con
       f.h = fmaf(a, f.h, x);
     }
     f.a *= a;
+  }
   }
   if (kBackward) {
     b.a = f.a;
@@ -391,7 +413,14 @@ __global__ void __launch_bounds__(kThreads, kBackward ? 3 : 4) narrow_kernel(con
   if (mine > 0) {
     float h = fx.cut ? fx.h : fmaf(fx.a, sm.wh[warp][c], fx.h);
     float *ox = sx + g * xl.stride + c;
-    if (!kBackward) {
+    if (!kBackward && stateless && !A.state_out) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        const bool st = m.start >> k & 1u;
+        h = fmaf(st ? 0.0f : pg[k * gates], st ? 0.0f : h, px[k * w]);
+        ox[k * w] = (m.live >> k & 1u) ? h : 0.0f;
+      }
+    } else if (!kBackward) {
 #pragma unroll
       for (int k = 0; k < K; ++k) {
         const float a = pg[k * gates], x = px[k * w];
@@ -440,7 +469,7 @@ __global__ void __launch_bounds__(kThreads, kBackward ? 3 : 4) narrow_kernel(con
     const int64_t row = row_of(P, i), b0 = quotient(row, A.time);
     return row - b0 * A.time < __ldg(A.lengths + b0);
   };
-  const NarrowWalk xw(P, i0, n, xl, K, P.rows, 0, w), gwalk(P, i0, n, gl, K, P.rows, 0, gates);
+  const Walk xw(P, i0, n, xl, P.rows, 0, w), gwalk(P, i0, n, gl, P.rows, 0, gates);
   TX *to = static_cast<TX *>(kBackward ? A.dx : A.out) + xw.base;
   const float *from = kBackward ? sd : sx;
   int scan, ch;
@@ -473,7 +502,9 @@ int launch_narrow(Params &p, bool backward, cudaStream_t stream) {
   p.ncol = 1;
   p.blocks_per_gate = 1;
   if (p.chain) GEARB_CUDA(cudaMemsetAsync(p.ticket, 0xff, static_cast<size_t>(p.chain_bytes), stream));
-  void (*kernel)(Params) = backward ? narrow_kernel<TX, TA, K, true> : narrow_kernel<TX, TA, K, false>;
+  void (*kernel)(Params);
+  if (w == 1) kernel = backward ? narrow_kernel<TX, TA, K, true, true> : narrow_kernel<TX, TA, K, false, true>;
+  else kernel = backward ? narrow_kernel<TX, TA, K, true, false> : narrow_kernel<TX, TA, K, false, false>;
   if (smem > 40 * 1024) GEARB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   kernel<<<static_cast<unsigned>(p.tiles), kThreads, smem, stream>>>(p);
   GEARB_CUDA(cudaGetLastError());
