@@ -8,8 +8,8 @@
 //   layout_scan_kernel    one CTA, eight requests a thread: up to 8192 requests in one round.
 //   layout_sums_kernel, layout_offsets_kernel   more requests: 4096 a CTA; a CTA adds up the sums before its own.
 //   layout_fill_kernel    every warp takes one stretch of the tokens, looks its first request up once and walks on from
-//                         there: 128 tokens a step, four a lane, while they belong to one request; otherwise 32 a step,
-//                         each lane finding its request among the next 32 offsets, which the warp holds.
+//                         there: up to 128 tokens of one request a step, four a lane; where less than 32 are left of
+//                         it, 32 a step, each lane finding its request among the next 32 offsets, which the warp holds.
 // Up to 8192 requests and 16384 slots the scan and the fill are one launch of one CTA.  Measured: 131072 requests,
 // 65 M tokens: 1950 us with a binary search per token and one CTA's prefix sums.
 #include "common.h"
@@ -24,6 +24,7 @@ constexpr int64_t kScanMost = kScanThreads * kPer;
 constexpr int64_t kFusedSlots = 16384;                 // beyond them the fill gets the whole GPU
 constexpr int kBlock = 4096;                           // requests a CTA of the longer way
 constexpr int kFillThreads = 256;
+constexpr int kFillCtas = 6;                           // an SM: what the registers allow
 constexpr int kStep = 128;                             // tokens a warp step
 constexpr unsigned kAll = 0xffffffffu;
 
@@ -168,39 +169,56 @@ __device__ __forceinline__ void fill_stretch(const LayoutParams &P, int64_t tota
     // last request whose offset is <= i: it has this token
     Request q = load_request(P, warp_upper_bound<int64_t>(a.offsets, 0, a.requests, i, lane, LoadPlain()) - 1);
     while (i < hi && i < total) {
-      if (i >= q.end) {  // usually among the next 32 requests
-        const int64_t near = q.r + 31 < a.requests ? q.r + 31 : a.requests;
-        q = load_request(P, warp_upper_bound<int64_t>(a.offsets, q.r, a.offsets[near] > i ? near : a.requests, i, lane,
-                                                      LoadPlain()) - 1);
+      if (i >= q.end) {  // usually the next request's
+        q = load_request(P, q.r + 1);
+        if (i >= q.end)
+          q = load_request(P, warp_upper_bound<int64_t>(a.offsets, q.r, a.requests, i, lane, LoadPlain()) - 1);
       }
-      const int64_t stop = i + kStep < hi ? i + kStep : hi;
-      if (stop == i + kStep && stop <= q.end && (stop <= a.max_tokens || i >= a.max_tokens)) {
-        // 128 tokens of one request, four a lane
-        const int64_t t = i + 4 * lane;
-        const unsigned pos = static_cast<unsigned>(q.past + (t - q.first)), blk = page_of(P, pos);
-        const unsigned in_page = pos - blk * static_cast<unsigned>(a.page);
-        int64_t s[4];
-        if (static_cast<int64_t>(in_page) + 3 < a.page) {
-          int32_t *entry = a.block_table + q.r * a.max_blocks + blk;
-          const bool fresh = blk >= q.have;
-          const int32_t page = fresh ? page_at(a, q.page0 + (blk - q.have)) : *entry;
-          if (fresh && in_page == 0) *entry = page;
-          const int64_t base = static_cast<int64_t>(page) * a.page + in_page;
+      const int64_t rest = q.end < hi ? q.end - i : hi - i;  // tokens of this request
+      if (rest >= 32) {
+        // up to 128 tokens of one request, in groups of four that begin on a multiple of four; counted in 32 bits from
+        // the request's first
+        const int64_t from = i & ~int64_t(3), stop = i + rest < from + kStep ? i + rest : from + kStep;
+        const int lo = static_cast<int>(i - q.first), end = static_cast<int>(stop - q.first);
+        const int rel = static_cast<int>(from - q.first) + 4 * lane, skip = rel < lo ? lo - rel : 0;  // first that counts
+        if (rel + skip < end) {
+          const unsigned size = static_cast<unsigned>(a.page), have = static_cast<unsigned>(q.have);
+          const unsigned pos = static_cast<unsigned>(q.past) + static_cast<unsigned>(rel + skip), blk = page_of(P, pos);
+          const unsigned in_page = pos - blk * size, left = size - in_page;  // tokens the page has room for
+          int32_t *entries = a.block_table + q.r * a.max_blocks;
+          auto look_up = [&](unsigned b, bool first) -> int64_t {
+            if (b < have) return entries[b];
+            const int32_t page = page_at(a, q.page0 + (b - have));
+            if (first) entries[b] = page;
+            return page;
+          };
+          int64_t page = look_up(blk, in_page == 0);
+          int64_t base = page < 0 ? -1 : page * a.page + in_page;
+          unsigned b = blk, used = 0, room = left;
+          int64_t s[4];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) s[k] = page < 0 ? -1 : base + k;
-        } else {
+          for (int k = 0; k < 4; ++k) {
+            s[k] = -1;
+            if (k < skip || rel + k >= end) continue;
+            if (used == room) {  // the next page; only pages of less than four rows come here twice
+              page = look_up(++b, true);
+              base = page < 0 ? -1 : page * a.page;
+              used = 0;
+              room = size;
+            }
+            s[k] = base < 0 ? -1 : base + used;
+            ++used;
+          }
+          const int64_t t = from + 4 * lane;
+          if (skip == 0 && rel + 4 <= end && P.vector && t + 4 <= a.max_tokens) {
+            longlong2 *to = reinterpret_cast<longlong2 *>(a.slot_map + t);
+            __stcs(to, make_longlong2(s[0], s[1]));
+            __stcs(to + 1, make_longlong2(s[2], s[3]));
+          } else {
 #pragma unroll
-          for (int k = 0; k < 4; ++k) s[k] = place_token(P, q, t + k);
-        }
-        if (i >= a.max_tokens) {
-          // rows without an entry: their pages only
-        } else if (P.vector) {
-          longlong2 *to = reinterpret_cast<longlong2 *>(a.slot_map + t);
-          __stcs(to, make_longlong2(s[0], s[1]));
-          __stcs(to + 1, make_longlong2(s[2], s[3]));
-        } else {
-#pragma unroll
-          for (int k = 0; k < 4; ++k) a.slot_map[t + k] = s[k];
+            for (int k = 0; k < 4; ++k)
+              if (k >= skip && rel + k < end && t + k < a.max_tokens) a.slot_map[t + k] = s[k];
+          }
         }
         i = stop;
         continue;
@@ -303,7 +321,7 @@ __global__ void __launch_bounds__(kScanThreads) layout_offsets_kernel(const __gr
   if (flags && P.a.status) atomicOr(reinterpret_cast<unsigned *>(P.a.status), flags);
 }
 
-__global__ void __launch_bounds__(kFillThreads) layout_fill_kernel(const __grid_constant__ LayoutParams P) {
+__global__ void __launch_bounds__(kFillThreads, kFillCtas) layout_fill_kernel(const __grid_constant__ LayoutParams P) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const gearb_layout_args &a = P.a;
   const int64_t total = a.offsets[a.requests];
@@ -383,7 +401,7 @@ int gearb_layout_paged(const gearb_layout_args *args, void *stream) {
     const int rc = launch_after(layout_offsets_kernel, static_cast<unsigned>(p.blocks), kScanThreads, p, st);
     if (rc != GEARB_OK) return rc;
   }
-  return launch_after(layout_fill_kernel, static_cast<unsigned>(sm_count() * 8), kFillThreads, p, st);
+  return launch_after(layout_fill_kernel, static_cast<unsigned>(sm_count() * kFillCtas), kFillThreads, p, st);
 }
 
 }  // extern "C"
