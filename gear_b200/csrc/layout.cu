@@ -85,18 +85,28 @@ __device__ __forceinline__ void block_sums(int64_t &x, int64_t &y, int64_t &tx, 
   __syncthreads();
 }
 
+// What placing one request's tokens takes.
+struct Request {
+  int64_t r, first, end;   // its tokens are [first, end) of the batch
+  int64_t past, have, page0;
+};
 // `per` requests a thread from r0 on, in front of them `tokens` tokens and `pages` pages; what follows is added to both.
+// `own` gets what the thread's (last) request is told.
 template <int kRequests>
 __device__ __forceinline__ void place_requests(const LayoutParams &P, int64_t r0, int64_t end, int64_t &tokens, int64_t &pages,
-                                               unsigned &flags, int64_t (*sm)[32]) {
+                                               unsigned &flags, int64_t (*sm)[32], Request *own = nullptr) {
   const gearb_layout_args &a = P.a;
   int64_t n[kRequests], need[kRequests], x = 0, y = 0, tx, ty;
   const int64_t r = r0 + static_cast<int64_t>(threadIdx.x) * kRequests;
 #pragma unroll
   for (int k = 0; k < kRequests; ++k) {
     n[k] = need[k] = 0;
-    int64_t past, have;
+    int64_t past = 0, have = 0;
     if (r + k < end) request_need(P, r + k, past, n[k], have, need[k], flags);
+    if (own) {
+      own->past = past;
+      own->have = have;
+    }
     x += n[k];
     y += need[k];
   }
@@ -108,6 +118,7 @@ __device__ __forceinline__ void place_requests(const LayoutParams &P, int64_t r0
     if (r + k < end) {
       a.offsets[r + k] = t;
       P.first_page[r + k] = p;
+      if (own) *own = Request{r + k, t, t + n[k], own->past, own->have, p};
       t += n[k];
       p += need[k];
     }
@@ -133,11 +144,6 @@ __device__ __forceinline__ int32_t page_at(const gearb_layout_args &a, int64_t k
   return a.free_pages ? __ldg(a.free_pages + k) : static_cast<int32_t>(k);
 }
 
-// What placing one request's tokens takes.
-struct Request {
-  int64_t r, first, end;   // its tokens are [first, end) of the batch
-  int64_t past, have, page0;
-};
 __device__ __forceinline__ Request load_request(const LayoutParams &P, int64_t r) {
   Request q;
   int64_t n, need;
@@ -264,12 +270,21 @@ __global__ void __launch_bounds__(kScanThreads) layout_scan_kernel(const __grid_
   int64_t tokens = 0, pages = used_before(a);
   unsigned flags = 0;
   __syncthreads();  // everybody has read used_in: used_out may be the same word
-  if (a.requests <= kScanThreads) place_requests<1>(P, 0, a.requests, tokens, pages, flags, sm);
+  Request own{0, 0, 0, 0, 0, 0};
+  if (a.requests <= kScanThreads) place_requests<1>(P, 0, a.requests, tokens, pages, flags, sm, &own);
   else place_requests<kPer>(P, 0, a.requests, tokens, pages, flags, sm);
   if (threadIdx.x == 0) finish_sums(a, tokens, pages, flags);
   if (flags && a.status) atomicOr(reinterpret_cast<unsigned *>(a.status), flags);
   if constexpr (kFill) {
-    __syncthreads();
+    // A decoding step: a thread places the few tokens of its request itself.
+    if (!__syncthreads_or(a.requests > kScanThreads || own.end - own.first > 4)) {
+      for (int64_t t = own.first; t < own.end; ++t) {
+        const int64_t slot = place_token(P, own, t);
+        if (t < a.max_tokens) a.slot_map[t] = slot;
+      }
+      for (int64_t t = tokens + threadIdx.x; t < a.max_tokens; t += kScanThreads) a.slot_map[t] = -1;
+      return;
+    }
     const int64_t end = tokens > a.max_tokens ? tokens : a.max_tokens;
     const int64_t each = ((end + 31) / 32 + kStep - 1) / kStep * kStep, lo = (threadIdx.x >> 5) * each;
     if (lo < end) fill_stretch(P, tokens, lo, lo + each < end ? lo + each : end, threadIdx.x & 31);
