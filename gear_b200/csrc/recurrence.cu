@@ -313,7 +313,10 @@ int launch(const gearb_recurrence_args &a, bool backward, cudaStream_t stream) {
   p.flat = p.x_period == p.rows && p.gate_period == p.rows && (!backward || p.dout_period == p.rows);
   // Channels a lane: as many as alignment allows and the width (of a gate's channels) fills.
   const bool shared = a.gates < a.width;
-  const int64_t unit = shared ? p.per : a.width;
+  // A gate's gradient is summed over the warp where a block lies inside one gate; gates of up to 16 channels would leave
+  // half of its lanes idle.
+  p.by_gate = shared && backward && p.per > 16;
+  const int64_t unit = p.by_gate ? p.per : a.width;
   const int xs = a.x_dtype == GEARB_DT_F32 ? 4 : 2, gs = a.gate_dtype == GEARB_DT_F32 ? 4 : 2;
   for (p.V = 4; p.V > 1; p.V /= 2) {
     const int v = p.V;

@@ -87,6 +87,10 @@ __device__ __forceinline__ void store_pack(T *p, const float (&f)[V]) {
   *reinterpret_cast<Pack<T, V> *>(p) = r;
 }
 
+// How a block of channels gets its gates: a gate each; one for the whole block; or any that it spans, each lane finding
+// its own (in the streaming kernel, from a table of a few).
+enum { kOwn = 0, kOne = 1, kTable = 2 };
+
 // The rows of a tile among the sequences, for the streaming kernels.
 struct alignas(16) TileRec {
   unsigned char live[kWarps], start[kWarps], end[kWarps];  // bits: rows of each warp
@@ -112,6 +116,8 @@ struct Params {
   int chain;             // tiles publish to each other
   int per;               // channels per gate
   int blocks_per_gate;   // column blocks of a gate's channels (shared gates)
+  int by_gate;           // shared gates: column blocks inside one gate each (wide kernels)
+  int block;             // channels of a column block where gates are not one per block
   int ncol;              // column blocks
   int flat;              // every tensor's rows lie one stride apart over the whole batch
   // Address periods: rows per batch entry, or all rows where one row stride covers the whole batch.
@@ -305,7 +311,7 @@ struct Place {
   int part;        // which column block of the gate
 };
 
-template <int V, bool kShared>
+template <int V, int kGate>
 __device__ __forceinline__ Place take_place(const Params &P, unsigned *smem_ticket, bool backward) {
   unsigned item;
   if (P.chain) {
@@ -321,7 +327,7 @@ __device__ __forceinline__ Place take_place(const Params &P, unsigned *smem_tick
   p.tile = backward ? P.tiles - 1 - t : t;
   p.i0 = p.tile * P.tile_rows;
   p.i1 = p.i0 + P.tile_rows < P.rows ? p.i0 + P.tile_rows : P.rows;
-  if (kShared) {
+  if (kGate == kOne) {
     p.gate = c / P.blocks_per_gate;
     p.part = c - static_cast<int>(p.gate) * P.blocks_per_gate;
     p.d0 = p.gate * P.per + static_cast<int64_t>(p.part) * 32 * V;
@@ -329,8 +335,8 @@ __device__ __forceinline__ Place take_place(const Params &P, unsigned *smem_tick
   } else {
     p.gate = 0;
     p.part = 0;
-    p.d0 = static_cast<int64_t>(c) * 32 * V;
-    p.d1 = P.A.width;
+    p.d0 = static_cast<int64_t>(c) * P.block;
+    p.d1 = p.d0 + P.block < P.A.width ? p.d0 + P.block : P.A.width;
   }
   return p;
 }
@@ -386,7 +392,7 @@ __device__ __forceinline__ TileRows tile_rows_packed(const Params &P, const Plac
   return t;
 }
 
-// V consecutive channels of a warp's n rows of the scan (zeros where there is no row or channel).  
+// V consecutive channels of a warp's n rows of the scan (zeros where there is no row or channel).
 template <typename T, int V>
 __device__ __forceinline__ void load_rows(const T *base, const Params &P, const Place &pl, const TileRows &tr, int64_t period,
                                           int64_t sb, int64_t sr, int warp, int n, int64_t d, bool on, Pack<T, V> (&r)[kRows]) {

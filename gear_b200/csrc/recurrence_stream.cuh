@@ -31,8 +31,6 @@ constexpr unsigned kLag = 2;  // tiles that compute warps begin before they come
 constexpr unsigned kRing = kLag + 1;
 constexpr int kMostStages = 6;
 constexpr int kRecorders = 2;  // one takes 3 us a tile: two dependent trips to L2
-// How a block of channels gets its gates: a gate each; one for the whole block; by a table of the few that it spans.
-enum { kOwn = 0, kOne = 1, kTable = 2 };
 constexpr int kTableGates = 8;
 
 constexpr unsigned kWaitLimit = 1u << 20;  // mbarrier polls before a copy is declared lost

@@ -10,17 +10,29 @@
 namespace gearb {
 namespace rec {
 
-template <typename TA, int V, bool kShared>
+template <typename TA, int V, int kGate>
 __device__ __forceinline__ void load_gate(const Params &P, const Place &pl, const TileRows &tr, int warp, int n, int64_t d,
-                                          bool on, float (&a)[kRows][kShared ? 1 : V]) {
-  constexpr int kG = kShared ? 1 : V;
-  Pack<TA, kG> raw[kRows];
-  load_rows<TA, kG>(static_cast<const TA *>(P.A.gate), P, pl, tr, P.gate_period, P.A.gate_batch_stride, P.A.gate_row_stride,
-                    warp, n, kShared ? pl.gate : d, on, raw);
+                                          bool on, float (&a)[kRows][kGate == kOne ? 1 : V]) {
+  const TA *gate = static_cast<const TA *>(P.A.gate);
+  if constexpr (kGate == kTable) {
 #pragma unroll
-  for (int k = 0; k < kRows; ++k)
+    for (int v = 0; v < V; ++v) {
+      Pack<TA, 1> raw[kRows];
+      load_rows<TA, 1>(gate, P, pl, tr, P.gate_period, P.A.gate_batch_stride, P.A.gate_row_stride, warp, n,
+                       on ? (static_cast<int>(d) + v) / P.per : 0, on, raw);
 #pragma unroll
-    for (int v = 0; v < kG; ++v) a[k][v] = to_f(raw[k].v[v]);
+      for (int k = 0; k < kRows; ++k) a[k][v] = to_f(raw[k].v[0]);
+    }
+  } else {
+    constexpr int kG = kGate == kOne ? 1 : V;
+    Pack<TA, kG> raw[kRows];
+    load_rows<TA, kG>(gate, P, pl, tr, P.gate_period, P.A.gate_batch_stride, P.A.gate_row_stride, warp, n,
+                      kGate == kOne ? pl.gate : d, on, raw);
+#pragma unroll
+    for (int k = 0; k < kRows; ++k)
+#pragma unroll
+      for (int v = 0; v < kG; ++v) a[k][v] = to_f(raw[k].v[v]);
+  }
 }
 
 template <int kG>
@@ -80,9 +92,9 @@ __device__ __forceinline__ void state_store(float *p, int seq, int64_t width, in
     for (int v = 0; v < V; ++v) p[static_cast<int64_t>(seq) * width + d + v] = r[v];
 }
 
-template <typename TX, typename TA, int V, bool kShared>
+template <typename TX, typename TA, int V, int kGate>
 __global__ void __launch_bounds__(kThreads, V == 4 ? 2 : 2) forward_kernel(const __grid_constant__ Params P) {
-  constexpr int kG = kShared ? 1 : V;
+  constexpr int kG = kGate == kOne ? 1 : V;
   constexpr int kW = 32 * V;  // channels of a block
   __shared__ float sa[kWarps][kW], sh[kWarps][kW];
   __shared__ int scut[kWarps];
@@ -91,7 +103,7 @@ __global__ void __launch_bounds__(kThreads, V == 4 ? 2 : 2) forward_kernel(const
   __shared__ int64_t sfirst;  // scan index at which the first row's sequence starts, or -1: nothing is needed from before
   const gearb_recurrence_args &A = P.A;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const Place pl = take_place<V, kShared>(P, &sticket, false);
+  const Place pl = take_place<V, kGate>(P, &sticket, false);
   const int64_t d = pl.d0 + lane * V;
   const bool on = d < pl.d1;
   const int64_t i0 = pl.i0 + warp * kRows;
@@ -101,7 +113,7 @@ __global__ void __launch_bounds__(kThreads, V == 4 ? 2 : 2) forward_kernel(const
   float a[kRows][kG];
   TileRows tr = rows_of_tile(P, pl);
   load_rows<TX, V>(static_cast<const TX *>(A.x), P, pl, tr, P.x_period, A.x_batch_stride, A.x_row_stride, warp, n, d, on, x);
-  load_gate<TA, V, kShared>(P, pl, tr, warp, n, d, on, a);
+  load_gate<TA, V, kGate>(P, pl, tr, warp, n, d, on, a);
   const RowMap m = rows_of_warp(P, pl, tr, srows, i0, n, warp, lane);
   if (A.gate_log) exp_gate(a);
   const bool plain = m.live == kAllRows && (m.start | m.end) == 0;
@@ -115,7 +127,7 @@ __global__ void __launch_bounds__(kThreads, V == 4 ? 2 : 2) forward_kernel(const
     for (int k = 0; k < kRows; ++k)
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        const float av = a[k][kShared ? 0 : v];
+        const float av = a[k][kGate == kOne ? 0 : v];
         ch[v] = fmaf(av, ch[v], to_f(x[k].v[v]));
         ca[v] *= av;
       }
@@ -128,7 +140,7 @@ __global__ void __launch_bounds__(kThreads, V == 4 ? 2 : 2) forward_kernel(const
       if (st) state_load<V>(A.h0, __shfl_sync(kAll, m.seq, k), A.width, d, on, s);
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        const float av = a[k][kShared ? 0 : v], xv = to_f(x[k].v[v]);
+        const float av = a[k][kGate == kOne ? 0 : v], xv = to_f(x[k].v[v]);
         if (st) ch[v] = A.h0 ? fmaf(av, s[v], xv) : xv;
         else ch[v] = fmaf(av, ch[v], xv);
         ca[v] *= av;
@@ -189,7 +201,7 @@ __global__ void __launch_bounds__(kThreads, V == 4 ? 2 : 2) forward_kernel(const
 #pragma unroll
       for (int k = 0; k < kRows; ++k) {
 #pragma unroll
-        for (int v = 0; v < V; ++v) h[v] = fmaf(a[k][kShared ? 0 : v], h[v], to_f(x[k].v[v]));
+        for (int v = 0; v < V; ++v) h[v] = fmaf(a[k][kGate == kOne ? 0 : v], h[v], to_f(x[k].v[v]));
         if (on) store_pack<TX, V>(out + k * step, h);
       }
     } else {
@@ -210,11 +222,11 @@ __global__ void __launch_bounds__(kThreads, V == 4 ? 2 : 2) forward_kernel(const
 #pragma unroll
           for (int v = 0; v < V; ++v) {
             const float xv = to_f(x[k].v[v]);
-            h[v] = A.h0 ? fmaf(a[k][kShared ? 0 : v], s[v], xv) : xv;
+            h[v] = A.h0 ? fmaf(a[k][kGate == kOne ? 0 : v], s[v], xv) : xv;
           }
         } else {
 #pragma unroll
-          for (int v = 0; v < V; ++v) h[v] = fmaf(a[k][kShared ? 0 : v], h[v], to_f(x[k].v[v]));
+          for (int v = 0; v < V; ++v) h[v] = fmaf(a[k][kGate == kOne ? 0 : v], h[v], to_f(x[k].v[v]));
         }
         if (on) store_pack<TX, V>(out + k * step, h);
         if (m.end >> k & 1u) state_store<V>(A.state_out, seq, A.width, d, on, h);
@@ -243,9 +255,9 @@ __device__ __forceinline__ float sum_rows(float (&v)[kRows], int lane) {
   return v[0];
 }
 
-template <typename TX, typename TA, int V, bool kShared>
+template <typename TX, typename TA, int V, int kGate>
 __global__ void __launch_bounds__(kThreads, V == 4 ? 1 : 2) backward_kernel(const __grid_constant__ Params P) {
-  constexpr int kG = kShared ? 1 : V;
+  constexpr int kG = kGate == kOne ? 1 : V;
   constexpr int kW = 32 * V;
   __shared__ float sa[kWarps][kW], sh[kWarps][kW], sc[kWarps][kW];
   __shared__ int scut[kWarps], send[kWarps];
@@ -255,7 +267,7 @@ __global__ void __launch_bounds__(kThreads, V == 4 ? 1 : 2) backward_kernel(cons
   __shared__ int sopen;       // the first row continues a sequence of an earlier tile
   const gearb_recurrence_args &A = P.A;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const Place pl = take_place<V, kShared>(P, &sticket, true);
+  const Place pl = take_place<V, kGate>(P, &sticket, true);
   const int64_t d = pl.d0 + lane * V;
   const bool on = d < pl.d1;
   const int64_t i0 = pl.i0 + warp * kRows;
@@ -265,7 +277,7 @@ __global__ void __launch_bounds__(kThreads, V == 4 ? 1 : 2) backward_kernel(cons
   float a[kRows][kG];
   TileRows tr = rows_of_tile(P, pl);
   load_rows<TX, V>(static_cast<const TX *>(A.x), P, pl, tr, P.x_period, A.x_batch_stride, A.x_row_stride, warp, n, d, on, x);
-  load_gate<TA, V, kShared>(P, pl, tr, warp, n, d, on, a);
+  load_gate<TA, V, kGate>(P, pl, tr, warp, n, d, on, a);
   load_rows<TX, V>(static_cast<const TX *>(A.dout), P, pl, tr, P.dout_period, A.dout_batch_stride, A.dout_row_stride, warp, n,
                    d, on, dh);
   const RowMap m = rows_of_warp(P, pl, tr, srows, i0, n, warp, lane);
@@ -281,14 +293,14 @@ __global__ void __launch_bounds__(kThreads, V == 4 ? 1 : 2) backward_kernel(cons
     for (int k = 0; k < kRows; ++k)
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        const float av = a[k][kShared ? 0 : v];
+        const float av = a[k][kGate == kOne ? 0 : v];
         ch[v] = fmaf(av, ch[v], to_f(x[k].v[v]));
         ca[v] *= av;
       }
 #pragma unroll
     for (int k = kRows - 1; k >= 0; --k)
 #pragma unroll
-      for (int v = 0; v < V; ++v) cc[v] = a[k][kShared ? 0 : v] * (to_f(dh[k].v[v]) + cc[v]);
+      for (int v = 0; v < V; ++v) cc[v] = a[k][kGate == kOne ? 0 : v] * (to_f(dh[k].v[v]) + cc[v]);
   } else {
 #pragma unroll
     for (int k = 0; k < kRows; ++k) {
@@ -298,7 +310,7 @@ __global__ void __launch_bounds__(kThreads, V == 4 ? 1 : 2) backward_kernel(cons
       if (st) state_load<V>(A.h0, __shfl_sync(kAll, m.seq, k), A.width, d, on, s);
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        const float av = a[k][kShared ? 0 : v], xv = to_f(x[k].v[v]);
+        const float av = a[k][kGate == kOne ? 0 : v], xv = to_f(x[k].v[v]);
         if (st) ch[v] = A.h0 ? fmaf(av, s[v], xv) : xv;
         else ch[v] = fmaf(av, ch[v], xv);
         ca[v] *= av;
@@ -309,7 +321,7 @@ __global__ void __launch_bounds__(kThreads, V == 4 ? 1 : 2) backward_kernel(cons
       if (!(m.live >> k & 1u)) continue;
       if (m.end >> k & 1u) state_load<V>(A.dstate, __shfl_sync(kAll, m.seq, k), A.width, d, on, cc);
 #pragma unroll
-      for (int v = 0; v < V; ++v) cc[v] = a[k][kShared ? 0 : v] * (to_f(dh[k].v[v]) + cc[v]);
+      for (int v = 0; v < V; ++v) cc[v] = a[k][kGate == kOne ? 0 : v] * (to_f(dh[k].v[v]) + cc[v]);
     }
   }
 #pragma unroll
@@ -385,17 +397,30 @@ __global__ void __launch_bounds__(kThreads, V == 4 ? 1 : 2) backward_kernel(cons
     float hp[kRows][V], h[V], c[V], part[kRows];  // hp: h_(t-1) of every row
 #pragma unroll
     for (int v = 0; v < V; ++v) { h[v] = sh[warp][lane * V + v]; c[v] = sc[warp][lane * V + v]; }
-    const int64_t row0 = row_of(P, i0), sign = A.reverse ? -1 : 1;
+    const int64_t row0 = row_of(P, i0), sign = A.reverse ? -1 : 1, xs = sign * A.width, gs = sign * A.gates;
     TX *dx = static_cast<TX *>(A.dx) + row0 * A.width + d;
-    TA *dgate = static_cast<TA *>(A.dgate) + row0 * A.gates + (kShared ? pl.gate : d);
-    const int64_t xs = sign * A.width, gs = sign * A.gates;
+    TA *dgate = static_cast<TA *>(A.dgate) + row0 * A.gates +
+                (kGate == kOne ? pl.gate : kGate == kTable ? pl.d0 / P.per : d);
+    // Gates of a few channels each: a row's products through shared memory, a lane a gate (blocks hold whole gates).
+    auto sum_gates = [&](int k, bool wanted, const float (&da)[V]) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) sa[warp][lane * V + v] = da[v];
+      __syncwarp();
+      const int cols = static_cast<int>(pl.d1 - pl.d0);
+      for (int j = lane; j * P.per < cols; j += 32) {
+        float sum = 0.0f;
+        for (int u = 0; u < P.per; ++u) sum += sa[warp][j * P.per + u];
+        if (wanted) dgate[k * gs + j] = from_f<TA>(sum);
+      }
+      __syncwarp();
+    };
     if (plain) {
 #pragma unroll
       for (int k = 0; k < kRows; ++k)
 #pragma unroll
         for (int v = 0; v < V; ++v) {
           hp[k][v] = h[v];
-          h[v] = fmaf(a[k][kShared ? 0 : v], h[v], to_f(x[k].v[v]));
+          h[v] = fmaf(a[k][kGate == kOne ? 0 : v], h[v], to_f(x[k].v[v]));
         }
 #pragma unroll
       for (int k = kRows - 1; k >= 0; --k) {
@@ -403,7 +428,7 @@ __global__ void __launch_bounds__(kThreads, V == 4 ? 1 : 2) backward_kernel(cons
         part[k] = 0.0f;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-          const float av = a[k][kShared ? 0 : v];
+          const float av = a[k][kGate == kOne ? 0 : v];
           g[v] = to_f(dh[k].v[v]) + c[v];
           c[v] = av * g[v];
           da[v] = (A.gate_log ? c[v] : g[v]) * hp[k][v];
@@ -411,8 +436,9 @@ __global__ void __launch_bounds__(kThreads, V == 4 ? 1 : 2) backward_kernel(cons
         }
         if (on) {
           store_pack<TX, V>(dx + k * xs, g);
-          if constexpr (!kShared) store_pack<TA, V>(dgate + k * gs, da);
+          if constexpr (kGate == kOwn) store_pack<TA, V>(dgate + k * gs, da);
         }
+        if constexpr (kGate == kTable) sum_gates(k, true, da);
       }
     } else {
 #pragma unroll
@@ -423,7 +449,7 @@ __global__ void __launch_bounds__(kThreads, V == 4 ? 1 : 2) backward_kernel(cons
         for (int v = 0; v < V; ++v) {
           const float xv = to_f(x[k].v[v]);
           hp[k][v] = h[v];
-          if (lv) h[v] = (st && !A.h0) ? xv : fmaf(a[k][kShared ? 0 : v], h[v], xv);
+          if (lv) h[v] = (st && !A.h0) ? xv : fmaf(a[k][kGate == kOne ? 0 : v], h[v], xv);
         }
       }
 #pragma unroll
@@ -436,7 +462,7 @@ __global__ void __launch_bounds__(kThreads, V == 4 ? 1 : 2) backward_kernel(cons
         float g[V], da[V];
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-          const float av = a[k][kShared ? 0 : v];
+          const float av = a[k][kGate == kOne ? 0 : v];
           g[v] = lv ? to_f(dh[k].v[v]) + c[v] : 0.0f;
           if (lv) c[v] = av * g[v];
           // the first row of a sequence without h0 is h = x: its gate plays no part
@@ -445,12 +471,13 @@ __global__ void __launch_bounds__(kThreads, V == 4 ? 1 : 2) backward_kernel(cons
         }
         if (on && (lv || A.zero_rest)) {
           store_pack<TX, V>(dx + k * xs, g);
-          if constexpr (!kShared) store_pack<TA, V>(dgate + k * gs, da);
+          if constexpr (kGate == kOwn) store_pack<TA, V>(dgate + k * gs, da);
         }
+        if constexpr (kGate == kTable) sum_gates(k, lv || A.zero_rest, da);
         if (st) state_store<V>(A.dh0, seq, A.width, d, on, c);
       }
     }
-    if constexpr (kShared) {
+    if constexpr (kGate == kOne) {
       const float sum = sum_rows(part, lane);
       const int k = row_of_lane(lane);
       if (lane % kSpare == 0 && k < n && ((m.live >> k & 1u) || A.zero_rest)) {
@@ -462,33 +489,38 @@ __global__ void __launch_bounds__(kThreads, V == 4 ? 1 : 2) backward_kernel(cons
   empty_sequences(P, pl, kW, A.dstate, A.dh0);
 }
 
-template <typename TX, typename TA, int V>
+template <typename TX, typename TA, int V, int kGate>
 int launch_wide(Params &p, bool backward, cudaStream_t stream) {
   const gearb_recurrence_args &a = p.A;
-  const bool shared = a.gates < a.width;
-  p.blocks_per_gate = shared ? (p.per + 32 * V - 1) / (32 * V) : 1;
-  const int64_t ncol = shared ? a.gates * p.blocks_per_gate : (a.width + 32 * V - 1) / (32 * V);
+  p.block = 32 * V;
+  if (kGate == kTable && backward) {  // whole gates, and whole vectors
+    const int unit = p.per % V == 0 ? p.per : (p.per % 2 == 0 && V == 4 ? 2 : V) * p.per;
+    p.block = 32 * V / unit * unit;
+  }
+  p.blocks_per_gate = kGate == kOne ? (p.per + 32 * V - 1) / (32 * V) : 1;
+  const int64_t ncol = kGate == kOne ? a.gates * p.blocks_per_gate : (a.width + p.block - 1) / p.block;
   GEARB_REQUIRE(p.tiles <= (int64_t(1) << 31) / ncol - 1, "recurrence: too many tiles for one launch");
   p.ncol = static_cast<int>(ncol);
   const unsigned grid = static_cast<unsigned>(p.tiles * ncol);
   if (p.chain) GEARB_CUDA(cudaMemsetAsync(p.ticket, 0xff, static_cast<size_t>(p.chain_bytes), stream));
-  if (backward) {
-    if (shared) backward_kernel<TX, TA, V, true><<<grid, kThreads, 0, stream>>>(p);
-    else backward_kernel<TX, TA, V, false><<<grid, kThreads, 0, stream>>>(p);
-  } else {
-    if (shared) forward_kernel<TX, TA, V, true><<<grid, kThreads, 0, stream>>>(p);
-    else forward_kernel<TX, TA, V, false><<<grid, kThreads, 0, stream>>>(p);
-  }
+  if (backward) backward_kernel<TX, TA, V, kGate><<<grid, kThreads, 0, stream>>>(p);
+  else if constexpr (kGate != kOne) forward_kernel<TX, TA, V, kGate><<<grid, kThreads, 0, stream>>>(p);
   GEARB_CUDA(cudaGetLastError());
   return GEARB_OK;
+}
+
+template <typename TX, typename TA, int V>
+int launch_wide_gate(Params &p, bool backward, cudaStream_t stream) {
+  if (p.A.gates == p.A.width) return launch_wide<TX, TA, V, kOwn>(p, backward, stream);
+  return p.by_gate ? launch_wide<TX, TA, V, kOne>(p, backward, stream) : launch_wide<TX, TA, V, kTable>(p, backward, stream);
 }
 
 template <typename TX, typename TA>
 int launch_wide_any(Params &p, bool backward, cudaStream_t stream) {
   switch (p.V) {
-    case 4: return launch_wide<TX, TA, 4>(p, backward, stream);
-    case 2: return launch_wide<TX, TA, 2>(p, backward, stream);
-    default: return launch_wide<TX, TA, 1>(p, backward, stream);
+    case 4: return launch_wide_gate<TX, TA, 4>(p, backward, stream);
+    case 2: return launch_wide_gate<TX, TA, 2>(p, backward, stream);
+    default: return launch_wide_gate<TX, TA, 1>(p, backward, stream);
   }
 }
 
