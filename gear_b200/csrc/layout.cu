@@ -10,7 +10,7 @@
 //   layout_fill_kernel    every warp takes one stretch of the tokens, looks its first request up once and walks on from
 //                         there: up to 128 tokens of one request a step, four a lane; where less than 32 are left of
 //                         it, 32 a step, each lane finding its request among the next 32 offsets, which the warp holds.
-// Up to 8192 requests and 16384 slots the scan and the fill are one launch of one CTA.  Measured: 131072 requests,
+// Up to 1024 requests and 4096 slots the scan and the fill are one launch of one CTA.  Measured: 131072 requests,
 // 65 M tokens: 1950 us with a binary search per token and one CTA's prefix sums.
 #include "common.h"
 #include "warp_search.cuh"
@@ -21,7 +21,7 @@ namespace {
 constexpr int kScanThreads = 1024;
 constexpr int kPer = 8;                                // requests a thread
 constexpr int64_t kScanMost = kScanThreads * kPer;
-constexpr int64_t kFusedSlots = 16384;                 // beyond them the fill gets the whole GPU
+constexpr int64_t kFusedSlots = 4096;                  // beyond them the fill gets the whole GPU
 constexpr int kBlock = 4096;                           // requests a CTA of the longer way
 constexpr int kFillThreads = 256;
 constexpr int kFillCtas = 6;                           // an SM: what the registers allow
@@ -403,7 +403,7 @@ int gearb_layout_paged(const gearb_layout_args *args, void *stream) {
   p.vector = reinterpret_cast<uintptr_t>(a.slot_map) % 16 == 0;
   cudaStream_t st = as_stream(stream);
   if (p.blocks == 0) {
-    if (a.max_tokens > 0 && a.max_tokens <= kFusedSlots) {
+    if (a.max_tokens > 0 && a.max_tokens <= kFusedSlots && a.requests <= kScanThreads) {
       layout_scan_kernel<true><<<1, kScanThreads, 0, st>>>(p);
       GEARB_CUDA(cudaGetLastError());
       return GEARB_OK;

@@ -93,7 +93,7 @@ __device__ __forceinline__ void state_store(float *p, int seq, int64_t width, in
 }
 
 template <typename TX, typename TA, int V, int kGate>
-__global__ void __launch_bounds__(kThreads, V == 4 ? 2 : 2) forward_kernel(const __grid_constant__ Params P) {
+__global__ void __launch_bounds__(kThreads, V == 4 ? 2 : V == 2 ? 3 : 5) forward_kernel(const __grid_constant__ Params P) {
   constexpr int kG = kGate == kOne ? 1 : V;
   constexpr int kW = 32 * V;  // channels of a block
   __shared__ float sa[kWarps][kW], sh[kWarps][kW];
@@ -256,7 +256,7 @@ __device__ __forceinline__ float sum_rows(float (&v)[kRows], int lane) {
 }
 
 template <typename TX, typename TA, int V, int kGate>
-__global__ void __launch_bounds__(kThreads, V == 4 ? 1 : 2) backward_kernel(const __grid_constant__ Params P) {
+__global__ void __launch_bounds__(kThreads, V == 4 ? 2 : V == 2 ? 3 : 4) backward_kernel(const __grid_constant__ Params P) {
   constexpr int kG = kGate == kOne ? 1 : V;
   constexpr int kW = 32 * V;
   __shared__ float sa[kWarps][kW], sh[kWarps][kW], sc[kWarps][kW];
