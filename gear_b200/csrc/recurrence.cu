@@ -221,7 +221,7 @@ Tiling tiling_of(const gearb_recurrence_args &a) {
 }
 
 struct Scratch {
-  int64_t agg, super, recs, part, chain_bytes, total;
+  int64_t agg, super, section, recs, part, chain_bytes, total;
 };
 Scratch scratch_of(const gearb_recurrence_args &a, bool backward) {
   const Tiling t = tiling_of(a);
@@ -230,7 +230,8 @@ Scratch scratch_of(const gearb_recurrence_args &a, bool backward) {
   if (t.chain) {
     s.agg = 256;
     s.super = s.agg + up256(tiles * a.width * 8);
-    s.chain_bytes = s.super + up256((tiles / kSuper + 1) * a.width * 4);
+    s.section = s.super + up256((tiles / kSuper + 1) * a.width * 8);
+    s.chain_bytes = s.section + up256((tiles / kSuper + 1) * a.width * 4);
   }
   s.recs = s.chain_bytes;
   s.part = s.recs + up256(tiles * static_cast<int64_t>(sizeof(TileRec)));
@@ -301,7 +302,8 @@ int launch(const gearb_recurrence_args &a, bool backward, cudaStream_t stream) {
     char *base = static_cast<char *>(a.scratch);
     p.ticket = reinterpret_cast<unsigned *>(base);
     p.agg = reinterpret_cast<float2 *>(base + s.agg);
-    p.super = reinterpret_cast<float *>(base + s.super);
+    p.super = reinterpret_cast<float2 *>(base + s.super);
+    p.section = reinterpret_cast<float *>(base + s.section);
     p.chain_bytes = s.chain_bytes;
   }
   p.recs = reinterpret_cast<TileRec *>(static_cast<char *>(a.scratch) + s.recs);

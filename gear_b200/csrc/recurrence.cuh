@@ -12,11 +12,16 @@
 // gate and x in registers (eight rows a warp, up to four channels a lane), forms (A, H), learns the state before
 // its tile, and runs its rows again from there.  Every input is read once and every output written once.
 //
-// The state before a tile.  Tiles publish their (A, H); 8 consecutive tiles form a superblock, and the last
-// tile of one publishes the state behind it.  A tile composes the tiles before it in its superblock, in
-// order, onto the state in front of the superblock: the same operations whatever the timing, so results are the
-// same bits every time, and the chain of waiting CTAs has one link per 512 rows.  A tile needs nothing from
-// before the start of the sequence its first row belongs to.  Tiles are handed out by a counter in scan order,
+// The state before a tile.  Tiles publish their (A, H).  8 consecutive tiles form a superblock, whose last tile
+// publishes the superblock's (A, H); 8 superblocks form a section, whose last tile publishes the state behind it.  A tile
+// applies the superblocks before it in its section to the state in front of the section, in order, and composes the
+// tiles before it in its superblock onto that: the same operations whatever the timing, so results are the same bits
+// every time, and the chain of CTAs that wait for one another has one link (0.5 to 0.65 us) per 4096 rows.  Where
+// there are more than five column blocks, so that 512 rows of all channels take longer than a link, or few rows a
+// sequence, a superblock is a section by itself: one thing less to wait for.  Measured, short sections and long:
+// 54 x 10752 x 48 float32 630 and 362 us, 1 x 580000 x 16 158 and 109, 4 x 65536 x 512 bf16 (4 blocks) 376 and 328,
+// 4 x 32768 x 768 (6 blocks) 217 and 229, 1 x 32768 x 2048 (16 blocks) 113 and 124, 3000 x 300 x 64 171 and 235.
+// A tile needs nothing from before the start of the sequence its first row belongs to.  Tiles are handed out by a counter in scan order,
 // so a CTA only ever waits for CTAs that are already running; every wait has a limit, after which the
 // launch goes on with NaN and says so in the status word.  Published words are 32 bits that read
 // 0xffffffff until they are written (a value of those bits is published as another NaN), so no flags and
@@ -42,6 +47,9 @@ constexpr int kThreads = kWarps * 32;
 constexpr int kRows = 8;                     // rows a warp keeps in registers
 constexpr int kTile = kWarps * kRows;        // rows per tile
 constexpr int kSuper = 8;                    // tiles per superblock
+constexpr int kShortSection = 3, kLongSection = 6;  // tiles per section (powers of two): one superblock, or eight
+constexpr int kLongColumns = 5;              // most column blocks with long sections,
+constexpr int kLongRows = 2048;              // and fewest rows a sequence
 constexpr unsigned kAll = 0xffffffffu;
 constexpr unsigned kAllRows = (1u << kRows) - 1u;
 constexpr unsigned kUnset = 0xffffffffu;     // a published word that has not been written
@@ -114,6 +122,7 @@ struct Params {
   int backward;
   int narrow_rows;       // rows a thread takes in narrow_kernel; 0: another kernel
   int chain;             // tiles publish to each other
+  int section_shift;     // kShortSection or kLongSection
   int per;               // channels per gate
   int blocks_per_gate;   // column blocks of a gate's channels (shared gates)
   int by_gate;           // shared gates: column blocks inside one gate each (wide kernels)
@@ -124,7 +133,8 @@ struct Params {
   int64_t x_period, gate_period, dout_period;
   unsigned *ticket;
   float2 *agg;           // [tiles][width]: (A, H) of every tile
-  float *super;          // [superblocks][width]: state in front of every superblock
+  float2 *super;         // [superblocks][width]: (A, H) of every superblock, in long sections
+  float *section;        // [sections][width]: state in front of every section
   int V;                 // channels a lane, by alignment and width
   TileRec *recs;         // [tiles]
   int64_t chain_bytes;   // at `ticket`: to be set to 0xff before tiles publish
@@ -421,33 +431,77 @@ __device__ __forceinline__ void load_rows(const T *base, const Params &P, const 
   }
 }
 
-// What the tiles before this one (in the order of the tickets, `at` of them) hand on: the state of channel d in front of
-// the tile.  lo: the first tile that matters.
-__device__ __forceinline__ float look_back(const Params &P, int64_t at, int64_t lo, int64_t d, bool &lost) {
-  const int64_t sb = at / kSuper, sb0 = sb * kSuper;
-  const bool need_super = lo < sb0;
-  const int64_t j0 = need_super ? sb0 : lo;
-  const int count = static_cast<int>(at - j0);
-  const float2 *p = P.agg + j0 * P.A.width + d;
-  float pa = 1.0f, ph = 0.0f;
-  for (int j = 0; j < count; j += 5) {
-    float2 q[5];
+// The state of channel d in front of tile `at` (in the order of the tickets), from what the tiles before it published;
+// the last tile of a superblock publishes for it on the way, that of a section too.  lo: the first tile that matters
+// (`at`: none).  own() gives the tile's own (A, H), asked for by such last tiles only; cut: a sequence starts in the tile.
+// kAhead pairs are asked for at a time: all seven by warps that have nothing else to hold in registers.  kShift: the
+// section's shift where it is known in advance, or 0.
+template <int kAhead, int kShift, typename Index, typename Own>
+__device__ __forceinline__ float look_back(const Params &P, Index at, Index lo, Index d, Own &&own, bool cut,
+                                           bool &lost) {
+  const int shift = kShift > 0 ? kShift : P.section_shift;
+  const int64_t width = P.A.width;
+  const Index sb = at / kSuper, sec = at >> shift, sec0 = sec << shift;
+  const bool by_super = lo < sb * kSuper, by_section = lo < sec0;
+  const Index t0 = by_super ? sb * kSuper : lo, s0 = (by_section ? sec0 : lo) / kSuper;
+  const int tiles = static_cast<int>(at - t0), supers = kShift != kShortSection && by_super ? static_cast<int>(sb - s0) : 0;
+  const float2 *tp = P.agg + t0 * width + d, *sp = P.super + s0 * width + d;
+  constexpr bool kAll7 = kAhead == kSuper - 1;
+  float2 t[kAhead], s[kAhead];
+  auto peek = [&](float2(&q)[kAhead], const float2 *p, int from, int n) {
 #pragma unroll
-    for (int u = 0; u < 5; ++u)
-      if (j + u < count) q[u] = peek_pair(p + (j + u) * P.A.width);
+    for (int u = 0; u < kAhead; ++u)
+      if (from + u < n) q[u] = peek_pair(p + (from + u) * width);
+  };
+  auto settle = [&](float2 &q, const float2 *p) {
+    if (__float_as_uint(q.x) == kUnset || __float_as_uint(q.y) == kUnset) q = poll_pair(p, lost);
+  };
+  unsigned word = 0;
+  peek(t, tp, 0, tiles);
+  if (kAll7) peek(s, sp, 0, supers);
+  if (by_section) asm volatile("ld.relaxed.gpu.global.u32 %0, [%1];" : "=r"(word) : "l"(P.section + sec * width + d) : "memory");
+
+  float pa = 1.0f, ph = 0.0f;  // of the tiles before this one in its superblock
+  for (int j = 0; j < tiles; j += kAhead) {
+    if (j > 0) peek(t, tp, j, tiles);
 #pragma unroll
-    for (int u = 0; u < 5; ++u)
-      if (j + u < count) {
-        if (__float_as_uint(q[u].x) == kUnset || __float_as_uint(q[u].y) == kUnset)
-          q[u] = poll_pair(p + (j + u) * P.A.width, lost);
+    for (int u = 0; u < kAhead; ++u)
+      if (j + u < tiles) {
+        settle(t[u], tp + (j + u) * width);
         // nothing in front of the sequence's start counts
-        ph = (j + u == 0 && !need_super) ? q[u].y : fmaf(q[u].x, ph, q[u].y);
-        pa *= q[u].x;
+        ph = (j + u == 0 && !by_super) ? t[u].y : fmaf(t[u].x, ph, t[u].y);
+        pa *= t[u].x;
       }
   }
-  if (!need_super) return ph;
-  const float s = __uint_as_float(poll_word(reinterpret_cast<const unsigned *>(P.super + sb * P.A.width + d), lost));
-  return fmaf(pa, s, ph);
+  const bool last = at % kSuper == kSuper - 1 && at + 1 < static_cast<Index>(P.tiles);
+  const bool very_last = last && at + 1 == (sec + 1) << shift;
+  if (last && !very_last) {
+    const float2 t = own();
+    publish_pair(P.super + sb * width + d, t.x * pa, cut ? t.y : fmaf(t.x, ph, t.y));
+  }
+  float in = ph;
+  if (by_super) {
+    float h = 0.0f;
+    if (by_section) {
+      if (word == kUnset) word = poll_word(reinterpret_cast<const unsigned *>(P.section + sec * width + d), lost);
+      h = __uint_as_float(word);
+    }
+    for (int j = 0; j < supers; j += kAhead) {
+      if (!kAll7) peek(s, sp, j, supers);
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u)
+        if (j + u < supers) {
+          settle(s[u], sp + (j + u) * width);
+          h = (j + u == 0 && !by_section) ? s[u].y : fmaf(s[u].x, h, s[u].y);
+        }
+    }
+    in = fmaf(pa, h, ph);
+  }
+  if (very_last) {
+    const float2 t = own();
+    publish_word(P.section + (sec + 1) * width + d, cut ? t.y : fmaf(t.x, in, t.y));
+  }
+  return in;
 }
 
 // e^x in float32 from 2^t (one instruction, 2 units in the last place): with t = x / ln 2 rounded, e^x = 2^t * e^r for
@@ -491,6 +545,11 @@ __device__ __forceinline__ void empty_sequences(const Params &P, const Place &pl
 // Whether rows can be read or written v values at a time.
 inline bool vector_ok(const void *p, int64_t sb, int64_t sr, int size, int v) {
   return reinterpret_cast<uintptr_t>(p) % (size * v) == 0 && sb % v == 0 && sr % v == 0;
+}
+
+// Long sections where the chain would take longer than the work, and sequences are long enough to feel it.
+inline bool long_sections(const Params &p, int ncol) {
+  return ncol <= kLongColumns && p.rows / kLongRows >= p.A.sequences;
 }
 
 // In front of a streaming kernel: finds out about the tiles' rows, and clears what they publish in.

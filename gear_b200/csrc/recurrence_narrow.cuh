@@ -366,14 +366,11 @@ __global__ void __launch_bounds__(kThreads, kBackward ? 3 : 4) narrow_kernel(con
     if (P.chain) {
       if (!kBackward) {
         publish_pair(P.agg + tile * w + ch, t.a, t.h);
-        if (sm.open) {
-          bool lost = false;
-          in = look_back(P, tile, quotient(sm.first, P.tile_rows), ch, lost);
-          if (lost && A.status) atomicOr(reinterpret_cast<unsigned *>(A.status), GEARB_ST_SCAN_ABORTED);
-          if (A.carry) A.carry[tile * w + ch] = in;
-        }
-        if (tile % kSuper == kSuper - 1 && tile + 1 < P.tiles)
-          publish_word(P.super + (tile / kSuper + 1) * w + ch, t.cut ? t.h : fmaf(t.a, in, t.h));
+        bool lost = false;
+        in = look_back<4, 0, int64_t>(P, tile, sm.open ? quotient(sm.first, P.tile_rows) : tile, ch,
+                                   [&] { return make_float2(t.a, t.h); }, t.cut != 0, lost);
+        if (lost && A.status) atomicOr(reinterpret_cast<unsigned *>(A.status), GEARB_ST_SCAN_ABORTED);
+        if (sm.open && A.carry) A.carry[tile * w + ch] = in;
       } else if (sm.open) {
         in = __ldg(A.carry + tile * w + ch);
       }
@@ -396,13 +393,10 @@ __global__ void __launch_bounds__(kThreads, kBackward ? 3 : 4) narrow_kernel(con
     if (P.chain) {
       publish_pair(P.agg + at_tile * w + ch, t.a, t.h);
       const int64_t lo = sm.last >= 0 ? P.tiles - 1 - quotient(sm.last, P.tile_rows) : at_tile;
-      if (lo < at_tile) {
-        bool lost = false;
-        in = look_back(P, at_tile, lo, ch, lost);
-        if (lost && A.status) atomicOr(reinterpret_cast<unsigned *>(A.status), GEARB_ST_SCAN_ABORTED);
-      }
-      if (at_tile % kSuper == kSuper - 1 && at_tile + 1 < P.tiles)
-        publish_word(P.super + (at_tile / kSuper + 1) * w + ch, t.cut ? t.h : fmaf(t.a, in, t.h));
+      bool lost = false;
+      in = look_back<4, 0, int64_t>(P, at_tile, lo < at_tile ? lo : at_tile, ch, [&] { return make_float2(t.a, t.h); },
+                                 t.cut != 0, lost);
+      if (lost && A.status) atomicOr(reinterpret_cast<unsigned *>(A.status), GEARB_ST_SCAN_ABORTED);
     }
 #pragma unroll
     for (int q = 0; q < kWarps; ++q) sm.wc[q][ch] = cut[q] ? ph[q] : fmaf(pa[q], in, ph[q]);
@@ -500,6 +494,7 @@ int launch_narrow(Params &p, bool backward, cudaStream_t stream) {
   const int smem = groups * ((backward ? 2 : 1) * xl.stride + gl.stride) * 4;
   GEARB_REQUIRE(p.tiles < (int64_t(1) << 31), "recurrence: too many tiles for one launch");
   p.ncol = 1;
+  p.section_shift = long_sections(p, p.ncol) ? kLongSection : kShortSection;
   p.blocks_per_gate = 1;
   if (p.chain) GEARB_CUDA(cudaMemsetAsync(p.ticket, 0xff, static_cast<size_t>(p.chain_bytes), stream));
   void (*kernel)(Params);

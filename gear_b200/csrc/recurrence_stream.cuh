@@ -193,30 +193,30 @@ struct StreamShared {
   uint64_t paired[kRing], ready[kRing], read[kRing];   // the warps' pairs; turned and edge.a, edge.h there; read again
 };
 
-// The tile before (in the order of the tickets): what its predecessors published, asked for early.
+// Short sections: what the tiles before one (in the order of the tickets) published, asked for at once.
 struct Peek {
   float2 q[kSuper - 1];
   float s;
 };
 __device__ __forceinline__ void peek_back(const Params &P, int at, int lo, int d, Peek &k) {
   const int sb = at / kSuper, sb0 = sb * kSuper;
-  const bool need_super = lo < sb0;
-  const int j0 = need_super ? sb0 : lo, count = at - j0;
+  const bool need_section = lo < sb0;
+  const int j0 = need_section ? sb0 : lo, count = at - j0;
   const float2 *p = P.agg + j0 * P.A.width + d;
 #pragma unroll
   for (int u = 0; u < kSuper - 1; ++u)
     if (u < count) k.q[u] = peek_pair(p + u * P.A.width);
-  if (need_super) {
+  if (need_section) {
     unsigned w;
-    asm volatile("ld.relaxed.gpu.global.u32 %0, [%1];" : "=r"(w) : "l"(P.super + sb * P.A.width + d) : "memory");
+    asm volatile("ld.relaxed.gpu.global.u32 %0, [%1];" : "=r"(w) : "l"(P.section + sb * P.A.width + d) : "memory");
     k.s = __uint_as_float(w);
   }
 }
 // The state in front of tile `at`: as look_back, from what was peeked at, waiting for what was not there yet.
 __device__ __forceinline__ float settle_back(const Params &P, int at, int lo, int d, Peek &k, bool &lost) {
   const int sb = at / kSuper, sb0 = sb * kSuper;
-  const bool need_super = lo < sb0;
-  const int j0 = need_super ? sb0 : lo, count = at - j0;
+  const bool need_section = lo < sb0;
+  const int j0 = need_section ? sb0 : lo, count = at - j0;
   const float2 *p = P.agg + j0 * P.A.width + d;
   float pa = 1.0f, ph = 0.0f;
 #pragma unroll
@@ -224,12 +224,12 @@ __device__ __forceinline__ float settle_back(const Params &P, int at, int lo, in
     if (u < count) {
       if (__float_as_uint(k.q[u].x) == kUnset || __float_as_uint(k.q[u].y) == kUnset)
         k.q[u] = poll_pair(p + u * P.A.width, lost);
-      ph = (u == 0 && !need_super) ? k.q[u].y : fmaf(k.q[u].x, ph, k.q[u].y);
+      ph = (u == 0 && !need_section) ? k.q[u].y : fmaf(k.q[u].x, ph, k.q[u].y);
       pa *= k.q[u].x;
     }
-  if (!need_super) return ph;
+  if (!need_section) return ph;
   if (__float_as_uint(k.s) == kUnset)
-    k.s = __uint_as_float(poll_word(reinterpret_cast<const unsigned *>(P.super + sb * P.A.width + d), lost));
+    k.s = __uint_as_float(poll_word(reinterpret_cast<const unsigned *>(P.section + sb * P.A.width + d), lost));
   return fmaf(pa, k.s, ph);
 }
 
@@ -433,8 +433,8 @@ __device__ __forceinline__ void step_row(const gearb_recurrence_args &A, const P
   fma_v(h, a, h, x);
 }
 
-// Finishers: the state in front of every tile (backward: behind it), and that in front of the next superblock.
-template <typename TX, typename TA, int V, int kGate, bool kBackward>
+// Finishers: the state in front of every tile (backward: behind it), and what its superblock and section publish.
+template <typename TX, typename TA, int V, int kGate, bool kBackward, bool kLong>
 __device__ __forceinline__ bool finish_tiles(const Params &P, StreamShared<TX, TA, V, kGate, kBackward> &sm, int c, int lane) {
   using Shared = StreamShared<TX, TA, V, kGate, kBackward>;
   const gearb_recurrence_args &A = P.A;
@@ -448,19 +448,28 @@ __device__ __forceinline__ bool finish_tiles(const Params &P, StreamShared<TX, T
     const int tile = kBackward ? static_cast<int>(P.tiles) - 1 - pl.tile : pl.tile, lo = kBackward ? pl.rec.lo_back : pl.rec.lo, d = pl.d0 + c;
     const bool on = c < pl.cols;
     float in = 0.0f;
-    if (on && lo >= 0) {
-      Peek peek;
-      peek_back(P, tile, lo, d, peek);
-      in = settle_back(P, tile, lo, d, peek, lost);
-      if (!kBackward && A.carry) A.carry[pl.tile * A.width + d] = in;
-    }
-    if (P.chain && tile % kSuper == kSuper - 1 && tile + 1 < P.tiles) {
-      const bool cut = (kBackward ? pl.rec.bcut : pl.rec.cut) >> kWarps & 1u;
-      if (!warp_wait(&sm.ready[pair.i], pair.parity)) return true;
-      if (on) {
-        const float h = sm.edge[stage].h[c];
-        publish_word(P.super + ((tile / kSuper + 1) * A.width + d), cut ? h : fmaf(sm.edge[stage].a[c], in, h));
+    const bool cut = (kBackward ? pl.rec.bcut : pl.rec.cut) >> kWarps & 1u;
+    if constexpr (!kLong) {
+      if (on && lo >= 0) {
+        Peek peek;
+        peek_back(P, tile, lo, d, peek);
+        in = settle_back(P, tile, lo, d, peek, lost);
+        if (!kBackward && A.carry) A.carry[pl.tile * A.width + d] = in;
       }
+      if (P.chain && tile % kSuper == kSuper - 1 && tile + 1 < P.tiles) {
+        if (!warp_wait(&sm.ready[pair.i], pair.parity)) return true;
+        if (on) {
+          const float h = sm.edge[stage].h[c];
+          publish_word(P.section + ((tile / kSuper + 1) * A.width + d), cut ? h : fmaf(sm.edge[stage].a[c], in, h));
+        }
+      }
+    } else if (on && (lo >= 0 || (P.chain && tile % kSuper == kSuper - 1))) {
+      auto own = [&] {
+        lost |= !mbar_wait(&sm.ready[pair.i], pair.parity);
+        return make_float2(sm.edge[stage].a[c], sm.edge[stage].h[c]);
+      };
+      in = look_back<kSuper - 1, kLongSection, int>(P, tile, lo >= 0 ? lo : tile, d, own, cut, lost);
+      if (!kBackward && A.carry && lo >= 0) A.carry[pl.tile * A.width + d] = in;
     }
     if (c < 32 * V) {
       sm.edge[stage].in[c] = in;
@@ -843,7 +852,7 @@ __device__ __forceinline__ void init_barriers(StreamShared<TX, TA, V, kGate, kBa
   __syncthreads();
 }
 
-template <typename TX, typename TA, int V, int kGate>
+template <typename TX, typename TA, int V, int kGate, bool kLong>
 __global__ void __launch_bounds__(kStreamThreads, 1) forward_stream_kernel(const __grid_constant__ Params P,
                                                                            const __grid_constant__ Maps maps) {
   using Shared = StreamShared<TX, TA, V, kGate, false>;
@@ -854,13 +863,13 @@ __global__ void __launch_bounds__(kStreamThreads, 1) forward_stream_kernel(const
   bool lost = false;
   if (warp < kWarps) lost = compute_forward<TX, TA, V, kGate>(P, sm, warp, lane);
   else if (warp < kWarps + 4) lost = publish_tiles<TX, TA, V, kGate, false>(P, sm, threadIdx.x - kThreads, lane);
-  else if (warp < kWarps + 8) lost = finish_tiles<TX, TA, V, kGate, false>(P, sm, threadIdx.x - kThreads - 128, lane);
+  else if (warp < kWarps + 8) lost = finish_tiles<TX, TA, V, kGate, false, kLong>(P, sm, threadIdx.x - kThreads - 128, lane);
   else if (warp < kWarps + 8 + kRecorders) lost = record_tiles<TX, TA, V, kGate, false>(P, sm, warp - kWarps - 8, lane);
   else if (lane == 0) lost = issue_tiles<TX, TA, V, kGate, false>(P, maps, sm);
   if (lost && lane == 0 && P.A.status) atomicOr(reinterpret_cast<unsigned *>(P.A.status), GEARB_ST_SCAN_ABORTED);
 }
 
-template <typename TX, typename TA, int V, int kGate>
+template <typename TX, typename TA, int V, int kGate, bool kLong>
 __global__ void __launch_bounds__(kStreamThreads, 1) backward_stream_kernel(const __grid_constant__ Params P,
                                                                             const __grid_constant__ Maps maps) {
   using Shared = StreamShared<TX, TA, V, kGate, true>;
@@ -871,7 +880,7 @@ __global__ void __launch_bounds__(kStreamThreads, 1) backward_stream_kernel(cons
   bool lost = false;
   if (warp < kWarps) lost = compute_backward<TX, TA, V, kGate>(P, sm, warp, lane);
   else if (warp < kWarps + 4) lost = publish_tiles<TX, TA, V, kGate, true>(P, sm, threadIdx.x - kThreads, lane);
-  else if (warp < kWarps + 8) lost = finish_tiles<TX, TA, V, kGate, true>(P, sm, threadIdx.x - kThreads - 128, lane);
+  else if (warp < kWarps + 8) lost = finish_tiles<TX, TA, V, kGate, true, kLong>(P, sm, threadIdx.x - kThreads - 128, lane);
   else if (warp < kWarps + 8 + kRecorders) lost = record_tiles<TX, TA, V, kGate, true>(P, sm, warp - kWarps - 8, lane);
   else if (lane == 0) lost = issue_tiles<TX, TA, V, kGate, true>(P, maps, sm);
   if (lost && lane == 0 && P.A.status) atomicOr(reinterpret_cast<unsigned *>(P.A.status), GEARB_ST_SCAN_ABORTED);
@@ -902,8 +911,11 @@ int launch_stream(Params &p, cudaStream_t stream) {
   constexpr int kSmem = sizeof(StreamShared<TX, TA, V, kGate, kBackward>);
   static_assert(kSmem <= kSmemMost, "fits one SM");
   void (*kernel)(Params, Maps);
-  if constexpr (kBackward) kernel = backward_stream_kernel<TX, TA, V, kGate>;
-  else kernel = forward_stream_kernel<TX, TA, V, kGate>;
+  // a kernel each: with both ways in one, packed heads take 10 % longer
+  const bool far = p.chain && long_sections(p, p.ncol);
+  p.section_shift = far ? kLongSection : kShortSection;
+  if constexpr (kBackward) kernel = far ? backward_stream_kernel<TX, TA, V, kGate, true> : backward_stream_kernel<TX, TA, V, kGate, false>;
+  else kernel = far ? forward_stream_kernel<TX, TA, V, kGate, true> : forward_stream_kernel<TX, TA, V, kGate, false>;
   GEARB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
   const int64_t most = sm_count(), items = p.tiles * ncol;
   kernel<<<static_cast<unsigned>(items < most ? items : most), kStreamThreads, kSmem, stream>>>(p, maps);

@@ -173,14 +173,10 @@ __global__ void __launch_bounds__(kThreads, V == 4 ? 2 : V == 2 ? 3 : 5) forward
     if (P.chain) {
       publish_pair(P.agg + pl.tile * A.width + ch2, ta, th);
       const int64_t lo = sfirst >= 0 ? quotient(sfirst, P.tile_rows) : pl.tile;
-      if (lo < pl.tile) {
-        bool lost = false;
-        cin = look_back(P, pl.tile, lo, ch2, lost);
-        if (lost && A.status) atomicOr(reinterpret_cast<unsigned *>(A.status), GEARB_ST_SCAN_ABORTED);
-        if (A.carry) A.carry[pl.tile * A.width + ch2] = cin;
-      }
-      if (pl.tile % kSuper == kSuper - 1 && pl.tile + 1 < P.tiles)
-        publish_word(P.super + (pl.tile / kSuper + 1) * A.width + ch2, cut ? th : fmaf(ta, cin, th));
+      bool lost = false;
+      cin = look_back<4, 0, int64_t>(P, pl.tile, lo, ch2, [&] { return make_float2(ta, th); }, cut, lost);
+      if (lost && A.status) atomicOr(reinterpret_cast<unsigned *>(A.status), GEARB_ST_SCAN_ABORTED);
+      if (lo < pl.tile && A.carry) A.carry[pl.tile * A.width + ch2] = cin;
     }
     cut = false;
 #pragma unroll
@@ -359,13 +355,9 @@ __global__ void __launch_bounds__(kThreads, V == 4 ? 2 : V == 2 ? 3 : 4) backwar
       if (P.chain) {
         publish_pair(P.agg + at * A.width + ch2, ta, tc);
         const int64_t lo = slast >= 0 ? P.tiles - 1 - quotient(slast, P.tile_rows) : at;
-        if (lo < at) {
-          bool lost = false;
-          cin = look_back(P, at, lo, ch2, lost);
-          if (lost && A.status) atomicOr(reinterpret_cast<unsigned *>(A.status), GEARB_ST_SCAN_ABORTED);
-        }
-        if (at % kSuper == kSuper - 1 && at + 1 < P.tiles)
-          publish_word(P.super + (at / kSuper + 1) * A.width + ch2, cut ? tc : fmaf(ta, cin, tc));
+        bool lost = false;
+        cin = look_back<4, 0, int64_t>(P, at, lo < at ? lo : at, ch2, [&] { return make_float2(ta, tc); }, cut, lost);
+        if (lost && A.status) atomicOr(reinterpret_cast<unsigned *>(A.status), GEARB_ST_SCAN_ABORTED);
       }
       cut = false;
 #pragma unroll
@@ -501,6 +493,7 @@ int launch_wide(Params &p, bool backward, cudaStream_t stream) {
   const int64_t ncol = kGate == kOne ? a.gates * p.blocks_per_gate : (a.width + p.block - 1) / p.block;
   GEARB_REQUIRE(p.tiles <= (int64_t(1) << 31) / ncol - 1, "recurrence: too many tiles for one launch");
   p.ncol = static_cast<int>(ncol);
+  p.section_shift = long_sections(p, p.ncol) ? kLongSection : kShortSection;
   const unsigned grid = static_cast<unsigned>(p.tiles * ncol);
   if (p.chain) GEARB_CUDA(cudaMemsetAsync(p.ticket, 0xff, static_cast<size_t>(p.chain_bytes), stream));
   if (backward) backward_kernel<TX, TA, V, kGate><<<grid, kThreads, 0, stream>>>(p);

@@ -133,6 +133,41 @@ def test_padded(width, gates, reverse, time):
     run_and_check(x, gate, state_of(time, 9, width), lengths=torch.from_numpy(lens).to(DEV), reverse=reverse, log=True)
 
 
+def slow(seed, lead, width, gates, dtype, gate_dtype):
+    """Log gates that remember thousands of rows."""
+    rng = np.random.default_rng(seed)
+    x = torch.from_numpy(rng.standard_normal(lead + (width,)).astype(np.float32)).to(dtype).to(DEV)
+    g = torch.from_numpy((-rng.uniform(0, 1e-3, lead + (gates,))).astype(np.float32)).to(gate_dtype).to(DEV)
+    return x, g
+
+
+# One channel block of the streaming kernels, rows that only the fallback reads, few channels at 4 and 16 rows a thread.
+@pytest.mark.parametrize("batch,time,width,gates", [(1, 9500, 48, 48), (2, 8500, 64, 4), (1, 9500, 43, 43), (2, 4400, 33, 3),
+                                                    (2, 9000, 16, 16), (1, 40000, 16, 4), (1, 140000, 1, 1)])
+@pytest.mark.parametrize("reverse", [False, True])
+def test_states_over_thousands_of_rows(batch, time, width, gates, reverse):
+    x, gate = slow(time + width, (batch, time), width, gates, F32, F32)
+    run_and_check(x, gate, h0=state_of(8, batch, width), reverse=reverse, log=True)
+
+
+@pytest.mark.parametrize("width,gates", [(48, 48), (43, 43), (64, 2), (12, 12)])
+@pytest.mark.parametrize("reverse", [False, True])
+def test_packed_starts_anywhere_in_thousands_of_rows(width, gates, reverse):
+    # starts on, before and behind the ends of tiles, of eight tiles and of sixty-four
+    lens = [3, 700, 3393, 4096, 0, 1, 4607, 512, 63, 5000, 1, 4200]
+    off = torch.tensor(np.cumsum([0] + lens), dtype=torch.int64, device=DEV)
+    x, gate = slow(17, (int(off[-1]),), width, gates, BF16, F32)
+    run_and_check(x, gate, h0=state_of(9, len(lens), width), offsets=off, reverse=reverse, log=True)
+
+
+@pytest.mark.parametrize("width", [48, 45, 5])
+def test_padded_ends_anywhere_in_thousands_of_rows(width):
+    x, gate = slow(18, (4, 6000), width, width, F32, F32)
+    lens = torch.tensor([6000, 4097, 0, 4544], dtype=torch.int64, device=DEV)
+    for reverse in (False, True):
+        run_and_check(x, gate, lengths=lens, reverse=reverse, log=True)
+
+
 def test_offsets_need_not_start_at_row_zero():
     off = torch.tensor([10, 10, 75, 200], device=DEV)
     for width, reverse in ((1, True), (70, False), (70, True), (4, False)):
