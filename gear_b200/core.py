@@ -278,6 +278,9 @@ class StorageHandler:
         if out is not None and out.numel() != n:
             raise GearError(N.ERR_INVALID, "out must have one entry per request")
         ptrs = [_dev_i64(t, w) for t, w in ((idx, "idx"), (ts, "ts"), (ln, "len"))]
+        for t, w in ((ts, "ts"), (ln, "len"), (out, "out")):
+            if t is not None and t.device != idx.device:
+                raise GearError(N.ERR_INVALID, f"{w} is on {t.device}, idx on {idx.device}")
         with _Scope(idx.device, stream):
             if out is None:
                 out = torch.empty(n, dtype=torch.int64, device=idx.device)
@@ -319,6 +322,8 @@ class StorageHandler:
             if block_table.dtype != torch.int32 or not block_table.is_cuda or not block_table.is_contiguous() \
                     or block_table.dim() != 2 or block_table.shape[0] != n:
                 raise GearError(N.ERR_INVALID, "block_table must be a contiguous int32 CUDA tensor [requests, max_blocks]")
+            if not 1 <= int(page) <= 1 << 31:
+                raise GearError(N.ERR_INVALID, "page must be 1 to 2^31")
             bt, max_blocks = block_table, block_table.shape[1]
         if past is not None and past.numel() != n:
             raise GearError(N.ERR_INVALID, "past must have one entry per request")

@@ -261,7 +261,7 @@ __device__ __forceinline__ void fill_stretch(const LayoutParams &P, int64_t tota
     if (t < a.max_tokens) a.slot_map[t] = -1;
 }
 
-// One CTA: the prefix sums, and with kFill everything.
+// One CTA: the prefix sums, and with kFill (a request a thread at most) everything.
 template <bool kFill>
 __global__ void __launch_bounds__(kScanThreads) layout_scan_kernel(const __grid_constant__ LayoutParams P) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -271,13 +271,13 @@ __global__ void __launch_bounds__(kScanThreads) layout_scan_kernel(const __grid_
   unsigned flags = 0;
   __syncthreads();  // everybody has read used_in: used_out may be the same word
   Request own{0, 0, 0, 0, 0, 0};
-  if (a.requests <= kScanThreads) place_requests<1>(P, 0, a.requests, tokens, pages, flags, sm, &own);
+  if (kFill || a.requests <= kScanThreads) place_requests<1>(P, 0, a.requests, tokens, pages, flags, sm, &own);
   else place_requests<kPer>(P, 0, a.requests, tokens, pages, flags, sm);
   if (threadIdx.x == 0) finish_sums(a, tokens, pages, flags);
   if (flags && a.status) atomicOr(reinterpret_cast<unsigned *>(a.status), flags);
   if constexpr (kFill) {
     // A decoding step: a thread places the few tokens of its request itself.
-    if (!__syncthreads_or(a.requests > kScanThreads || own.end - own.first > 4)) {
+    if (!__syncthreads_or(own.end - own.first > 4)) {
       for (int64_t t = own.first; t < own.end; ++t) {
         const int64_t slot = place_token(P, own, t);
         if (t < a.max_tokens) a.slot_map[t] = slot;

@@ -77,10 +77,12 @@ def paged_layout(lengths: torch.Tensor, page: int, block_table: torch.Tensor, us
     at_used = _need(used, "used", torch.int64, dev, 1)
     if free_pages is None and num_pages is None:
         raise GearError(N.ERR_INVALID, "paged_layout: num_pages is required without free_pages")
-    pages = free_pages.numel() if num_pages is None else int(num_pages)
+    pages = free_pages.numel() if num_pages is None else num_pages
     if free_pages is not None and pages > free_pages.numel():
         raise GearError(N.ERR_INVALID, "paged_layout: num_pages is more than free_pages has")
-    max_tokens = int(max_tokens)
+    page, pages, max_tokens = int(page), int(pages), int(max_tokens)
+    if not 1 <= page <= 1 << 31 or not 0 <= pages <= 1 << 31:
+        raise GearError(N.ERR_INVALID, "paged_layout: page must be 1 to 2^31, num_pages 0 to 2^31")
     if slot_map is not None:
         _need(slot_map, "slot_map", torch.int64, dev)
         if max_tokens not in (0, slot_map.numel()):
@@ -102,7 +104,7 @@ def paged_layout(lengths: torch.Tensor, page: int, block_table: torch.Tensor, us
             used_out = torch.empty(1, dtype=torch.int64, device=dev)
         nbytes = lib.gearb_layout_scratch_bytes(r)
         scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        check(_LAYOUT(N.LAYOUT_ARGS.pack(at_lengths, at_past, r, int(page), shape[1], at_table, at_free, pages, at_used,
+        check(_LAYOUT(N.LAYOUT_ARGS.pack(at_lengths, at_past, r, page, shape[1], at_table, at_free, pages, at_used,
                                          used_out.data_ptr(), offsets.data_ptr(),
                                          0 if slot_map is None else slot_map.data_ptr(), max_tokens,
                                          scratch.data_ptr(), nbytes, at_status), _stream()))

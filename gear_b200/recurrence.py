@@ -160,8 +160,11 @@ def linear_recurrence(x: torch.Tensor, gate: torch.Tensor, *, h0: Optional[torch
 
     Arithmetic and state are float32 whatever x's type; h is rounded once to x's type.  The bits of the result
     depend on nothing but the inputs' values and shape.  Differentiable once in x, gate and h0; the backward pass
-    recomputes h in float32.  Gates whose product over some thousand rows passes float32's range (|a| well
-    above 1) overflow."""
+    recomputes h in float32.  Products of a sequence's gates over up to 512 rows (32768 of a single channel) must stay
+    inside float32's range, and so must exp(gate): where they pass it (|a| well above 1) h is infinite or NaN.
+
+    Capturing a backward pass into a CUDA graph: as for any autograd function, let no eager graph of the same leaves
+    live meanwhile, and warm up on a side stream."""
     if not isinstance(x, torch.Tensor) or not isinstance(gate, torch.Tensor):
         _bad("x and gate must be tensors")
     xd, gd = _DTYPES.get(x.dtype), _DTYPES.get(gate.dtype)

@@ -246,3 +246,96 @@ def test_from_a_draw_to_advantages(O):
                        for k in range(len(seg))])
         assert np.abs(d[go[r]: go[r + 1], 0].cpu().numpy() - gk).max() <= 1e-5 * max(1.0, np.abs(gk).max())
     assert (ret[total:] == 0).all() and (d[total:] == 0).all()
+
+
+def test_refuses_pages_beyond_the_argument():
+    t, _ = make_table([8], 20, 4)
+    h = core.StorageHandler(t)
+    h.set([0], [core.SubscribePattern(0, 20, 0)])
+    z = torch.zeros(2, dtype=torch.int64, device=DEV)
+    for page in (1 << 70, (1 << 64) + 16, -1):
+        with pytest.raises(core.GearError) as e:
+            h.gather_packed([0], z, z, z + 20, torch.tensor([0, 20, 40], device=DEV), [torch.zeros(64, 8, dtype=torch.uint8, device=DEV)],
+                            block_table=torch.zeros(2, 2, dtype=torch.int32, device=DEV), page=page)
+        assert e.value.code == N.ERR_INVALID
+
+
+def test_destinations_beyond_32_bits():
+    """Rows past 2^31 of a packed destination, pages past 2^31 rows of a pool; the same trajectory twice."""
+    rows, T, cap = [4, 1], 40, 3
+    t, img = make_table(rows, T, cap)
+    h = core.StorageHandler(t)
+    h.set([0, 1], [core.SubscribePattern(0, T, 0)] * 2)
+    big = (1 << 31) + 200
+    dsts = [torch.zeros(big, r, dtype=torch.uint8, device=DEV) for r in rows]
+    idx = torch.tensor([2, 2], dtype=torch.int64, device=DEV)
+    z = torch.zeros(2, dtype=torch.int64, device=DEV)
+    off = torch.tensor([big - 80, big - 40, big], device=DEV)
+    h.gather_packed([0, 1], idx, z, z + T, off, dsts)
+    for c in (0, 1):
+        base = 2 * t.trajectory_stride + t.column_offset(c)
+        want = torch.from_numpy(img[base: base + T * rows[c]].reshape(T, rows[c]).copy()).to(DEV)
+        assert torch.equal(dsts[c][big - 80: big - 40], want) and torch.equal(dsts[c][big - 40:], want)
+        assert int(dsts[c][: big - 80].max()) == 0
+        dsts[c].zero_()
+    last = big // 8 - 5
+    table = torch.arange(last, last - 10, -1, dtype=torch.int32, device=DEV).reshape(2, 5)
+    h.gather_packed([0, 1], idx, z, z + T, off, dsts, block_table=table, page=8)
+    for c in (0, 1):
+        base = 2 * t.trajectory_stride + t.column_offset(c)
+        want = torch.from_numpy(img[base: base + T * rows[c]].reshape(T, rows[c]).copy()).to(DEV)
+        pages = dsts[c][: big // 8 * 8].reshape(big // 8, 8, rows[c])
+        for r in range(2):
+            assert torch.equal(pages[table[r].long()].reshape(T, rows[c]), want)
+        assert int(dsts[c][: (last - 9) * 8].max()) == 0
+    assert h.status() == 0
+
+
+def test_layout_and_gather_captured_once_follow_their_inputs():
+    """One graph from lengths to rows, replayed with other requests, beside the same graph on a second stream."""
+    rows, T, cap, n, page = [12, 4], 60, 9, 50, 8
+    t, img = make_table(rows, T, cap)
+    rng = np.random.default_rng(4)
+    blocks = -(-T // page)
+    graphs = []
+    for _ in range(2):
+        h = core.StorageHandler(t)
+        h.set([0, 1], [core.SubscribePattern(-3, T, 0)] * 2)
+        inp = [torch.zeros(n, dtype=torch.int64, device=DEV) for _ in range(3)]
+        used = torch.zeros(1, dtype=torch.int64, device=DEV)
+        table = torch.full((n, blocks), -1, dtype=torch.int32, device=DEV)
+        pools = [torch.zeros(n * blocks * page, r, dtype=torch.uint8, device=DEV) for r in rows]
+
+        def step():
+            lens = h.segment_lengths(*inp, 0)
+            lay = layout.paged_layout(lens, page, table, used, num_pages=n * blocks, max_tokens=64)
+            h.gather_packed([0, 1], *inp, lay.offsets, pools, block_table=table, page=page)
+            return lens, lay
+        step()
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            res = step()
+        graphs.append((g, inp, table, pools, res, torch.cuda.Stream(), h))
+    for _ in range(3):
+        wants = []
+        for g, inp, table, pools, res, st, h in graphs:
+            req = requests(rng, n, T, cap)
+            for a, b in zip(inp, req):
+                a.copy_(torch.from_numpy(b))
+            for p in pools:
+                p.zero_()
+            start, count = clip(t, core.SubscribePattern(-3, T, 0), *req)
+            wants.append((req, start, count))
+        torch.cuda.synchronize()
+        for g, _i, _t, _p, _r, st, _h in graphs:
+            with torch.cuda.stream(st):
+                g.replay()
+        torch.cuda.synchronize()
+        for (g, inp, table, pools, (lens, lay), st, h), (req, start, count) in zip(graphs, wants):
+            offsets = np.concatenate([[0], np.cumsum(count)])
+            assert np.array_equal(lens.cpu().numpy(), count) and np.array_equal(lay.offsets.cpu().numpy(), offsets)
+            tab = table.cpu().numpy()
+            for c in (0, 1):
+                want = plain(t, img, c, start, count, req[0], offsets, np.zeros((n * blocks * page, rows[c]), np.uint8), tab, page)
+                assert np.array_equal(pools[c].cpu().numpy(), want)

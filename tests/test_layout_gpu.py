@@ -194,3 +194,47 @@ def test_refusals():
         with pytest.raises(core.GearError) as e:
             f()
         assert e.value.code == N.ERR_INVALID, i
+
+
+def test_refuses_sizes_beyond_the_argument_block():
+    L = torch.ones(4, dtype=torch.int64, device=DEV)
+    T = torch.zeros(4, 2, dtype=torch.int32, device=DEV)
+    U = torch.zeros(1, dtype=torch.int64, device=DEV)
+    for kw in (dict(page=1 << 70, num_pages=5), dict(page=16, num_pages=1 << 70), dict(page=(1 << 64) + 16, num_pages=5),
+               dict(page=16, num_pages=-(1 << 70))):
+        with pytest.raises(core.GearError) as e:
+            layout.paged_layout(L, block_table=T, used=U, **kw)
+        assert e.value.code == N.ERR_INVALID
+
+
+@pytest.mark.parametrize("requests,most", [(1024, 3), (1024, 30), (1025, 3), (1, 4096), (700, 5), (8192, 2), (8193, 2), (20000, 1)])
+@pytest.mark.parametrize("room", [1, 4096, 4097])
+def test_ways_of_the_scan_and_of_the_fill(requests, most, room):
+    """Sizes on both sides of every choice: requests a thread, one launch or several, tokens a request."""
+    rng = np.random.default_rng(requests + most)
+    lengths = rng.integers(0, most + 1, requests)
+    past = rng.integers(0, 20, requests)
+    page, blocks = 8, -(-(most + 20) // 8)
+    have = -(-past // page)
+    table = np.full((requests, blocks), -1, np.int32)
+    nxt = 0
+    for r in range(requests):
+        table[r, :have[r]] = np.arange(nxt, nxt + have[r])
+        nxt += have[r]
+    free = (nxt + np.random.default_rng(1).permutation(requests * blocks)).astype(np.int32)
+    dev = lambda a: torch.from_numpy(np.ascontiguousarray(a)).to(DEV)
+    used = torch.tensor([7], dtype=torch.int64, device=DEV)
+    lay = layout.paged_layout(dev(lengths), page, dev(table), used, free_pages=dev(free), past=dev(past), max_tokens=room)
+    want_table, at, slots = table.copy(), 7, []
+    for r in range(requests):
+        need = -(-(past[r] + lengths[r]) // page) - have[r]
+        want_table[r, have[r]:have[r] + need] = free[at:at + need]
+        at += need
+        for t in range(past[r], past[r] + lengths[r]):
+            slots.append(int(want_table[r, t // page]) * page + t % page)
+    want_slots = np.full(room, -1, np.int64)
+    want_slots[:min(room, len(slots))] = slots[:room]
+    assert np.array_equal(lay.offsets.cpu().numpy(), np.concatenate([[0], np.cumsum(lengths)]))
+    assert np.array_equal(lay.block_table.cpu().numpy(), want_table)
+    assert int(lay.used) == at
+    assert np.array_equal(lay.slot_map.cpu().numpy(), want_slots)

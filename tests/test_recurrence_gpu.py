@@ -454,3 +454,76 @@ def test_refusals():
     d, = torch.autograd.grad(h.sum(), xg, create_graph=True)
     with pytest.raises(RuntimeError):
         d.sum().backward()
+
+
+@pytest.mark.parametrize("width,gates", [(96, 48), (96, 32), (99, 33), (99, 9), (102, 6), (130, 10), (128, 8), (143, 11), (66, 3),
+                                         (96, 4), (50, 2), (58, 2), (200, 1), (63, 7), (18, 9), (260, 130)])
+@pytest.mark.parametrize("dtype,gate_dtype", [(F32, F32), (BF16, BF16)])
+def test_shared_gates_of_any_share(width, gates, dtype, gate_dtype):
+    """Shares of 2 to 200 channels, with blocks that hold many gates, a few or a part of one."""
+    x, gate = make(width + gates, (2, 150), width, gates, dtype, gate_dtype, False)
+    run_and_check(x, gate, h0=state_of(1, 2, width))
+    off = torch.tensor([0, 40, 41, 200, 290], dtype=torch.int64, device=DEV)
+    run_and_check(x.reshape(300, width), gate.reshape(300, gates), h0=state_of(2, 4, width), offsets=off, reverse=True)
+
+
+@pytest.mark.parametrize("width,gates", [(64, 64), (64, 16), (63, 63), (63, 9), (64, 1)])
+def test_rows_that_start_anywhere(width, gates):
+    """Tensors inside larger ones, at offsets of one element: no vector access, no tensor copy."""
+    big = torch.empty(2, 70, width + 3, dtype=BF16, device=DEV)
+    gbig = torch.empty(2, 70, gates + 5, dtype=F32, device=DEV)
+    x, gate = make(5, (2, 70), width, gates, BF16, F32, False)
+    big[..., 1:1 + width], gbig[..., 3:3 + gates] = x, gate
+    xv, gv = big[..., 1:1 + width], gbig[..., 3:3 + gates]
+    want, ws = run_and_check(x, gate)
+    h, st = recurrence.linear_recurrence(xv, gv)
+    assert torch.equal(h, want) and torch.equal(st, ws)
+    # one row a sequence
+    h0 = state_of(3, 2, width)
+    one, s1 = recurrence.linear_recurrence(x[:, :1], gate[:, :1], h0=h0)
+    two, s2 = recurrence.linear_recurrence(xv[:, :1], gv[:, :1], h0=h0)
+    assert torch.equal(one, two) and torch.equal(s1, s2)
+    ref = R.reference(dbl(x[:, 0]), dbl(gate[:, 0]), [(0, 1), (1, 2)], dbl(h0))
+    R.check(one, ref["h"], BF16, "h")
+    R.check(s1, ref["state"], F32, "state")
+
+
+@pytest.mark.parametrize("width", [5, 40, 64])
+def test_state_in_place_with_one_row(width):
+    """state_out may be h0: padded and packed rows of one step too."""
+    x, gate = make(6, (7, 1), width, width, F32, F32, False)
+    h0 = state_of(4, 7, width)
+    for kw in (dict(lengths=torch.tensor([1, 0, 1, 1, 0, 1, 1], device=DEV)), {}):
+        want, ws = recurrence.linear_recurrence(x, gate, h0=h0, **kw)
+        state = h0.clone()
+        got, _ = recurrence.linear_recurrence(x, gate, h0=state, state_out=state, **kw)
+        assert torch.equal(got, want) and torch.equal(state, ws)
+    off = torch.tensor([0, 0, 1, 1], device=DEV)
+    want, ws = recurrence.linear_recurrence(x[0], gate[0], h0=h0[:3], offsets=off)
+    state = h0[:3].clone()
+    got, _ = recurrence.linear_recurrence(x[0], gate[0], h0=state, offsets=off, state_out=state)
+    assert torch.equal(got, want) and torch.equal(state, ws) and torch.equal(ws[0], h0[0])
+
+
+@pytest.mark.parametrize("width", [64, 33, 1])
+def test_beyond_32_bits(width):
+    """A sequence behind element 2^31 of every tensor, in the streaming, the fallback and the narrow kernels."""
+    tail = 5000
+    rows = (1 << 31) // width + 3 * tail
+    x = torch.zeros(rows, width, dtype=BF16, device=DEV)
+    gate = torch.full((rows, width), 0.5, dtype=BF16, device=DEV)
+    xs, gs = make(3, (tail,), width, width, BF16, BF16, False)
+    x[-tail:], gate[-tail:] = xs, gs
+    dh = torch.zeros_like(x)
+    dh[-tail:] = torch.randn(tail, width, device=DEV).to(BF16)
+    off = torch.tensor([0, rows - tail, rows], device=DEV)
+    x.requires_grad_(True), gate.requires_grad_(True)
+    h, state = recurrence.linear_recurrence(x, gate, offsets=off)
+    dx, dgate = torch.autograd.grad(h, [x, gate], dh)
+    want = R.reference(dbl(xs), dbl(gs), [(0, tail)], dh=dbl(dh[-tail:]))
+    R.check(h[-tail:], want["h"], BF16, "h")
+    R.check(state[1:], want["state"], F32, "state")
+    R.check(dx[-tail:], want["dx"], BF16, "dx")
+    R.check(dgate[-tail:], want["dgate"], BF16, "dgate")
+    for t in (h, dx, dgate):
+        assert not t[:-tail].any()
