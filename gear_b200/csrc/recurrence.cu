@@ -50,12 +50,15 @@ __global__ void __launch_bounds__(kThreads) gate_sum_kernel(const __grid_constan
   const int64_t n = P.rows * A.gates;
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < n;
        i += static_cast<int64_t>(gridDim.x) * kThreads) {
-    if (!A.zero_rest) {
+    if (A.offsets || A.lengths) {
       const int64_t row = i / A.gates;
       bool live;
       if (A.offsets) live = row >= __ldg(A.offsets) && row < __ldg(A.offsets + A.sequences);
-      else live = !A.lengths || row % A.time < __ldg(A.lengths + row / A.time);
-      if (!live) continue;
+      else live = row % A.time < __ldg(A.lengths + row / A.time);
+      if (!live) {
+        if (A.zero_rest) static_cast<TA *>(A.dgate)[i] = from_f<TA>(0.0f);
+        continue;
+      }
     }
     float sum = P.gate_part[i];
     for (int b = 1; b < P.blocks_per_gate; ++b) sum += P.gate_part[b * n + i];
@@ -70,13 +73,34 @@ __global__ void states_kernel(const float *from, float *to, int64_t n) {
     to[i] = from ? from[i] : 0.0f;
 }
 
-// One warp per tile: its rows among the sequences.  All warps: 0xff where tiles will publish.
+__device__ __forceinline__ void zero_span(char *p, int64_t n, int64_t me, int64_t threads) {
+  int64_t head = (16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15;
+  if (head > n) head = n;
+  const int64_t vecs = (n - head) / 16, done = head + vecs * 16;
+  if (me < head) p[me] = 0;
+  if (me < n - done) p[done + me] = 0;
+  for (int64_t i = me; i < vecs; i += threads) reinterpret_cast<uint4 *>(p + head)[i] = make_uint4(0, 0, 0, 0);
+}
+
+// One warp per tile: its rows among the sequences.  All warps: 0xff where tiles will publish, and zeros where packed
+// sequences leave whole tiles.
 __global__ void __launch_bounds__(kThreads) prepare_kernel(const __grid_constant__ Params P) {
   const gearb_recurrence_args &A = P.A;
   const int lane = threadIdx.x & 31;
   const int64_t threads = static_cast<int64_t>(gridDim.x) * kThreads, me = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
   uint4 *fill = reinterpret_cast<uint4 *>(P.ticket);  // whole multiples of 256 bytes
   for (int64_t i = me; i < P.chain_bytes / 16; i += threads) fill[i] = make_uint4(kUnset, kUnset, kUnset, kUnset);
+  const LiveTiles live_range = live_tiles(P);
+  if (A.offsets && A.zero_rest) {
+    const int64_t end = live_range.end * P.tile_rows, d0 = live_range.first * P.tile_rows, d1 = end < P.rows ? end : P.rows;
+    auto zero = [&](void *base, int64_t row_bytes) {
+      char *b = static_cast<char *>(base);
+      zero_span(A.reverse ? b + (P.rows - d0) * row_bytes : b, d0 * row_bytes, me, threads);
+      zero_span(A.reverse ? b : b + d1 * row_bytes, (P.rows - d1) * row_bytes, me, threads);
+    };
+    zero(P.backward ? A.dx : A.out, A.width * (A.x_dtype == GEARB_DT_F32 ? 4 : 2));
+    if (P.backward && P.blocks_per_gate == 1) zero(A.dgate, A.gates * (A.gate_dtype == GEARB_DT_F32 ? 4 : 2));
+  }
   // sequences without rows keep their state (backward: their gradient)
   float *to = P.backward ? A.dh0 : A.state_out;
   const float *old = P.backward ? A.dstate : A.h0;
@@ -86,7 +110,7 @@ __global__ void __launch_bounds__(kThreads) prepare_kernel(const __grid_constant
       if ((A.offsets ? so.at(s + 1) - so.at(s) : __ldg(A.lengths + s)) > 0) continue;
       for (int64_t d = lane; d < A.width; d += 32) to[s * A.width + d] = old ? old[s * A.width + d] : 0.0f;
     }
-  for (int64_t tile = me >> 5; tile < P.tiles; tile += threads >> 5) {
+  for (int64_t tile = live_range.first + (me >> 5); tile < live_range.end; tile += threads >> 5) {
     Place at = {};
     at.tile = tile;
     at.i0 = tile * P.tile_rows;
@@ -358,6 +382,10 @@ int run(const gearb_recurrence_args *args, bool backward, void *stream) {
 int rec::launch_prepare(const Params &p, cudaStream_t stream) {
   int64_t warps = p.tiles > p.chain_bytes / 2048 ? p.tiles : p.chain_bytes / 2048;  // up to 64 bytes a thread
   if ((p.A.offsets || p.A.lengths) && warps < p.A.sequences) warps = p.A.sequences;
+  if (p.A.offsets && p.A.zero_rest) {  // up to 256 bytes a thread, were there no sequences at all
+    const int64_t bytes = p.rows * p.A.width * (p.A.x_dtype == GEARB_DT_F32 ? 4 : 2);
+    if (warps < bytes / 8192) warps = bytes / 8192;
+  }
   const int64_t blocks = (warps + kWarps - 1) / kWarps, most = static_cast<int64_t>(sm_count()) * 8;
   prepare_kernel<<<static_cast<unsigned>(blocks < most ? (blocks > 0 ? blocks : 1) : most), kThreads, 0, stream>>>(p);
   GEARB_CUDA(cudaGetLastError());

@@ -402,6 +402,21 @@ __device__ __forceinline__ TileRows tile_rows_packed(const Params &P, const Plac
   return t;
 }
 
+// Tiles with rows of sequences, [first, end): packed sequences may leave rows in front of the first and behind the last.
+struct LiveTiles {
+  int64_t first, end;
+};
+__device__ __forceinline__ LiveTiles live_tiles(const Params &P) {
+  if (!P.A.offsets) return {0, P.tiles};
+  const ScanOffsets so{P.A.offsets, P.rows, P.A.sequences, P.A.reverse};
+  const int64_t lo = so.at(0), hi = so.at(P.A.sequences);
+  LiveTiles t;
+  t.first = quotient(lo, P.tile_rows);
+  t.end = quotient(hi + P.tile_rows - 1, P.tile_rows);
+  if (hi <= lo) t.end = t.first;
+  return t;
+}
+
 // V consecutive channels of a warp's n rows of the scan (zeros where there is no row or channel).
 template <typename T, int V>
 __device__ __forceinline__ void load_rows(const T *base, const Params &P, const Place &pl, const TileRows &tr, int64_t period,

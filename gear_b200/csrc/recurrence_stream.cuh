@@ -33,6 +33,7 @@ constexpr int kMostStages = 6;
 constexpr int kRecorders = 2;  // one takes 3 us a tile: two dependent trips to L2
 constexpr int kTableGates = 8;
 
+constexpr unsigned kNoItem = 0xffffffffu;
 constexpr unsigned kWaitLimit = 1u << 20;  // mbarrier polls before a copy is declared lost
 
 __device__ __forceinline__ uint32_t smem_addr(const void *p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
@@ -254,22 +255,19 @@ template <typename TX, typename TA, int V, int kGate, bool kBackward>
 __device__ __forceinline__ bool issue_tiles(const Params &P, const Maps &maps, StreamShared<TX, TA, V, kGate, kBackward> &sm) {
   using Shared = StreamShared<TX, TA, V, kGate, kBackward>;
   const gearb_recurrence_args &A = P.A;
-  const unsigned items = static_cast<unsigned>(P.tiles * P.ncol);
-  // Packed rows of no sequence need no copies.
-  int64_t lo = 0, hi = P.rows;
-  if (A.offsets) {
-    const ScanOffsets so{A.offsets, P.rows, A.sequences, A.reverse};
-    lo = so.at(0);
-    hi = so.at(A.sequences);
-  }
+  // Tiles without sequences are no items: the launch before has zeroed their rows.  (Taken through the pipeline, the
+  // 43 % of a packed batch's room that no sequence filled cost a quarter of the time.)
+  const LiveTiles live = live_tiles(P);
+  const unsigned base = static_cast<unsigned>((kBackward ? P.tiles - live.end : live.first) * P.ncol);
+  const unsigned items = base + static_cast<unsigned>((live.end - live.first) * P.ncol);
   // One number at a time from the start: CTAs that took several at once would come to tiles much later than others come to
   // the tiles behind them, and those would wait.
-  unsigned next = P.chain ? atomicAdd(P.ticket, 1u) + 1u : blockIdx.x;  // the counter starts at 0xffffffff
+  unsigned next = base + (P.chain ? atomicAdd(P.ticket, 1u) + 1u : blockIdx.x);  // the counter starts at 0xffffffff
   Turn<Shared::kStages> now;
   for (unsigned m = 0;; ++m, now.next()) {
     if (m >= Shared::kStages && !mbar_wait(&sm.empty[now.i], now.parity ^ 1u)) return true;
     const unsigned item = next;
-    sm.item[now.i] = item;
+    sm.item[now.i] = item < items ? item : kNoItem;
     if (item >= items) {
       mbar_arrive(&sm.full[now.i]);
       for (int r = 0; r < kRecorders; ++r) {  // every recorder has to learn that there are no more
@@ -278,25 +276,21 @@ __device__ __forceinline__ bool issue_tiles(const Params &P, const Maps &maps, S
         if (r + 1 < kRecorders) {
           ++m;
           if (m >= Shared::kStages && !mbar_wait(&sm.empty[now.i], now.parity ^ 1u)) return true;
-          sm.item[now.i] = item;
+          sm.item[now.i] = kNoItem;
         }
       }
       return false;
     }
     const Place at = place_of_item<V, kGate, kBackward>(P, item);
     uint64_t *full = &sm.full[now.i];
-    if (at.i0 < hi && at.i1 > lo) {
-      // a reverse call's tile ends at row_of(i0): its box begins kTile - 1 rows before, if need be in front of the matrix
-      const int row0 = static_cast<int>(row_of(P, at.i0)), c = static_cast<int>(at.d0), r = A.reverse ? row0 - (kTile - 1) : row0;
-      mbar_expect(full, Shared::StageT::kBytes);
-      tensor_load(sm.stage[now.i].x, &maps.x, c, r, full);
-      if constexpr (kGate == kOwn) tensor_load(sm.stage[now.i].gate, &maps.gate, c, r, full);
-      if constexpr (kBackward) tensor_load(sm.stage[now.i].dout, &maps.dout, c, r, full);
-    } else {
-      mbar_arrive(full);
-    }
+    // a reverse call's tile ends at row_of(i0): its box begins kTile - 1 rows before, if need be in front of the matrix
+    const int row0 = static_cast<int>(row_of(P, at.i0)), c = static_cast<int>(at.d0), r = A.reverse ? row0 - (kTile - 1) : row0;
+    mbar_expect(full, Shared::StageT::kBytes);
+    tensor_load(sm.stage[now.i].x, &maps.x, c, r, full);
+    if constexpr (kGate == kOwn) tensor_load(sm.stage[now.i].gate, &maps.gate, c, r, full);
+    if constexpr (kBackward) tensor_load(sm.stage[now.i].dout, &maps.dout, c, r, full);
     mbar_arrive(&sm.issued[now.i]);
-    next = P.chain ? atomicAdd(P.ticket, 1u) + 1u : item + gridDim.x;  // needed a tile later
+    next = P.chain ? base + atomicAdd(P.ticket, 1u) + 1u : item + gridDim.x;  // needed a tile later
   }
 }
 
@@ -305,14 +299,13 @@ template <typename TX, typename TA, int V, int kGate, bool kBackward>
 __device__ __forceinline__ bool record_tiles(const Params &P, StreamShared<TX, TA, V, kGate, kBackward> &sm, int which, int lane) {
   using Shared = StreamShared<TX, TA, V, kGate, kBackward>;
   const gearb_recurrence_args &A = P.A;
-  const unsigned items = static_cast<unsigned>(P.tiles * P.ncol);
   Turn<Shared::kStages> now;
   for (int k = 0; k < which; ++k) now.next();
   for (;;) {
     if (!warp_wait(&sm.issued[now.i], now.parity)) return true;
     const unsigned item = sm.item[now.i];
     Plan &pl = sm.plan[now.i];
-    if (item >= items) {
+    if (item == kNoItem) {
       if (lane == 0) {
         pl.valid = 0;
         mbar_arrive(&sm.full[now.i]);
