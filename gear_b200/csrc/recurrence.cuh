@@ -21,11 +21,10 @@
 // sequence, a superblock is a section by itself: one thing less to wait for.  Measured, short sections and long:
 // 54 x 10752 x 48 float32 630 and 362 us, 1 x 580000 x 16 158 and 109, 4 x 65536 x 512 bf16 (4 blocks) 376 and 328,
 // 4 x 32768 x 768 (6 blocks) 217 and 229, 1 x 32768 x 2048 (16 blocks) 113 and 124, 3000 x 300 x 64 171 and 235.
-// A tile needs nothing from before the start of the sequence its first row belongs to.  Tiles are handed out by a counter in scan order,
-// so a CTA only ever waits for CTAs that are already running; every wait has a limit, after which the
-// launch goes on with NaN and says so in the status word.  Published words are 32 bits that read
-// 0xffffffff until they are written (a value of those bits is published as another NaN), so no flags and
-// fences are needed beside them.
+// A tile needs nothing from before the start of the sequence its first row belongs to.  Tiles are handed out by a counter
+// in scan order, so a CTA only ever waits for CTAs that are already running; every wait has a limit, after which the
+// launch goes on with NaN and says so in the status word.  Published words are 32 bits that read 0xffffffff until they
+// are written (a value of those bits is published as another NaN), so no flags and fences are needed beside them.
 //
 // Backward.  In terms of c_t = a_t * g_t the gradients obey c_t = a_t * c_(t+1) + a_t * dh_t, the same
 // recurrence from the last row to the first, over the same tiles.  h_(t-1) is not read back (it was rounded to

@@ -5,6 +5,11 @@
 // eight warps follow one another.  (A, H) of the groups are joined by a shuffle scan in the warp and one thread per
 // channel across the warps; tiles hand their state on as in the other kernels.  Rows are laid out so that the threads
 // of a warp, which read K rows apart, fall into different banks: a group's stride is the width modulo 32.
+//
+// 16384 packed sequences of up to 1000 rows of one channel, 8.6 M rows: 64 us (15 at the copy rate); a warp a row 2300,
+// with loads one after the other 203, with the general code for one channel 142.  Issue slots are taken in 51 % of
+// the cycles, mostly by the bookkeeping of rows (which start and end a sequence) rather than by the two
+// multiply-adds a row; barriers between the phases are the first of the stalls.
 #pragma once
 
 #include "recurrence_wide.cuh"

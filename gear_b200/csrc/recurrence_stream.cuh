@@ -2,19 +2,24 @@
 //
 // The tiles are those of recurrence_wide.cuh, but the CTAs stay, one per SM, and their warps have roles, so that
 // nothing waits in line:
-//   planner     takes the next tile's number from the counter and starts its copies (one tensor copy per input);
-//               which of its rows start or end a sequence was found out by the launch before, once for all columns
-//   compute     first look at tile m: (A, H) of each warp's rows; then, tile m - 1 again: its rows from the state
+//   issuer      takes the next tile's number from the counter and starts its copies (one tensor copy per input)
+//   recorders   fetch what the launch before found out about the tile's rows (which start or end a sequence: once for all
+//               column blocks), and shared gates
+//   compute     first look at tile m: (A, H) of each warp's rows; then, tile m - 2 again: its rows from the state
 //               before them, and out
 //   publishers  one thread per channel: turn the warps' pairs into those of all rows before each warp, publish the
 //               tile's
 //   finishers   one thread per channel: the state in front of the tile from what the tiles before published
-// They meet at mbarriers only.  Measured on the way, 2 x 16384 x 2048 bf16 with float32 gates (82 us at the copy rate):
+// They meet at mbarriers only.  2 x 16384 x 2048 bf16 with float32 log gates takes 113 us, 4.75 TB/s of 6.55 (82 us);
+// the backward pass of 4 x 4096 x 2048 117 us, beside 60 us forward.  What bounds it now: 19 warps of one CTA issue in
+// 51 % of the cycles (the two looks at every element, exponentials and conversions), and the rest is the latency
+// of what they hand each other (long scoreboard 4.3 of 8 stall cycles an issue); two CTAs an SM do not fit the
+// registers.  Measured on the way:
 // a CTA per tile 170 us whatever the types; CTAs that stay but finish a tile before they begin the next: every tile
 // spent 6700 of 11000 cycles looking back; one bulk copy per row: an SM starts one about every 35 cycles, 180 us;
 // every warp finding its rows' place itself: 600 of 1000 instructions; both phases' rows in registers: spills, 234 us;
-// the planner looking the rows up in the offsets: 4 us a tile; several tiles' numbers taken at once: tiles wait for others far back in another CTA's queue, 250 to 600 us; two CTA
-// barriers a tile in place of the roles: 136 us.
+// the issuer looking the rows up in the offsets: 4 us a tile; several tiles' numbers taken at once: tiles wait for
+// others far back in another CTA's queue, 250 to 600 us; two CTA barriers a tile in place of the roles: 136 us.
 #pragma once
 
 #include <cuda.h>
@@ -535,7 +540,7 @@ __device__ __forceinline__ bool compute_forward(const Params &P, StreamShared<TX
   const gearb_recurrence_args &A = P.A;
   Turn<Shared::kStages> now, old;
   Turn<kRing> pair, opair;
-  unsigned m = 0, tiles = 0xffffffffu;  // tiles of this CTA, known when the planner has said that there are no more
+  unsigned m = 0, tiles = 0xffffffffu;  // tiles of this CTA, known when the issuer has said that there are no more
   for (; m < kLag || m - kLag < tiles; ++m) {
     if (tiles == 0xffffffffu) {
       if (!warp_wait(&sm.full[now.i], now.parity)) return true;
