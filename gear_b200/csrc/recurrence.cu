@@ -354,6 +354,10 @@ int launch(const gearb_recurrence_args &a, bool backward, cudaStream_t stream) {
     if (!vector_ok(a.dout, a.dout_batch_stride, a.dout_row_stride, xs, v)) continue;
     if (shared || vector_ok(a.dgate, 0, 0, gs, v)) break;
   }
+  if (p.V == 1 && unit > 32) {
+    p.V = 2;
+    p.apart = 1;
+  }
   const int rc = a.x_dtype == GEARB_DT_F32 ? launch_f32(p, backward, stream)
                  : a.x_dtype == GEARB_DT_F16 ? launch_f16(p, backward, stream) : launch_bf16(p, backward, stream);
   if (rc != GEARB_OK || !backward || p.blocks_per_gate <= 1) return rc;

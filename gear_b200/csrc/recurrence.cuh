@@ -135,6 +135,7 @@ struct Params {
   float2 *super;         // [superblocks][width]: (A, H) of every superblock, in long sections
   float *section;        // [sections][width]: state in front of every section
   int V;                 // channels a lane, by alignment and width
+  int apart;             // with V = 2: channels 32 apart, where vectors are not aligned (wide kernels)
   TileRec *recs;         // [tiles]
   int64_t chain_bytes;   // at `ticket`: to be set to 0xff before tiles publish
   float *gate_part;      // [blocks_per_gate][rows][gates], when a gate's channels span several column blocks
@@ -416,31 +417,62 @@ __device__ __forceinline__ LiveTiles live_tiles(const Params &P) {
   return t;
 }
 
-// V consecutive channels of a warp's n rows of the scan (zeros where there is no row or channel).
-template <typename T, int V>
+// V channels a lane of a warp's n rows of the scan (zeros where there is no row or channel): consecutive ones from d on, or,
+// with kApart, every 32nd.  Where vectors are not aligned, two channels apart a lane are as many bytes in flight as
+// vectors of two, and read memory in order.
+template <int V, bool kApart>
+struct Channels {
+  int d, end;  // the lane's first channel, the block's end
+  __device__ __forceinline__ Channels(int d_, int end_) : d(d_), end(end_) {}
+  __device__ __forceinline__ Channels(const Place &pl, int lane)
+      : d(static_cast<int>(pl.d0) + (kApart ? lane : lane * V)), end(static_cast<int>(pl.d1)) {}
+  __device__ __forceinline__ static int of(int lane, int v) { return kApart ? lane + 32 * v : lane * V + v; }  // in the block
+  __device__ __forceinline__ int at(int v) const { return d + (kApart ? 32 * v : v); }
+  __device__ __forceinline__ bool on(int v) const { return at(v) < end; }
+  template <typename T>
+  __device__ __forceinline__ Pack<T, V> load(const T *row) const {
+    Pack<T, V> r;
+    if constexpr (kApart) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) r.v[v] = on(v) ? load_pack<T, 1>(row + at(v)).v[0] : from_f<T>(0.0f);
+    } else {
+      if (on(0)) return load_pack<T, V>(row + d);
+#pragma unroll
+      for (int v = 0; v < V; ++v) r.v[v] = from_f<T>(0.0f);
+    }
+    return r;
+  }
+  template <typename T>
+  __device__ __forceinline__ void store(T *row, const float (&f)[V]) const {
+    if constexpr (kApart) {
+#pragma unroll
+      for (int v = 0; v < V; ++v)
+        if (on(v)) row[at(v)] = from_f<T>(f[v]);
+    } else {
+      if (on(0)) store_pack<T, V>(row + d, f);
+    }
+  }
+};
+template <typename T, int V, bool kApart>
 __device__ __forceinline__ void load_rows(const T *base, const Params &P, const Place &pl, const TileRows &tr, int64_t period,
-                                          int64_t sb, int64_t sr, int warp, int n, int64_t d, bool on, Pack<T, V> (&r)[kRows]) {
+                                          int64_t sb, int64_t sr, int warp, int n, const Channels<V, kApart> &ch,
+                                          Pack<T, V> (&r)[kRows]) {
   if (n == kRows && tr.linear) {
     const int64_t step = P.A.reverse ? -sr : sr;
-    const T *p = base + (tr.bb * sb + tr.tt * sr + warp * kRows * step + d);
+    const T *p = base + (tr.bb * sb + tr.tt * sr + warp * kRows * step);
 #pragma unroll
-    for (int k = 0; k < kRows; ++k) {
-      if (on) r[k] = load_pack<T, V>(p + k * step);
-      else
-#pragma unroll
-        for (int v = 0; v < V; ++v) r[k].v[v] = from_f<T>(0.0f);
-    }
+    for (int k = 0; k < kRows; ++k) r[k] = ch.load(p + k * step);
     return;
   }
 #pragma unroll
   for (int k = 0; k < kRows; ++k)
 #pragma unroll
     for (int v = 0; v < V; ++v) r[k].v[v] = from_f<T>(0.0f);
-  if (n == 0 || !on) return;
+  if (n == 0) return;
   RowWalk w(row_of(P, pl.i0 + warp * kRows), period, sb, sr, P.A.reverse);
 #pragma unroll
   for (int k = 0; k < kRows; ++k) {
-    if (k < n) r[k] = load_pack<T, V>(base + w.off + d);
+    if (k < n) r[k] = ch.load(base + w.off);
     w.next();
   }
 }

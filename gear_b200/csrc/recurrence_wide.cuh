@@ -5,7 +5,9 @@
 // each warp; then every warp runs its rows from there.  These take what the streaming kernels cannot: rows that are not
 // one matrix on 16-byte boundaries, odd widths, gates of up to 32 channels in the backward pass.  Bound by the latency
 // of the phases: a CTA takes some 13 us for its tile, whatever its types, so what counts is how many fit an SM
-// (2 to 5, by V).  54 x 10733 x 43 float16 224 us, 2 x 16384 x 2048 bf16 170 us (113 in the streaming kernels).
+// (2 to 5, by V) and how many bytes each has under way.  Where rows are not aligned for vectors a lane takes two
+// channels 32 apart; with one channel a lane 650 x 64 x 1233 float16 with float32 gates took 235 us, now 148 (63 at
+// the copy rate), 54 x 10733 x 43 221, now 156.  2 x 16384 x 2048 bf16 170 us (113 in the streaming kernels).
 #pragma once
 
 #include "recurrence.cuh"
@@ -13,28 +15,29 @@
 namespace gearb {
 namespace rec {
 
-template <typename TA, int V, int kGate>
-__device__ __forceinline__ void load_gate(const Params &P, const Place &pl, const TileRows &tr, int warp, int n, int64_t d,
-                                          bool on, float (&a)[kRows][kGate == kOne ? 1 : V]) {
+template <typename TA, int V, int kGate, bool kApart>
+__device__ __forceinline__ void load_gate(const Params &P, const Place &pl, const TileRows &tr, int warp, int n,
+                                          const Channels<V, kApart> &ch, float (&a)[kRows][kGate == kOne ? 1 : V]) {
   const TA *gate = static_cast<const TA *>(P.A.gate);
+  auto one = [&](int g, bool on, int v) {  // gate g, for the lane's channel v
+    const Channels<1, false> at(g, on ? g + 1 : g);
+    Pack<TA, 1> raw[kRows];
+    load_rows<TA>(gate, P, pl, tr, P.gate_period, P.A.gate_batch_stride, P.A.gate_row_stride, warp, n, at, raw);
+#pragma unroll
+    for (int k = 0; k < kRows; ++k) a[k][v] = to_f(raw[k].v[0]);
+  };
   if constexpr (kGate == kTable) {
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      Pack<TA, 1> raw[kRows];
-      load_rows<TA, 1>(gate, P, pl, tr, P.gate_period, P.A.gate_batch_stride, P.A.gate_row_stride, warp, n,
-                       on ? (static_cast<int>(d) + v) / P.per : 0, on, raw);
-#pragma unroll
-      for (int k = 0; k < kRows; ++k) a[k][v] = to_f(raw[k].v[0]);
-    }
+    for (int v = 0; v < V; ++v) one(ch.on(v) ? ch.at(v) / P.per : 0, ch.on(v), v);
+  } else if constexpr (kGate == kOne) {
+    one(static_cast<int>(pl.gate), ch.on(0), 0);
   } else {
-    constexpr int kG = kGate == kOne ? 1 : V;
-    Pack<TA, kG> raw[kRows];
-    load_rows<TA, kG>(gate, P, pl, tr, P.gate_period, P.A.gate_batch_stride, P.A.gate_row_stride, warp, n,
-                      kGate == kOne ? pl.gate : d, on, raw);
+    Pack<TA, V> raw[kRows];
+    load_rows<TA>(gate, P, pl, tr, P.gate_period, P.A.gate_batch_stride, P.A.gate_row_stride, warp, n, ch, raw);
 #pragma unroll
     for (int k = 0; k < kRows; ++k)
 #pragma unroll
-      for (int v = 0; v < kG; ++v) a[k][v] = to_f(raw[k].v[v]);
+      for (int v = 0; v < V; ++v) a[k][v] = to_f(raw[k].v[v]);
   }
 }
 
@@ -82,7 +85,8 @@ __device__ __forceinline__ RowMap rows_of_warp(const Params &P, const Place &pl,
   return m;
 }
 
-// A float of every channel of [sequences][width], of V channels of one sequence.
+// A float of every channel of [sequences][width], of the lane's channels of one sequence (the streaming kernels: of V
+// consecutive ones).
 template <int V>
 __device__ __forceinline__ void state_load(const float *p, int seq, int64_t width, int64_t d, bool on, float (&r)[V]) {
 #pragma unroll
@@ -94,8 +98,20 @@ __device__ __forceinline__ void state_store(float *p, int seq, int64_t width, in
 #pragma unroll
     for (int v = 0; v < V; ++v) p[static_cast<int64_t>(seq) * width + d + v] = r[v];
 }
+template <int V, bool kApart>
+__device__ __forceinline__ void state_load(const float *p, int seq, int64_t width, const Channels<V, kApart> &ch, float (&r)[V]) {
+#pragma unroll
+  for (int v = 0; v < V; ++v) r[v] = (p && ch.on(v)) ? p[static_cast<int64_t>(seq) * width + ch.at(v)] : 0.0f;
+}
+template <int V, bool kApart>
+__device__ __forceinline__ void state_store(float *p, int seq, int64_t width, const Channels<V, kApart> &ch, const float (&r)[V]) {
+  if (p)
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      if (ch.on(v)) p[static_cast<int64_t>(seq) * width + ch.at(v)] = r[v];
+}
 
-template <typename TX, typename TA, int V, int kGate>
+template <typename TX, typename TA, int V, int kGate, bool kApart>
 __global__ void __launch_bounds__(kThreads, V == 4 ? 2 : V == 2 ? 3 : 5) forward_kernel(const __grid_constant__ Params P) {
   constexpr int kG = kGate == kOne ? 1 : V;
   constexpr int kW = 32 * V;  // channels of a block
@@ -107,16 +123,15 @@ __global__ void __launch_bounds__(kThreads, V == 4 ? 2 : V == 2 ? 3 : 5) forward
   const gearb_recurrence_args &A = P.A;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const Place pl = take_place<V, kGate>(P, &sticket, false);
-  const int64_t d = pl.d0 + lane * V;
-  const bool on = d < pl.d1;
+  const Channels<V, kApart> chans(pl, lane);
   const int64_t i0 = pl.i0 + warp * kRows;
   const int n = static_cast<int>(i0 >= pl.i1 ? 0 : (pl.i1 - i0 < kRows ? pl.i1 - i0 : kRows));
 
   Pack<TX, V> x[kRows];
   float a[kRows][kG];
   TileRows tr = rows_of_tile(P, pl);
-  load_rows<TX, V>(static_cast<const TX *>(A.x), P, pl, tr, P.x_period, A.x_batch_stride, A.x_row_stride, warp, n, d, on, x);
-  load_gate<TA, V, kGate>(P, pl, tr, warp, n, d, on, a);
+  load_rows<TX>(static_cast<const TX *>(A.x), P, pl, tr, P.x_period, A.x_batch_stride, A.x_row_stride, warp, n, chans, x);
+  load_gate<TA, V, kGate>(P, pl, tr, warp, n, chans, a);
   const RowMap m = rows_of_warp(P, pl, tr, srows, i0, n, warp, lane);
   if (A.gate_log) exp_gate(a);
   const bool plain = m.live == kAllRows && (m.start | m.end) == 0;
@@ -140,7 +155,7 @@ __global__ void __launch_bounds__(kThreads, V == 4 ? 2 : V == 2 ? 3 : 5) forward
       if (!(m.live >> k & 1u)) continue;
       const bool st = m.start >> k & 1u;
       float s[V];
-      if (st) state_load<V>(A.h0, __shfl_sync(kAll, m.seq, k), A.width, d, on, s);
+      if (st) state_load<V>(A.h0, __shfl_sync(kAll, m.seq, k), A.width, chans, s);
 #pragma unroll
       for (int v = 0; v < V; ++v) {
         const float av = a[k][kGate == kOne ? 0 : v], xv = to_f(x[k].v[v]);
@@ -151,7 +166,7 @@ __global__ void __launch_bounds__(kThreads, V == 4 ? 2 : V == 2 ? 3 : 5) forward
     }
   }
 #pragma unroll
-  for (int v = 0; v < V; ++v) { sa[warp][lane * V + v] = ca[v]; sh[warp][lane * V + v] = ch[v]; }
+  for (int v = 0; v < V; ++v) { sa[warp][chans.of(lane, v)] = ca[v]; sh[warp][chans.of(lane, v)] = ch[v]; }
   if (lane == 0) {
     scut[warp] = m.start != 0;
     if (warp == 0) sfirst = ((m.live & ~m.start) & 1u) ? m.first_start : -1;
@@ -193,31 +208,31 @@ __global__ void __launch_bounds__(kThreads, V == 4 ? 2 : V == 2 ? 3 : 5) forward
   if (n > 0) {
     float h[V];
 #pragma unroll
-    for (int v = 0; v < V; ++v) h[v] = sh[warp][lane * V + v];
-    TX *out = static_cast<TX *>(A.out) + row_of(P, i0) * A.width + d;
+    for (int v = 0; v < V; ++v) h[v] = sh[warp][chans.of(lane, v)];
+    TX *out = static_cast<TX *>(A.out) + row_of(P, i0) * A.width;
     const int64_t step = A.reverse ? -A.width : A.width;
     if (plain) {
 #pragma unroll
       for (int k = 0; k < kRows; ++k) {
 #pragma unroll
         for (int v = 0; v < V; ++v) h[v] = fmaf(a[k][kGate == kOne ? 0 : v], h[v], to_f(x[k].v[v]));
-        if (on) store_pack<TX, V>(out + k * step, h);
+        chans.store(out + k * step, h);
       }
     } else {
 #pragma unroll
       for (int k = 0; k < kRows; ++k) {
         if (k >= n) break;
         if (!(m.live >> k & 1u)) {
-          if (A.zero_rest && on) {
+          if (A.zero_rest) {
             const float z[V] = {};
-            store_pack<TX, V>(out + k * step, z);
+            chans.store(out + k * step, z);
           }
           continue;
         }
         const int seq = __shfl_sync(kAll, m.seq, k);
         if (m.start >> k & 1u) {
           float s[V];
-          state_load<V>(A.h0, seq, A.width, d, on, s);
+          state_load<V>(A.h0, seq, A.width, chans, s);
 #pragma unroll
           for (int v = 0; v < V; ++v) {
             const float xv = to_f(x[k].v[v]);
@@ -227,8 +242,8 @@ __global__ void __launch_bounds__(kThreads, V == 4 ? 2 : V == 2 ? 3 : 5) forward
 #pragma unroll
           for (int v = 0; v < V; ++v) h[v] = fmaf(a[k][kGate == kOne ? 0 : v], h[v], to_f(x[k].v[v]));
         }
-        if (on) store_pack<TX, V>(out + k * step, h);
-        if (m.end >> k & 1u) state_store<V>(A.state_out, seq, A.width, d, on, h);
+        chans.store(out + k * step, h);
+        if (m.end >> k & 1u) state_store<V>(A.state_out, seq, A.width, chans, h);
       }
     }
   }
@@ -254,7 +269,7 @@ __device__ __forceinline__ float sum_rows(float (&v)[kRows], int lane) {
   return v[0];
 }
 
-template <typename TX, typename TA, int V, int kGate>
+template <typename TX, typename TA, int V, int kGate, bool kApart>
 __global__ void __launch_bounds__(kThreads, V == 4 ? 2 : V == 2 ? 3 : 4) backward_kernel(const __grid_constant__ Params P) {
   constexpr int kG = kGate == kOne ? 1 : V;
   constexpr int kW = 32 * V;
@@ -267,18 +282,17 @@ __global__ void __launch_bounds__(kThreads, V == 4 ? 2 : V == 2 ? 3 : 4) backwar
   const gearb_recurrence_args &A = P.A;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const Place pl = take_place<V, kGate>(P, &sticket, true);
-  const int64_t d = pl.d0 + lane * V;
-  const bool on = d < pl.d1;
+  const Channels<V, kApart> chans(pl, lane);
   const int64_t i0 = pl.i0 + warp * kRows;
   const int n = static_cast<int>(i0 >= pl.i1 ? 0 : (pl.i1 - i0 < kRows ? pl.i1 - i0 : kRows));
 
   Pack<TX, V> x[kRows], dh[kRows];
   float a[kRows][kG];
   TileRows tr = rows_of_tile(P, pl);
-  load_rows<TX, V>(static_cast<const TX *>(A.x), P, pl, tr, P.x_period, A.x_batch_stride, A.x_row_stride, warp, n, d, on, x);
-  load_gate<TA, V, kGate>(P, pl, tr, warp, n, d, on, a);
-  load_rows<TX, V>(static_cast<const TX *>(A.dout), P, pl, tr, P.dout_period, A.dout_batch_stride, A.dout_row_stride, warp, n,
-                   d, on, dh);
+  load_rows<TX>(static_cast<const TX *>(A.x), P, pl, tr, P.x_period, A.x_batch_stride, A.x_row_stride, warp, n, chans, x);
+  load_gate<TA, V, kGate>(P, pl, tr, warp, n, chans, a);
+  load_rows<TX>(static_cast<const TX *>(A.dout), P, pl, tr, P.dout_period, A.dout_batch_stride, A.dout_row_stride, warp, n,
+                chans, dh);
   const RowMap m = rows_of_warp(P, pl, tr, srows, i0, n, warp, lane);
   if (A.gate_log) exp_gate(a);
   const bool plain = m.live == kAllRows && (m.start | m.end) == 0;
@@ -306,7 +320,7 @@ __global__ void __launch_bounds__(kThreads, V == 4 ? 2 : V == 2 ? 3 : 4) backwar
       if (!(m.live >> k & 1u)) continue;
       const bool st = m.start >> k & 1u;
       float s[V];
-      if (st) state_load<V>(A.h0, __shfl_sync(kAll, m.seq, k), A.width, d, on, s);
+      if (st) state_load<V>(A.h0, __shfl_sync(kAll, m.seq, k), A.width, chans, s);
 #pragma unroll
       for (int v = 0; v < V; ++v) {
         const float av = a[k][kGate == kOne ? 0 : v], xv = to_f(x[k].v[v]);
@@ -318,16 +332,16 @@ __global__ void __launch_bounds__(kThreads, V == 4 ? 2 : V == 2 ? 3 : 4) backwar
 #pragma unroll
     for (int k = kRows - 1; k >= 0; --k) {
       if (!(m.live >> k & 1u)) continue;
-      if (m.end >> k & 1u) state_load<V>(A.dstate, __shfl_sync(kAll, m.seq, k), A.width, d, on, cc);
+      if (m.end >> k & 1u) state_load<V>(A.dstate, __shfl_sync(kAll, m.seq, k), A.width, chans, cc);
 #pragma unroll
       for (int v = 0; v < V; ++v) cc[v] = a[k][kGate == kOne ? 0 : v] * (to_f(dh[k].v[v]) + cc[v]);
     }
   }
 #pragma unroll
   for (int v = 0; v < V; ++v) {
-    sa[warp][lane * V + v] = ca[v];
-    sh[warp][lane * V + v] = ch[v];
-    sc[warp][lane * V + v] = cc[v];
+    sa[warp][chans.of(lane, v)] = ca[v];
+    sh[warp][chans.of(lane, v)] = ch[v];
+    sc[warp][chans.of(lane, v)] = cc[v];
   }
   if (lane == 0) {
     scut[warp] = m.start != 0;
@@ -391,15 +405,15 @@ __global__ void __launch_bounds__(kThreads, V == 4 ? 2 : V == 2 ? 3 : 4) backwar
   if (n > 0) {
     float hp[kRows][V], h[V], c[V], part[kRows];  // hp: h_(t-1) of every row
 #pragma unroll
-    for (int v = 0; v < V; ++v) { h[v] = sh[warp][lane * V + v]; c[v] = sc[warp][lane * V + v]; }
+    for (int v = 0; v < V; ++v) { h[v] = sh[warp][chans.of(lane, v)]; c[v] = sc[warp][chans.of(lane, v)]; }
     const int64_t row0 = row_of(P, i0), sign = A.reverse ? -1 : 1, xs = sign * A.width, gs = sign * A.gates;
-    TX *dx = static_cast<TX *>(A.dx) + row0 * A.width + d;
+    TX *dx = static_cast<TX *>(A.dx) + row0 * A.width;
     TA *dgate = static_cast<TA *>(A.dgate) + row0 * A.gates +
-                (kGate == kOne ? pl.gate : kGate == kTable ? pl.d0 / P.per : d);
+                (kGate == kOne ? pl.gate : kGate == kTable ? pl.d0 / P.per : 0);
     // Gates of a few channels each: a row's products through shared memory, a lane a gate (blocks hold whole gates).
     auto sum_gates = [&](int k, bool wanted, const float (&da)[V]) {
 #pragma unroll
-      for (int v = 0; v < V; ++v) sa[warp][lane * V + v] = da[v];
+      for (int v = 0; v < V; ++v) sa[warp][chans.of(lane, v)] = da[v];
       __syncwarp();
       const int cols = static_cast<int>(pl.d1 - pl.d0);
       for (int j = lane; j * P.per < cols; j += 32) {
@@ -427,19 +441,17 @@ __global__ void __launch_bounds__(kThreads, V == 4 ? 2 : V == 2 ? 3 : 4) backwar
           g[v] = to_f(dh[k].v[v]) + c[v];
           c[v] = av * g[v];
           da[v] = (A.gate_log ? c[v] : g[v]) * hp[k][v];
-          part[k] += on ? da[v] : 0.0f;
+          part[k] += chans.on(v) ? da[v] : 0.0f;
         }
-        if (on) {
-          store_pack<TX, V>(dx + k * xs, g);
-          if constexpr (kGate == kOwn) store_pack<TA, V>(dgate + k * gs, da);
-        }
+        chans.store(dx + k * xs, g);
+        if constexpr (kGate == kOwn) chans.store(dgate + k * gs, da);
         if constexpr (kGate == kTable) sum_gates(k, true, da);
       }
     } else {
 #pragma unroll
       for (int k = 0; k < kRows; ++k) {
         const bool st = m.start >> k & 1u, lv = m.live >> k & 1u;
-        if (st) state_load<V>(A.h0, __shfl_sync(kAll, m.seq, k), A.width, d, on, h);
+        if (st) state_load<V>(A.h0, __shfl_sync(kAll, m.seq, k), A.width, chans, h);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
           const float xv = to_f(x[k].v[v]);
@@ -453,7 +465,7 @@ __global__ void __launch_bounds__(kThreads, V == 4 ? 2 : V == 2 ? 3 : 4) backwar
         if (k >= n) continue;
         const bool lv = m.live >> k & 1u, st = m.start >> k & 1u;
         const int seq = __shfl_sync(kAll, m.seq, k);
-        if (m.end >> k & 1u) state_load<V>(A.dstate, seq, A.width, d, on, c);
+        if (m.end >> k & 1u) state_load<V>(A.dstate, seq, A.width, chans, c);
         float g[V], da[V];
 #pragma unroll
         for (int v = 0; v < V; ++v) {
@@ -462,14 +474,14 @@ __global__ void __launch_bounds__(kThreads, V == 4 ? 2 : V == 2 ? 3 : 4) backwar
           if (lv) c[v] = av * g[v];
           // the first row of a sequence without h0 is h = x: its gate plays no part
           da[v] = (lv && !(st && !A.h0)) ? (A.gate_log ? c[v] : g[v]) * hp[k][v] : 0.0f;
-          part[k] += on ? da[v] : 0.0f;
+          part[k] += chans.on(v) ? da[v] : 0.0f;
         }
-        if (on && (lv || A.zero_rest)) {
-          store_pack<TX, V>(dx + k * xs, g);
-          if constexpr (kGate == kOwn) store_pack<TA, V>(dgate + k * gs, da);
+        if (lv || A.zero_rest) {
+          chans.store(dx + k * xs, g);
+          if constexpr (kGate == kOwn) chans.store(dgate + k * gs, da);
         }
         if constexpr (kGate == kTable) sum_gates(k, lv || A.zero_rest, da);
-        if (st) state_store<V>(A.dh0, seq, A.width, d, on, c);
+        if (st) state_store<V>(A.dh0, seq, A.width, chans, c);
       }
     }
     if constexpr (kGate == kOne) {
@@ -484,12 +496,12 @@ __global__ void __launch_bounds__(kThreads, V == 4 ? 2 : V == 2 ? 3 : 4) backwar
   empty_sequences(P, pl, kW, A.dstate, A.dh0);
 }
 
-template <typename TX, typename TA, int V, int kGate>
+template <typename TX, typename TA, int V, int kGate, bool kApart>
 int launch_wide(Params &p, bool backward, cudaStream_t stream) {
   const gearb_recurrence_args &a = p.A;
   p.block = 32 * V;
   if (kGate == kTable && backward) {  // whole gates, and whole vectors
-    const int unit = p.per % V == 0 ? p.per : (p.per % 2 == 0 && V == 4 ? 2 : V) * p.per;
+    const int unit = kApart || p.per % V == 0 ? p.per : (p.per % 2 == 0 && V == 4 ? 2 : V) * p.per;
     p.block = 32 * V / unit * unit;
   }
   p.blocks_per_gate = kGate == kOne ? (p.per + 32 * V - 1) / (32 * V) : 1;
@@ -499,24 +511,26 @@ int launch_wide(Params &p, bool backward, cudaStream_t stream) {
   p.section_shift = long_sections(p, p.ncol) ? kLongSection : kShortSection;
   const unsigned grid = static_cast<unsigned>(p.tiles * ncol);
   if (p.chain) GEARB_CUDA(cudaMemsetAsync(p.ticket, 0xff, static_cast<size_t>(p.chain_bytes), stream));
-  if (backward) backward_kernel<TX, TA, V, kGate><<<grid, kThreads, 0, stream>>>(p);
-  else if constexpr (kGate != kOne) forward_kernel<TX, TA, V, kGate><<<grid, kThreads, 0, stream>>>(p);
+  if (backward) backward_kernel<TX, TA, V, kGate, kApart><<<grid, kThreads, 0, stream>>>(p);
+  else if constexpr (kGate != kOne) forward_kernel<TX, TA, V, kGate, kApart><<<grid, kThreads, 0, stream>>>(p);
   GEARB_CUDA(cudaGetLastError());
   return GEARB_OK;
 }
 
-template <typename TX, typename TA, int V>
+template <typename TX, typename TA, int V, bool kApart>
 int launch_wide_gate(Params &p, bool backward, cudaStream_t stream) {
-  if (p.A.gates == p.A.width) return launch_wide<TX, TA, V, kOwn>(p, backward, stream);
-  return p.by_gate ? launch_wide<TX, TA, V, kOne>(p, backward, stream) : launch_wide<TX, TA, V, kTable>(p, backward, stream);
+  if (p.A.gates == p.A.width) return launch_wide<TX, TA, V, kOwn, kApart>(p, backward, stream);
+  return p.by_gate ? launch_wide<TX, TA, V, kOne, kApart>(p, backward, stream) : launch_wide<TX, TA, V, kTable, kApart>(p, backward, stream);
 }
 
 template <typename TX, typename TA>
 int launch_wide_any(Params &p, bool backward, cudaStream_t stream) {
   switch (p.V) {
-    case 4: return launch_wide_gate<TX, TA, 4>(p, backward, stream);
-    case 2: return launch_wide_gate<TX, TA, 2>(p, backward, stream);
-    default: return launch_wide_gate<TX, TA, 1>(p, backward, stream);
+    case 4: return launch_wide_gate<TX, TA, 4, false>(p, backward, stream);
+    case 2:
+      return p.apart ? launch_wide_gate<TX, TA, 2, true>(p, backward, stream)
+                     : launch_wide_gate<TX, TA, 2, false>(p, backward, stream);
+    default: return launch_wide_gate<TX, TA, 1, false>(p, backward, stream);
   }
 }
 
