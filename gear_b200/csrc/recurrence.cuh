@@ -17,8 +17,8 @@
 // applies the superblocks before it in its section to the state in front of the section, in order, and composes the
 // tiles before it in its superblock onto that: the same operations whatever the timing, so results are the same bits
 // every time, and the chain of CTAs that wait for one another has one link (0.5 to 0.65 us) per 4096 rows.  Where
-// there are more than five column blocks, so that 512 rows of all channels take longer than a link, or few rows a
-// sequence, a superblock is a section by itself: one thing less to wait for.  Measured, short sections and long:
+// there are more than 512 channels, so that 512 rows of all of them take longer than a link, or few rows a sequence, a
+// superblock is a section by itself: one thing less to wait for.  Measured, short sections and long:
 // 54 x 10752 x 48 float32 630 and 362 us, 1 x 580000 x 16 158 and 109, 4 x 65536 x 512 bf16 (4 blocks) 376 and 328,
 // 4 x 32768 x 768 (6 blocks) 217 and 229, 1 x 32768 x 2048 (16 blocks) 113 and 124, 3000 x 300 x 64 171 and 235.
 // A tile needs nothing from before the start of the sequence its first row belongs to.  Tiles are handed out by a counter
@@ -47,7 +47,7 @@ constexpr int kRows = 8;                     // rows a warp keeps in registers
 constexpr int kTile = kWarps * kRows;        // rows per tile
 constexpr int kSuper = 8;                    // tiles per superblock
 constexpr int kShortSection = 3, kLongSection = 6;  // tiles per section (powers of two): one superblock, or eight
-constexpr int kLongColumns = 5;              // most column blocks with long sections,
+constexpr int kLongWidth = 512;              // most channels with long sections,
 constexpr int kLongRows = 2048;              // and fewest rows a sequence
 constexpr unsigned kAll = 0xffffffffu;
 constexpr unsigned kAllRows = (1u << kRows) - 1u;
@@ -593,9 +593,10 @@ inline bool vector_ok(const void *p, int64_t sb, int64_t sr, int size, int v) {
   return reinterpret_cast<uintptr_t>(p) % (size * v) == 0 && sb % v == 0 && sr % v == 0;
 }
 
-// Long sections where the chain would take longer than the work, and sequences are long enough to feel it.
-inline bool long_sections(const Params &p, int ncol) {
-  return ncol <= kLongColumns && p.rows / kLongRows >= p.A.sequences;
+// Long sections where the chain would take longer than the work, and sequences are long enough to feel it.  By the sizes
+// alone: the section decides how a state is rounded, and every kernel gives the same bits.
+inline int section_shift_of(const Params &p) {
+  return p.A.width <= kLongWidth && p.rows / kLongRows >= p.A.sequences ? kLongSection : kShortSection;
 }
 
 // In front of a streaming kernel: finds out about the tiles' rows, and clears what they publish in.

@@ -499,7 +499,7 @@ int launch_narrow(Params &p, bool backward, cudaStream_t stream) {
   const int smem = groups * ((backward ? 2 : 1) * xl.stride + gl.stride) * 4;
   GEARB_REQUIRE(p.tiles < (int64_t(1) << 31), "recurrence: too many tiles for one launch");
   p.ncol = 1;
-  p.section_shift = long_sections(p, p.ncol) ? kLongSection : kShortSection;
+  p.section_shift = section_shift_of(p);
   p.blocks_per_gate = 1;
   if (p.chain) GEARB_CUDA(cudaMemsetAsync(p.ticket, 0xff, static_cast<size_t>(p.chain_bytes), stream));
   void (*kernel)(Params);

@@ -763,7 +763,7 @@ __device__ __forceinline__ bool compute_backward(const Params &P, StreamShared<T
             mul_v(c, as[k], g);
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-              da[v] = (A.gate_log ? c[v] : g[v]) * hp[k][v];
+              da[v] = __fmul_rn(A.gate_log ? c[v] : g[v], hp[k][v]);
               part[k] += on ? da[v] : 0.0f;
             }
             if (on) {
@@ -800,9 +800,9 @@ __device__ __forceinline__ bool compute_backward(const Params &P, StreamShared<T
             for (int v = 0; v < V; ++v) {
               const float av = as[k][kGate == kOne ? 0 : v];
               g[v] = lv ? g[v] + c[v] : 0.0f;
-              if (lv) c[v] = av * g[v];
+              if (lv) c[v] = __fmul_rn(av, g[v]);
               // the first row of a sequence without h0 is h = x: its gate plays no part
-              da[v] = (lv && !(st && !A.h0)) ? (A.gate_log ? c[v] : g[v]) * hp[k][v] : 0.0f;
+              da[v] = (lv && !(st && !A.h0)) ? __fmul_rn(A.gate_log ? c[v] : g[v], hp[k][v]) : 0.0f;
               part[k] += on ? da[v] : 0.0f;
             }
             if (on && (lv || (A.zero_rest && k < n))) {
@@ -910,8 +910,8 @@ int launch_stream(Params &p, cudaStream_t stream) {
   static_assert(kSmem <= kSmemMost, "fits one SM");
   void (*kernel)(Params, Maps);
   // a kernel each: with both ways in one, packed heads take 10 % longer
-  const bool far = p.chain && long_sections(p, p.ncol);
-  p.section_shift = far ? kLongSection : kShortSection;
+  p.section_shift = section_shift_of(p);
+  const bool far = p.chain && p.section_shift == kLongSection;
   if constexpr (kBackward) kernel = far ? backward_stream_kernel<TX, TA, V, kGate, true> : backward_stream_kernel<TX, TA, V, kGate, false>;
   else kernel = far ? forward_stream_kernel<TX, TA, V, kGate, true> : forward_stream_kernel<TX, TA, V, kGate, false>;
   GEARB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));

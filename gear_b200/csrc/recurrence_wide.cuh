@@ -269,6 +269,8 @@ __device__ __forceinline__ float sum_rows(float (&v)[kRows], int lane) {
   return v[0];
 }
 
+// Products are rounded (__fmul_rn) before they are added, as in the streaming kernels: left to the compiler, some would be
+// fused with the addition in one kernel and not in the other.
 template <typename TX, typename TA, int V, int kGate, bool kApart>
 __global__ void __launch_bounds__(kThreads, V == 4 ? 2 : V == 2 ? 3 : 4) backward_kernel(const __grid_constant__ Params P) {
   constexpr int kG = kGate == kOne ? 1 : V;
@@ -313,7 +315,7 @@ __global__ void __launch_bounds__(kThreads, V == 4 ? 2 : V == 2 ? 3 : 4) backwar
 #pragma unroll
     for (int k = kRows - 1; k >= 0; --k)
 #pragma unroll
-      for (int v = 0; v < V; ++v) cc[v] = a[k][kGate == kOne ? 0 : v] * (to_f(dh[k].v[v]) + cc[v]);
+      for (int v = 0; v < V; ++v) cc[v] = __fmul_rn(a[k][kGate == kOne ? 0 : v], to_f(dh[k].v[v]) + cc[v]);
   } else {
 #pragma unroll
     for (int k = 0; k < kRows; ++k) {
@@ -334,7 +336,7 @@ __global__ void __launch_bounds__(kThreads, V == 4 ? 2 : V == 2 ? 3 : 4) backwar
       if (!(m.live >> k & 1u)) continue;
       if (m.end >> k & 1u) state_load<V>(A.dstate, __shfl_sync(kAll, m.seq, k), A.width, chans, cc);
 #pragma unroll
-      for (int v = 0; v < V; ++v) cc[v] = a[k][kGate == kOne ? 0 : v] * (to_f(dh[k].v[v]) + cc[v]);
+      for (int v = 0; v < V; ++v) cc[v] = __fmul_rn(a[k][kGate == kOne ? 0 : v], to_f(dh[k].v[v]) + cc[v]);
     }
   }
 #pragma unroll
@@ -439,8 +441,8 @@ __global__ void __launch_bounds__(kThreads, V == 4 ? 2 : V == 2 ? 3 : 4) backwar
         for (int v = 0; v < V; ++v) {
           const float av = a[k][kGate == kOne ? 0 : v];
           g[v] = to_f(dh[k].v[v]) + c[v];
-          c[v] = av * g[v];
-          da[v] = (A.gate_log ? c[v] : g[v]) * hp[k][v];
+          c[v] = __fmul_rn(av, g[v]);
+          da[v] = __fmul_rn(A.gate_log ? c[v] : g[v], hp[k][v]);
           part[k] += chans.on(v) ? da[v] : 0.0f;
         }
         chans.store(dx + k * xs, g);
@@ -471,9 +473,9 @@ __global__ void __launch_bounds__(kThreads, V == 4 ? 2 : V == 2 ? 3 : 4) backwar
         for (int v = 0; v < V; ++v) {
           const float av = a[k][kGate == kOne ? 0 : v];
           g[v] = lv ? to_f(dh[k].v[v]) + c[v] : 0.0f;
-          if (lv) c[v] = av * g[v];
+          if (lv) c[v] = __fmul_rn(av, g[v]);
           // the first row of a sequence without h0 is h = x: its gate plays no part
-          da[v] = (lv && !(st && !A.h0)) ? (A.gate_log ? c[v] : g[v]) * hp[k][v] : 0.0f;
+          da[v] = (lv && !(st && !A.h0)) ? __fmul_rn(A.gate_log ? c[v] : g[v], hp[k][v]) : 0.0f;
           part[k] += chans.on(v) ? da[v] : 0.0f;
         }
         if (lv || A.zero_rest) {
@@ -508,7 +510,7 @@ int launch_wide(Params &p, bool backward, cudaStream_t stream) {
   const int64_t ncol = kGate == kOne ? a.gates * p.blocks_per_gate : (a.width + p.block - 1) / p.block;
   GEARB_REQUIRE(p.tiles <= (int64_t(1) << 31) / ncol - 1, "recurrence: too many tiles for one launch");
   p.ncol = static_cast<int>(ncol);
-  p.section_shift = long_sections(p, p.ncol) ? kLongSection : kShortSection;
+  p.section_shift = section_shift_of(p);
   const unsigned grid = static_cast<unsigned>(p.tiles * ncol);
   if (p.chain) GEARB_CUDA(cudaMemsetAsync(p.ticket, 0xff, static_cast<size_t>(p.chain_bytes), stream));
   if (backward) backward_kernel<TX, TA, V, kGate, kApart><<<grid, kThreads, 0, stream>>>(p);

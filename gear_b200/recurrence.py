@@ -159,7 +159,7 @@ def linear_recurrence(x: torch.Tensor, gate: torch.Tensor, *, h0: Optional[torch
     stream      where to launch (None: the current stream of x's device); gradients follow it
 
     Arithmetic and state are float32 whatever x's type; h is rounded once to x's type.  The bits of the result
-    depend on nothing but the inputs' values and shape.  Differentiable once in x, gate and h0; the backward pass
+    depend on nothing but the inputs' values and shape (a shared gate's gradient: and their alignment).  Differentiable once in x, gate and h0; the backward pass
     recomputes h in float32.  Products of a sequence's gates over up to 512 rows (32768 of a single channel) must stay
     inside float32's range, and so must exp(gate): where they pass it (|a| well above 1) h is infinite or NaN.
 

@@ -553,7 +553,7 @@ int gearb_layout_paged(const gearb_layout_args *args, void *stream);
  * float32 [sequences][width], each may be NULL (h0: zeros); state_out of an empty sequence is its h0.
  * Nothing that is written may overlap what is read, except that with time 1 state_out may be h0.
  * Types: x, out, dout, dx of x_dtype; gate, dgate of gate_dtype, either x_dtype or GEARB_DT_F32.
- * All arithmetic is float32; the result does not depend on timing.
+ * All arithmetic is float32; the result does not depend on timing, nor, but for the sums of shared gates, on alignment.
  * carry: what the backward pass needs besides x and gate, written by the forward pass when not NULL.
  * gearb_recurrence_bytes gives the sizes of scratch (contents irrelevant, one per call in flight) and
  * carry.  The backward pass reads x, gate, h0, dout, dstate and carry, writes dx, dgate and dh0.     */

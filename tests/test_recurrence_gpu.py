@@ -527,3 +527,25 @@ def test_beyond_32_bits(width):
     R.check(dgate[-tail:], want["dgate"], BF16, "dgate")
     for t in (h, dx, dgate):
         assert not t[:-tail].any()
+
+
+@pytest.mark.parametrize("width", [64, 200, 320, 512, 520, 640])
+@pytest.mark.parametrize("time", [300, 6000])
+@pytest.mark.parametrize("gate_dtype", [F32, BF16])
+def test_the_same_bits_whatever_the_alignment(width, time, gate_dtype):
+    x, gate = slow(width, (2, time), width, width, BF16, gate_dtype)
+    dh = torch.randn(2, time, width, device=DEV).to(BF16)
+    h0 = state_of(6, 2, width)
+
+    def both(x, gate):
+        leaves = [x.detach().requires_grad_(True), gate.detach().requires_grad_(True)]
+        h, s = recurrence.linear_recurrence(*leaves, h0=h0, gate_kind="log")
+        return [h, s] + list(torch.autograd.grad(h, leaves, dh))
+
+    shifted = []
+    for t in (x, gate):
+        room = torch.empty(2, time, width + 3, dtype=t.dtype, device=DEV)
+        room[..., 1:1 + width] = t
+        shifted.append(room[..., 1:1 + width])
+    for a, b in zip(both(x, gate), both(*shifted)):
+        assert torch.equal(a, b)
