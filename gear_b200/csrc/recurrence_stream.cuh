@@ -26,6 +26,7 @@
 
 #include "recurrence_narrow.cuh"
 #include "recurrence_wide.cuh"
+#include "ring.h"
 
 namespace gearb {
 namespace rec {
@@ -129,17 +130,6 @@ __device__ __forceinline__ void mbar_arrive(uint64_t *bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
 }
 
-// A place in a ring of barriers, and the parity of its use.
-template <unsigned kSize>
-struct Turn {
-  unsigned i = 0, parity = 0;
-  __device__ __forceinline__ void next() {
-    if (++i == kSize) {
-      i = 0;
-      parity ^= 1u;
-    }
-  }
-};
 // Shared memory of one stage.  A tensor copy writes to 128-byte boundaries.
 template <typename TX, typename TA, int V, int kGate, bool kBackward>
 struct Stage {
@@ -438,8 +428,8 @@ __device__ __forceinline__ bool finish_tiles(const Params &P, StreamShared<TX, T
   const gearb_recurrence_args &A = P.A;
   bool lost = false;
   unsigned stage = 0, parity = 0;
-  Turn<kRing> pair;
-  for (;; pair.next()) {
+  Follower<kRing> ready;
+  for (;;) {
     if (!warp_wait(&sm.full[stage], parity)) return true;
     const Plan &pl = sm.plan[stage];
     if (!pl.valid) return lost;
@@ -454,20 +444,21 @@ __device__ __forceinline__ bool finish_tiles(const Params &P, StreamShared<TX, T
         in = settle_back(P, tile, lo, d, peek, lost);
         if (!kBackward && A.carry) A.carry[pl.tile * A.width + d] = in;
       }
-      if (P.chain && tile % kSuper == kSuper - 1 && tile + 1 < P.tiles) {
-        if (!warp_wait(&sm.ready[pair.i], pair.parity)) return true;
-        if (on) {
-          const float h = sm.edge[stage].h[c];
-          publish_word(P.section + ((tile / kSuper + 1) * A.width + d), cut ? h : fmaf(sm.edge[stage].a[c], in, h));
-        }
-      }
     } else if (on && (lo >= 0 || (P.chain && tile % kSuper == kSuper - 1))) {
       auto own = [&] {
-        lost |= !mbar_wait(&sm.ready[pair.i], pair.parity);
+        lost |= !mbar_wait(&sm.ready[ready.turn.i], ready.turn.parity);
         return make_float2(sm.edge[stage].a[c], sm.edge[stage].h[c]);
       };
       in = look_back<kSuper - 1, kLongSection, int>(P, tile, lo >= 0 ? lo : tile, d, own, cut, lost);
       if (!kBackward && A.carry && lo >= 0) A.carry[pl.tile * A.width + d] = in;
+    }
+    // The tile's own pair, which the compute warps wait for as well.  Every tile's: see Follower.
+    if (!ready.pass([&](unsigned i, unsigned p) { return warp_wait(&sm.ready[i], p); })) return true;
+    if constexpr (!kLong) {
+      if (on && P.chain && tile % kSuper == kSuper - 1 && tile + 1 < P.tiles) {
+        const float h = sm.edge[stage].h[c];
+        publish_word(P.section + ((tile / kSuper + 1) * A.width + d), cut ? h : fmaf(sm.edge[stage].a[c], in, h));
+      }
     }
     if (c < 32 * V) {
       sm.edge[stage].in[c] = in;

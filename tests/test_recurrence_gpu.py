@@ -549,3 +549,44 @@ def test_the_same_bits_whatever_the_alignment(width, time, gate_dtype):
         shifted.append(room[..., 1:1 + width])
     for a, b in zip(both(x, gate), both(*shifted)):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("width,gates,dtype", [(64, 64, F32), (256, 256, F32), (256, 2, BF16), (700, 700, F32), (520, 4, BF16)])
+@pytest.mark.parametrize("reverse", [False, True])
+def test_states_behind_tiles_that_wait_for_nothing(width, gates, dtype, reverse):
+    """Tiles of many short sequences with states (slow to look at), then one that starts a sequence in the last tile of
+    eight, so that the state behind the eight depends on that tile's own rows alone; and padding.  Every time the bits of
+    the kernels without roles."""
+    rng = np.random.default_rng(width)
+    lens = []
+    for _ in range(40):                       # 512 rows: short ones up to row 448 or so, one over the end of the eight tiles
+        room = 448 - (64 if lens else 0)
+        while room > 0:
+            lens.append(int(min(room, rng.integers(1, 6))))
+            room -= lens[-1]
+        lens.append(128)
+    lens += [0, 3000, 5]
+    off = torch.tensor(np.cumsum([0] + lens), dtype=torch.int64, device=DEV)
+    rows = int(off[-1]) + 1500                # rows of no sequence behind the last
+    x, gate = slow(width, (rows,), width, gates, dtype, F32)
+    h0 = state_of(5, len(lens), width)
+    dh = torch.randn(rows, width, device=DEV).to(dtype)
+    dst = state_of(6, len(lens), width)
+
+    def once(x, gate):
+        leaves = [t.detach().requires_grad_(True) for t in (x, gate, h0)]
+        h, s = recurrence.linear_recurrence(*leaves[:2], h0=leaves[2], offsets=off, reverse=reverse, gate_kind="log")
+        return [h, s, *torch.autograd.grad([h, s], leaves, [dh, dst])]
+
+    room = torch.empty(rows, width + 1, dtype=dtype, device=DEV)
+    room[:, 1:] = x
+    groom = torch.empty(rows, gates + 1, dtype=F32, device=DEV)
+    groom[:, 1:] = gate
+    want = once(room[:, 1:], groom[:, 1:])
+    for _ in range(20):
+        got = once(x, gate)
+        for i, (a, b) in enumerate(zip(got, want)):
+            if i != 3 or gates == width:      # the sums of shared gates depend on alignment
+                assert torch.equal(a, b), i
+    if not reverse:
+        run_and_check(x, gate, h0, offsets=off, log=True)
