@@ -170,6 +170,7 @@ _SIGS = {
     "gearb_layout_scratch_bytes": (i64, [i64]),
     "gearb_layout_paged": (C.c_int, [vp, vp]),
     "gearb_recurrence_bytes": (C.c_int, [vp, C.c_int, pi64, pi64]),
+    "gearb_recurrence_wait_limit": (C.c_int, [C.c_int]),
     "gearb_recurrence_forward": (C.c_int, [vp, vp]),
     "gearb_recurrence_backward": (C.c_int, [vp, vp]),
     "gearb_fill": (C.c_int, [vp, i64, C.c_int, u64, u64, f64, f64, vp]),

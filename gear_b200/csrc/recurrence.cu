@@ -42,6 +42,8 @@ int encode_map(CUtensorMap *map, CUtensorMapDataType type, void *base, int64_t w
 
 namespace {
 
+std::atomic<int> g_wait_limit{-1};  // as gearb_recurrence_wait_limit has set it
+
 // Joins the column blocks' sums of a gate whose channels span several of them, in order.  Rows of no
 // sequence hold zeros when zero_rest is set; otherwise they are left as they are.
 template <typename TA>
@@ -304,6 +306,9 @@ int launch(const gearb_recurrence_args &a, bool backward, cudaStream_t stream) {
   p.tile_rows = t.tile_rows;
   p.chain = t.chain;
   p.narrow_rows = t.narrow_rows;
+  const int limit = g_wait_limit.load(std::memory_order_relaxed);
+  p.poll_limit = limit < 0 ? kPollLimit : limit;
+  p.no_waits = limit == 0;
   if (p.rows == 0) {
     const float *from = backward ? a.dstate : a.h0;
     float *to = backward ? a.dh0 : a.state_out;
@@ -411,6 +416,8 @@ int gearb_recurrence_bytes(const gearb_recurrence_args *args, int backward, int6
   *carry_bytes = t.chain ? t.tiles * args->width * 4 : 0;
   return GEARB_OK;
 }
+
+int gearb_recurrence_wait_limit(int polls) { return g_wait_limit.exchange(polls < 0 ? -1 : polls); }
 
 int gearb_recurrence_forward(const gearb_recurrence_args *args, void *stream) {
   TraceRange trace("gearb:recurrence");

@@ -23,7 +23,7 @@
 // 4 x 32768 x 768 (6 blocks) 217 and 229, 1 x 32768 x 2048 (16 blocks) 113 and 124, 3000 x 300 x 64 171 and 235.
 // A tile needs nothing from before the start of the sequence its first row belongs to.  Tiles are handed out by a counter
 // in scan order, so a CTA only ever waits for CTAs that are already running; every wait has a limit, after which the
-// launch goes on with NaN and says so in the status word.  Published words are 32 bits that read 0xffffffff until they
+// launch says so in the status word and the rows concerned, their states and what depends on them are NaN.  Published words are 32 bits that read 0xffffffff until they
 // are written (a value of those bits is published as another NaN), so no flags and fences are needed beside them.
 //
 // Backward.  In terms of c_t = a_t * g_t the gradients obey c_t = a_t * c_(t+1) + a_t * dh_t, the same
@@ -53,6 +53,7 @@ constexpr unsigned kAll = 0xffffffffu;
 constexpr unsigned kAllRows = (1u << kRows) - 1u;
 constexpr unsigned kUnset = 0xffffffffu;     // a published word that has not been written
 constexpr int kPollLimit = 1 << 20;          // polls of one word, the better part of a second
+constexpr unsigned kWaitLimit = 1u << 20;    // polls of an mbarrier, 4 s
 
 template <typename T> __device__ __forceinline__ float to_f(T v);
 template <> __device__ __forceinline__ float to_f(float v) { return v; }
@@ -139,14 +140,16 @@ struct Params {
   TileRec *recs;         // [tiles]
   int64_t chain_bytes;   // at `ticket`: to be set to 0xff before tiles publish
   float *gate_part;      // [blocks_per_gate][rows][gates], when a gate's channels span several column blocks
+  int poll_limit;        // polls of a published word before the wait is given up
+  int no_waits;          // the roles of a streaming kernel give up at once
 };
 
-__device__ __forceinline__ unsigned poll_word(const unsigned *p, bool &lost) {
+__device__ __forceinline__ unsigned poll_word(const unsigned *p, int limit, bool &lost) {
   unsigned v;
   for (int n = 0;; ++n) {
     asm volatile("ld.relaxed.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
     if (v != kUnset) return v;
-    if (lost || n == kPollLimit) break;
+    if (lost || n == limit) break;
     __nanosleep(20);
   }
   lost = true;
@@ -157,12 +160,12 @@ __device__ __forceinline__ float2 peek_pair(const float2 *p) {
   asm volatile("ld.relaxed.gpu.global.v2.u32 {%0,%1}, [%2];" : "=r"(a), "=r"(h) : "l"(p) : "memory");
   return make_float2(__uint_as_float(a), __uint_as_float(h));
 }
-__device__ __forceinline__ float2 poll_pair(const float2 *p, bool &lost) {
+__device__ __forceinline__ float2 poll_pair(const float2 *p, int limit, bool &lost) {
   unsigned a, h;
   for (int n = 0;; ++n) {
     asm volatile("ld.relaxed.gpu.global.v2.u32 {%0,%1}, [%2];" : "=r"(a), "=r"(h) : "l"(p) : "memory");
     if (a != kUnset && h != kUnset) return make_float2(__uint_as_float(a), __uint_as_float(h));
-    if (lost || n == kPollLimit) break;
+    if (lost || n == limit) break;
     __nanosleep(20);
   }
   lost = true;
@@ -500,7 +503,7 @@ __device__ __forceinline__ float look_back(const Params &P, Index at, Index lo, 
       if (from + u < n) q[u] = peek_pair(p + (from + u) * width);
   };
   auto settle = [&](float2 &q, const float2 *p) {
-    if (__float_as_uint(q.x) == kUnset || __float_as_uint(q.y) == kUnset) q = poll_pair(p, lost);
+    if (__float_as_uint(q.x) == kUnset || __float_as_uint(q.y) == kUnset) q = poll_pair(p, P.poll_limit, lost);
   };
   unsigned word = 0;
   peek(t, tp, 0, tiles);
@@ -529,7 +532,7 @@ __device__ __forceinline__ float look_back(const Params &P, Index at, Index lo, 
   if (by_super) {
     float h = 0.0f;
     if (by_section) {
-      if (word == kUnset) word = poll_word(reinterpret_cast<const unsigned *>(P.section + sec * width + d), lost);
+      if (word == kUnset) word = poll_word(reinterpret_cast<const unsigned *>(P.section + sec * width + d), P.poll_limit, lost);
       h = __uint_as_float(word);
     }
     for (int j = 0; j < supers; j += kAhead) {

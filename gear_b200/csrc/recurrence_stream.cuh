@@ -40,7 +40,6 @@ constexpr int kRecorders = 2;  // one takes 3 us a tile: two dependent trips to 
 constexpr int kTableGates = 8;
 
 constexpr unsigned kNoItem = 0xffffffffu;
-constexpr unsigned kWaitLimit = 1u << 20;  // mbarrier polls before a copy is declared lost
 
 __device__ __forceinline__ uint32_t smem_addr(const void *p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 __device__ __forceinline__ void mbar_init(uint64_t *bar) {
@@ -49,7 +48,10 @@ __device__ __forceinline__ void mbar_init(uint64_t *bar) {
 __device__ __forceinline__ void mbar_expect(uint64_t *bar, unsigned bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_addr(bar)), "r"(bytes) : "memory");
 }
+// Every try waits up to 4 us by itself; with a hint it may wait as long as the hint says, and 2^20 times that is no limit.  The
+// limit is a constant: as a parameter of the launch it made packed heads 5 % slower.
 __device__ __forceinline__ bool mbar_wait(uint64_t *bar, unsigned parity) {
+#pragma unroll 1
   for (unsigned n = 0; n < kWaitLimit; ++n) {
     unsigned ok;
     asm volatile(
@@ -187,6 +189,10 @@ struct StreamShared {
   unsigned item[kStages];
   uint64_t entered[kStages];               // edge.in is there
   uint64_t paired[kRing], ready[kRing], read[kRing];   // the warps' pairs; turned and edge.a, edge.h there; read again
+  // How far the roles have come when they end, for abandon(): tiles issued, the item behind them, tiles that each compute warp
+  // has done with, the turn of the first tile that each recorder has not recorded.
+  unsigned issued_tiles, next, done[kWarps];
+  Turn<kStages> recorded[kRecorders];
 };
 
 // Short sections: what the tiles before one (in the order of the tickets) published, asked for at once.
@@ -219,13 +225,13 @@ __device__ __forceinline__ float settle_back(const Params &P, int at, int lo, in
   for (int u = 0; u < kSuper - 1; ++u)
     if (u < count) {
       if (__float_as_uint(k.q[u].x) == kUnset || __float_as_uint(k.q[u].y) == kUnset)
-        k.q[u] = poll_pair(p + u * P.A.width, lost);
+        k.q[u] = poll_pair(p + u * P.A.width, P.poll_limit, lost);
       ph = (u == 0 && !need_section) ? k.q[u].y : fmaf(k.q[u].x, ph, k.q[u].y);
       pa *= k.q[u].x;
     }
   if (!need_section) return ph;
   if (__float_as_uint(k.s) == kUnset)
-    k.s = __uint_as_float(poll_word(reinterpret_cast<const unsigned *>(P.section + sb * P.A.width + d), lost));
+    k.s = __uint_as_float(poll_word(reinterpret_cast<const unsigned *>(P.section + sb * P.A.width + d), P.poll_limit, lost));
   return fmaf(pa, k.s, ph);
 }
 
@@ -245,32 +251,52 @@ __device__ __forceinline__ Place place_of_item(const Params &P, unsigned item) {
   return at;
 }
 
+// The items of a call: tiles without sequences are none, the launch before has zeroed their rows.  (Taken through the
+// pipeline, the 43 % of a packed batch's room that no sequence filled cost a quarter of the time.)
+struct Items {
+  unsigned base, end;
+};
+template <bool kBackward>
+__device__ __forceinline__ Items items_of(const Params &P) {
+  const LiveTiles live = live_tiles(P);
+  Items t;
+  t.base = static_cast<unsigned>((kBackward ? P.tiles - live.end : live.first) * P.ncol);
+  t.end = t.base + static_cast<unsigned>((live.end - live.first) * P.ncol);
+  return t;
+}
+// The item behind `item` for this CTA.
+__device__ __forceinline__ unsigned item_behind(const Params &P, const Items &items, unsigned item) {
+  return P.chain ? items.base + atomicAdd(P.ticket, 1u) + 1u : item + gridDim.x;  // the counter starts at 0xffffffff
+}
+
 // The issuing warp (one lane of it): numbers and copies.
 template <typename TX, typename TA, int V, int kGate, bool kBackward>
 __device__ __forceinline__ bool issue_tiles(const Params &P, const Maps &maps, StreamShared<TX, TA, V, kGate, kBackward> &sm) {
   using Shared = StreamShared<TX, TA, V, kGate, kBackward>;
   const gearb_recurrence_args &A = P.A;
-  // Tiles without sequences are no items: the launch before has zeroed their rows.  (Taken through the pipeline, the
-  // 43 % of a packed batch's room that no sequence filled cost a quarter of the time.)
-  const LiveTiles live = live_tiles(P);
-  const unsigned base = static_cast<unsigned>((kBackward ? P.tiles - live.end : live.first) * P.ncol);
-  const unsigned items = base + static_cast<unsigned>((live.end - live.first) * P.ncol);
+  const Items items = items_of<kBackward>(P);
   // One number at a time from the start: CTAs that took several at once would come to tiles much later than others come to
   // the tiles behind them, and those would wait.
-  unsigned next = base + (P.chain ? atomicAdd(P.ticket, 1u) + 1u : blockIdx.x);  // the counter starts at 0xffffffff
+  unsigned next = P.chain ? item_behind(P, items, 0) : items.base + blockIdx.x;
   Turn<Shared::kStages> now;
+  bool lost = false;
   for (unsigned m = 0;; ++m, now.next()) {
-    if (m >= Shared::kStages && !mbar_wait(&sm.empty[now.i], now.parity ^ 1u)) return true;
+    lost = m >= Shared::kStages && (P.no_waits || !mbar_wait(&sm.empty[now.i], now.parity ^ 1u));
+    if (lost || next >= items.end) {
+      sm.issued_tiles = m;
+      sm.next = next;
+      if (lost) return true;
+    }
     const unsigned item = next;
-    sm.item[now.i] = item < items ? item : kNoItem;
-    if (item >= items) {
+    sm.item[now.i] = item < items.end ? item : kNoItem;
+    if (item >= items.end) {
       mbar_arrive(&sm.full[now.i]);
       for (int r = 0; r < kRecorders; ++r) {  // every recorder has to learn that there are no more
         mbar_arrive(&sm.issued[now.i]);
         now.next();
         if (r + 1 < kRecorders) {
           ++m;
-          if (m >= Shared::kStages && !mbar_wait(&sm.empty[now.i], now.parity ^ 1u)) return true;
+          if (m >= Shared::kStages && (P.no_waits || !mbar_wait(&sm.empty[now.i], now.parity ^ 1u))) return true;
           sm.item[now.i] = kNoItem;
         }
       }
@@ -285,7 +311,7 @@ __device__ __forceinline__ bool issue_tiles(const Params &P, const Maps &maps, S
     if constexpr (kGate == kOwn) tensor_load(sm.stage[now.i].gate, &maps.gate, c, r, full);
     if constexpr (kBackward) tensor_load(sm.stage[now.i].dout, &maps.dout, c, r, full);
     mbar_arrive(&sm.issued[now.i]);
-    next = P.chain ? base + atomicAdd(P.ticket, 1u) + 1u : item + gridDim.x;  // needed a tile later
+    next = item_behind(P, items, item);  // needed a tile later
   }
 }
 
@@ -297,12 +323,16 @@ __device__ __forceinline__ bool record_tiles(const Params &P, StreamShared<TX, T
   Turn<Shared::kStages> now;
   for (int k = 0; k < which; ++k) now.next();
   for (;;) {
-    if (!warp_wait(&sm.issued[now.i], now.parity)) return true;
+    if (!warp_wait(&sm.issued[now.i], now.parity)) {
+      if (lane == 0) sm.recorded[which] = now;
+      return true;
+    }
     const unsigned item = sm.item[now.i];
     Plan &pl = sm.plan[now.i];
     if (item == kNoItem) {
       if (lane == 0) {
         pl.valid = 0;
+        sm.recorded[which] = now;
         mbar_arrive(&sm.full[now.i]);
       }
       return false;
@@ -446,8 +476,10 @@ __device__ __forceinline__ bool finish_tiles(const Params &P, StreamShared<TX, T
       }
     } else if (on && (lo >= 0 || (P.chain && tile % kSuper == kSuper - 1))) {
       auto own = [&] {
-        lost |= !mbar_wait(&sm.ready[ready.turn.i], ready.turn.parity);
-        return make_float2(sm.edge[stage].a[c], sm.edge[stage].h[c]);
+        if (mbar_wait(&sm.ready[ready.turn.i], ready.turn.parity))
+          return make_float2(sm.edge[stage].a[c], sm.edge[stage].h[c]);
+        lost = true;
+        return make_float2(__uint_as_float(0x7fffffffu), __uint_as_float(0x7fffffffu));
       };
       in = look_back<kSuper - 1, kLongSection, int>(P, tile, lo >= 0 ? lo : tile, d, own, cut, lost);
       if (!kBackward && A.carry && lo >= 0) A.carry[pl.tile * A.width + d] = in;
@@ -524,15 +556,15 @@ __device__ __forceinline__ bool publish_tiles(const Params &P, StreamShared<TX, 
 }
 
 template <typename TX, typename TA, int V, int kGate>
-__device__ __forceinline__ bool compute_forward(const Params &P, StreamShared<TX, TA, V, kGate, false> &sm, int warp,
-                                                int lane) {
+__device__ __forceinline__ bool compute_forward(const Params &P, StreamShared<TX, TA, V, kGate, false> &sm, unsigned &m,
+                                                int warp, int lane) {
   using Shared = StreamShared<TX, TA, V, kGate, false>;
   constexpr int kG = kGate == kOne ? 1 : V, R = kRows;
   const gearb_recurrence_args &A = P.A;
   Turn<Shared::kStages> now, old;
   Turn<kRing> pair, opair;
-  unsigned m = 0, tiles = 0xffffffffu;  // tiles of this CTA, known when the issuer has said that there are no more
-  for (; m < kLag || m - kLag < tiles; ++m) {
+  unsigned tiles = 0xffffffffu;  // of this CTA, known when the issuer has said that there are no more
+  for (m = 0; m < kLag || m - kLag < tiles; ++m) {
     if (tiles == 0xffffffffu) {
       if (!warp_wait(&sm.full[now.i], now.parity)) return true;
       if (!sm.plan[now.i].valid) tiles = m;
@@ -638,14 +670,15 @@ __device__ __forceinline__ bool compute_forward(const Params &P, StreamShared<TX
 }
 
 template <typename TX, typename TA, int V, int kGate>
-__device__ __forceinline__ bool compute_backward(const Params &P, StreamShared<TX, TA, V, kGate, true> &sm, int warp, int lane) {
+__device__ __forceinline__ bool compute_backward(const Params &P, StreamShared<TX, TA, V, kGate, true> &sm, unsigned &m,
+                                                 int warp, int lane) {
   using Shared = StreamShared<TX, TA, V, kGate, true>;
   constexpr int kG = kGate == kOne ? 1 : V, R = kRows;
   const gearb_recurrence_args &A = P.A;
   Turn<Shared::kStages> now, old;
   Turn<kRing> pair, opair;
-  unsigned m = 0, tiles = 0xffffffffu;
-  for (; m < kLag || m - kLag < tiles; ++m) {
+  unsigned tiles = 0xffffffffu;
+  for (m = 0; m < kLag || m - kLag < tiles; ++m) {
     if (tiles == 0xffffffffu) {
       if (!warp_wait(&sm.full[now.i], now.parity)) return true;
       if (!sm.plan[now.i].valid) tiles = m;
@@ -822,6 +855,85 @@ __device__ __forceinline__ bool compute_backward(const Params &P, StreamShared<T
   return false;
 }
 
+// What an item's rows, states and published words hold when it was given up: NaN, but for rows of no sequence and words
+// that were there already.  All threads.
+template <typename TX, typename TA, int V, int kGate, bool kBackward>
+__device__ void give_up_item(const Params &P, unsigned item) {
+  const gearb_recurrence_args &A = P.A;
+  const float nan = __uint_as_float(0x7fffffffu);
+  const Place at = place_of_item<V, kGate, kBackward>(P, item);
+  const TileRec &rec = P.recs[at.tile];
+  const int n = static_cast<int>(at.i1 - at.i0), cols = static_cast<int>(at.d1 - at.d0 < 32 * V ? at.d1 - at.d0 : 32 * V);
+  TX *rows = static_cast<TX *>(kBackward ? A.dx : A.out);
+  float *states = kBackward ? A.dh0 : A.state_out;
+  for (int e = threadIdx.x; e < n * cols; e += kStreamThreads) {
+    const int k = e / cols;
+    const int64_t row = row_of(P, at.i0 + k), d = at.d0 + (e - k * cols);
+    const bool live = rec.live[k / kRows] >> (k % kRows) & 1u;
+    const float v = live ? nan : 0.0f;
+    if (live || A.zero_rest) {
+      rows[row * A.width + d] = from_f<TX>(v);
+      if (kBackward && kGate == kOwn) static_cast<TA *>(A.dgate)[row * A.gates + d] = from_f<TA>(v);
+      if (kBackward && kGate == kOne && e == k * cols) {
+        if (P.blocks_per_gate == 1) static_cast<TA *>(A.dgate)[row * A.gates + at.gate] = from_f<TA>(v);
+        else P.gate_part[(at.part * P.rows + row) * A.gates + at.gate] = v;
+      }
+    }
+    if (states && ((kBackward ? rec.start : rec.end)[k / kRows] >> (k % kRows) & 1u))
+      states[static_cast<int64_t>(rec.seq[k]) * A.width + d] = nan;
+  }
+  if (!P.chain) return;
+  const int64_t t = kBackward ? P.tiles - 1 - at.tile : at.tile, sb = t / kSuper, sec = t >> P.section_shift;
+  for (int c = threadIdx.x; c < cols; c += kStreamThreads) {
+    const int64_t d = at.d0 + c;
+    if (!kBackward && A.carry && rec.open) A.carry[at.tile * A.width + d] = nan;
+    auto unset = [](const float2 &q) { return __float_as_uint(q.x) == kUnset || __float_as_uint(q.y) == kUnset; };
+    float2 *own = P.agg + t * A.width + d;
+    if (unset(peek_pair(own))) publish_pair(own, nan, nan);
+    if (t % kSuper != kSuper - 1 || t + 1 >= P.tiles) continue;
+    if (t + 1 == (sec + 1) << P.section_shift) {
+      float *state = P.section + (sec + 1) * A.width + d;
+      bool seen = true;
+      if (poll_word(reinterpret_cast<const unsigned *>(state), 0, seen) == 0x7fffffffu) publish_word(state, nan);
+    } else if (unset(peek_pair(P.super + sb * A.width + d))) {
+      publish_pair(P.super + sb * A.width + d, nan, nan);
+    }
+  }
+}
+
+// A wait ran into its limit: the roles have ended somewhere.  Copies under way have to land before the CTA leaves its shared
+// memory; tiles that are not done, and those that nobody has taken, are given up, so that no row is left unwritten and no
+// CTA waits for what will not come.  All threads.
+template <typename TX, typename TA, int V, int kGate, bool kBackward>
+__device__ __noinline__ void abandon(const Params &P, StreamShared<TX, TA, V, kGate, kBackward> &sm) {
+  constexpr unsigned kStages = StreamShared<TX, TA, V, kGate, kBackward>::kStages;
+  unsigned from = sm.done[0];
+  for (int w = 1; w < kWarps; ++w) from = sm.done[w] < from ? sm.done[w] : from;
+  const unsigned to = sm.issued_tiles;  // at most kStages more: a stage is used again when all warps are done with it
+  if (threadIdx.x == 0) {
+    if (P.A.status) atomicOr(reinterpret_cast<unsigned *>(P.A.status), GEARB_ST_SCAN_ABORTED);
+    bool recorded[kRecorders];  // whether the recorder has been at the tiles so far
+    for (int r = 0; r < kRecorders; ++r) recorded[r] = true;
+    for (unsigned m = from; m < to; ++m) {
+      const unsigned stage = m % kStages, parity = m / kStages & 1u, r = m % kRecorders;
+      if (sm.recorded[r].i == stage && sm.recorded[r].parity == parity) recorded[r] = false;
+      if (!recorded[r]) mbar_arrive(&sm.full[stage]);  // in its recorder's place
+      mbar_wait(&sm.full[stage], parity);
+    }
+  }
+  __syncthreads();
+  for (unsigned m = from; m < to; ++m) give_up_item<TX, TA, V, kGate, kBackward>(P, sm.item[m % kStages]);
+  const Items items = items_of<kBackward>(P);
+  for (;;) {
+    const unsigned item = sm.next;
+    if (item >= items.end) return;
+    give_up_item<TX, TA, V, kGate, kBackward>(P, item);
+    __syncthreads();
+    if (threadIdx.x == 0) sm.next = item_behind(P, items, item);
+    __syncthreads();
+  }
+}
+
 template <typename TX, typename TA, int V, int kGate, bool kBackward>
 __device__ __forceinline__ void init_barriers(StreamShared<TX, TA, V, kGate, kBackward> &sm) {
   if (threadIdx.x == 0) {
@@ -850,12 +962,28 @@ __global__ void __launch_bounds__(kStreamThreads, 1) forward_stream_kernel(const
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   init_barriers(sm);
   bool lost = false;
-  if (warp < kWarps) lost = compute_forward<TX, TA, V, kGate>(P, sm, warp, lane);
-  else if (warp < kWarps + 4) lost = publish_tiles<TX, TA, V, kGate, false>(P, sm, threadIdx.x - kThreads, lane);
-  else if (warp < kWarps + 8) lost = finish_tiles<TX, TA, V, kGate, false, kLong>(P, sm, threadIdx.x - kThreads - 128, lane);
-  else if (warp < kWarps + 8 + kRecorders) lost = record_tiles<TX, TA, V, kGate, false>(P, sm, warp - kWarps - 8, lane);
-  else if (lane == 0) lost = issue_tiles<TX, TA, V, kGate, false>(P, maps, sm);
-  if (lost && lane == 0 && P.A.status) atomicOr(reinterpret_cast<unsigned *>(P.A.status), GEARB_ST_SCAN_ABORTED);
+  if (warp == kWarps + 8 + kRecorders) {
+    if (lane == 0) lost = issue_tiles<TX, TA, V, kGate, false>(P, maps, sm);
+  } else if (P.no_waits) {
+    lost = true;
+    if (threadIdx.x < kWarps) sm.done[threadIdx.x] = 0;
+    if (threadIdx.x < kRecorders) {
+      sm.recorded[threadIdx.x].i = threadIdx.x;
+      sm.recorded[threadIdx.x].parity = 0;
+    }
+  } else if (warp < kWarps) {
+    unsigned m;
+    lost = compute_forward<TX, TA, V, kGate>(P, sm, m, warp, lane);
+    if (lane == 0) sm.done[warp] = m < kLag ? 0 : m - kLag;
+  } else if (warp < kWarps + 4) {
+    lost = publish_tiles<TX, TA, V, kGate, false>(P, sm, threadIdx.x - kThreads, lane);
+  } else if (warp < kWarps + 8) {
+    lost = finish_tiles<TX, TA, V, kGate, false, kLong>(P, sm, threadIdx.x - kThreads - 128, lane);
+  } else {
+    lost = record_tiles<TX, TA, V, kGate, false>(P, sm, warp - kWarps - 8, lane);
+  }
+  __syncwarp();
+  if (__syncthreads_or(lost)) abandon(P, sm);
 }
 
 template <typename TX, typename TA, int V, int kGate, bool kLong>
@@ -867,12 +995,28 @@ __global__ void __launch_bounds__(kStreamThreads, 1) backward_stream_kernel(cons
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   init_barriers(sm);
   bool lost = false;
-  if (warp < kWarps) lost = compute_backward<TX, TA, V, kGate>(P, sm, warp, lane);
-  else if (warp < kWarps + 4) lost = publish_tiles<TX, TA, V, kGate, true>(P, sm, threadIdx.x - kThreads, lane);
-  else if (warp < kWarps + 8) lost = finish_tiles<TX, TA, V, kGate, true, kLong>(P, sm, threadIdx.x - kThreads - 128, lane);
-  else if (warp < kWarps + 8 + kRecorders) lost = record_tiles<TX, TA, V, kGate, true>(P, sm, warp - kWarps - 8, lane);
-  else if (lane == 0) lost = issue_tiles<TX, TA, V, kGate, true>(P, maps, sm);
-  if (lost && lane == 0 && P.A.status) atomicOr(reinterpret_cast<unsigned *>(P.A.status), GEARB_ST_SCAN_ABORTED);
+  if (warp == kWarps + 8 + kRecorders) {
+    if (lane == 0) lost = issue_tiles<TX, TA, V, kGate, true>(P, maps, sm);
+  } else if (P.no_waits) {
+    lost = true;
+    if (threadIdx.x < kWarps) sm.done[threadIdx.x] = 0;
+    if (threadIdx.x < kRecorders) {
+      sm.recorded[threadIdx.x].i = threadIdx.x;
+      sm.recorded[threadIdx.x].parity = 0;
+    }
+  } else if (warp < kWarps) {
+    unsigned m;
+    lost = compute_backward<TX, TA, V, kGate>(P, sm, m, warp, lane);
+    if (lane == 0) sm.done[warp] = m < kLag ? 0 : m - kLag;
+  } else if (warp < kWarps + 4) {
+    lost = publish_tiles<TX, TA, V, kGate, true>(P, sm, threadIdx.x - kThreads, lane);
+  } else if (warp < kWarps + 8) {
+    lost = finish_tiles<TX, TA, V, kGate, true, kLong>(P, sm, threadIdx.x - kThreads - 128, lane);
+  } else {
+    lost = record_tiles<TX, TA, V, kGate, true>(P, sm, warp - kWarps - 8, lane);
+  }
+  __syncwarp();
+  if (__syncthreads_or(lost)) abandon(P, sm);
 }
 
 // A matrix of [rows][width] for boxes of kTile rows and 32 * V channels.

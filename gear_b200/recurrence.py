@@ -154,8 +154,8 @@ def linear_recurrence(x: torch.Tensor, gate: torch.Tensor, *, h0: Optional[torch
     state       float32 [sequences, width] (None with return_state=False); an empty sequence keeps its h0
     out, state_out   write there instead of allocating (no gradients then); with `out` the rows of no
                 sequence are left as they were.  state_out may be h0 itself; apart from that nothing may overlap
-    status      int32[4] as of the other launches: ST_SCAN_ABORTED if a wait inside the launch ran out (h is
-                not valid then)
+    status      int32[4] as of the other launches: ST_SCAN_ABORTED if a wait inside the launch ran out (rows and
+                states that were not worked out, and those that depend on them, are NaN then, status or not)
     stream      where to launch (None: the current stream of x's device); gradients follow it
 
     Arithmetic and state are float32 whatever x's type; h is rounded once to x's type.  The bits of the result

@@ -583,6 +583,12 @@ typedef struct gearb_recurrence_args {
 } gearb_recurrence_args;
 int gearb_recurrence_bytes(const gearb_recurrence_args *args, int backward, int64_t *scratch_bytes,
                            int64_t *carry_bytes);
+/* Waits inside a launch have a limit; where one runs out the launch ends with GEARB_ST_SCAN_ABORTED in status[0], and
+ * NaN in the rows and states that were not worked out and in those that depend on them.  This sets the limit, for the
+ * launches that follow, by any thread, and returns the one before: polls of a word that another part of the launch
+ * publishes (below 0: the default, the better part of a second).  0: nothing is waited for at all.  For tests, and for
+ * tools under which kernels run much slower.                                                                */
+int gearb_recurrence_wait_limit(int polls);
 int gearb_recurrence_forward(const gearb_recurrence_args *args, void *stream);
 int gearb_recurrence_backward(const gearb_recurrence_args *args, void *stream);
 

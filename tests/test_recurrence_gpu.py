@@ -590,3 +590,74 @@ def test_states_behind_tiles_that_wait_for_nothing(width, gates, dtype, reverse)
                 assert torch.equal(a, b), i
     if not reverse:
         run_and_check(x, gate, h0, offsets=off, log=True)
+
+
+class polls:
+    """Waits inside the launches of the block give up after `n` polls."""
+
+    def __init__(self, n):
+        self.n = n
+
+    def __enter__(self):
+        self.before = N.lib.gearb_recurrence_wait_limit(self.n)
+
+    def __exit__(self, *exc):
+        torch.cuda.synchronize()
+        N.lib.gearb_recurrence_wait_limit(self.before)
+
+
+# streaming (a gate per channel, shared; long sections and short ones), a CTA per tile, few channels
+WAITS = [(64, 64, F32, False), (1024, 1024, BF16, False), (256, 4, BF16, False), (80, 1, F32, False), (63, 63, F32, True),
+         (130, 10, BF16, True), (1, 1, F32, True), (6, 2, F32, True)]
+
+
+@pytest.mark.parametrize("width,gates,dtype,polled", WAITS)
+@pytest.mark.parametrize("reverse", [False, True])
+def test_a_wait_that_runs_out(width, gates, dtype, polled, reverse):
+    """With no polls at all: the status says so, and what was not worked out is NaN, nothing else; `polled`: kernels that
+    only wait for words of other tiles, and may find them there at the first look."""
+    rows = 60000 if width <= 16 else 9000
+    lens = [700, 0, rows - 1500, 1, 99]
+    off = torch.tensor(np.cumsum([0] + lens), dtype=torch.int64, device=DEV)
+    owned = int(off[-1])
+    x, gate = slow(width, (rows,), width, gates, dtype, F32)
+    h0 = state_of(1, len(lens), width)
+    dh = torch.randn(rows, width, device=DEV).to(dtype)
+    dst = state_of(2, len(lens), width)
+
+    def forward(status=None):
+        leaves = [t.detach().requires_grad_(True) for t in (x, gate, h0)]
+        h, s = recurrence.linear_recurrence(*leaves[:2], h0=leaves[2], offsets=off, reverse=reverse, gate_kind="log",
+                                            status=status)
+        return leaves, h, s
+
+    def backward(leaves, h, s):
+        return torch.autograd.grad([h, s], leaves, [dh, dst], retain_graph=True)
+
+    leaves, h, s = forward()
+    want = [h, s, *backward(leaves, h, s)]
+    for n in (0, 1, 3):
+        status = torch.zeros(N.STATUS_WORDS, dtype=torch.int32, device=DEV)
+        leaves, h, s = forward(status)
+        with polls(n):
+            _, bad_h, bad_s = forward(status)
+        gave_up = bool(status[0].item() & N.ST_SCAN_ABORTED)
+        status.zero_()
+        with polls(n):
+            grads = backward(leaves, h, s)
+        gave_up_back = bool(status[0].item() & N.ST_SCAN_ABORTED)
+        got = [bad_h, bad_s, *grads]
+        for i, (a, b) in enumerate(zip(got, want)):
+            lost = torch.isnan(a)
+            assert torch.equal(torch.where(lost, b, a), b), (n, i)
+            assert not lost.any() or (gave_up if i < 2 else gave_up_back), (n, i)
+        assert not any(torch.isnan(t[owned:]).any() for t in (bad_h, grads[0], grads[1]))
+        assert torch.equal(bad_s[1], h0[1]) and torch.equal(grads[2][1], dst[1])
+        if n == 0 and not polled:
+            assert gave_up and gave_up_back
+            assert torch.isnan(bad_h[:owned]).all() and torch.isnan(grads[0][:owned]).all() and torch.isnan(grads[1][:owned]).all()
+            assert torch.isnan(bad_s[[0, 2, 3, 4]]).all() and torch.isnan(grads[2][[0, 2, 3, 4]]).all()
+    # and the next launches are as ever
+    leaves, h, s = forward()
+    for a, b in zip([h, s, *backward(leaves, h, s)], want):
+        assert torch.equal(a, b)
