@@ -128,9 +128,10 @@ __device__ __forceinline__ void place_requests(const LayoutParams &P, int64_t r0
   pages += ty;
 }
 
+// Inside the pool, whatever the counter holds: sums of pages behind it stay inside 64 bits.
 __device__ __forceinline__ int64_t used_before(const gearb_layout_args &a) {
   const int64_t u = *a.used_in;
-  return u < 0 ? 0 : u;
+  return u < 0 ? 0 : (u > a.num_pages ? a.num_pages : u);
 }
 __device__ __forceinline__ void finish_sums(const gearb_layout_args &a, int64_t tokens, int64_t pages, unsigned &flags) {
   a.offsets[a.requests] = tokens;

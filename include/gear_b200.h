@@ -516,7 +516,8 @@ int gearb_handler_gather_packed(gearb_handler *h, const int32_t *columns, int nc
  *   block_table[r][ceil(past[r] / page) ...] = those pages; its other entries are left as they are
  *   slot_map[offsets[r] + t] = block_table[r][(past[r]+t) / page] * page + (past[r]+t) % page;
  *                entries from offsets[requests] to max_tokens are -1
- *   used_out   = min(used_in + sum of need_r, num_pages); may be the same address as used_in
+ *   used_out   = min(used_in + sum of need_r, num_pages); may be the same address as used_in (which is
+ *                cut to [0, num_pages])
  * Where the pool runs out the entries and slots are -1 (GEARB_ST_NO_PAGE).  Tokens beyond max_tokens have
  * their pages but no entry in slot_map.  past may be NULL (all 0); slot_map may be NULL (max_tokens 0).
  * scratch: gearb_layout_scratch_bytes(requests) bytes, contents irrelevant, one per call in flight.   */

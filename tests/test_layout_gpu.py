@@ -238,3 +238,19 @@ def test_ways_of_the_scan_and_of_the_fill(requests, most, room):
     assert np.array_equal(lay.block_table.cpu().numpy(), want_table)
     assert int(lay.used) == at
     assert np.array_equal(lay.slot_map.cpu().numpy(), want_slots)
+
+
+@pytest.mark.parametrize("requests", [3, 9000])
+def test_counter_at_and_behind_the_end_of_the_pool(requests):
+    """Nothing is needed, so nothing is missing; the counter comes back as the pool's size."""
+    for used in (7, 8, 1 << 40):
+        check([0] * requests, 8, 4, num_pages=7, used=used)
+        check([5] * requests, 8, 4, past=[3] * requests, num_pages=7, used=used)     # in the page there is
+
+
+@pytest.mark.parametrize("requests", [3, 9000])
+def test_wild_counters(requests):
+    """Page numbers that would pass 64 bits name no page."""
+    free = np.arange(40, dtype=np.int32)
+    for used in ((1 << 63) - 1, (1 << 63) - 2, -(1 << 63), 1 << 62):
+        check([20] * requests, 8, 4, free=free, used=used)
