@@ -185,14 +185,15 @@ __device__ __forceinline__ void fill_stretch(const LayoutParams &P, int64_t tota
       }
       const int64_t rest = q.end < hi ? q.end - i : hi - i;  // tokens of this request
       if (rest >= 32) {
-        // up to 128 tokens of one request, in groups of four that begin on a multiple of four; counted in 32 bits from
-        // the request's first
+        // up to 128 tokens of one request, a group of four a lane, from a multiple of four on.  Counted from the lane's group: a
+        // request may have 2^31 tokens, so counted from its first they pass 31 bits.
         const int64_t from = i & ~int64_t(3), stop = i + rest < from + kStep ? i + rest : from + kStep;
-        const int lo = static_cast<int>(i - q.first), end = static_cast<int>(stop - q.first);
-        const int rel = static_cast<int>(from - q.first) + 4 * lane, skip = rel < lo ? lo - rel : 0;  // first that counts
-        if (rel + skip < end) {
+        const int before = static_cast<int>(i - from) - 4 * lane, skip = before > 0 ? before : 0;  // of the group, not its own
+        const int end = static_cast<int>(stop - from) - 4 * lane;
+        if (skip < end) {
           const unsigned size = static_cast<unsigned>(a.page), have = static_cast<unsigned>(q.have);
-          const unsigned pos = static_cast<unsigned>(q.past) + static_cast<unsigned>(rel + skip), blk = page_of(P, pos);
+          const unsigned pos = static_cast<unsigned>(q.past) + static_cast<unsigned>(i - q.first) + static_cast<unsigned>(skip - before),
+                         blk = page_of(P, pos);
           const unsigned in_page = pos - blk * size, left = size - in_page;  // tokens the page has room for
           int32_t *entries = a.block_table + q.r * a.max_blocks;
           auto look_up = [&](unsigned b, bool first) -> int64_t {
@@ -208,7 +209,7 @@ __device__ __forceinline__ void fill_stretch(const LayoutParams &P, int64_t tota
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             s[k] = -1;
-            if (k < skip || rel + k >= end) continue;
+            if (k < skip || k >= end) continue;
             if (used == room) {  // the next page; only pages of less than four rows come here twice
               page = look_up(++b, true);
               base = page < 0 ? -1 : page * a.page;
@@ -219,14 +220,14 @@ __device__ __forceinline__ void fill_stretch(const LayoutParams &P, int64_t tota
             ++used;
           }
           const int64_t t = from + 4 * lane;
-          if (skip == 0 && rel + 4 <= end && P.vector && t + 4 <= a.max_tokens) {
+          if (skip == 0 && end >= 4 && P.vector && t + 4 <= a.max_tokens) {
             longlong2 *to = reinterpret_cast<longlong2 *>(a.slot_map + t);
             __stcs(to, make_longlong2(s[0], s[1]));
             __stcs(to + 1, make_longlong2(s[2], s[3]));
           } else {
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-              if (k >= skip && rel + k < end && t + k < a.max_tokens) a.slot_map[t + k] = s[k];
+              if (k >= skip && k < end && t + k < a.max_tokens) a.slot_map[t + k] = s[k];
           }
         }
         i = stop;

@@ -254,3 +254,38 @@ def test_wild_counters(requests):
     free = np.arange(40, dtype=np.int32)
     for used in ((1 << 63) - 1, (1 << 63) - 2, -(1 << 63), 1 << 62):
         check([20] * requests, 8, 4, free=free, used=used)
+
+
+@pytest.mark.parametrize("tokens,past", [((1 << 31) - 1, 0), ((1 << 31) - 130, 0), ((1 << 31) - 130, 129), ((1 << 31) - 4, 3)])
+def test_requests_as_long_as_they_may_be(tokens, past):
+    """Every slot of a request of some 2^31 tokens, and of the one behind it."""
+    page, blocks = 64, 1 << 25
+    table = torch.full((2, blocks), -1, dtype=torch.int32, device=DEV)
+    have = -(-past // page)
+    if have:
+        table[0, :have] = torch.arange(have, device=DEV, dtype=torch.int32)
+    free = torch.arange(have, blocks + 2, device=DEV, dtype=torch.int32)
+    status = torch.zeros(4, dtype=torch.int32, device=DEV)
+    lay = layout.paged_layout(torch.tensor([tokens, 5], device=DEV), page, table, torch.zeros(1, dtype=torch.int64, device=DEV),
+                              free_pages=free, past=torch.tensor([past, 0], device=DEV), max_tokens=tokens + 7, status=status)
+    pages = -(-(past + tokens) // page)
+    assert lay.offsets.tolist() == [0, tokens, tokens + 5] and int(lay.used) == pages + 1 - have and int(status[0]) == 0
+    assert torch.equal(table[0, :pages], torch.arange(pages, device=DEV, dtype=torch.int32)) and (table[0, pages:] == -1).all()
+    assert int(table[1, 0]) == pages and (table[1, 1:] == -1).all()
+    for t in range(0, tokens, 1 << 28):             # the pages follow one another, so do the slots
+        part = lay.slot_map[t:min(t + (1 << 28), tokens)]
+        assert torch.equal(part, torch.arange(t + past, t + past + part.numel(), device=DEV))
+    assert lay.slot_map[tokens:].tolist() == [pages * page + t for t in range(5)] + [-1, -1]
+
+
+@pytest.mark.parametrize("page", [64, 48, 1 << 20, 1 << 31])
+def test_pages_of_requests_as_long_as_they_may_be(page):
+    blocks = (1 << 31) // page
+    room = blocks * page
+    table = torch.full((2, blocks), -1, dtype=torch.int32, device=DEV)
+    lay = layout.paged_layout(torch.tensor([room, room], device=DEV), page, table, torch.zeros(1, dtype=torch.int64, device=DEV),
+                              num_pages=3 * blocks // 2)
+    assert lay.offsets.tolist() == [0, room, 2 * room] and int(lay.used) == 3 * blocks // 2
+    want = torch.arange(2 * blocks, device=DEV, dtype=torch.int32)
+    want[3 * blocks // 2:] = -1
+    assert torch.equal(table.reshape(-1), want)
