@@ -10,6 +10,8 @@
 //   layout_fill_kernel    every warp takes one stretch of the tokens, looks its first request up once and walks on from
 //                         there: up to 128 tokens of one request a step, four a lane; where less than 32 are left of
 //                         it, 32 a step, each lane finding its request among the next 32 offsets, which the warp holds.
+//                         Of tokens without slots only the pages are looked at.  How many there are is known on the device
+//                         alone: 1024 requests of 16 M tokens with 64 slots, token by token, took one CTA 3.8 s.
 // Up to 1024 requests and 4096 slots the scan and the fill are one launch of one CTA.  Measured: 131072 requests,
 // 65 M tokens: 195 us (82 at the copy rate; issue slots are taken in 74 % of the cycles, by 64-bit slots' arithmetic), 254
 // with 64-bit arithmetic throughout, 1950 with a binary search per token and one CTA's prefix sums.  256 requests, one
@@ -170,9 +172,40 @@ __device__ __forceinline__ int64_t place_token(const LayoutParams &P, const Requ
   return page < 0 ? -1 : static_cast<int64_t>(page) * a.page + in_page;
 }
 
-// Tokens [lo, hi) by one warp.
-__device__ __forceinline__ void fill_stretch(const LayoutParams &P, int64_t total, int64_t lo, int64_t hi, int lane) {
+// Tokens [lo, hi) of the batch, which have no slots: the table entries of the pages that begin with one of them.  32 requests
+// at a time, a lane each; the pages of long ones by the whole warp.
+__device__ __forceinline__ void fill_pages(const LayoutParams &P, int64_t lo, int64_t hi, int lane) {
   const gearb_layout_args &a = P.a;
+  if (lo >= hi) return;
+  auto pages_of = [&](int64_t rows) -> int64_t { return rows > 0 ? int64_t(page_of(P, static_cast<unsigned>(rows - 1))) + 1 : 0; };
+  int64_t r = warp_upper_bound<int64_t>(a.offsets, 0, a.requests, lo, lane, LoadPlain()) - 1;
+  for (; r < a.requests && a.offsets[r] < hi; r += 32) {
+    int64_t b = 0, end = 0, shift = 0;  // pages, and where they are in the free list
+    if (r + lane < a.requests) {
+      const Request q = load_request(P, r + lane);
+      const int64_t t0 = q.first > lo ? q.first : lo, t1 = q.end < hi ? q.end : hi;
+      if (t0 < t1) {
+        b = pages_of(q.past + (t0 - q.first));
+        if (b < q.have) b = q.have;
+        end = pages_of(q.past + (t1 - q.first));
+        shift = q.page0 - q.have;
+      }
+    }
+    if (__all_sync(kAll, end - b <= 4)) {
+      for (; b < end; ++b) a.block_table[(r + lane) * a.max_blocks + b] = page_at(a, shift + b);
+      continue;
+    }
+    for (int l = 0; l < 32; ++l) {
+      const int64_t from = __shfl_sync(kAll, b, l), to = __shfl_sync(kAll, end, l), in_list = __shfl_sync(kAll, shift, l);
+      for (int64_t k = from + lane; k < to; k += 32) a.block_table[(r + l) * a.max_blocks + k] = page_at(a, in_list + k);
+    }
+  }
+}
+
+// Tokens [lo, stretch) by one warp.
+__device__ __forceinline__ void fill_stretch(const LayoutParams &P, int64_t total, int64_t lo, int64_t stretch, int lane) {
+  const gearb_layout_args &a = P.a;
+  const int64_t hi = stretch < a.max_tokens ? stretch : a.max_tokens;  // with slots
   int64_t i = lo;
   if (i < total && i < hi) {
     // last request whose offset is <= i: it has this token
@@ -220,14 +253,14 @@ __device__ __forceinline__ void fill_stretch(const LayoutParams &P, int64_t tota
             ++used;
           }
           const int64_t t = from + 4 * lane;
-          if (skip == 0 && end >= 4 && P.vector && t + 4 <= a.max_tokens) {
+          if (skip == 0 && end >= 4 && P.vector) {
             longlong2 *to = reinterpret_cast<longlong2 *>(a.slot_map + t);
             __stcs(to, make_longlong2(s[0], s[1]));
             __stcs(to + 1, make_longlong2(s[2], s[3]));
           } else {
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-              if (k >= skip && k < end && t + k < a.max_tokens) a.slot_map[t + k] = s[k];
+              if (k >= skip && k < end) a.slot_map[t + k] = s[k];
           }
         }
         i = stop;
@@ -255,14 +288,13 @@ __device__ __forceinline__ void fill_stretch(const LayoutParams &P, int64_t tota
       }
       if (mine) {
         const Request own = r == q.r ? q : load_request(P, r);
-        const int64_t slot = place_token(P, own, t);
-        if (t < a.max_tokens) a.slot_map[t] = slot;
+        a.slot_map[t] = place_token(P, own, t);
       }
       i += 32;
     }
   }
-  for (int64_t t = (total > lo ? total : lo) + lane; t < hi; t += 32)  // behind the last token
-    if (t < a.max_tokens) a.slot_map[t] = -1;
+  for (int64_t t = (total > lo ? total : lo) + lane; t < hi; t += 32) a.slot_map[t] = -1;  // behind the last token
+  fill_pages(P, lo > hi ? lo : hi, stretch < total ? stretch : total, lane);
 }
 
 // One CTA: the prefix sums, and with kFill (a request a thread at most) everything.

@@ -289,3 +289,36 @@ def test_pages_of_requests_as_long_as_they_may_be(page):
     want = torch.arange(2 * blocks, device=DEV, dtype=torch.int32)
     want[3 * blocks // 2:] = -1
     assert torch.equal(table.reshape(-1), want)
+
+
+@pytest.mark.parametrize("requests,page,room", [(1024, 4096, 64), (1024, 4099, 0), (9000, 4096, 64), (1, 64, 1000)])
+def test_tokens_without_slots_cost_their_pages_only(requests, page, room):
+    """Far more tokens than slots (every path of the fill): all pages, and in the time of the pages."""
+    blocks = (1 << 24) // page
+    tokens = torch.full((requests,), blocks * page - 5, dtype=torch.int64, device=DEV)
+    past = torch.zeros(requests, dtype=torch.int64, device=DEV)
+    past[::3] = 3 * page + 1
+    tokens[::3] -= 3 * page + 1
+    have = -(-past // page)
+    table = torch.full((requests, blocks), -1, dtype=torch.int32, device=DEV)
+    used = torch.zeros(1, dtype=torch.int64, device=DEV)
+
+    def call(t):
+        return layout.paged_layout(tokens, page, t, used, num_pages=1 << 31, past=past, max_tokens=room)
+
+    call(table.clone())
+    t0, t1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    t0.record()
+    lay = call(table)
+    t1.record()
+    torch.cuda.synchronize()
+    per = blocks - have
+    start = torch.cumsum(per, 0) - per
+    col = torch.arange(blocks, device=DEV)[None]
+    want = torch.where(col < have[:, None], -1, start[:, None] + col - have[:, None])
+    assert torch.equal(lay.block_table.long(), want) and int(lay.used) == int(per.sum())
+    for t in range(0, room, 7):                 # the first request has them all
+        pos = int(past[0]) + t
+        at = int(want[0, pos // page])
+        assert int(lay.slot_map[t]) == (at * page + pos % page if at >= 0 else -1)
+    assert t0.elapsed_time(t1) < 50             # milliseconds; token by token it was hundreds
