@@ -21,6 +21,7 @@ import functools
 from typing import NamedTuple, Optional
 
 import torch
+import torch.autograd.forward_ad as _forward_ad
 
 from . import _native as N
 from ._native import GearError, check, lib
@@ -47,6 +48,13 @@ def _vector(t, what: str, dtype: torch.dtype, shape: tuple, device) -> None:
 def _unit(t: torch.Tensor) -> torch.Tensor:
     """The tensor itself where its last dimension is consecutive (any other strides), else a copy."""
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def _no_tangents(*tensors) -> None:
+    if getattr(_forward_ad, "_current_level", 0) >= 0:     # inside a dual level
+        for t in tensors:
+            if t is not None and _forward_ad.unpack_dual(t).tangent is not None:
+                _bad("forward-mode derivatives are not supported: the tangent would be dropped")
 
 
 def _at(t) -> int:
@@ -119,6 +127,7 @@ class _LinearRecurrence(torch.autograd.Function):
     def backward(ctx, dh, dstate):
         x, gate, h0, offsets, lengths, carry = ctx.saved_tensors
         s = ctx.s
+        _no_tangents(dh, dstate)
         with _Scope(x.device):
             dh = torch.zeros_like(x) if dh is None else _unit(dh)
             dstate = None if dstate is None else dstate.contiguous()
@@ -159,8 +168,8 @@ def linear_recurrence(x: torch.Tensor, gate: torch.Tensor, *, h0: Optional[torch
     stream      where to launch (None: the current stream of x's device); gradients follow it
 
     Arithmetic and state are float32 whatever x's type; h is rounded once to x's type.  The bits of the result
-    depend on nothing but the inputs' values and shape (a shared gate's gradient: and their alignment).  Differentiable once in x, gate and h0; the backward pass
-    recomputes h in float32.  Products of a sequence's gates over up to 512 rows (32768 of a single channel) must stay
+    depend on nothing but the inputs' values and shape (a shared gate's gradient: and their alignment).  Differentiable
+    once in x, gate and h0, in reverse mode (forward mode is refused); the backward pass recomputes h in float32.  Products of a sequence's gates over up to 512 rows (32768 of a single channel) must stay
     inside float32's range, and so must exp(gate): where they pass it (|a| well above 1) h is infinite or NaN.
 
     Capturing a backward pass into a CUDA graph: as for any autograd function, let no eager graph of the same leaves
@@ -196,6 +205,7 @@ def linear_recurrence(x: torch.Tensor, gate: torch.Tensor, *, h0: Optional[torch
         _bad(f"gate is on {gate.device}, x on {dev}")
     if h0 is not None:
         _vector(h0, "h0", torch.float32, (sequences, width), dev)
+    _no_tangents(x, gate, h0)
     if not x.is_cuda:
         _bad("x must be a CUDA tensor")
     if status is not None and (status.dtype != torch.int32 or status.numel() < N.STATUS_WORDS

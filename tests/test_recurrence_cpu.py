@@ -19,3 +19,28 @@ def test_waits_that_leave_turns_out_end_behind_their_own_phase(tmp_path):
     assert build.returncode == 0, build.stderr[-2000:]
     run = subprocess.run([str(exe)], capture_output=True, text=True, timeout=60)
     assert run.returncode == 0 and "states ok" in run.stdout, run.stdout
+
+
+def test_forward_mode_derivatives_are_refused():
+    """The launch knows nothing of tangents: dropping one would be a derivative of zero."""
+    import torch
+    import torch.autograd.forward_ad as fwd
+
+    from gear_b200 import _native as N
+    from gear_b200 import core, recurrence
+    x, g, h0 = torch.ones(2, 3, 4), torch.ones(2, 3, 4), torch.ones(2, 4)
+    for at in range(3):
+        with fwd.dual_level():
+            t = [x, g, h0]
+            t[at] = fwd.make_dual(t[at], torch.ones_like(t[at]))
+            with pytest.raises(core.GearError, match="forward-mode") as e:
+                recurrence.linear_recurrence(t[0], t[1], h0=t[2])
+            assert e.value.code == N.ERR_INVALID
+    for leaf in (x, g, h0):       # beside reverse mode, too
+        leaf.requires_grad_(True)
+    with fwd.dual_level(), pytest.raises(core.GearError, match="forward-mode"):
+        recurrence.linear_recurrence(fwd.make_dual(x, torch.ones_like(x)), g, h0=h0)
+    with fwd.dual_level(), pytest.raises(core.GearError, match="CUDA"):      # a level alone changes nothing
+        recurrence.linear_recurrence(x, g, h0=h0)
+    with pytest.raises(core.GearError, match="forward-mode"):
+        torch.func.jvp(lambda t: recurrence.linear_recurrence(t, g.detach())[0], (x.detach(),), (x.detach(),))

@@ -661,3 +661,42 @@ def test_a_wait_that_runs_out(width, gates, dtype, polled, reverse):
     leaves, h, s = forward()
     for a, b in zip([h, s, *backward(leaves, h, s)], want):
         assert torch.equal(a, b)
+
+
+def test_transforms_that_the_launch_cannot_follow_are_refused():
+    import torch.autograd.forward_ad as fwd
+    x, gate = make(1, (2, 30), 8, 8, F32, F32, False)
+    x.requires_grad_(True)
+    h, _ = recurrence.linear_recurrence(x, gate)
+    with fwd.dual_level():
+        with pytest.raises(core.GearError, match="forward-mode"):
+            recurrence.linear_recurrence(x, fwd.make_dual(gate, gate))
+        with pytest.raises(core.GearError, match="forward-mode"):         # of a gradient
+            torch.autograd.grad(h, x, fwd.make_dual(torch.ones_like(h), torch.ones_like(h)), retain_graph=True)
+        plain, = torch.autograd.grad(h, x, torch.ones_like(h))
+        assert torch.isfinite(plain).all()
+    x = x.detach()
+    for f in (lambda: torch.func.vmap(lambda t: recurrence.linear_recurrence(t, gate)[0])(torch.stack([x, x])),
+              lambda: torch.func.grad(lambda t: recurrence.linear_recurrence(t, gate)[0].sum())(x),
+              lambda: torch.func.jvp(lambda t: recurrence.linear_recurrence(t, gate)[0], (x,), (x,))):
+        with pytest.raises(RuntimeError):
+            f()
+
+
+@pytest.mark.parametrize("width,gates", [(1, 1), (12, 3), (64, 64), (64, 1), (45, 45)])
+def test_gradients_of_some_inputs_and_of_the_state_alone(width, gates):
+    x, gate = make(21, (3, 200), width, gates, F32, F32, True)
+    h0 = state_of(22, 3, width)
+    rng = np.random.default_rng(5)
+    dst = torch.from_numpy(rng.standard_normal((3, width)).astype(np.float32)).to(DEV)
+    flat = lambda t, c: dbl(t).reshape(600, c)
+    want = R.reference(flat(x, width), flat(gate, gates), R.spans(600, 200, None, None), dbl(h0), False, True,
+                       np.zeros((600, width)), dbl(dst))
+    for wanted in ((1, 1, 1), (1, 0, 0), (0, 1, 0), (0, 0, 1)):
+        leaves = [t.clone().requires_grad_(bool(w)) for t, w in zip((x, gate, h0), wanted)]
+        _, s = recurrence.linear_recurrence(leaves[0], leaves[1], h0=leaves[2], gate_kind="log")
+        s.backward(dst)
+        for t, w, key in zip(leaves, wanted, ("dx", "dgate", "dh0")):
+            assert (t.grad is not None) == bool(w)
+            if w:
+                R.check(t.grad, want[key], F32, key)
