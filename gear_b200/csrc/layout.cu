@@ -430,6 +430,7 @@ int gearb_layout_paged(const gearb_layout_args *args, void *stream) {
   GEARB_REQUIRE(a.max_tokens == 0 || a.slot_map, "layout: max_tokens without a slot map");
   GEARB_REQUIRE(a.scratch_bytes >= gearb_layout_scratch_bytes(a.requests) && (a.requests == 0 || a.scratch),
                 "layout: scratch of %lld bytes needed", (long long)gearb_layout_scratch_bytes(a.requests));
+  GEARB_REQUIRE(reinterpret_cast<uintptr_t>(a.scratch) % 8 == 0, "layout: scratch must start on 8 bytes");
   p.first_page = static_cast<int64_t *>(a.scratch);
   p.blocks = a.requests > kScanMost ? (a.requests + kBlock - 1) / kBlock : 0;
   p.sums = p.first_page + a.requests;

@@ -382,6 +382,7 @@ int run(const gearb_recurrence_args *args, bool backward, void *stream) {
   if (rc != GEARB_OK) return rc;
   GEARB_REQUIRE(args->scratch_bytes >= scratch && (scratch == 0 || args->scratch),
                 "recurrence: scratch of %lld bytes needed", (long long)scratch);
+  GEARB_REQUIRE(reinterpret_cast<uintptr_t>(args->scratch) % 16 == 0, "recurrence: scratch must start on 16 bytes");
   GEARB_REQUIRE(!backward || carry == 0 || args->carry, "recurrence: the backward pass needs the forward pass's carry");
   return launch(*args, backward, as_stream(stream));
 }

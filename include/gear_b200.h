@@ -520,7 +520,8 @@ int gearb_handler_gather_packed(gearb_handler *h, const int32_t *columns, int nc
  *                cut to [0, num_pages])
  * Where the pool runs out the entries and slots are -1 (GEARB_ST_NO_PAGE).  Tokens beyond max_tokens have
  * their pages but no entry in slot_map.  past may be NULL (all 0); slot_map may be NULL (max_tokens 0).
- * scratch: gearb_layout_scratch_bytes(requests) bytes, contents irrelevant, one per call in flight.   */
+ * scratch: gearb_layout_scratch_bytes(requests) bytes that start on a multiple of 8, contents irrelevant, one per
+ * call in flight.                                                                                    */
 typedef struct gearb_layout_args {
   const int64_t *lengths;
   const int64_t *past;
@@ -556,8 +557,8 @@ int gearb_layout_paged(const gearb_layout_args *args, void *stream);
  * Types: x, out, dout, dx of x_dtype; gate, dgate of gate_dtype, either x_dtype or GEARB_DT_F32.
  * All arithmetic is float32; the result does not depend on timing, nor, but for the sums of shared gates, on alignment.
  * carry: what the backward pass needs besides x and gate, written by the forward pass when not NULL.
- * gearb_recurrence_bytes gives the sizes of scratch (contents irrelevant, one per call in flight) and
- * carry.  The backward pass reads x, gate, h0, dout, dstate and carry, writes dx, dgate and dh0.     */
+ * gearb_recurrence_bytes gives the sizes of scratch (starts on a multiple of 16 bytes, contents irrelevant, one per
+ * call in flight) and carry.  Every other tensor starts on a multiple of its element.  The backward pass reads x, gate, h0, dout, dstate and carry, writes dx, dgate and dh0.     */
 typedef struct gearb_recurrence_args {
   const void *x;
   const void *gate;

@@ -44,3 +44,32 @@ def test_forward_mode_derivatives_are_refused():
         recurrence.linear_recurrence(x, g, h0=h0)
     with pytest.raises(core.GearError, match="forward-mode"):
         torch.func.jvp(lambda t: recurrence.linear_recurrence(t, g.detach())[0], (x.detach(),), (x.detach(),))
+
+
+@pytest.mark.parametrize("backward", [False, True])
+def test_scratch_that_is_not_aligned_is_refused(backward):
+    import ctypes as C
+
+    from gear_b200 import _native as N
+    a = N.RecurrenceArgs(x=256, gate=256, x_dtype=N.DT_F32, gate_dtype=N.DT_F32, batch=1, time=100, width=64, gates=64,
+                         sequences=1, out=256, dout=256, dx=256, dgate=256, carry=256)
+    scratch, carry = C.c_int64(0), C.c_int64(0)
+    assert N.lib.gearb_recurrence_bytes(C.byref(a), int(backward), C.byref(scratch), C.byref(carry)) == N.OK
+    a.scratch_bytes = scratch.value
+    run = N.lib.gearb_recurrence_backward if backward else N.lib.gearb_recurrence_forward
+    for at in (1, 4, 8, 15):
+        a.scratch = 4096 + at
+        assert run(C.byref(a), None) == N.ERR_INVALID
+        assert "16 bytes" in N.lib.gearb_last_error().decode()
+
+
+def test_layout_scratch_that_is_not_aligned_is_refused():
+    import ctypes as C
+
+    from gear_b200 import _native as N
+    a = N.LayoutArgs(lengths=256, requests=3, page=16, max_blocks=4, block_table=256, num_pages=5, used_in=256, used_out=256,
+                     offsets=256, scratch_bytes=N.lib.gearb_layout_scratch_bytes(3))
+    for at in (1, 4):
+        a.scratch = 4096 + at
+        assert N.lib.gearb_layout_paged(C.byref(a), None) == N.ERR_INVALID
+        assert "8 bytes" in N.lib.gearb_last_error().decode()
