@@ -1056,9 +1056,10 @@ int launch_stream(Params &p, cudaStream_t stream) {
   return GEARB_OK;
 }
 
-// TMA takes a matrix whose base and rows start on 16 bytes, and copies that start on 16 bytes.
-inline bool matrix_ok(const void *p, int64_t sr, int size) {
-  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && sr > 0 && sr * size % 16 == 0 && sr * size < (int64_t(1) << 40);
+// TMA takes a matrix whose base and rows start on 16 bytes, and copies that start on 16 bytes; rows that overlap (sr below
+// the width) are not among the layouts that its documentation describes.
+inline bool matrix_ok(const void *p, int64_t width, int64_t sr, int size) {
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && sr >= width && sr < (int64_t(1) << 37) && sr * size % 16 == 0;
 }
 
 // Channels a lane in the streaming kernel, 0: not for it.
@@ -1066,10 +1067,10 @@ template <typename TX, typename TA>
 int stream_width(const Params &p, bool backward) {
   const gearb_recurrence_args &a = p.A;
   const bool shared = a.gates < a.width;
-  if (!p.flat || p.rows >= (int64_t(1) << 31) || !matrix_ok(a.x, a.x_row_stride, sizeof(TX))) return 0;
-  if (!shared && !matrix_ok(a.gate, a.gate_row_stride, sizeof(TA))) return 0;
+  if (!p.flat || p.rows >= (int64_t(1) << 31) || !matrix_ok(a.x, a.width, a.x_row_stride, sizeof(TX))) return 0;
+  if (!shared && !matrix_ok(a.gate, a.width, a.gate_row_stride, sizeof(TA))) return 0;
   if (backward) {
-    if (!matrix_ok(a.dout, a.dout_row_stride, sizeof(TX)) || a.width % 2 != 0) return 0;
+    if (!matrix_ok(a.dout, a.width, a.dout_row_stride, sizeof(TX)) || a.width % 2 != 0) return 0;
     if (!vector_ok(a.dx, 0, 0, sizeof(TX), 2) || (!shared && !vector_ok(a.dgate, 0, 0, sizeof(TA), 2))) return 0;
     if (shared ? (p.per <= 32 || p.per * sizeof(TX) % 16 != 0) : a.width <= 32) return 0;
     return 2;

@@ -700,3 +700,29 @@ def test_gradients_of_some_inputs_and_of_the_state_alone(width, gates):
             assert (t.grad is not None) == bool(w)
             if w:
                 R.check(t.grad, want[key], F32, key)
+
+
+@pytest.mark.parametrize("width,gates", [(64, 64), (96, 2), (160, 160), (8, 8), (43, 43)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("step", [8, 16, 0])
+def test_rows_that_overlap(width, gates, dtype, step):
+    """Windows over one line of values: rows fewer elements apart than they are wide (or all the same one)."""
+    rows = 300
+    line, gline = make(3, (rows * max(step, 1) + width,), 1, 1, dtype, F32, False)
+    x = line.reshape(-1).as_strided((rows, width), (step, 1))
+    gate = gline.reshape(-1).as_strided((rows, gates), (step, 1))
+    dh = torch.randn(rows * max(step, 1) + width, device=DEV).to(dtype).as_strided((rows, width), (step, 1))
+    off = torch.tensor([0, 100, 101, 290], device=DEV)
+
+    def once(x, gate, dh, **kw):
+        leaves = [x.detach(), gate.detach()]
+        for t in leaves:
+            t.requires_grad_(True)
+        h, s = recurrence.linear_recurrence(*leaves, **kw)
+        return [h, s, *torch.autograd.grad(h, leaves, dh)]
+
+    for a, b in zip(once(x, gate, dh, offsets=off), once(x.contiguous(), gate.contiguous(), dh.contiguous(), offsets=off)):
+        assert torch.equal(a, b)
+    batch = lambda t: t.as_strided((3, 100, t.shape[1]), (100 * step, step, 1))
+    for a, b in zip(once(*map(batch, (x, gate, dh))), once(*(batch(t).contiguous() for t in (x, gate, dh)))):
+        assert torch.equal(a, b)
