@@ -257,7 +257,7 @@ __global__ void __launch_bounds__(kThreads, kBackward ? 3 : 4) narrow_kernel(con
   float h0v = 0.0f;  // of the last start looked at
   auto first_state = [&](const float *p, int k) { return p ? p[sequence_of(A, P.rows, i0 + at + k) * w + c] : 0.0f; };
   Group f{1.0f, 0.0f, m.start != 0}, b{1.0f, 0.0f, m.end != 0};
-  // Without states of their own sequences start from nothing: no branches.  (What a row of no sequence leaves is not
+  // Without states of their own sequences start from nothing: no branches (0 * -0 + x is x, to the sign of a zero).  (What a row of no sequence leaves is not
   // used: the next row of one is its first.)
   const bool stateless = !A.h0 && !(kBackward ? A.dstate : nullptr);
   if (stateless && mine > 0) {
@@ -265,7 +265,7 @@ __global__ void __launch_bounds__(kThreads, kBackward ? 3 : 4) narrow_kernel(con
     for (int k = 0; k < K; ++k) {
       const bool st = m.start >> k & 1u;
       const float a = pg[k * gates];
-      f.h = fmaf(st ? 0.0f : a, st ? 0.0f : f.h, px[k * w]);
+      f.h = fmaf(st ? 0.0f : a, st ? -0.0f : f.h, px[k * w]);
       f.a *= a;
     }
   } else {
@@ -416,7 +416,7 @@ __global__ void __launch_bounds__(kThreads, kBackward ? 3 : 4) narrow_kernel(con
 #pragma unroll
       for (int k = 0; k < K; ++k) {
         const bool st = m.start >> k & 1u;
-        h = fmaf(st ? 0.0f : pg[k * gates], st ? 0.0f : h, px[k * w]);
+        h = fmaf(st ? 0.0f : pg[k * gates], st ? -0.0f : h, px[k * w]);
         ox[k * w] = (m.live >> k & 1u) ? h : 0.0f;
       }
     } else if (!kBackward) {

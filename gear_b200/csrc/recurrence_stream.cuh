@@ -441,9 +441,9 @@ __device__ __forceinline__ void step_row(const gearb_recurrence_args &A, const P
   if (start >> k & 1u) {
     if (A.h0) {
       state_load<V>(A.h0, pl.rec.seq[row], A.width, d, on, h);
-    } else {
+    } else {  // 0 * -0 + x is x, to the sign of a zero
 #pragma unroll
-      for (int v = 0; v < V; ++v) h[v] = 0.0f;
+      for (int v = 0; v < V; ++v) h[v] = -0.0f;
 #pragma unroll
       for (int v = 0; v < kG; ++v) a[v] = 0.0f;
     }

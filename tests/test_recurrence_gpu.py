@@ -726,3 +726,31 @@ def test_rows_that_overlap(width, gates, dtype, step):
     batch = lambda t: t.as_strided((3, 100, t.shape[1]), (100 * step, step, 1))
     for a, b in zip(once(*map(batch, (x, gate, dh))), once(*(batch(t).contiguous() for t in (x, gate, dh)))):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("width,gates", [(64, 64), (66, 66), (256, 4), (96, 48), (1, 1), (6, 2)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("with_state", [False, True])
+def test_the_sign_of_zero(width, gates, dtype, with_state):
+    """Without h0 a first row is x, to the sign of its zero; the same bits whatever the alignment, gradients too."""
+    lens = [5, 1, 64, 130, 0, 60, 40]
+    off = torch.tensor(np.cumsum([0] + lens), dtype=torch.int64, device=DEV)
+    rows = int(off[-1])
+    x, gate = make(31, (rows,), width, gates, dtype, F32, False)
+    x[torch.rand(rows, width, device=DEV, generator=torch.Generator(DEV).manual_seed(3)) < 0.5] = -0.0
+    first = off[:-1][torch.tensor(lens, device=DEV) > 0]
+    dh = torch.randn(rows, width, device=DEV).to(dtype)
+    bits = lambda t: t.view(torch.int32 if t.dtype is F32 else torch.int16)
+    room, groom = torch.empty(rows, width + 1, dtype=dtype, device=DEV), torch.empty(rows, gates + 1, device=DEV)
+    room[:, 1:], groom[:, 1:] = x, gate
+
+    def once(x, gate):
+        leaves = [x.detach().requires_grad_(True), gate.detach().requires_grad_(True)]
+        h, s = recurrence.linear_recurrence(*leaves, offsets=off, return_state=with_state)
+        return [h, *torch.autograd.grad(h, leaves, dh)] + ([s] if with_state else [])
+
+    got, other = once(x, gate), once(room[:, 1:], groom[:, 1:])
+    assert torch.equal(bits(got[0])[first], bits(x)[first])
+    for i, (a, b) in enumerate(zip(got, other)):
+        if i != 2 or gates == width:              # the sums of shared gates depend on alignment
+            assert torch.equal(bits(a), bits(b)), i
