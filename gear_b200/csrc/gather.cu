@@ -154,8 +154,10 @@ __global__ void __launch_bounds__(kThreads, 6) gather_packed_kernel(const __grid
   if (o0 < 0 || past < 0 || past > D.room) {
     flags |= GEARB_ST_BAD_REQUEST;
     count64 = 0;
+  } else if (o1 <= o0) {  // before the difference, which may pass 64 bits
+    count64 = 0;
   } else if (count64 > o1 - o0) {
-    count64 = o1 > o0 ? o1 - o0 : 0;
+    count64 = o1 - o0;
   }
   const int count = static_cast<int>(count64);  // at most the pattern's length
   const uint8_t *base = P.table + idx * P.traj_stride;

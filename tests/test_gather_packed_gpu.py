@@ -339,3 +339,55 @@ def test_layout_and_gather_captured_once_follow_their_inputs():
             for c in (0, 1):
                 want = plain(t, img, c, start, count, req[0], offsets, np.zeros((n * blocks * page, rows[c]), np.uint8), tab, page)
                 assert np.array_equal(pools[c].cpu().numpy(), want)
+
+
+@pytest.mark.parametrize("page", [0, 8])
+def test_offsets_that_fall_by_more_than_63_bits(page):
+    """A request whose end lies in front of its start has no rows, however far in front."""
+    rows, T, cap = [24, 5], 40, 5
+    t, img = make_table(rows, T, cap)
+    h = core.StorageHandler(t)
+    h.set([0, 1], [core.SubscribePattern(0, 20)] * 2)
+    idx, ts, ln = (np.full(3, v, np.int64) for v in (2, 3, 40))
+    start, count = clip(t, core.SubscribePattern(0, 20), idx, ts, ln)
+    for end in (-(1 << 63), -(1 << 63) + 5, -1, 0, 10):
+        offsets = [0, 10, end, 30]
+        table = np.arange(9, dtype=np.int32).reshape(3, 3) if page else None
+        dsts = [np.full((80, r), 0xA5, np.uint8) for r in rows]
+        ddst = [torch.from_numpy(d).to(DEV) for d in dsts]
+        h.gather_packed([0, 1], *(torch.from_numpy(a).to(DEV) for a in (idx, ts, ln)), torch.tensor(offsets, device=DEV), ddst,
+                        block_table=None if table is None else torch.from_numpy(table).to(DEV), page=page)
+        torch.cuda.synchronize()
+        # request 2 begins where `end` says: in front of row 0 it is refused as a whole
+        own = [min(int(count[r]), max(0, offsets[r + 1] - offsets[r])) if offsets[r] >= 0 else 0 for r in range(3)]
+        for c in (0, 1):
+            want = plain(t, img, c, start, own, idx, [0, 10, max(end, 0), 30], dsts[c], table, page)
+            if end < 10:                                  # `plain` takes what the offsets leave: nothing of request 1
+                assert own[1] == 0
+            assert np.array_equal(ddst[c].cpu().numpy(), want), (c, end)
+
+
+@pytest.mark.parametrize("residency", [N.RES_HOST, N.RES_HOST | N.RES_HBM])
+@pytest.mark.parametrize("page", [1, 8, 100])
+def test_pages_filled_from_the_host(residency, page):
+    rows, T, cap = [156, 24, 4, 1, 16], 50, 7
+    t, img = make_table(rows, T, cap, residency)
+    h = core.StorageHandler(t)
+    pat = core.SubscribePattern(0, 30)
+    cols = list(range(5))
+    h.set(cols, [pat] * 5)
+    rng = np.random.default_rng(3)
+    idx, ts, ln = requests(rng, 60, T, cap)
+    start, count = clip(t, pat, idx, ts, ln)
+    offsets = np.concatenate([[0], np.cumsum(count)])
+    past = rng.integers(0, 20, 60)
+    m = -(-50 // page)
+    table = rng.permutation(60 * m).astype(np.int32).reshape(60, m)
+    dev = [torch.from_numpy(a).to(DEV) for a in (idx, ts, ln, offsets)]
+    dsts = [np.full((60 * m * page, r), 0x5A, np.uint8) for r in rows]
+    ddst = [torch.from_numpy(d).to(DEV) for d in dsts]
+    h.gather_packed(cols, *dev[:3], dev[3], ddst, block_table=torch.from_numpy(table).to(DEV), page=page,
+                    past=torch.from_numpy(past).to(DEV))
+    for c in cols:
+        want = plain(t, img, c, start, count, idx, offsets, dsts[c], table, page, past)
+        assert np.array_equal(ddst[c].cpu().numpy(), want), c
