@@ -169,8 +169,12 @@ def linear_recurrence(x: torch.Tensor, gate: torch.Tensor, *, h0: Optional[torch
 
     Arithmetic and state are float32 whatever x's type; h is rounded once to x's type.  The bits of the result
     depend on nothing but the inputs' values and shape (a shared gate's gradient: and their alignment).  Differentiable
-    once in x, gate and h0, in reverse mode (forward mode is refused); the backward pass recomputes h in float32.  Products of a sequence's gates over up to 512 rows (32768 of a single channel) must stay
-    inside float32's range, and so must exp(gate): where they pass it (|a| well above 1) h is infinite or NaN.
+    once in x, gate and h0, in reverse mode (forward mode is refused); the backward pass recomputes h in float32.
+
+    Rows are worked on in parallel, by products of gates: of up to 512 consecutive rows of a sequence, of up to 16
+    channels 32768 / channels rows.  These, and exp(gate), must stay inside float32's range.  Where |a| is above 1 for so
+    long that they pass it, h is infinite or NaN, even where it is zero by the formula; and an infinite h may become
+    NaN, as products below the range are zero.
 
     Capturing a backward pass into a CUDA graph: as for any autograd function, let no eager graph of the same leaves
     live meanwhile, and warm up on a side stream."""

@@ -555,6 +555,8 @@ int gearb_layout_paged(const gearb_layout_args *args, void *stream);
  * float32 [sequences][width], each may be NULL (h0: zeros); state_out of an empty sequence is its h0.
  * Nothing that is written may overlap what is read, except that with time 1 state_out may be h0.
  * Types: x, out, dout, dx of x_dtype; gate, dgate of gate_dtype, either x_dtype or GEARB_DT_F32.
+ * Products of a sequence's gates over up to 512 rows (width <= 16: 32768 / width rows), and exp(gate), must stay inside
+ * float32's range; where they pass it, results are infinite or NaN.
  * All arithmetic is float32; the result does not depend on timing, nor, but for the sums of shared gates, on alignment.
  * carry: what the backward pass needs besides x and gate, written by the forward pass when not NULL.
  * gearb_recurrence_bytes gives the sizes of scratch (starts on a multiple of 16 bytes, contents irrelevant, one per

@@ -754,3 +754,34 @@ def test_the_sign_of_zero(width, gates, dtype, with_state):
     for i, (a, b) in enumerate(zip(got, other)):
         if i != 2 or gates == width:              # the sums of shared gates depend on alignment
             assert torch.equal(bits(a), bits(b)), i
+
+
+@pytest.mark.parametrize("width", [1, 2, 3, 5, 8, 16, 17, 64, 512])
+@pytest.mark.parametrize("reverse", [False, True])
+def test_gates_above_one_up_to_the_stated_products(width, reverse):
+    """Gates whose products over the stated number of rows just stay in range, over four times as many rows: where there is
+    nothing to multiply, zeros and finite gradients (a product beyond the range would make them NaN)."""
+    reach = 32768 // width if width <= 16 else 512
+    rows, tail = 4 * reach + 77, 60
+    a = float(np.float32(np.exp(86.0 / reach)))           # float32 ends at e^88.7
+    x = torch.zeros(1, rows, width, device=DEV)
+    gate = torch.full((1, rows, width), a, device=DEV)
+    dh = torch.zeros_like(x)
+    last, first = (slice(0, tail), slice(rows - tail, rows)) if reverse else (slice(rows - tail, rows), slice(0, tail))
+    rng = np.random.default_rng(width)
+    x[0, last] = torch.from_numpy(rng.standard_normal((tail, width)).astype(np.float32)).to(DEV)
+    dh[0, first] = torch.from_numpy(rng.standard_normal((tail, width)).astype(np.float32)).to(DEV)
+    for h0 in (None, torch.zeros(1, width, device=DEV)):
+        leaves = [x.clone().requires_grad_(True), gate.clone().requires_grad_(True)]
+        h, s = recurrence.linear_recurrence(*leaves, h0=h0, reverse=reverse)
+        dx, dg = torch.autograd.grad(h, leaves, dh)
+        want = R.reference(dbl(x[0, last]), dbl(gate[0, last]), [(0, tail)], np.zeros((1, width)), reverse)
+        R.check(h[0, last], want["h"], F32, "h")
+        R.check(s, want["state"], F32, "state")
+        h[0, last] = 0
+        assert (h == 0).all()
+        back = R.reference(np.zeros((tail, width)), dbl(gate[0, first]), [(0, tail)], np.zeros((1, width)), reverse,
+                           dh=dbl(dh[0, first]))
+        R.check(dx[0, first], back["dx"], F32, "dx")
+        dx[0, first] = 0
+        assert (dx == 0).all() and (dg == 0).all()
