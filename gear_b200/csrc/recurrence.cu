@@ -226,6 +226,9 @@ struct Tiling {
   int64_t rows, tiles;
   int tile_rows, chain, narrow_rows;
 };
+// SMs of a full B200.  A constant in place of sm_count(): tiles decide how states are rounded and how long the carry is, and
+// these go by the sizes of a call alone, whatever part of a GPU it runs on.
+constexpr int kFullSms = 148;
 Tiling tiling_of(const gearb_recurrence_args &a) {
   Tiling t = {};
   t.rows = a.batch * a.time;
@@ -233,7 +236,7 @@ Tiling tiling_of(const gearb_recurrence_args &a) {
   if (a.width <= kNarrowWidth) {
     // 16 rows a thread keep the memory busy; with 4 a small call is spread over four times as many SMs
     const int groups = kWarps * narrow_groups(static_cast<int>(a.width));
-    t.narrow_rows = t.rows > int64_t(16) * groups * 148 ? 16 : 4;
+    t.narrow_rows = t.rows > int64_t(16) * groups * kFullSms ? 16 : 4;
     most = t.narrow_rows * groups;
   }
   t.tile_rows = most;

@@ -569,13 +569,10 @@ __device__ __forceinline__ float exp_of(float x) {
 
 // Hands a sequence without rows its state (forward) or its gradient (backward): the CTAs of a launch share the
 // sequences among them.
-__device__ __forceinline__ void empty_sequences(const Params &P, const Place &pl, int64_t block, const float *from,
-                                                float *to, int lane = -1) {
+__device__ __forceinline__ void empty_sequences(const Params &P, const Place &pl, int64_t block, const float *from, float *to) {
   const gearb_recurrence_args &A = P.A;
   if (!to) return;
-  // by all threads of the CTA, or by one warp's lanes
-  const int64_t each = lane < 0 ? kThreads : 32, step = P.tiles * each;
-  for (int64_t s = pl.tile * each + (lane < 0 ? threadIdx.x : lane); s < A.sequences; s += step) {
+  for (int64_t s = pl.tile * kThreads + threadIdx.x; s < A.sequences; s += P.tiles * kThreads) {
     int64_t n;
     if (A.offsets) {
       const ScanOffsets so{A.offsets, P.rows, A.sequences, 0};

@@ -27,7 +27,7 @@ struct NarrowLayout {
 };
 __host__ __device__ inline int narrow_groups(int width) { return 32 / width; }  // of a warp
 
-// start, end and live bits of K rows, and the first of their sequences (dense and padded rows).
+// Live, start and end bits of K rows.
 struct GroupRows {
   unsigned live, start, end;
 };

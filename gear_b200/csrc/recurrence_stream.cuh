@@ -42,9 +42,6 @@ constexpr int kTableGates = 8;
 constexpr unsigned kNoItem = 0xffffffffu;
 
 __device__ __forceinline__ uint32_t smem_addr(const void *p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
-__device__ __forceinline__ void mbar_init(uint64_t *bar) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(smem_addr(bar)));
-}
 __device__ __forceinline__ void mbar_expect(uint64_t *bar, unsigned bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_addr(bar)), "r"(bytes) : "memory");
 }
@@ -559,7 +556,8 @@ template <typename TX, typename TA, int V, int kGate>
 __device__ __forceinline__ bool compute_forward(const Params &P, StreamShared<TX, TA, V, kGate, false> &sm, unsigned &m,
                                                 int warp, int lane) {
   using Shared = StreamShared<TX, TA, V, kGate, false>;
-  constexpr int kG = kGate == kOne ? 1 : V, R = kRows;
+  static_assert(kGate != kOne, "forward calls take a table of gates");
+  constexpr int kG = V, R = kRows;
   const gearb_recurrence_args &A = P.A;
   Turn<Shared::kStages> now, old;
   Turn<kRing> pair, opair;

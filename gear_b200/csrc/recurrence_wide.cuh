@@ -113,7 +113,7 @@ __device__ __forceinline__ void state_store(float *p, int seq, int64_t width, co
 
 template <typename TX, typename TA, int V, int kGate, bool kApart>
 __global__ void __launch_bounds__(kThreads, V == 4 ? 2 : V == 2 ? 3 : 5) forward_kernel(const __grid_constant__ Params P) {
-  constexpr int kG = kGate == kOne ? 1 : V;
+  static_assert(kGate != kOne, "forward calls take a table of gates");
   constexpr int kW = 32 * V;  // channels of a block
   __shared__ float sa[kWarps][kW], sh[kWarps][kW];
   __shared__ int scut[kWarps];
@@ -128,7 +128,7 @@ __global__ void __launch_bounds__(kThreads, V == 4 ? 2 : V == 2 ? 3 : 5) forward
   const int n = static_cast<int>(i0 >= pl.i1 ? 0 : (pl.i1 - i0 < kRows ? pl.i1 - i0 : kRows));
 
   Pack<TX, V> x[kRows];
-  float a[kRows][kG];
+  float a[kRows][V];
   TileRows tr = rows_of_tile(P, pl);
   load_rows<TX>(static_cast<const TX *>(A.x), P, pl, tr, P.x_period, A.x_batch_stride, A.x_row_stride, warp, n, chans, x);
   load_gate<TA, V, kGate>(P, pl, tr, warp, n, chans, a);
@@ -145,7 +145,7 @@ __global__ void __launch_bounds__(kThreads, V == 4 ? 2 : V == 2 ? 3 : 5) forward
     for (int k = 0; k < kRows; ++k)
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        const float av = a[k][kGate == kOne ? 0 : v];
+        const float av = a[k][v];
         ch[v] = fmaf(av, ch[v], to_f(x[k].v[v]));
         ca[v] *= av;
       }
@@ -158,7 +158,7 @@ __global__ void __launch_bounds__(kThreads, V == 4 ? 2 : V == 2 ? 3 : 5) forward
       if (st) state_load<V>(A.h0, __shfl_sync(kAll, m.seq, k), A.width, chans, s);
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        const float av = a[k][kGate == kOne ? 0 : v], xv = to_f(x[k].v[v]);
+        const float av = a[k][v], xv = to_f(x[k].v[v]);
         if (st) ch[v] = A.h0 ? fmaf(av, s[v], xv) : xv;
         else ch[v] = fmaf(av, ch[v], xv);
         ca[v] *= av;
@@ -215,7 +215,7 @@ __global__ void __launch_bounds__(kThreads, V == 4 ? 2 : V == 2 ? 3 : 5) forward
 #pragma unroll
       for (int k = 0; k < kRows; ++k) {
 #pragma unroll
-        for (int v = 0; v < V; ++v) h[v] = fmaf(a[k][kGate == kOne ? 0 : v], h[v], to_f(x[k].v[v]));
+        for (int v = 0; v < V; ++v) h[v] = fmaf(a[k][v], h[v], to_f(x[k].v[v]));
         chans.store(out + k * step, h);
       }
     } else {
@@ -236,11 +236,11 @@ __global__ void __launch_bounds__(kThreads, V == 4 ? 2 : V == 2 ? 3 : 5) forward
 #pragma unroll
           for (int v = 0; v < V; ++v) {
             const float xv = to_f(x[k].v[v]);
-            h[v] = A.h0 ? fmaf(a[k][kGate == kOne ? 0 : v], s[v], xv) : xv;
+            h[v] = A.h0 ? fmaf(a[k][v], s[v], xv) : xv;
           }
         } else {
 #pragma unroll
-          for (int v = 0; v < V; ++v) h[v] = fmaf(a[k][kGate == kOne ? 0 : v], h[v], to_f(x[k].v[v]));
+          for (int v = 0; v < V; ++v) h[v] = fmaf(a[k][v], h[v], to_f(x[k].v[v]));
         }
         chans.store(out + k * step, h);
         if (m.end >> k & 1u) state_store<V>(A.state_out, seq, A.width, chans, h);
