@@ -13,9 +13,9 @@
 //                         Of tokens without slots only the pages are looked at.  How many there are is known on the device
 //                         alone: 1024 requests of 16 M tokens with 64 slots, token by token, took one CTA 3.8 s.
 // Up to 1024 requests and 4096 slots the scan and the fill are one launch of one CTA.  Measured: 131072 requests,
-// 65 M tokens: 195 us (82 at the copy rate; issue slots are taken in 74 % of the cycles, by 64-bit slots' arithmetic), 254
+// 65 M tokens: 189 us (82 at the copy rate; issue slots are taken in 75 % of the cycles, by 64-bit slots' arithmetic), 254
 // with 64-bit arithmetic throughout, 1950 with a binary search per token and one CTA's prefix sums.  256 requests, one
-// token each: 4.3 us, a launch.
+// token each: 3.5 us, a launch.
 #include "common.h"
 #include "warp_search.cuh"
 

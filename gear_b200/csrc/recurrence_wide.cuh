@@ -7,7 +7,7 @@
 // of the phases: a CTA takes some 13 us for its tile, whatever its types, so what counts is how many fit an SM
 // (2 to 5, by V) and how many bytes each has under way.  Where rows are not aligned for vectors a lane takes two
 // channels 32 apart; with one channel a lane 650 x 64 x 1233 float16 with float32 gates took 235 us, now 148 (63 at
-// the copy rate), 54 x 10733 x 43 221, now 156.  2 x 16384 x 2048 bf16 170 us (113 in the streaming kernels).
+// the copy rate), 54 x 10733 x 43 221, now 156.  2 x 16384 x 2048 bf16 170 us (115 in the streaming kernels).
 #pragma once
 
 #include "recurrence.cuh"
