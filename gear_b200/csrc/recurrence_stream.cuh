@@ -10,11 +10,11 @@
 //   publishers  one thread per channel: turn the warps' pairs into those of all rows before each warp, publish the
 //               tile's
 //   finishers   one thread per channel: the state in front of the tile from what the tiles before published
-// They meet at mbarriers only, and once more when they end: where a wait ran into its limit, abandon() leaves NaN.  2 x 16384 x 2048 bf16 with float32 log gates takes 115 us, 4.67 TB/s of 6.55 (82 us);
-// the backward pass of 4 x 4096 x 2048 118 us, beside 62 us forward.  What bounds it now: 19 warps of one CTA issue in
-// 52 % of the cycles (the two looks at every element, exponentials and conversions), and the rest is the latency
-// of what they hand each other (long scoreboard 3.8 of 8 stall cycles an issue); two CTAs an SM do not fit the
-// registers.  Measured on the way:
+// They meet at mbarriers only, and once more when they end: where a wait ran into its limit, abandon() leaves NaN.
+// 2 x 16384 x 2048 bf16 with float32 log gates takes 115 us, 4.67 TB/s of 6.55 (82 us); the backward pass of
+// 4 x 4096 x 2048 118 us, beside 62 us forward.  What bounds it now: 19 warps of one CTA issue in 52 % of the cycles (the
+// two looks at every element, exponentials and conversions), and the rest is the latency of what they hand each other
+// (long scoreboard 3.8 of 8 stall cycles an issue); two CTAs an SM do not fit the registers.  Measured on the way:
 // a CTA per tile 170 us whatever the types; CTAs that stay but finish a tile before they begin the next: every tile
 // spent 6700 of 11000 cycles looking back; one bulk copy per row: an SM starts one about every 35 cycles, 180 us;
 // every warp finding its rows' place itself: 600 of 1000 instructions; both phases' rows in registers: spills, 234 us;
