@@ -913,10 +913,10 @@ __device__ __noinline__ void abandon(const Params &P, StreamShared<TX, TA, V, kG
     bool recorded[kRecorders];  // whether the recorder has been at the tiles so far
     for (int r = 0; r < kRecorders; ++r) recorded[r] = true;
     for (unsigned m = from; m < to; ++m) {
-      const unsigned stage = m % kStages, parity = m / kStages & 1u, r = m % kRecorders;
-      if (sm.recorded[r].i == stage && sm.recorded[r].parity == parity) recorded[r] = false;
+      const unsigned stage = m % kStages, r = m % kRecorders;
+      if (is_turn(sm.recorded[r], m)) recorded[r] = false;
       if (!recorded[r]) mbar_arrive(&sm.full[stage]);  // in its recorder's place
-      mbar_wait(&sm.full[stage], parity);
+      mbar_wait(&sm.full[stage], m / kStages & 1u);
     }
   }
   __syncthreads();

@@ -22,6 +22,12 @@ struct Turn {
   }
 };
 
+// Whether `t` is the place of turn m, where it is known to be less than 2 * kSize turns away.
+template <unsigned kSize>
+GEARB_RING_FN bool is_turn(const Turn<kSize> &t, unsigned m) {
+  return t.i == m % kSize && t.parity == (m / kSize & 1u);
+}
+
 // Waits for the phase of every turn, in order.  A wait knows the parity of a phase only: while the phase of kSize turns
 // ago runs, that of 2 * kSize turns ago looks like this turn's, ended.  So no turn may be left out, not even one whose
 // data is not needed.  (Waiting for the phase before first would not do: when this turn's has ended already, that one

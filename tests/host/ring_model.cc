@@ -48,8 +48,34 @@ unsigned faults(unsigned stages, unsigned every, unsigned &checked) {
   return bad;
 }
 
+// Two recorders take every other turn and leave the place of the first that they have not recorded.  Turns [from, to) are
+// gone through as a launch that gives up does: which of them has its recorder left out?
+template <unsigned kStages>
+bool left_out_is_found(unsigned &checked) {
+  constexpr unsigned kRecorders = 2;
+  for (unsigned from = 0; from < 60; ++from)
+    for (unsigned to = from; to <= from + kStages; ++to)
+      for (unsigned r = 0; r < kRecorders; ++r)
+        for (unsigned first = from + (from % kRecorders != r); first <= to + 1; first += kRecorders) {
+          gearb::rec::Turn<kStages> place;
+          for (unsigned k = 0; k < first; ++k) place.next();
+          bool recorded = true;
+          for (unsigned m = from; m < to; ++m) {
+            if (m % kRecorders != r) continue;
+            if (gearb::rec::is_turn(place, m)) recorded = false;
+            if (recorded != (m < first)) return false;
+            ++checked;
+          }
+        }
+  return true;
+}
+
 int main() {
   unsigned checked = 0;
+  if (!left_out_is_found<4>(checked) || !left_out_is_found<5>(checked) || !left_out_is_found<6>(checked)) {
+    std::printf("a turn that was not recorded is taken for one that was, or the other way round\n");
+    return 1;
+  }
   for (unsigned stages = 4; stages <= 6; ++stages) {
     if (faults(stages, 1, checked) != 0) {
       std::printf("%u stages: a wait ended early, or never\n", stages);
